@@ -46,6 +46,9 @@ typedef int rtq_status;
  * Their forward takes f32 activations (no activation quantisation) and runs as f32 GEMMs. */
 #define RTQ_TYPE_F32 0
 #define RTQ_TYPE_TQ8_0 264
+/* element types of rows of logits (beside RTQ_TYPE_F32; ggml ids) */
+#define RTQ_TYPE_F16 1
+#define RTQ_TYPE_BF16 30
 
 typedef struct rtq_ctx rtq_ctx;
 typedef struct rtq_weight rtq_weight;
@@ -153,6 +156,72 @@ rtq_status rtq_lm_head(rtq_ctx* ctx, const rtq_weight* lm_head, const float* nor
 rtq_status rtq_lm_head_d(rtq_ctx* ctx, const rtq_weight* lm_head, const float* norm_w, float eps, float offset,
                          const float* x, int64_t t, const int32_t* pos, const int32_t* tok, const float* weights,
                          int64_t n, float* logp, int32_t* hit, float* dx, void* stream);
+
+/* ---- rows of vocabulary logits: top logits, distillation, drafted tokens ----
+ * No counterpart in the reference.  A row is `vocab` logits (vocab <= 2^20) of type RTQ_TYPE_F32, _F16
+ * or _BF16, rows `ld` >= vocab elements apart, at any alignment of an element; what lies between vocab
+ * and ld is neither read nor written.  Temperatures lie in [1e-4, 1e4].  The host versions are synchronous,
+ * take the same arrays on the host and refuse token ids out of range; the `_d` versions take device
+ * pointers, only enqueue, and treat ids out of range as stated.  A `_d` call of this section may be
+ * captured into a HIP graph once an eager call of the same sizes (or larger) has run on the context,
+ * whose workspace cannot grow under capture (RTQ_ERR_INVALID); the graph uses that workspace, so it
+ * replays on the one stream that the context's other calls are issued on. */
+#define RTQ_TOP_MAX 256 /* most listed tokens a row */
+/* A teacher's top logits, as rtq_top_logits writes them.  Its distribution has k + 1 buckets: the listed
+ * tokens, with weight exp(vals / temperature), and all others together, with weight exp(rest).  An id
+ * outside [0, vocab) marks an empty slot (host version: >= vocab is refused); slots naming one token
+ * add.  A row with no listed token above -inf and no rest has no teacher: its divergence and the
+ * divergence's gradient are 0. */
+typedef struct rtq_teacher {
+  int64_t k;           /* slots per row, 1 .. RTQ_TOP_MAX */
+  const int32_t* ids;  /* [n x k] */
+  const float* vals;   /* [n x k] logits, before the temperature */
+  const float* rest;   /* [n] log of the sum of exp(logit / temperature) over the other tokens; NULL: none */
+  float temperature;
+} rtq_teacher;
+/* The k largest logits of each of n rows, largest first, equal logits by the lower id (a NaN is above
+ * every number): vals [n x k], ids [n x k]; rest [n] (or NULL) = log of the sum of exp(logit /
+ * temperature) over the others, -inf where there are none.  1 <= k <= min(vocab, RTQ_TOP_MAX). */
+rtq_status rtq_top_logits(rtq_ctx* ctx, const void* logits, int type, int64_t n, int64_t vocab, int64_t ld, int64_t k,
+                          float temperature, float* vals, int32_t* ids, float* rest);
+rtq_status rtq_top_logits_d(rtq_ctx* ctx, const void* logits, int type, int64_t n, int64_t vocab, int64_t ld, int64_t k,
+                            float temperature, float* vals, int32_t* ids, float* rest, void* stream);
+/* Distillation of n rows of student logits z.  With p the teacher's k + 1 buckets, q = softmax(z / T) summed
+ * over the same buckets (T = teacher->temperature):
+ *   kl[i]   = sum over the buckets of p log(p / q);
+ *   logp[i] = log softmax(z)[tok[i]] (temperature 1; tok and logp may both be NULL, then hard must be 0).
+ * A label outside [0, vocab) is none: logp NaN, no gradient from it (host version: refused).
+ * With weights (else NULL, and dlogits unused), for L = sum weights[i] ((1 - hard) T^2 kl[i] - hard logp[i]),
+ * hard in [0, 1]: dlogits [n x vocab], rows ldd elements apart, = dL/dz in the logits' type, OVERWRITTEN;
+ * it may be the logits themselves (same ldd), and must not overlap them otherwise.  A row of weight 0
+ * has gradient 0.  A NaN logit, or a row of -inf alone, makes the row's outputs NaN. */
+rtq_status rtq_distill(rtq_ctx* ctx, const void* logits, int type, int64_t n, int64_t vocab, int64_t ld,
+                       const rtq_teacher* teacher, const int32_t* tok, const float* weights, float hard, float* kl,
+                       float* logp, void* dlogits, int64_t ldd);
+rtq_status rtq_distill_d(rtq_ctx* ctx, const void* logits, int type, int64_t n, int64_t vocab, int64_t ld,
+                         const rtq_teacher* teacher, const int32_t* tok, const float* weights, float hard, float* kl,
+                         float* logp, void* dlogits, int64_t ldd, void* stream);
+/* Verifies drafted tokens of b sequences against the target's logits (speculative sampling: what comes
+ * out is distributed as samples of the target).  logits: b (d + 1) rows, row i (d + 1) + j the target's
+ * after j of sequence i's drafted tokens; draft: b d rows, row i d + j the logits that drafted[i d + j]
+ * was drawn from, or NULL for drafts that were not drawn (all probability on the token); uniforms
+ * [b x (d + 1)] in [0, 1); lens [b] drafted tokens per sequence, clamped to [0, d] (host version:
+ * refused outside), or NULL for d.  With p, q the softmax of a row / temperature, in 64 bits:
+ *   tokens j = 0, 1, ... are accepted while uniforms[j] q_j(x_j) < p_j(x_j) and j < lens;
+ *   then one more is drawn: from max(p - q, 0) at a rejection (from p if that is nowhere positive), from p
+ *   after all: the first id whose running sum passes uniforms[d] times the total.
+ * temperature 0: accepted while x_j is the row's largest logit (the lowest id of equals), which is also the
+ * token drawn; draft and uniforms are not read.  accepted [b]; tokens [b x (d + 1)]: the accepted ones,
+ * the drawn one, -1 after.  A drafted id outside [0, vocab) is rejected (host version: refused).  Rows
+ * past a sequence's length are not read.  A row without a distribution (a NaN, or -inf alone) accepts
+ * nothing and draws -1. */
+rtq_status rtq_verify_draft(rtq_ctx* ctx, const void* logits, int type, int64_t ld, const void* draft, int64_t ldq,
+                            int64_t b, int64_t d, int64_t vocab, const int32_t* drafted, const int32_t* lens,
+                            const float* uniforms, float temperature, int32_t* accepted, int32_t* tokens);
+rtq_status rtq_verify_draft_d(rtq_ctx* ctx, const void* logits, int type, int64_t ld, const void* draft, int64_t ldq,
+                              int64_t b, int64_t d, int64_t vocab, const int32_t* drafted, const int32_t* lens,
+                              const float* uniforms, float temperature, int32_t* accepted, int32_t* tokens,
+                              void* stream);
 
 /* ---- device-resident training step (Model::forward_backward over the frozen linears) ----
  * A GGUF Qwen / Llama decoder (load_gguf_from, src/rie.rs:164-260) with every frozen tensor, norm

@@ -17,6 +17,9 @@ STATUS_NAMES = {0: "OK", 1: "ERR_INVALID", 2: "ERR_UNSUPPORTED", 3: "ERR_HIP", 4
 TYPE_Q4_0, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K = 2, 8, 12, 14
 # trainer-native FrozenWeight storage (src/frozen.rs:33-45): f32, and Q8_0 with f32 block scales
 TYPE_F32, TYPE_TQ8_0 = 0, 264
+# element types of rows of logits, beside TYPE_F32
+TYPE_F16, TYPE_BF16 = 1, 30
+TOP_MAX = 256  # most listed tokens a row
 
 # every symbol include/rtq.h declares, with (restype, argtypes)
 _p = ctypes.c_void_p
@@ -32,6 +35,14 @@ class RtqLora(ctypes.Structure):
 
 
 _LP = ctypes.POINTER(RtqLora)
+
+
+class RtqTeacher(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_int64), ("ids", ctypes.c_void_p), ("vals", ctypes.c_void_p), ("rest", ctypes.c_void_p),
+                ("temperature", ctypes.c_float)]
+
+
+_TP = ctypes.POINTER(RtqTeacher)
 
 
 class RtqModelConfig(ctypes.Structure):
@@ -77,6 +88,13 @@ SIGNATURES = {
     "rtq_frozen_gather_d": (_i, [_p, _p, _p, _i64, _p, _p]),
     "rtq_lm_head": (_i, [_p, _p, _p, _f, _f, _p, _i64, _p, _p, _p, _i64, _p, ctypes.POINTER(_i64), _p]),
     "rtq_lm_head_d": (_i, [_p, _p, _p, _f, _f, _p, _i64, _p, _p, _p, _i64, _p, _p, _p, _p]),
+    # rows of vocabulary logits
+    "rtq_top_logits": (_i, [_p, _p, _i, _i64, _i64, _i64, _i64, _f, _p, _p, _p]),
+    "rtq_top_logits_d": (_i, [_p, _p, _i, _i64, _i64, _i64, _i64, _f, _p, _p, _p, _p]),
+    "rtq_distill": (_i, [_p, _p, _i, _i64, _i64, _i64, _TP, _p, _p, _f, _p, _p, _p, _i64]),
+    "rtq_distill_d": (_i, [_p, _p, _i, _i64, _i64, _i64, _TP, _p, _p, _f, _p, _p, _p, _i64, _p]),
+    "rtq_verify_draft": (_i, [_p, _p, _i, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _f, _p, _p]),
+    "rtq_verify_draft_d": (_i, [_p, _p, _i, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _f, _p, _p, _p]),
     # device-resident training step
     "rtq_linear_forward_noalloc_d": (_i, [_p, _p, _p, _LP, _p, _i64, _p, _p]),
     "rtq_model_from_gguf": (_i, [_p, _p, ctypes.POINTER(_p)]),

@@ -352,6 +352,64 @@ struct HeadArgs {
   float* dx;           // [t x d] dL/dx (rows without a target are cleared separately)
 };
 
+// ---------------------------------------------------------------- rows of vocabulary logits
+// z: rows of V logits (f32, f16 or bf16), stride ld elements; a row is cut into G slices of L
+// logits.  ch + cl = log2(e) / temp.
+struct TopArgs {
+  const void* z;
+  int64_t ld;
+  int n, V, k, G, L;
+  float temp, ch, cl;
+  uint64_t* lists;  // [n x G x k] each slice's largest, in order (G > 1)
+  float* pm;        // [n x G] maximum of each slice's others
+  double* ps;       // [n x G] their sum of exp((z - pm) / temp)
+  float* vals;      // [n x k]
+  int32_t* ids;     // [n x k]
+  float* rest;      // [n] or null
+};
+
+struct DistillArgs {
+  const void* z;
+  void* dz;  // [n x V] gradient, stride ldd (may be z itself)
+  int64_t ld, ldd;
+  int n, V, k, G, L;
+  float temp, ch, cl, hard;
+  const int32_t* ids;  // [n x k] the teacher's tokens (outside [0, V): no token)
+  const float* tv;     // [n x k] its logits
+  const float* rest;   // [n] log-sum-exp of its other logits / temp, or null
+  const int32_t* tok;  // [n] labels, or null
+  const float* w;      // [n] loss weights, or null (no gradient)
+  float* pm;           // [n x G] maximum of each slice's unlisted logits
+  double* psT;         // [n x G] their sums of exp((z - pm) / temp)
+  double* ps1;         // [n x G] and of exp(z - pm) (with labels)
+  int32_t* twice;      // [n x G] a token of the slice is listed twice
+  float* zs;           // [n x k] the student's logits of the listed tokens
+  float* zt;           // [n] and of the labels
+  float* kl;           // [n]
+  float* logp;         // [n] or null
+};
+
+struct VerifyPick {  // the row that sequence i's next token is drawn from
+  double pm, ps, qm, qs;  // maxima and reciprocal sums of the target's and the draft's row
+  int row, not_x, minus_q, pad;
+};
+struct VerifyArgs {
+  const void* z;  // [b (d + 1)] target rows, stride ld
+  const void* q;  // [b d] draft rows, stride ldq, or null
+  int64_t ld, ldq;
+  int b, d, V, G, L;
+  float temp;
+  const int32_t* drafted;  // [b x d]
+  const int32_t* lens;     // [b] or null: d
+  const float* u;          // [b x (d + 1)]
+  int32_t* accepted;       // [b]
+  int32_t* tokens;         // [b x (d + 1)]
+  uint64_t* pk;            // [rows x G] rank key of each slice's maximum
+  double* ps;              // [rows x G] sum of exp((z - max) / temp)
+  VerifyPick* pick;        // [b]
+  double* mass;            // [b x G x 2] sums of the weights and of p over the row's slices
+};
+
 // ---------------------------------------------------------------- model-level step
 // The decoder block around the frozen linears (src/model.rs:165-197, src/attention.rs:162-367,
 // src/model.rs:113-134, src/ops.rs:14-56, :118-196), all tensors row-major f32 on the device.

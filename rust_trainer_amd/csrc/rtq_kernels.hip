@@ -4601,6 +4601,9 @@ extern "C" __global__ __launch_bounds__(256) void rtq_head_norm_bwd(HeadArgs a) 
   }
 }
 
+// ============================================================== rows of vocabulary logits
+#include "rtq_vocab.hip"
+
 // ============================================================== decoder block (model-level step)
 #include "rtq_dense.hip"
 #include "rtq_model_kernels.hip"

@@ -165,7 +165,15 @@ enum Kid {
   K_HEAD_NORM_BWD,
   K_ACT_PREP8,   // Q8_0 activations of the block norms on 8-token tiles
   K_ACT_PREP4,   // the same on 4-token tiles
-  K_ROWS,        // + format
+  K_TOP,         // + type + 3 * (the longer slices): top logits of a slice, of a row from its slices
+  K_TOP_MERGE = K_TOP + 6,
+  K_DISTILL_STATS,  // + type
+  K_DISTILL_GRAD = K_DISTILL_STATS + 3,
+  K_VERIFY_STATS = K_DISTILL_GRAD + 3,
+  K_VERIFY_ACCEPT = K_VERIFY_STATS + 3,
+  K_VERIFY_MASS = K_VERIFY_ACCEPT + 3,
+  K_VERIFY_PICK = K_VERIFY_MASS + 3,
+  K_ROWS = K_VERIFY_PICK + 3,  // + format
   K_MODEL = K_ROWS + F_COUNT,  // + RtqModelKernel: the decoder block (rtq_model.cpp)
   K_COUNT = K_MODEL + KM_COUNT
 };
@@ -196,6 +204,14 @@ constexpr const char* kKernelNames[] = {
     "rtq_dense_bwd32",      "rtq_dense_bwd32_q8",   "rtq_dense_bwd64",      "rtq_dense_bwd64_q8",
     "rtq_head_norm",        "rtq_head_max",         "rtq_head_sum",         "rtq_head_grad",
     "rtq_head_norm_bwd",    "rtq_act_prep8_q8_0",   "rtq_act_prep4_q8_0",
+    "rtq_top_f32_s",        "rtq_top_f16_s",        "rtq_top_bf16_s",       "rtq_top_f32_l",        "rtq_top_f16_l",
+    "rtq_top_bf16_l",       "rtq_top_merge",
+    "rtq_distill_stats_f32", "rtq_distill_stats_f16", "rtq_distill_stats_bf16",
+    "rtq_distill_grad_f32", "rtq_distill_grad_f16", "rtq_distill_grad_bf16",
+    "rtq_verify_stats_f32", "rtq_verify_stats_f16", "rtq_verify_stats_bf16",
+    "rtq_verify_accept_f32", "rtq_verify_accept_f16", "rtq_verify_accept_bf16",
+    "rtq_verify_mass_f32",  "rtq_verify_mass_f16",  "rtq_verify_mass_bf16",
+    "rtq_verify_pick_f32",  "rtq_verify_pick_f16",  "rtq_verify_pick_bf16",
     "rtq_rows_q4_0",        "rtq_rows_q8_0",        "rtq_rows_q4_k",        "rtq_rows_q6_k",
     "rtq_m_rmsnorm",        "rtq_m_rmsnorm_bwd",    "rtq_m_qk_prep",        "rtq_m_qk_bwd",
     "rtq_m_gemm",           "rtq_m_softmax",        "rtq_m_softmax_bwd",    "rtq_m_group_sum",
@@ -226,6 +242,8 @@ struct rtq_ctx {
   void* ws = nullptr;
   size_t ws_bytes = 0;
   uint64_t ws_gen = 0;  // bumped whenever ws moves (graphs that captured its address are stale)
+  bool ws_captured = false;    // a caller's graph holds ws's address: when it is outgrown it is kept,
+  std::vector<void*> retired;  // here, until the context goes, so that the graph can still replay
   bool timing = false;
   int timing_only = -1;  // -1: every kernel
   std::vector<TimedLaunch> pending;
@@ -342,6 +360,12 @@ struct Arena {
 rtq_status ensure_ws(rtq_ctx* c, size_t bytes) {
   if (bytes <= c->ws_bytes) return RTQ_OK;
   size_t want = std::max<size_t>(bytes + bytes / 4, 1 << 20);
+  if (c->ws && c->ws_captured) {
+    c->retired.push_back(c->ws);
+    c->ws = nullptr;
+    c->ws_bytes = 0;
+    c->ws_captured = false;
+  }
   if (c->ws) {
     HIP_TRY(hipDeviceSynchronize());
     HIP_TRY(hipFree(c->ws));
@@ -1438,6 +1462,7 @@ void rtq_ctx_destroy(rtq_ctx* c) {
   }
   for (auto e : c->free_events) (void)hipEventDestroy(e);
   if (c->ws) (void)hipFree(c->ws);
+  for (void* p : c->retired) (void)hipFree(p);
   if (c->stream) (void)hipStreamDestroy(c->stream);
   if (c->mod) (void)hipModuleUnload(c->mod);
   delete c;
@@ -1835,6 +1860,257 @@ rtq_status rtq_lm_head_d(rtq_ctx* c, const rtq_weight* w, const float* norm, flo
   return enqueue_head(c, w, norm, eps, offset, x, t, pos, tok, weights, n, logp, hit, dx, hp, ar, st);
 }
 
+// ------------------------------------------------------------------ rows of vocabulary logits
+namespace {
+
+constexpr int64_t kVocabMax = 1 << 20;
+constexpr int64_t kTopMergeMax = 8192;  // list entries that rtq_top_merge sorts at most (64 KiB of LDS)
+
+int logit_type(int type) { return type == RTQ_TYPE_F32 ? 0 : type == RTQ_TYPE_F16 ? 1 : type == RTQ_TYPE_BF16 ? 2 : -1; }
+int64_t logit_bytes(int type) { return type == RTQ_TYPE_F32 ? 4 : 2; }
+
+// the workspace of a call on `st`: it does not grow under capture, and a graph that captured it keeps it
+rtq_status row_ws(rtq_ctx* c, size_t bytes, hipStream_t st) {
+  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+  HIP_TRY(hipStreamIsCapturing(st, &cs));
+  if (cs != hipStreamCaptureStatusNone) {
+    if (bytes > c->ws_bytes)
+      return fail(RTQ_ERR_INVALID,
+                  "the workspace (%zu bytes, %zu needed) cannot grow under capture: make an eager call of this size first",
+                  c->ws_bytes, bytes);
+    c->ws_captured = true;
+    return RTQ_OK;
+  }
+  return ensure_ws(c, bytes);
+}
+
+rtq_status check_rows(const void* z, int type, int64_t n, int64_t vocab, int64_t ld) {
+  if (logit_type(type) < 0) return fail(RTQ_ERR_UNSUPPORTED, "logits of type %d (F32, F16 and BF16 are supported)", type);
+  if (n < 0 || n > 65535) return fail(RTQ_ERR_INVALID, "row count %lld out of range [0, 65535]", (long long)n);
+  if (vocab < 1 || vocab > kVocabMax)
+    return fail(RTQ_ERR_INVALID, "vocabulary of %lld out of range [1, %lld]", (long long)vocab, (long long)kVocabMax);
+  if (ld < vocab || ld > (1LL << 40)) return fail(RTQ_ERR_INVALID, "row stride %lld with a vocabulary of %lld", (long long)ld, (long long)vocab);
+  if (n > 0 && !z) return fail(RTQ_ERR_INVALID, "null logits");
+  if ((uintptr_t)z % (uintptr_t)logit_bytes(type)) return fail(RTQ_ERR_INVALID, "logits not aligned to their elements");
+  return RTQ_OK;
+}
+
+rtq_status check_ctx(const rtq_ctx* c) { return c ? RTQ_OK : fail(RTQ_ERR_INVALID, "null context"); }
+
+rtq_status check_temperature(float t) {
+  if (!(t >= 1e-4f && t <= 1e4f)) return fail(RTQ_ERR_INVALID, "temperature %g out of range [1e-4, 1e4]", (double)t);
+  return RTQ_OK;
+}
+
+// log2(e) / t as the sum of two floats
+void exp_scale(float t, float* hi, float* lo) {
+  const double e = 1.4426950408889634 / (double)t;
+  *hi = (float)e;
+  *lo = (float)(e - (double)*hi);
+}
+
+// ---- top logits
+struct TopPlan {
+  bool large;  // the longer slices
+  int64_t G, L;
+  size_t bytes;
+};
+
+TopPlan top_plan(int type, int64_t n, int64_t V, int64_t k) {
+  const int64_t per = 1024 * 16 / logit_bytes(type);  // logits a workgroup loads at once
+  TopPlan p{};
+  p.L = 2 * per;
+  if (cdiv(V, p.L) * k > kTopMergeMax) p.large = true, p.L = (type == RTQ_TYPE_F32 ? 8 : 4) * per;
+  p.G = cdiv(V, p.L);
+  if (p.G > 1) p.bytes = (size_t)(n * p.G * k) * 8 + (size_t)(n * p.G) * 12 + 4 * 256;
+  return p;
+}
+
+rtq_status check_top(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V, int64_t ld, int64_t k, float temp,
+                     const float* vals, const int32_t* ids) {
+  RTQ_TRY(check_rows(z, type, n, V, ld));
+  RTQ_TRY(check_temperature(temp));
+  if (k < 1 || k > RTQ_TOP_MAX || k > V)
+    return fail(RTQ_ERR_INVALID, "k = %lld out of range [1, min(%lld, %d)]", (long long)k, (long long)V, RTQ_TOP_MAX);
+  if (n > 0 && (!vals || !ids)) return fail(RTQ_ERR_INVALID, "null vals/ids");
+  return check_ctx(c);
+}
+
+rtq_status enqueue_top(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V, int64_t ld, int64_t k, float temp,
+                       float* vals, int32_t* ids, float* rest, const TopPlan& p, Arena& ar, hipStream_t st) {
+  TopArgs a{};
+  a.z = z, a.ld = ld, a.n = (int)n, a.V = (int)V, a.k = (int)k, a.G = (int)p.G, a.L = (int)p.L;
+  a.temp = temp;
+  exp_scale(temp, &a.ch, &a.cl);
+  a.vals = vals, a.ids = ids, a.rest = rest;
+  if (p.G > 1) {
+    a.lists = ar.take<uint64_t>((size_t)(n * p.G * k));
+    a.ps = ar.take<double>((size_t)(n * p.G));
+    a.pm = ar.take<float>((size_t)(n * p.G));
+    if (ar.off > ar.cap) return fail(RTQ_ERR_INVALID, "internal: workspace too small");
+  }
+  RTQ_TRY(launch(c, K_TOP + logit_type(type) + (p.large ? 3 : 0), dim3((unsigned)p.G, (unsigned)n), dim3(1024), st, a));
+  if (p.G == 1) return RTQ_OK;
+  unsigned P = 2;
+  while (P < p.G * k) P <<= 1;
+  return launch(c, K_TOP_MERGE, dim3((unsigned)n), dim3(1024), st, a, P * 8);
+}
+
+// ---- distillation
+struct DistillPlan {
+  int64_t G, L;
+  size_t bytes;
+};
+
+DistillPlan distill_plan(int64_t n, int64_t V, int64_t k) {
+  DistillPlan p{};
+  p.L = 8192;
+  p.G = cdiv(V, p.L);
+  p.bytes = (size_t)(n * p.G) * 24 + (size_t)(n * k + n) * 4 + 8 * 256;
+  return p;
+}
+
+rtq_status check_distill(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V, int64_t ld, const rtq_teacher* t,
+                         const int32_t* tok, const float* w, float hard, const float* kl, const float* logp,
+                         const void* dz, int64_t ldd) {
+  RTQ_TRY(check_rows(z, type, n, V, ld));
+  if (!t) return fail(RTQ_ERR_INVALID, "null teacher");
+  RTQ_TRY(check_temperature(t->temperature));
+  if (t->k < 1 || t->k > RTQ_TOP_MAX)
+    return fail(RTQ_ERR_INVALID, "%lld slots per row out of range [1, %d]", (long long)t->k, RTQ_TOP_MAX);
+  if (!(hard >= 0.0f && hard <= 1.0f)) return fail(RTQ_ERR_INVALID, "hard = %g out of range [0, 1]", (double)hard);
+  if ((tok == nullptr) != (logp == nullptr)) return fail(RTQ_ERR_INVALID, "tok and logp go together");
+  if (!tok && hard > 0.0f) return fail(RTQ_ERR_INVALID, "hard > 0 without labels");
+  if (n > 0 && (!t->ids || !t->vals || !kl)) return fail(RTQ_ERR_INVALID, "null ids/vals/kl");
+  if (!w) return check_ctx(c);
+  if (n > 0 && !dz) return fail(RTQ_ERR_INVALID, "weights given without dlogits");
+  if (ldd < V || ldd > (1LL << 40)) return fail(RTQ_ERR_INVALID, "gradient row stride %lld with a vocabulary of %lld", (long long)ldd, (long long)V);
+  const int64_t es = logit_bytes(type);
+  if ((uintptr_t)dz % (uintptr_t)es) return fail(RTQ_ERR_INVALID, "dlogits not aligned to its elements");
+  if (n > 0) {
+    const uintptr_t z0 = (uintptr_t)z, z1 = z0 + (uintptr_t)(((n - 1) * ld + V) * es);
+    const uintptr_t d0 = (uintptr_t)dz, d1 = d0 + (uintptr_t)(((n - 1) * ldd + V) * es);
+    if (d0 < z1 && z0 < d1 && !(z0 == d0 && (ld == ldd || n == 1)))
+      return fail(RTQ_ERR_INVALID, "dlogits overlaps the logits without being them");
+  }
+  return check_ctx(c);
+}
+
+rtq_status enqueue_distill(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V, int64_t ld, const rtq_teacher& t,
+                           const int32_t* tok, const float* w, float hard, float* kl, float* logp, void* dz,
+                           int64_t ldd, const DistillPlan& p, Arena& ar, hipStream_t st) {
+  DistillArgs a{};
+  a.z = z, a.dz = dz, a.ld = ld, a.ldd = ldd;
+  a.n = (int)n, a.V = (int)V, a.k = (int)t.k, a.G = (int)p.G, a.L = (int)p.L;
+  a.temp = t.temperature;
+  exp_scale(t.temperature, &a.ch, &a.cl);
+  a.hard = hard, a.ids = t.ids, a.tv = t.vals, a.rest = t.rest, a.tok = tok, a.w = w, a.kl = kl, a.logp = logp;
+  a.psT = ar.take<double>((size_t)(n * p.G));
+  a.ps1 = ar.take<double>((size_t)(n * p.G));
+  a.pm = ar.take<float>((size_t)(n * p.G));
+  a.twice = ar.take<int32_t>((size_t)(n * p.G));
+  a.zs = ar.take<float>((size_t)(n * t.k));
+  a.zt = ar.take<float>((size_t)n);
+  if (ar.off > ar.cap) return fail(RTQ_ERR_INVALID, "internal: workspace too small");
+  const dim3 grid((unsigned)p.G, (unsigned)n);
+  RTQ_TRY(launch(c, K_DISTILL_STATS + logit_type(type), grid, dim3(256), st, a, (unsigned)(p.L / 8)));
+  return launch(c, K_DISTILL_GRAD + logit_type(type), w ? grid : dim3(1, (unsigned)n), dim3(256), st, a);
+}
+
+// ---- drafted tokens
+struct VerifyPlan {
+  int64_t G, L, rows;
+  size_t bytes;
+};
+
+VerifyPlan verify_plan(int64_t b, int64_t d, int64_t V, bool draft) {
+  VerifyPlan p{};
+  p.L = 8192;
+  p.G = cdiv(V, p.L);
+  p.rows = b * (d + 1) + (draft ? b * d : 0);
+  p.bytes = (size_t)(p.rows * p.G) * 16 + (size_t)b * sizeof(VerifyPick) + (size_t)(b * p.G) * 16 + 8 * 256;
+  return p;
+}
+
+rtq_status check_verify(rtq_ctx* c, const void* z, int type, int64_t ld, const void* q, int64_t ldq, int64_t b, int64_t d,
+                        int64_t V, const int32_t* drafted, const float* u, float temp, const int32_t* accepted,
+                        const int32_t* tokens) {
+  if (b < 0 || b > 65535 || d < 0 || d > 65535 || b * (2 * d + 1) > (1 << 24))
+    return fail(RTQ_ERR_INVALID, "%lld sequences of %lld drafted tokens", (long long)b, (long long)d);
+  RTQ_TRY(check_rows(z, type, b, V, ld));
+  if (temp != 0.0f) RTQ_TRY(check_temperature(temp));
+  if (q && (ldq < V || ldq > (1LL << 40))) return fail(RTQ_ERR_INVALID, "draft row stride %lld with a vocabulary of %lld", (long long)ldq, (long long)V);
+  if ((uintptr_t)q % (uintptr_t)logit_bytes(type)) return fail(RTQ_ERR_INVALID, "draft logits not aligned to their elements");
+  if (b > 0 && ((d > 0 && !drafted) || !accepted || !tokens)) return fail(RTQ_ERR_INVALID, "null drafted/accepted/tokens");
+  if (b > 0 && temp != 0.0f && !u) return fail(RTQ_ERR_INVALID, "null uniforms");
+  return check_ctx(c);
+}
+
+rtq_status enqueue_verify(rtq_ctx* c, const void* z, int type, int64_t ld, const void* q, int64_t ldq, int64_t b, int64_t d,
+                          int64_t V, const int32_t* drafted, const int32_t* lens, const float* u, float temp,
+                          int32_t* accepted, int32_t* tokens, const VerifyPlan& p, Arena& ar, hipStream_t st) {
+  VerifyArgs a{};
+  a.z = z, a.q = q, a.ld = ld, a.ldq = ldq;
+  a.b = (int)b, a.d = (int)d, a.V = (int)V, a.G = (int)p.G, a.L = (int)p.L, a.temp = temp;
+  a.drafted = drafted, a.lens = lens, a.u = u, a.accepted = accepted, a.tokens = tokens;
+  a.pk = ar.take<uint64_t>((size_t)(p.rows * p.G));
+  a.ps = ar.take<double>((size_t)(p.rows * p.G));
+  a.pick = ar.take<VerifyPick>((size_t)b);
+  a.mass = ar.take<double>((size_t)(b * p.G * 2));
+  if (ar.off > ar.cap) return fail(RTQ_ERR_INVALID, "internal: workspace too small");
+  const int ty = logit_type(type);
+  const int64_t gy = std::min<int64_t>(p.rows, 65535);
+  RTQ_TRY(launch(c, K_VERIFY_STATS + ty, dim3((unsigned)p.G, (unsigned)gy, (unsigned)cdiv(p.rows, 65535)), dim3(256), st, a));
+  RTQ_TRY(launch(c, K_VERIFY_ACCEPT + ty, dim3((unsigned)b), dim3(64), st, a));
+  if (temp == 0.0f) return RTQ_OK;
+  RTQ_TRY(launch(c, K_VERIFY_MASS + ty, dim3((unsigned)p.G, (unsigned)b), dim3(256), st, a));
+  return launch(c, K_VERIFY_PICK + ty, dim3((unsigned)b), dim3(256), st, a);
+}
+
+}  // namespace
+
+rtq_status rtq_top_logits_d(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V, int64_t ld, int64_t k, float temp,
+                            float* vals, int32_t* ids, float* rest, void* stream) {
+  RTQ_TRY(check_top(c, z, type, n, V, ld, k, temp, vals, ids));
+  if (n == 0) return RTQ_OK;
+  std::lock_guard<std::mutex> lk(c->mu);
+  HIP_TRY(hipSetDevice(c->device));
+  hipStream_t st = (hipStream_t)stream;
+  const TopPlan p = top_plan(type, n, V, k);
+  RTQ_TRY(row_ws(c, p.bytes, st));
+  Arena ar{(char*)c->ws, c->ws_bytes, 0};
+  return enqueue_top(c, z, type, n, V, ld, k, temp, vals, ids, rest, p, ar, st);
+}
+
+rtq_status rtq_distill_d(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V, int64_t ld, const rtq_teacher* t,
+                         const int32_t* tok, const float* w, float hard, float* kl, float* logp, void* dz, int64_t ldd,
+                         void* stream) {
+  RTQ_TRY(check_distill(c, z, type, n, V, ld, t, tok, w, hard, kl, logp, dz, ldd));
+  if (n == 0) return RTQ_OK;
+  std::lock_guard<std::mutex> lk(c->mu);
+  HIP_TRY(hipSetDevice(c->device));
+  hipStream_t st = (hipStream_t)stream;
+  const DistillPlan p = distill_plan(n, V, t->k);
+  RTQ_TRY(row_ws(c, p.bytes, st));
+  Arena ar{(char*)c->ws, c->ws_bytes, 0};
+  return enqueue_distill(c, z, type, n, V, ld, *t, tok, w, hard, kl, logp, dz, ldd, p, ar, st);
+}
+
+rtq_status rtq_verify_draft_d(rtq_ctx* c, const void* z, int type, int64_t ld, const void* q, int64_t ldq, int64_t b,
+                              int64_t d, int64_t V, const int32_t* drafted, const int32_t* lens, const float* u, float temp,
+                              int32_t* accepted, int32_t* tokens, void* stream) {
+  RTQ_TRY(check_verify(c, z, type, ld, q, ldq, b, d, V, drafted, u, temp, accepted, tokens));
+  if (b == 0) return RTQ_OK;
+  std::lock_guard<std::mutex> lk(c->mu);
+  HIP_TRY(hipSetDevice(c->device));
+  hipStream_t st = (hipStream_t)stream;
+  if (temp == 0.0f || d == 0) q = nullptr;
+  const VerifyPlan p = verify_plan(b, d, V, q != nullptr);
+  RTQ_TRY(row_ws(c, p.bytes, st));
+  Arena ar{(char*)c->ws, c->ws_bytes, 0};
+  return enqueue_verify(c, z, type, ld, q, ldq, b, d, V, drafted, lens, u, temp, accepted, tokens, p, ar, st);
+}
+
 // ------------------------------------------------------------------ host-pointer API
 namespace {
 
@@ -2033,6 +2309,126 @@ rtq_status rtq_lm_head(rtq_ctx* c, const rtq_weight* w, const float* norm, float
     for (int32_t h : hv) s += h;
     *hits = s;
   }
+  return RTQ_OK;
+}
+
+// ------------------------------------------------------------------ rows of vocabulary logits, on host arrays
+namespace {
+// n rows of V elements of es bytes, ld apart on the host, back to back on the device
+rtq_status h2d_rows(void* d, const void* h, int64_t n, int64_t V, int64_t ld, int64_t es, hipStream_t st) {
+  HIP_TRY(hipMemcpy2DAsync(d, (size_t)(V * es), h, (size_t)(ld * es), (size_t)(V * es), (size_t)n, hipMemcpyHostToDevice, st));
+  return RTQ_OK;
+}
+rtq_status d2h_rows(void* h, const void* d, int64_t n, int64_t V, int64_t ld, int64_t es, hipStream_t st) {
+  HIP_TRY(hipMemcpy2DAsync(h, (size_t)(ld * es), d, (size_t)(V * es), (size_t)(V * es), (size_t)n, hipMemcpyDeviceToHost, st));
+  return RTQ_OK;
+}
+rtq_status check_teacher_ids(const rtq_teacher* t, int64_t n, int64_t V) {
+  for (int64_t i = 0; i < n * t->k; i++)
+    if (t->ids[i] >= V) return fail(RTQ_ERR_INVALID, "teacher token %d of row %lld out of vocab", t->ids[i], (long long)(i / t->k));
+  return RTQ_OK;
+}
+}  // namespace
+
+rtq_status rtq_top_logits(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V, int64_t ld, int64_t k, float temp,
+                          float* vals, int32_t* ids, float* rest) {
+  RTQ_TRY(check_top(c, z, type, n, V, ld, k, temp, vals, ids));
+  if (n == 0) return RTQ_OK;
+  HostCall hc(c);
+  HIP_TRY(hipSetDevice(c->device));
+  hipStream_t st = c->stream;
+  const TopPlan p = top_plan(type, n, V, k);
+  const int64_t es = logit_bytes(type);
+  RTQ_TRY(ensure_ws(c, p.bytes + (size_t)(n * V * es + n * (8 * k + 4)) + 4 * 256));
+  Arena ar{(char*)c->ws, c->ws_bytes, 0};
+  char* zd = ar.take<char>((size_t)(n * V * es));
+  float* vd = ar.take<float>((size_t)(n * k));
+  int32_t* kd = ar.take<int32_t>((size_t)(n * k));
+  float* rd = rest ? ar.take<float>((size_t)n) : nullptr;
+  RTQ_TRY(h2d_rows(zd, z, n, V, ld, es, st));
+  RTQ_TRY(enqueue_top(c, zd, type, n, V, V, k, temp, vd, kd, rd, p, ar, st));
+  RTQ_TRY(d2h(vals, vd, (size_t)(n * k) * 4, st));
+  RTQ_TRY(d2h(ids, kd, (size_t)(n * k) * 4, st));
+  if (rest) RTQ_TRY(d2h(rest, rd, (size_t)n * 4, st));
+  HIP_TRY(hipStreamSynchronize(st));
+  return RTQ_OK;
+}
+
+rtq_status rtq_distill(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V, int64_t ld, const rtq_teacher* t,
+                       const int32_t* tok, const float* w, float hard, float* kl, float* logp, void* dz, int64_t ldd) {
+  RTQ_TRY(check_distill(c, z, type, n, V, ld, t, tok, w, hard, kl, logp, dz, ldd));
+  if (n == 0) return RTQ_OK;
+  RTQ_TRY(check_teacher_ids(t, n, V));
+  for (int64_t i = 0; tok && i < n; i++)
+    if (tok[i] < 0 || tok[i] >= V) return fail(RTQ_ERR_INVALID, "label %d of row %lld out of vocab", tok[i], (long long)i);
+  HostCall hc(c);
+  HIP_TRY(hipSetDevice(c->device));
+  hipStream_t st = c->stream;
+  const DistillPlan p = distill_plan(n, V, t->k);
+  const int64_t es = logit_bytes(type), k = t->k;
+  RTQ_TRY(ensure_ws(c, p.bytes + (size_t)(n * V * es + n * (8 * k + 20)) + 8 * 256));
+  Arena ar{(char*)c->ws, c->ws_bytes, 0};
+  char* zd = ar.take<char>((size_t)(n * V * es));  // the gradient is written over it
+  int32_t* idd = ar.take<int32_t>((size_t)(n * k));
+  float* vd = ar.take<float>((size_t)(n * k));
+  float* rd = t->rest ? ar.take<float>((size_t)n) : nullptr;
+  int32_t* kd = tok ? ar.take<int32_t>((size_t)n) : nullptr;
+  float* wd = w ? ar.take<float>((size_t)n) : nullptr;
+  float* kld = ar.take<float>((size_t)n);
+  float* lpd = tok ? ar.take<float>((size_t)n) : nullptr;
+  RTQ_TRY(h2d_rows(zd, z, n, V, ld, es, st));
+  RTQ_TRY(h2d(idd, t->ids, (size_t)(n * k) * 4, st));
+  RTQ_TRY(h2d(vd, t->vals, (size_t)(n * k) * 4, st));
+  if (rd) RTQ_TRY(h2d(rd, t->rest, (size_t)n * 4, st));
+  if (kd) RTQ_TRY(h2d(kd, tok, (size_t)n * 4, st));
+  if (wd) RTQ_TRY(h2d(wd, w, (size_t)n * 4, st));
+  const rtq_teacher td{k, idd, vd, rd, t->temperature};
+  RTQ_TRY(enqueue_distill(c, zd, type, n, V, V, td, kd, wd, hard, kld, lpd, zd, V, p, ar, st));
+  RTQ_TRY(d2h(kl, kld, (size_t)n * 4, st));
+  if (lpd) RTQ_TRY(d2h(logp, lpd, (size_t)n * 4, st));
+  if (w) RTQ_TRY(d2h_rows(dz, zd, n, V, ldd, es, st));
+  HIP_TRY(hipStreamSynchronize(st));
+  return RTQ_OK;
+}
+
+rtq_status rtq_verify_draft(rtq_ctx* c, const void* z, int type, int64_t ld, const void* q, int64_t ldq, int64_t b,
+                            int64_t d, int64_t V, const int32_t* drafted, const int32_t* lens, const float* u, float temp,
+                            int32_t* accepted, int32_t* tokens) {
+  RTQ_TRY(check_verify(c, z, type, ld, q, ldq, b, d, V, drafted, u, temp, accepted, tokens));
+  if (b == 0) return RTQ_OK;
+  for (int64_t i = 0; i < b; i++) {
+    if (lens && (lens[i] < 0 || lens[i] > d)) return fail(RTQ_ERR_INVALID, "sequence %lld has %d of %lld drafted tokens", (long long)i, lens[i], (long long)d);
+    for (int64_t j = 0; j < (lens ? lens[i] : d); j++)
+      if (drafted[i * d + j] < 0 || drafted[i * d + j] >= V)
+        return fail(RTQ_ERR_INVALID, "drafted token %d of sequence %lld out of vocab", drafted[i * d + j], (long long)i);
+  }
+  if (temp != 0.0f)
+    for (int64_t i = 0; i < b * (d + 1); i++)
+      if (!(u[i] >= 0.0f && u[i] < 1.0f)) return fail(RTQ_ERR_INVALID, "uniform number %g out of range [0, 1)", (double)u[i]);
+  HostCall hc(c);
+  HIP_TRY(hipSetDevice(c->device));
+  hipStream_t st = c->stream;
+  if (temp == 0.0f || d == 0) q = nullptr;
+  const VerifyPlan p = verify_plan(b, d, V, q != nullptr);
+  const int64_t es = logit_bytes(type), tr = b * (d + 1);
+  RTQ_TRY(ensure_ws(c, p.bytes + (size_t)(p.rows * V * es + b * (2 + d) * 4 + tr * 8) + 8 * 256));
+  Arena ar{(char*)c->ws, c->ws_bytes, 0};
+  char* zd = ar.take<char>((size_t)(tr * V * es));
+  char* qd = q ? ar.take<char>((size_t)(b * d * V * es)) : nullptr;
+  int32_t* xd = ar.take<int32_t>((size_t)(b * d));
+  int32_t* nd = lens ? ar.take<int32_t>((size_t)b) : nullptr;
+  float* ud = temp != 0.0f ? ar.take<float>((size_t)tr) : nullptr;
+  int32_t* ad = ar.take<int32_t>((size_t)b);
+  int32_t* kd = ar.take<int32_t>((size_t)tr);
+  RTQ_TRY(h2d_rows(zd, z, tr, V, ld, es, st));
+  if (q) RTQ_TRY(h2d_rows(qd, q, b * d, V, ldq, es, st));
+  RTQ_TRY(h2d(xd, drafted, (size_t)(b * d) * 4, st));
+  if (nd) RTQ_TRY(h2d(nd, lens, (size_t)b * 4, st));
+  if (ud) RTQ_TRY(h2d(ud, u, (size_t)tr * 4, st));
+  RTQ_TRY(enqueue_verify(c, zd, type, V, qd, V, b, d, V, xd, nd, ud, temp, ad, kd, p, ar, st));
+  RTQ_TRY(d2h(accepted, ad, (size_t)b * 4, st));
+  RTQ_TRY(d2h(tokens, kd, (size_t)tr * 4, st));
+  HIP_TRY(hipStreamSynchronize(st));
   return RTQ_OK;
 }
 

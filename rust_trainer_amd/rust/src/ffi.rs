@@ -18,6 +18,9 @@ pub const RTQ_TYPE_Q8_0: c_int = 8;
 pub const RTQ_TYPE_Q4_K: c_int = 12;
 pub const RTQ_TYPE_Q6_K: c_int = 14;
 pub const RTQ_TYPE_TQ8_0: c_int = 264;
+pub const RTQ_TYPE_F16: c_int = 1;
+pub const RTQ_TYPE_BF16: c_int = 30;
+pub const RTQ_TOP_MAX: i64 = 256;
 
 #[repr(C)]
 pub struct rtq_ctx {
@@ -49,6 +52,17 @@ pub struct rtq_lora {
     pub a: *const f32,
     pub b: *const f32,
     pub enabled: c_int,
+}
+
+/// A teacher's top logits: ids and vals [n x k], rest [n] (or null).
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct rtq_teacher {
+    pub k: i64,
+    pub ids: *const i32,
+    pub vals: *const f32,
+    pub rest: *const f32,
+    pub temperature: f32,
 }
 
 #[repr(C)]
@@ -134,6 +148,27 @@ extern "C" {
     pub fn rtq_lm_head_d(ctx: *mut rtq_ctx, lm_head: *const rtq_weight, norm_w: *const f32, eps: f32, offset: f32,
                          x: *const f32, t: i64, pos: *const i32, tok: *const i32, weights: *const f32, n: i64,
                          logp: *mut f32, hit: *mut i32, dx: *mut f32, stream: *mut c_void) -> rtq_status;
+
+    // rows of vocabulary logits: top logits, distillation, drafted tokens
+    pub fn rtq_top_logits(ctx: *mut rtq_ctx, logits: *const c_void, type_: c_int, n: i64, vocab: i64, ld: i64, k: i64,
+                          temperature: f32, vals: *mut f32, ids: *mut i32, rest: *mut f32) -> rtq_status;
+    pub fn rtq_top_logits_d(ctx: *mut rtq_ctx, logits: *const c_void, type_: c_int, n: i64, vocab: i64, ld: i64,
+                            k: i64, temperature: f32, vals: *mut f32, ids: *mut i32, rest: *mut f32,
+                            stream: *mut c_void) -> rtq_status;
+    pub fn rtq_distill(ctx: *mut rtq_ctx, logits: *const c_void, type_: c_int, n: i64, vocab: i64, ld: i64,
+                       teacher: *const rtq_teacher, tok: *const i32, weights: *const f32, hard: f32, kl: *mut f32,
+                       logp: *mut f32, dlogits: *mut c_void, ldd: i64) -> rtq_status;
+    pub fn rtq_distill_d(ctx: *mut rtq_ctx, logits: *const c_void, type_: c_int, n: i64, vocab: i64, ld: i64,
+                         teacher: *const rtq_teacher, tok: *const i32, weights: *const f32, hard: f32, kl: *mut f32,
+                         logp: *mut f32, dlogits: *mut c_void, ldd: i64, stream: *mut c_void) -> rtq_status;
+    pub fn rtq_verify_draft(ctx: *mut rtq_ctx, logits: *const c_void, type_: c_int, ld: i64, draft: *const c_void,
+                            ldq: i64, b: i64, d: i64, vocab: i64, drafted: *const i32, lens: *const i32,
+                            uniforms: *const f32, temperature: f32, accepted: *mut i32,
+                            tokens: *mut i32) -> rtq_status;
+    pub fn rtq_verify_draft_d(ctx: *mut rtq_ctx, logits: *const c_void, type_: c_int, ld: i64, draft: *const c_void,
+                              ldq: i64, b: i64, d: i64, vocab: i64, drafted: *const i32, lens: *const i32,
+                              uniforms: *const f32, temperature: f32, accepted: *mut i32, tokens: *mut i32,
+                              stream: *mut c_void) -> rtq_status;
 
     // the device-resident training step (Model::forward_backward)
     pub fn rtq_model_from_gguf(ctx: *mut rtq_ctx, g: *const rtq_gguf, out: *mut *mut rtq_model) -> rtq_status;
