@@ -223,6 +223,24 @@ rtq_status rtq_verify_draft_d(rtq_ctx* ctx, const void* logits, int type, int64_
                               const float* uniforms, float temperature, int32_t* accepted, int32_t* tokens,
                               void* stream);
 
+/* The LM head's rows: rtq_top_logits and rtq_distill of the logits at positions pos[i] < t of hidden states
+ * x [t x d], with the final norm and the product of rtq_lm_head (the logits stay in the workspace).  With
+ * weights, dx [t x d] = dL/dx as rtq_lm_head's, OVERWRITTEN.  Positions out of range: refused (host
+ * version); vals, rest, kl and logp NaN, ids -1, no gradient (device version). */
+rtq_status rtq_lm_top_logits(rtq_ctx* ctx, const rtq_weight* lm_head, const float* norm_w, float eps, float offset,
+                             const float* x, int64_t t, const int32_t* pos, int64_t n, int64_t k, float temperature,
+                             float* vals, int32_t* ids, float* rest);
+rtq_status rtq_lm_top_logits_d(rtq_ctx* ctx, const rtq_weight* lm_head, const float* norm_w, float eps, float offset,
+                               const float* x, int64_t t, const int32_t* pos, int64_t n, int64_t k, float temperature,
+                               float* vals, int32_t* ids, float* rest, void* stream);
+rtq_status rtq_lm_distill(rtq_ctx* ctx, const rtq_weight* lm_head, const float* norm_w, float eps, float offset,
+                          const float* x, int64_t t, const int32_t* pos, const int32_t* tok, const float* weights,
+                          int64_t n, const rtq_teacher* teacher, float hard, float* kl, float* logp, float* dx);
+rtq_status rtq_lm_distill_d(rtq_ctx* ctx, const rtq_weight* lm_head, const float* norm_w, float eps, float offset,
+                            const float* x, int64_t t, const int32_t* pos, const int32_t* tok, const float* weights,
+                            int64_t n, const rtq_teacher* teacher, float hard, float* kl, float* logp, float* dx,
+                            void* stream);
+
 /* ---- device-resident training step (Model::forward_backward over the frozen linears) ----
  * A GGUF Qwen / Llama decoder (load_gguf_from, src/rie.rs:164-260) with every frozen tensor, norm
  * and adapter in device memory.  One call runs embed_tokens, the blocks (RMSNorm, q/k/v, QK-norm,
@@ -281,6 +299,24 @@ rtq_status rtq_model_forward_backward_packed(rtq_model* m, const int32_t* tokens
                                              const int32_t* positions, const int32_t* segments, const int32_t* pos,
                                              const int32_t* tok, const float* weights, int64_t n, float* logp,
                                              int64_t* hits);
+/* The same step with other heads (no counterpart in the reference).  positions and segments: both NULL
+ * (one sequence) or both given (a packed batch); rows are formed at pos[i] < t.
+ * rtq_model_top_logits: a teacher's pass, rtq_top_logits of n rows (no backward).
+ * rtq_model_forward_backward_distill: rtq_distill of n rows; with weights (else NULL: the losses alone)
+ * the adapters' gradients of its L accumulate.  tok and logp may both be NULL, then hard must be 0. */
+rtq_status rtq_model_top_logits(rtq_model* m, const int32_t* tokens, int64_t t, const int32_t* positions,
+                                const int32_t* segments, const int32_t* pos, int64_t n, int64_t k, float temperature,
+                                float* vals, int32_t* ids, float* rest);
+rtq_status rtq_model_forward_backward_distill(rtq_model* m, const int32_t* tokens, int64_t t, const int32_t* positions,
+                                              const int32_t* segments, const int32_t* pos, const int32_t* tok,
+                                              const float* weights, int64_t n, const rtq_teacher* teacher, float hard,
+                                              float* kl, float* logp);
+/* Verifies the last d of t tokens (0 <= d < t) against m's logits after each of the tokens before them:
+ * rtq_verify_draft with uniforms [d + 1], *accepted and out [d + 1].  draft: the model (of the same
+ * vocabulary, on the same device) that they were drawn from at this temperature, whose logits are formed
+ * from the same tokens; NULL: drafts that were not drawn. */
+rtq_status rtq_model_verify_draft(rtq_model* m, rtq_model* draft, const int32_t* tokens, int64_t t, int64_t d,
+                                  const float* uniforms, float temperature, int32_t* accepted, int32_t* out);
 /* Model::checkpointing (src/model.rs:299-300; the loader's default true, src/rie.rs:254): 1 keeps
  * only each block's input and recomputes its forward in the backward (src/model.rs:663-665,
  * 678-680); 0 keeps every block's activations; -1 (default) keeps them when they take at most half

@@ -95,6 +95,10 @@ SIGNATURES = {
     "rtq_distill_d": (_i, [_p, _p, _i, _i64, _i64, _i64, _TP, _p, _p, _f, _p, _p, _p, _i64, _p]),
     "rtq_verify_draft": (_i, [_p, _p, _i, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _f, _p, _p]),
     "rtq_verify_draft_d": (_i, [_p, _p, _i, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _f, _p, _p, _p]),
+    "rtq_lm_top_logits": (_i, [_p, _p, _p, _f, _f, _p, _i64, _p, _i64, _i64, _f, _p, _p, _p]),
+    "rtq_lm_top_logits_d": (_i, [_p, _p, _p, _f, _f, _p, _i64, _p, _i64, _i64, _f, _p, _p, _p, _p]),
+    "rtq_lm_distill": (_i, [_p, _p, _p, _f, _f, _p, _i64, _p, _p, _p, _i64, _TP, _f, _p, _p, _p]),
+    "rtq_lm_distill_d": (_i, [_p, _p, _p, _f, _f, _p, _i64, _p, _p, _p, _i64, _TP, _f, _p, _p, _p, _p]),
     # device-resident training step
     "rtq_linear_forward_noalloc_d": (_i, [_p, _p, _p, _LP, _p, _i64, _p, _p]),
     "rtq_model_from_gguf": (_i, [_p, _p, ctypes.POINTER(_p)]),
@@ -112,6 +116,9 @@ SIGNATURES = {
     "rtq_model_zero_grad": (_i, [_p]),
     "rtq_model_forward_backward": (_i, [_p, _p, _i64, _p, _p, _p, _i64, _p, ctypes.POINTER(_i64)]),
     "rtq_model_forward_backward_packed": (_i, [_p, _p, _i64, _p, _p, _p, _p, _p, _i64, _p, ctypes.POINTER(_i64)]),
+    "rtq_model_top_logits": (_i, [_p, _p, _i64, _p, _p, _p, _i64, _i64, _f, _p, _p, _p]),
+    "rtq_model_forward_backward_distill": (_i, [_p, _p, _i64, _p, _p, _p, _p, _p, _i64, _TP, _f, _p, _p]),
+    "rtq_model_verify_draft": (_i, [_p, _p, _p, _i64, _i64, _p, _f, ctypes.POINTER(ctypes.c_int32), _p]),
     "rtq_model_set_checkpointing": (_i, [_p, _i]),
     "rtq_model_checkpointing": (_i, [_p]),
     "rtq_model_set_attention": (_i, [_p, _i]),

@@ -53,6 +53,13 @@ int rtq_ctx_cu_count(const rtq_ctx* c);
 uint64_t rtq_ctx_ws_gen(const rtq_ctx* c);
 // per-launch timing is on (rtq_ctx_set_timing): launches record events
 bool rtq_ctx_timing_on(const rtq_ctx* c);
+// a capture of the library's own begins / ends (its graph is dropped when the workspace moves, so the
+// workspace need not be kept for it)
+void rtq_ctx_set_own_capture(rtq_ctx* c, bool on);
+rtq_status rtq_check_temperature(float t);
+// logits [n x vocab] of the hidden states x [t x d] at pos (final RMSNorm, lm_head.forward)
+extern "C" rtq_status rtq_lm_logits_d(rtq_ctx* c, const rtq_weight* lm_head, const float* norm_w, float eps, float offset,
+                                      const float* x, int64_t t, const int32_t* pos, int64_t n, float* out, void* stream);
 // floats of the LoRA-down partials a forward of t tokens at rank r can keep for the backward of the
 // same x (0: not kept for this weight - dense, or slicings that differ)
 int64_t rtq_lora_partial_floats(const rtq_weight* w, int64_t t, int64_t r);

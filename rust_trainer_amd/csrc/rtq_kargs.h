@@ -335,7 +335,7 @@ struct FillArgs {
 struct HeadArgs {
   const float* x;      // [t x d] final hidden states
   const int32_t* pos;  // [n] target positions
-  const int32_t* tok;  // [n] target tokens
+  const int32_t* tok;  // [n] target tokens (null where rows go by their position alone)
   const float* wts;    // [n] loss weights, or null (log-probs only)
   const float* norm;   // [d] final norm weight
   float eps, off;
@@ -366,6 +366,8 @@ struct TopArgs {
   float* vals;      // [n x k]
   int32_t* ids;     // [n x k]
   float* rest;      // [n] or null
+  const int32_t* pos;  // [n] positions that the rows were formed at, or null: a row whose position is
+  int t;               // outside [0, t) has no logits (vals and rest NaN, ids -1)
 };
 
 struct DistillArgs {
@@ -387,6 +389,8 @@ struct DistillArgs {
   float* zt;           // [n] and of the labels
   float* kl;           // [n]
   float* logp;         // [n] or null
+  const int32_t* pos;  // [n] positions that the rows were formed at, or null: a row whose position is
+  int t;               // outside [0, t) has no logits (kl and logp NaN, gradient 0)
 };
 
 struct VerifyPick {  // the row that sequence i's next token is drawn from

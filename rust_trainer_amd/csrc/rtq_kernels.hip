@@ -4433,7 +4433,7 @@ extern "C" __global__ __launch_bounds__(256) void rtq_rows_q6_k(RowArgs a) { row
 // A target outside [0, t) x [0, V) reads nothing: its normalised row is 0, logp NaN, gradient 0.
 
 __device__ __forceinline__ bool head_target_ok(const HeadArgs& a, int i) {
-  const int p = a.pos[i], k = a.tok[i];
+  const int p = a.pos[i], k = a.tok ? a.tok[i] : 0;
   return p >= 0 && p < a.t && k >= 0 && k < a.V;
 }
 

@@ -217,10 +217,31 @@ struct rtq_model {
   std::vector<uint64_t> gkey, prev_key;
   uint64_t gen = 0;
   int64_t graph_replays = 0;
+  // what the current step does with its rows' logits (null: cross-entropy), and the device copies of
+  // its arrays: teacher or top ids and logits [n x k], rest [n], kl [n]
+  const struct HeadJob* job = nullptr;
+  void* job_mem = nullptr;
+  size_t job_cap = 0;
+  int32_t* job_ids = nullptr;
+  float *job_vals = nullptr, *job_rest = nullptr, *job_kl = nullptr;
+  void* draft_mem = nullptr;  // rtq_model_verify_draft: the logits' rows and the small arrays
+  size_t draft_cap = 0;
   // pinned staging of the step's host inputs (tokens, target positions and tokens, weights) and
   // outputs (log-probs, hits)
   void* io_host = nullptr;
   size_t io_cap = 0;
+};
+
+// a step's head other than cross-entropy: top logits, distillation, or the logits' rows themselves
+struct HeadJob {
+  enum Kind { TOP = 1, DISTILL = 2, ROWS = 3 } kind;
+  int64_t k = 0;
+  float temp = 1.0f, hard = 0.0f;
+  const rtq_teacher* teacher = nullptr;  // host arrays
+  float *vals = nullptr, *rest = nullptr, *kl = nullptr;  // host outputs
+  int32_t* ids = nullptr;
+  float* rows = nullptr;  // ROWS: device, [n x vocab]
+  bool tok = false;
 };
 
 namespace {
@@ -1632,6 +1653,8 @@ void rtq_model_destroy(rtq_model* m) {
   if (m->lgt_host) (void)hipHostFree(m->lgt_host);
   if (m->attn_mem) (void)hipFree(m->attn_mem);
   if (m->seq_mem) (void)hipFree(m->seq_mem);
+  if (m->job_mem) (void)hipFree(m->job_mem);
+  if (m->draft_mem) (void)hipFree(m->draft_mem);
   delete m;
 }
 
@@ -1862,8 +1885,22 @@ rtq_status step_kernels(rtq_model* m, int64_t t, int64_t n, bool weights) {
     if (l == m->dbg_layer) M_TRY(dbg_forward(m, (int)l, t, x, y));
   }
   if (n == 0) return RTQ_OK;
-  M_TRY(rtq_lm_head_d(m->ctx, m->head, m->out_norm, c.rms_eps, c.norm_offset, m->X + c.n_layer * t * d, t, m->pos_d,
-                      m->tgt_d, weights ? m->wts_d : nullptr, n, m->logp_d, m->hit_d, weights ? m->dY : nullptr, st));
+  const float* xl = m->X + c.n_layer * t * d;
+  if (m->job && m->job->kind == HeadJob::TOP)
+    return rtq_lm_top_logits_d(m->ctx, m->head, m->out_norm, c.rms_eps, c.norm_offset, xl, t, m->pos_d, n, m->job->k,
+                               m->job->temp, m->job_vals, m->job_ids, m->job->rest ? m->job_rest : nullptr, st);
+  if (m->job && m->job->kind == HeadJob::ROWS)
+    return rtq_lm_logits_d(m->ctx, m->head, m->out_norm, c.rms_eps, c.norm_offset, xl, t, m->pos_d, n, m->job->rows, st);
+  if (m->job) {
+    const HeadJob& j = *m->job;
+    const rtq_teacher te{j.k, m->job_ids, m->job_vals, j.teacher->rest ? m->job_rest : nullptr, j.temp};
+    M_TRY(rtq_lm_distill_d(m->ctx, m->head, m->out_norm, c.rms_eps, c.norm_offset, xl, t, m->pos_d, j.tok ? m->tgt_d : nullptr,
+                           weights ? m->wts_d : nullptr, n, &te, j.hard, m->job_kl, j.tok ? m->logp_d : nullptr,
+                           weights ? m->dY : nullptr, st));
+  } else {
+    M_TRY(rtq_lm_head_d(m->ctx, m->head, m->out_norm, c.rms_eps, c.norm_offset, xl, t, m->pos_d, m->tgt_d,
+                        weights ? m->wts_d : nullptr, n, m->logp_d, m->hit_d, weights ? m->dY : nullptr, st));
+  }
   if (!weights) return RTQ_OK;
   m->lg_all.clear();
   for (int64_t l = c.n_layer - 1; l >= 0; l--) {
@@ -1895,7 +1932,9 @@ rtq_status capture_step(rtq_model* m, int64_t t, int64_t n, bool weights, const 
   if (hipStreamBeginCapture(st, hipStreamCaptureModeThreadLocal) != hipSuccess) {
     why = "hipStreamBeginCapture";
   } else {
+    rtq_ctx_set_own_capture(m->ctx, true);
     const rtq_status s = step_kernels(m, t, n, weights);
+    rtq_ctx_set_own_capture(m->ctx, false);
     hipGraph_t g = nullptr;
     const hipError_t e = hipStreamEndCapture(st, &g);
     hipGraphExec_t x = nullptr;
@@ -1915,11 +1954,53 @@ rtq_status capture_step(rtq_model* m, int64_t t, int64_t n, bool weights, const 
   return step_kernels(m, t, n, weights);
 }
 
+// the device arrays of a job of n rows, and its teacher's upload (pageable copies: the step ends synchronised)
+rtq_status upload_job(rtq_model* m, const HeadJob& j, int64_t n, hipStream_t st) {
+  if (j.kind == HeadJob::ROWS) return RTQ_OK;
+  const size_t lists = ((size_t)(n * j.k) * 4 + 255) / 256 * 256, row = ((size_t)n * 4 + 255) / 256 * 256;
+  const size_t need = 2 * lists + 2 * row;
+  if (need > m->job_cap) {
+    if (m->job_mem) {
+      M_HIP(hipStreamSynchronize(st));
+      M_HIP(hipFree(m->job_mem));
+      m->job_mem = nullptr;
+      m->job_cap = 0;
+    }
+    M_HIP(hipMalloc(&m->job_mem, need));
+    m->job_cap = need;
+    m->gen++;
+  }
+  char* p = (char*)m->job_mem;
+  m->job_ids = (int32_t*)p;
+  m->job_vals = (float*)(p + lists);
+  m->job_rest = (float*)(p + 2 * lists);
+  m->job_kl = (float*)(p + 2 * lists + row);
+  if (j.kind != HeadJob::DISTILL) return RTQ_OK;
+  M_HIP(hipMemcpyAsync(m->job_ids, j.teacher->ids, (size_t)(n * j.k) * 4, hipMemcpyHostToDevice, st));
+  M_HIP(hipMemcpyAsync(m->job_vals, j.teacher->vals, (size_t)(n * j.k) * 4, hipMemcpyHostToDevice, st));
+  if (j.teacher->rest) M_HIP(hipMemcpyAsync(m->job_rest, j.teacher->rest, (size_t)n * 4, hipMemcpyHostToDevice, st));
+  return RTQ_OK;
+}
+
+// a job's outputs to the host
+rtq_status download_job(rtq_model* m, const HeadJob& j, int64_t n, float* logp, hipStream_t st) {
+  if (j.kind == HeadJob::TOP) {
+    M_HIP(hipMemcpyAsync(j.vals, m->job_vals, (size_t)(n * j.k) * 4, hipMemcpyDeviceToHost, st));
+    M_HIP(hipMemcpyAsync(j.ids, m->job_ids, (size_t)(n * j.k) * 4, hipMemcpyDeviceToHost, st));
+    if (j.rest) M_HIP(hipMemcpyAsync(j.rest, m->job_rest, (size_t)n * 4, hipMemcpyDeviceToHost, st));
+  } else if (j.kind == HeadJob::DISTILL) {
+    M_HIP(hipMemcpyAsync(j.kl, m->job_kl, (size_t)n * 4, hipMemcpyDeviceToHost, st));
+    if (j.tok) M_HIP(hipMemcpyAsync(logp, m->logp_d, (size_t)n * 4, hipMemcpyDeviceToHost, st));
+  }
+  return RTQ_OK;
+}
+
 // one step (forward_backward_layout, src/model.rs:644-687): checks, buffers and tables, the
 // inputs' upload, the kernels (eager, captured or replayed), the outputs' download
 rtq_status step(rtq_model* m, const int32_t* tokens, int64_t t, const int32_t* positions, const int32_t* segments,
-                const int32_t* pos, const int32_t* tok, const float* weights, int64_t n, float* logp, int64_t* hits) {
-  if (!m || !tokens || t <= 0 || n < 0 || (n > 0 && (!pos || !tok || !logp)))
+                const int32_t* pos, const int32_t* tok, const float* weights, int64_t n, float* logp, int64_t* hits,
+                const HeadJob* job = nullptr) {
+  if (!m || !tokens || t <= 0 || n < 0 || (n > 0 && (!pos || (!job && (!tok || !logp)))))
     return rtq_fail(RTQ_ERR_INVALID, "null model/tokens/targets or empty sequence");
   const rtq_model_config& c = m->cfg;
   if (t > 65535) return rtq_fail(RTQ_ERR_INVALID, "sequence of %lld tokens too long", (long long)t);
@@ -1927,7 +2008,7 @@ rtq_status step(rtq_model* m, const int32_t* tokens, int64_t t, const int32_t* p
     if (tokens[i] < 0 || tokens[i] >= c.n_vocab)
       return rtq_fail(RTQ_ERR_INVALID, "token %d out of vocab", tokens[i]);  // src/model.rs:450
   for (int64_t i = 0; i < n; i++)
-    if (pos[i] < 0 || pos[i] >= t || tok[i] < 0 || tok[i] >= c.n_vocab)
+    if (pos[i] < 0 || pos[i] >= t || (tok && (tok[i] < 0 || tok[i] >= c.n_vocab)))
       return rtq_fail(RTQ_ERR_INVALID, "target %lld out of range", (long long)i);  // src/model.rs:575
   if (positions)
     for (int64_t i = 0; i < t; i++)
@@ -1936,6 +2017,7 @@ rtq_status step(rtq_model* m, const int32_t* tokens, int64_t t, const int32_t* p
     for (int64_t i = 0; i < t; i++)
       if (segments[i] < 0) return rtq_fail(RTQ_ERR_INVALID, "segment %lld is negative", (long long)i);
   M_HIP(hipSetDevice(rtq_ctx_device_id(m->ctx)));
+  m->job = job;
   m->attn_fused = m->attn_hd_ok && m->attn_mode != 0;
   M_TRY(choose_ckpt(m, t, n));
   M_TRY(choose_defer(m, t));
@@ -1963,14 +2045,17 @@ rtq_status step(rtq_model* m, const int32_t* tokens, int64_t t, const int32_t* p
   M_HIP(hipMemcpyAsync(m->tok_d, io, (size_t)t * 4, hipMemcpyHostToDevice, st));
   if (n > 0) {
     std::memcpy(io + t, pos, (size_t)n * 4);
-    std::memcpy(io + t + n, tok, (size_t)n * 4);
     M_HIP(hipMemcpyAsync(m->pos_d, io + t, (size_t)n * 4, hipMemcpyHostToDevice, st));
-    M_HIP(hipMemcpyAsync(m->tgt_d, io + t + n, (size_t)n * 4, hipMemcpyHostToDevice, st));
+    if (tok) {
+      std::memcpy(io + t + n, tok, (size_t)n * 4);
+      M_HIP(hipMemcpyAsync(m->tgt_d, io + t + n, (size_t)n * 4, hipMemcpyHostToDevice, st));
+    }
     if (weights) {
       std::memcpy(io + t + 2 * n, weights, (size_t)n * 4);
       M_HIP(hipMemcpyAsync(m->wts_d, io + t + 2 * n, (size_t)n * 4, hipMemcpyHostToDevice, st));
     }
   }
+  if (job && n > 0) M_TRY(upload_job(m, *job, n, st));
   // the launch key: everything the step's launches depend on besides gen (bumped by the rest)
   const bool graphable = m->graph_on && m->dbg_layer < 0 && !rtq_ctx_timing_on(m->ctx);
   std::vector<uint64_t> key;
@@ -1979,6 +2064,15 @@ rtq_status step(rtq_model* m, const int32_t* tokens, int64_t t, const int32_t* p
            m->ckpt ? 1u : 0u, m->defer_lg ? 1u : 0u, m->attn_fused ? 1u : 0u, (uint64_t)m->n_fwd,
            (uint64_t)m->n_kv, (uint64_t)m->n_mfwd, (uint64_t)m->n_mkv, m->packed && m->seq_on ? 1u : 0u,
            (uint64_t)m->tv, (uint64_t)m->n_sit, (uint64_t)m->n_smg, m->gen, rtq_ctx_ws_gen(m->ctx)};
+  if (graphable && job) {
+    uint32_t temp, hard;
+    std::memcpy(&temp, &job->temp, 4);
+    std::memcpy(&hard, &job->hard, 4);
+    const uint64_t rest = job->rest || (job->teacher && job->teacher->rest) ? 1u : 0u;
+    for (uint64_t v : {(uint64_t)job->kind, (uint64_t)job->k, (uint64_t)temp, (uint64_t)hard, (uint64_t)(job->tok ? 1 : 0), rest,
+                       (uint64_t)(uintptr_t)job->rows})
+      key.push_back(v);
+  }
   if (graphable && m->gexec && key == m->gkey) {
     M_HIP(hipGraphLaunch(m->gexec, st));
     m->graph_replays++;
@@ -1988,7 +2082,10 @@ rtq_status step(rtq_model* m, const int32_t* tokens, int64_t t, const int32_t* p
     M_TRY(step_kernels(m, t, n, weights != nullptr));
   }
   m->prev_key = key;
-  if (n > 0) {
+  if (job) {
+    if (n > 0) M_TRY(download_job(m, *job, n, logp, st));
+    M_HIP(hipStreamSynchronize(st));
+  } else if (n > 0) {
     float* lp = (float*)(io + t + 3 * n);
     int32_t* hv = io + t + 4 * n;
     M_HIP(hipMemcpyAsync(lp, m->logp_d, (size_t)n * 4, hipMemcpyDeviceToHost, st));
@@ -2022,6 +2119,94 @@ rtq_status rtq_model_forward_backward_packed(rtq_model* m, const int32_t* tokens
                                              int64_t* hits) {
   if (!positions || !segments) return rtq_fail(RTQ_ERR_INVALID, "packed step needs positions and segments");
   return step(m, tokens, t, positions, segments, pos, tok, weights, n, logp, hits);
+}
+
+rtq_status rtq_model_top_logits(rtq_model* m, const int32_t* tokens, int64_t t, const int32_t* positions,
+                                const int32_t* segments, const int32_t* pos, int64_t n, int64_t k, float temperature,
+                                float* vals, int32_t* ids, float* rest) {
+  if (!m) return rtq_fail(RTQ_ERR_INVALID, "null model");
+  if ((positions == nullptr) != (segments == nullptr)) return rtq_fail(RTQ_ERR_INVALID, "positions and segments go together");
+  if (n < 0 || n > 65535) return rtq_fail(RTQ_ERR_INVALID, "row count %lld out of range [0, 65535]", (long long)n);
+  if (k < 1 || k > RTQ_TOP_MAX || k > m->cfg.n_vocab)
+    return rtq_fail(RTQ_ERR_INVALID, "k = %lld out of range [1, min(%lld, %d)]", (long long)k, (long long)m->cfg.n_vocab, RTQ_TOP_MAX);
+  if (n > 0 && (!vals || !ids)) return rtq_fail(RTQ_ERR_INVALID, "null vals/ids");
+  M_TRY(rtq_check_temperature(temperature));
+  HeadJob j{HeadJob::TOP};
+  j.k = k, j.temp = temperature, j.vals = vals, j.ids = ids, j.rest = rest;
+  return step(m, tokens, t, positions, segments, pos, nullptr, nullptr, n, nullptr, nullptr, &j);
+}
+
+rtq_status rtq_model_forward_backward_distill(rtq_model* m, const int32_t* tokens, int64_t t, const int32_t* positions,
+                                              const int32_t* segments, const int32_t* pos, const int32_t* tok,
+                                              const float* weights, int64_t n, const rtq_teacher* teacher, float hard,
+                                              float* kl, float* logp) {
+  if (!m) return rtq_fail(RTQ_ERR_INVALID, "null model");
+  if ((positions == nullptr) != (segments == nullptr)) return rtq_fail(RTQ_ERR_INVALID, "positions and segments go together");
+  if (n < 0 || n > 65535) return rtq_fail(RTQ_ERR_INVALID, "row count %lld out of range [0, 65535]", (long long)n);
+  if (!teacher) return rtq_fail(RTQ_ERR_INVALID, "null teacher");
+  if (teacher->k < 1 || teacher->k > RTQ_TOP_MAX)
+    return rtq_fail(RTQ_ERR_INVALID, "%lld slots per row out of range [1, %d]", (long long)teacher->k, RTQ_TOP_MAX);
+  M_TRY(rtq_check_temperature(teacher->temperature));
+  if (!(hard >= 0.0f && hard <= 1.0f)) return rtq_fail(RTQ_ERR_INVALID, "hard = %g out of range [0, 1]", (double)hard);
+  if ((tok == nullptr) != (logp == nullptr)) return rtq_fail(RTQ_ERR_INVALID, "tok and logp go together");
+  if (!tok && hard > 0.0f) return rtq_fail(RTQ_ERR_INVALID, "hard > 0 without labels");
+  if (n > 0 && (!teacher->ids || !teacher->vals || !kl)) return rtq_fail(RTQ_ERR_INVALID, "null ids/vals/kl");
+  for (int64_t i = 0; i < n * teacher->k; i++)
+    if (teacher->ids[i] >= m->cfg.n_vocab)
+      return rtq_fail(RTQ_ERR_INVALID, "teacher token %d of row %lld out of vocab", teacher->ids[i], (long long)(i / teacher->k));
+  HeadJob j{HeadJob::DISTILL};
+  j.k = teacher->k, j.temp = teacher->temperature, j.hard = hard, j.teacher = teacher, j.kl = kl, j.tok = tok != nullptr;
+  return step(m, tokens, t, positions, segments, pos, tok, weights, n, logp, nullptr, &j);
+}
+
+rtq_status rtq_model_verify_draft(rtq_model* m, rtq_model* draft, const int32_t* tokens, int64_t t, int64_t d,
+                                  const float* uniforms, float temperature, int32_t* accepted, int32_t* out) {
+  if (!m || !tokens || !accepted || !out) return rtq_fail(RTQ_ERR_INVALID, "null model/tokens/accepted/out");
+  if (d < 0 || d >= t || t > 65535) return rtq_fail(RTQ_ERR_INVALID, "%lld drafted of %lld tokens", (long long)d, (long long)t);
+  if (temperature != 0.0f) M_TRY(rtq_check_temperature(temperature));
+  if (temperature != 0.0f && !uniforms) return rtq_fail(RTQ_ERR_INVALID, "null uniforms");
+  if (temperature != 0.0f)
+    for (int64_t i = 0; i <= d; i++)
+      if (!(uniforms[i] >= 0.0f && uniforms[i] < 1.0f))
+        return rtq_fail(RTQ_ERR_INVALID, "uniform number %g out of range [0, 1)", (double)uniforms[i]);
+  const int64_t V = m->cfg.n_vocab;
+  if (temperature == 0.0f || d == 0) draft = nullptr;
+  if (draft && (draft->cfg.n_vocab != V || rtq_ctx_device_id(draft->ctx) != rtq_ctx_device_id(m->ctx)))
+    return rtq_fail(RTQ_ERR_INVALID, "the draft model has another vocabulary or device");
+  M_HIP(hipSetDevice(rtq_ctx_device_id(m->ctx)));
+  hipStream_t st = stream_of(m);
+  const size_t rows = ((size_t)((d + 1) * V) * 4 + 255) / 256 * 256, small = ((size_t)(d + 1) * 4 + 255) / 256 * 256;
+  const size_t need = (draft ? 2 : 1) * rows + 4 * small;
+  if (need > m->draft_cap) {
+    if (m->draft_mem) {
+      M_HIP(hipStreamSynchronize(st));
+      M_HIP(hipFree(m->draft_mem));
+      m->draft_mem = nullptr;
+      m->draft_cap = 0;
+    }
+    M_HIP(hipMalloc(&m->draft_mem, need));
+    m->draft_cap = need;
+    m->gen++;
+  }
+  char* p = (char*)m->draft_mem;
+  int32_t *xd = (int32_t*)p, *ad = (int32_t*)(p + 2 * small), *od = (int32_t*)(p + 3 * small);
+  float *ud = (float*)(p + small), *zt = (float*)(p + 4 * small), *zq = (float*)(p + 4 * small + rows);
+  std::vector<int32_t> pos((size_t)(d + 1));
+  for (int64_t i = 0; i <= d; i++) pos[(size_t)i] = (int32_t)(t - d - 1 + i);
+  HeadJob j{HeadJob::ROWS};
+  if (draft) {
+    j.rows = zq;
+    M_TRY(step(draft, tokens, t, nullptr, nullptr, pos.data(), nullptr, nullptr, d, nullptr, nullptr, &j));
+  }
+  j.rows = zt;
+  M_TRY(step(m, tokens, t, nullptr, nullptr, pos.data(), nullptr, nullptr, d + 1, nullptr, nullptr, &j));
+  if (d > 0) M_HIP(hipMemcpyAsync(xd, tokens + t - d, (size_t)d * 4, hipMemcpyHostToDevice, st));
+  if (temperature != 0.0f) M_HIP(hipMemcpyAsync(ud, uniforms, (size_t)(d + 1) * 4, hipMemcpyHostToDevice, st));
+  M_TRY(rtq_verify_draft_d(m->ctx, zt, RTQ_TYPE_F32, V, draft ? zq : nullptr, V, 1, d, V, xd, nullptr, ud, temperature, ad, od, st));
+  M_HIP(hipMemcpyAsync(accepted, ad, 4, hipMemcpyDeviceToHost, st));
+  M_HIP(hipMemcpyAsync(out, od, (size_t)(d + 1) * 4, hipMemcpyDeviceToHost, st));
+  M_HIP(hipStreamSynchronize(st));
+  return RTQ_OK;
 }
 
 rtq_status rtq_model_set_checkpointing(rtq_model* m, int mode) {

@@ -242,6 +242,7 @@ struct rtq_ctx {
   void* ws = nullptr;
   size_t ws_bytes = 0;
   uint64_t ws_gen = 0;  // bumped whenever ws moves (graphs that captured its address are stale)
+  bool own_capture = false;    // the library's own capture (a model's step) is running: its graph goes by ws_gen
   bool ws_captured = false;    // a caller's graph holds ws's address: when it is outgrown it is kept,
   std::vector<void*> retired;  // here, until the context goes, so that the graph can still replay
   bool timing = false;
@@ -1376,6 +1377,11 @@ rtq_status rtq_model_launch(rtq_ctx* c, int km, dim3 grid, dim3 block, hipStream
 int rtq_ctx_device_id(const rtq_ctx* c) { return c ? c->device : -1; }
 int rtq_ctx_cu_count(const rtq_ctx* c) { return c ? (int)c->cu_count : 256; }
 uint64_t rtq_ctx_ws_gen(const rtq_ctx* c) { return c ? c->ws_gen : 0; }
+rtq_status rtq_check_temperature(float t) {
+  if (!(t >= 1e-4f && t <= 1e4f)) return fail(RTQ_ERR_INVALID, "temperature %g out of range [1e-4, 1e4]", (double)t);
+  return RTQ_OK;
+}
+void rtq_ctx_set_own_capture(rtq_ctx* c, bool on) { c->own_capture = on; }
 bool rtq_ctx_timing_on(const rtq_ctx* c) { return c && c->timing; }
 
 // error reporting shared with the other translation units of the library (rtq_gguf.cpp, rtq_model.cpp)
@@ -1878,7 +1884,7 @@ rtq_status row_ws(rtq_ctx* c, size_t bytes, hipStream_t st) {
       return fail(RTQ_ERR_INVALID,
                   "the workspace (%zu bytes, %zu needed) cannot grow under capture: make an eager call of this size first",
                   c->ws_bytes, bytes);
-    c->ws_captured = true;
+    c->ws_captured = c->ws_captured || !c->own_capture;
     return RTQ_OK;
   }
   return ensure_ws(c, bytes);
@@ -1896,11 +1902,6 @@ rtq_status check_rows(const void* z, int type, int64_t n, int64_t vocab, int64_t
 }
 
 rtq_status check_ctx(const rtq_ctx* c) { return c ? RTQ_OK : fail(RTQ_ERR_INVALID, "null context"); }
-
-rtq_status check_temperature(float t) {
-  if (!(t >= 1e-4f && t <= 1e4f)) return fail(RTQ_ERR_INVALID, "temperature %g out of range [1e-4, 1e4]", (double)t);
-  return RTQ_OK;
-}
 
 // log2(e) / t as the sum of two floats
 void exp_scale(float t, float* hi, float* lo) {
@@ -1929,7 +1930,7 @@ TopPlan top_plan(int type, int64_t n, int64_t V, int64_t k) {
 rtq_status check_top(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V, int64_t ld, int64_t k, float temp,
                      const float* vals, const int32_t* ids) {
   RTQ_TRY(check_rows(z, type, n, V, ld));
-  RTQ_TRY(check_temperature(temp));
+  RTQ_TRY(rtq_check_temperature(temp));
   if (k < 1 || k > RTQ_TOP_MAX || k > V)
     return fail(RTQ_ERR_INVALID, "k = %lld out of range [1, min(%lld, %d)]", (long long)k, (long long)V, RTQ_TOP_MAX);
   if (n > 0 && (!vals || !ids)) return fail(RTQ_ERR_INVALID, "null vals/ids");
@@ -1937,8 +1938,10 @@ rtq_status check_top(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V, 
 }
 
 rtq_status enqueue_top(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V, int64_t ld, int64_t k, float temp,
-                       float* vals, int32_t* ids, float* rest, const TopPlan& p, Arena& ar, hipStream_t st) {
+                       float* vals, int32_t* ids, float* rest, const TopPlan& p, Arena& ar, hipStream_t st,
+                       const int32_t* pos = nullptr, int64_t t = 0) {
   TopArgs a{};
+  a.pos = pos, a.t = (int)t;
   a.z = z, a.ld = ld, a.n = (int)n, a.V = (int)V, a.k = (int)k, a.G = (int)p.G, a.L = (int)p.L;
   a.temp = temp;
   exp_scale(temp, &a.ch, &a.cl);
@@ -1975,7 +1978,7 @@ rtq_status check_distill(rtq_ctx* c, const void* z, int type, int64_t n, int64_t
                          const void* dz, int64_t ldd) {
   RTQ_TRY(check_rows(z, type, n, V, ld));
   if (!t) return fail(RTQ_ERR_INVALID, "null teacher");
-  RTQ_TRY(check_temperature(t->temperature));
+  RTQ_TRY(rtq_check_temperature(t->temperature));
   if (t->k < 1 || t->k > RTQ_TOP_MAX)
     return fail(RTQ_ERR_INVALID, "%lld slots per row out of range [1, %d]", (long long)t->k, RTQ_TOP_MAX);
   if (!(hard >= 0.0f && hard <= 1.0f)) return fail(RTQ_ERR_INVALID, "hard = %g out of range [0, 1]", (double)hard);
@@ -1998,8 +2001,10 @@ rtq_status check_distill(rtq_ctx* c, const void* z, int type, int64_t n, int64_t
 
 rtq_status enqueue_distill(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V, int64_t ld, const rtq_teacher& t,
                            const int32_t* tok, const float* w, float hard, float* kl, float* logp, void* dz,
-                           int64_t ldd, const DistillPlan& p, Arena& ar, hipStream_t st) {
+                           int64_t ldd, const DistillPlan& p, Arena& ar, hipStream_t st, const int32_t* pos = nullptr,
+                           int64_t npos = 0) {
   DistillArgs a{};
+  a.pos = pos, a.t = (int)npos;
   a.z = z, a.dz = dz, a.ld = ld, a.ldd = ldd;
   a.n = (int)n, a.V = (int)V, a.k = (int)t.k, a.G = (int)p.G, a.L = (int)p.L;
   a.temp = t.temperature;
@@ -2038,7 +2043,7 @@ rtq_status check_verify(rtq_ctx* c, const void* z, int type, int64_t ld, const v
   if (b < 0 || b > 65535 || d < 0 || d > 65535 || b * (2 * d + 1) > (1 << 24))
     return fail(RTQ_ERR_INVALID, "%lld sequences of %lld drafted tokens", (long long)b, (long long)d);
   RTQ_TRY(check_rows(z, type, b, V, ld));
-  if (temp != 0.0f) RTQ_TRY(check_temperature(temp));
+  if (temp != 0.0f) RTQ_TRY(rtq_check_temperature(temp));
   if (q && (ldq < V || ldq > (1LL << 40))) return fail(RTQ_ERR_INVALID, "draft row stride %lld with a vocabulary of %lld", (long long)ldq, (long long)V);
   if ((uintptr_t)q % (uintptr_t)logit_bytes(type)) return fail(RTQ_ERR_INVALID, "draft logits not aligned to their elements");
   if (b > 0 && ((d > 0 && !drafted) || !accepted || !tokens)) return fail(RTQ_ERR_INVALID, "null drafted/accepted/tokens");
@@ -2109,6 +2114,143 @@ rtq_status rtq_verify_draft_d(rtq_ctx* c, const void* z, int type, int64_t ld, c
   RTQ_TRY(row_ws(c, p.bytes, st));
   Arena ar{(char*)c->ws, c->ws_bytes, 0};
   return enqueue_verify(c, z, type, ld, q, ldq, b, d, V, drafted, lens, u, temp, accepted, tokens, p, ar, st);
+}
+
+// ------------------------------------------------------------------ the LM head's top logits and distillation
+namespace {
+
+// logits [n x vocab] of the hidden states at pos: final RMSNorm, lm_head.forward (the first half of
+// enqueue_head); inv keeps 1 / rms for the backward.  A row whose position is out of range is formed from zeros.
+rtq_status enqueue_head_logits(rtq_ctx* c, const rtq_weight* w, const float* norm, float eps, float off, const float* x,
+                               int64_t t, const int32_t* pos, int64_t n, float* ns, float* inv, float* logits, Arena& ar,
+                               hipStream_t st) {
+  HeadArgs ha{};
+  ha.x = x, ha.pos = pos, ha.norm = norm, ha.eps = eps, ha.off = off;
+  ha.t = (int)t, ha.d = (int)w->cols, ha.n = (int)n, ha.V = (int)w->rows, ha.ns = ns, ha.inv = inv;
+  RTQ_TRY(launch(c, K_HEAD_NORM, dim3((unsigned)n), dim3(256), st, ha));
+  Arena fa = ar;
+  return enqueue_forward(c, w, ns, n, logits, nullptr, nullptr, nullptr, 0, 0.0f, nullptr, fa, st);
+}
+
+rtq_status enqueue_lm_top(rtq_ctx* c, const rtq_weight* w, const float* norm, float eps, float off, const float* x,
+                          int64_t t, const int32_t* pos, int64_t n, int64_t k, float temp, float* vals, int32_t* ids,
+                          float* rest, const TopPlan& p, Arena& ar, hipStream_t st) {
+  const int64_t V = w->rows, d = w->cols;
+  float* ns = ar.take<float>((size_t)(n * d));
+  float* inv = ar.take<float>((size_t)n);
+  float* logits = ar.take<float>((size_t)(n * V));
+  if (ar.off > ar.cap) return fail(RTQ_ERR_INVALID, "internal: workspace too small");
+  RTQ_TRY(enqueue_head_logits(c, w, norm, eps, off, x, t, pos, n, ns, inv, logits, ar, st));
+  Arena ta = ar;
+  return enqueue_top(c, logits, RTQ_TYPE_F32, n, V, V, k, temp, vals, ids, rest, p, ta, st, pos, t);
+}
+
+rtq_status enqueue_lm_distill(rtq_ctx* c, const rtq_weight* w, const float* norm, float eps, float off, const float* x,
+                              int64_t t, const int32_t* pos, const int32_t* tok, const float* wts, int64_t n,
+                              const rtq_teacher& te, float hard, float* kl, float* logp, float* dx, const DistillPlan& p,
+                              Arena& ar, hipStream_t st) {
+  const int64_t V = w->rows, d = w->cols;
+  float* ns = ar.take<float>((size_t)(n * d));
+  float* inv = ar.take<float>((size_t)n);
+  float* logits = ar.take<float>((size_t)(n * V));
+  float* dns = wts ? ar.take<float>((size_t)(n * d)) : nullptr;
+  if (ar.off > ar.cap) return fail(RTQ_ERR_INVALID, "internal: workspace too small");
+  RTQ_TRY(enqueue_head_logits(c, w, norm, eps, off, x, t, pos, n, ns, inv, logits, ar, st));
+  Arena da = ar;
+  RTQ_TRY(enqueue_distill(c, logits, RTQ_TYPE_F32, n, V, V, te, tok, wts, hard, kl, logp, logits, V, p, da, st, pos, t));
+  if (!wts) return RTQ_OK;
+  Arena ba = ar;
+  RTQ_TRY(enqueue_backward(c, w, logits, n, dns, false, nullptr, nullptr, nullptr, 0, 0.0f, nullptr, nullptr, ba, st));
+  FillArgs fz{dx, t * d};
+  RTQ_TRY(launch(c, K_FILL, dim3((unsigned)std::min<int64_t>(cdiv(t * d, 256), 4096)), dim3(256), st, fz));
+  HeadArgs ha{};
+  ha.x = x, ha.pos = pos, ha.norm = norm, ha.eps = eps, ha.off = off, ha.inv = inv, ha.dns = dns, ha.dx = dx;
+  ha.t = (int)t, ha.d = (int)d, ha.n = (int)n, ha.V = (int)V;
+  return launch(c, K_HEAD_NORM_BWD, dim3((unsigned)n), dim3(256), st, ha);
+}
+
+// the workspace of a head call over n rows: its buffers, then the largest of its products and `rows` bytes
+size_t lm_bytes(const rtq_ctx* c, const rtq_weight* w, int64_t n, bool grad, size_t rows) {
+  size_t sub = std::max(rows, fwd_ws_bytes(fwd_plan(w, n, 0)));
+  if (grad) sub = std::max(sub, bwd_ws_bytes(c, w, n, 0));
+  return (size_t)(n * w->cols) * 8 + (size_t)n * 4 + (size_t)(n * w->rows) * 4 + 8 * 256 + sub;
+}
+
+rtq_status check_lm_rows(rtq_ctx* c, const rtq_weight* w, const float* norm, const float* x, int64_t t, const int32_t* pos,
+                         int64_t n) {
+  RTQ_TRY(check_weight(c, w));
+  RTQ_TRY(check_t(t));
+  if (n < 0 || n > 65535) return fail(RTQ_ERR_INVALID, "row count %lld out of range [0, 65535]", (long long)n);
+  if (n > 0 && (!norm || !x || !pos)) return fail(RTQ_ERR_INVALID, "null norm/x/pos");
+  if ((double)n * (double)w->rows > 4e9) return fail(RTQ_ERR_INVALID, "n x vocab logits too large");
+  return RTQ_OK;
+}
+
+// the arguments of the row operators on f32 logits of the head (the logits themselves are the workspace's)
+const float* const kWsLogits = reinterpret_cast<const float*>((uintptr_t)256);
+
+rtq_status check_lm_top(rtq_ctx* c, const rtq_weight* w, const float* norm, const float* x, int64_t t, const int32_t* pos,
+                        int64_t n, int64_t k, float temp, const float* vals, const int32_t* ids) {
+  RTQ_TRY(check_lm_rows(c, w, norm, x, t, pos, n));
+  return check_top(c, kWsLogits, RTQ_TYPE_F32, n, w->rows, w->rows, k, temp, vals, ids);
+}
+
+rtq_status check_lm_distill(rtq_ctx* c, const rtq_weight* w, const float* norm, const float* x, int64_t t, const int32_t* pos,
+                            const int32_t* tok, const float* wts, int64_t n, const rtq_teacher* te, float hard,
+                            const float* kl, const float* logp, const float* dx) {
+  RTQ_TRY(check_lm_rows(c, w, norm, x, t, pos, n));
+  if (n > 0 && wts && !dx) return fail(RTQ_ERR_INVALID, "weights given without dx");
+  return check_distill(c, kWsLogits, RTQ_TYPE_F32, n, w->rows, w->rows, te, tok, wts, hard, kl, logp, kWsLogits, w->rows);
+}
+
+rtq_status fill_zero(rtq_ctx* c, float* p, int64_t n, hipStream_t st) {
+  FillArgs fz{p, n};
+  return launch(c, K_FILL, dim3((unsigned)std::min<int64_t>(cdiv(n, 256), 4096)), dim3(256), st, fz);
+}
+
+}  // namespace
+
+rtq_status rtq_lm_top_logits_d(rtq_ctx* c, const rtq_weight* w, const float* norm, float eps, float offset, const float* x,
+                               int64_t t, const int32_t* pos, int64_t n, int64_t k, float temp, float* vals, int32_t* ids,
+                               float* rest, void* stream) {
+  RTQ_TRY(check_lm_top(c, w, norm, x, t, pos, n, k, temp, vals, ids));
+  if (n == 0) return RTQ_OK;
+  std::lock_guard<std::mutex> lk(c->mu);
+  HIP_TRY(hipSetDevice(c->device));
+  hipStream_t st = (hipStream_t)stream;
+  const TopPlan p = top_plan(RTQ_TYPE_F32, n, w->rows, k);
+  RTQ_TRY(row_ws(c, lm_bytes(c, w, n, false, p.bytes), st));
+  Arena ar{(char*)c->ws, c->ws_bytes, 0};
+  return enqueue_lm_top(c, w, norm, eps, offset, x, t, pos, n, k, temp, vals, ids, rest, p, ar, st);
+}
+
+rtq_status rtq_lm_distill_d(rtq_ctx* c, const rtq_weight* w, const float* norm, float eps, float offset, const float* x,
+                            int64_t t, const int32_t* pos, const int32_t* tok, const float* weights, int64_t n,
+                            const rtq_teacher* teacher, float hard, float* kl, float* logp, float* dx, void* stream) {
+  RTQ_TRY(check_lm_distill(c, w, norm, x, t, pos, tok, weights, n, teacher, hard, kl, logp, dx));
+  std::lock_guard<std::mutex> lk(c->mu);
+  HIP_TRY(hipSetDevice(c->device));
+  hipStream_t st = (hipStream_t)stream;
+  if (n == 0) return weights && dx && t > 0 ? fill_zero(c, dx, t * w->cols, st) : RTQ_OK;
+  const DistillPlan p = distill_plan(n, w->rows, teacher->k);
+  RTQ_TRY(row_ws(c, lm_bytes(c, w, n, weights != nullptr, p.bytes), st));
+  Arena ar{(char*)c->ws, c->ws_bytes, 0};
+  return enqueue_lm_distill(c, w, norm, eps, offset, x, t, pos, tok, weights, n, *teacher, hard, kl, logp, dx, p, ar, st);
+}
+
+// the head's logits themselves (the model's draft verification): out [n x vocab]
+rtq_status rtq_lm_logits_d(rtq_ctx* c, const rtq_weight* w, const float* norm, float eps, float offset, const float* x,
+                           int64_t t, const int32_t* pos, int64_t n, float* out, void* stream) {
+  RTQ_TRY(check_lm_rows(c, w, norm, x, t, pos, n));
+  if (n == 0) return RTQ_OK;
+  std::lock_guard<std::mutex> lk(c->mu);
+  HIP_TRY(hipSetDevice(c->device));
+  hipStream_t st = (hipStream_t)stream;
+  RTQ_TRY(row_ws(c, lm_bytes(c, w, n, false, 0), st));
+  Arena ar{(char*)c->ws, c->ws_bytes, 0};
+  float* ns = ar.take<float>((size_t)(n * w->cols));
+  float* inv = ar.take<float>((size_t)n);
+  return enqueue_head_logits(c, w, norm, eps, offset, x, t, pos, n, ns, inv, out, ar, st);
 }
 
 // ------------------------------------------------------------------ host-pointer API
@@ -2328,6 +2470,16 @@ rtq_status check_teacher_ids(const rtq_teacher* t, int64_t n, int64_t V) {
     if (t->ids[i] >= V) return fail(RTQ_ERR_INVALID, "teacher token %d of row %lld out of vocab", t->ids[i], (long long)(i / t->k));
   return RTQ_OK;
 }
+rtq_status check_labels(const int32_t* tok, int64_t n, int64_t V) {
+  for (int64_t i = 0; tok && i < n; i++)
+    if (tok[i] < 0 || tok[i] >= V) return fail(RTQ_ERR_INVALID, "label %d of row %lld out of vocab", tok[i], (long long)i);
+  return RTQ_OK;
+}
+rtq_status check_positions(const int32_t* pos, int64_t n, int64_t t) {
+  for (int64_t i = 0; i < n; i++)
+    if (pos[i] < 0 || pos[i] >= t) return fail(RTQ_ERR_INVALID, "position %d of row %lld out of range", pos[i], (long long)i);
+  return RTQ_OK;
+}
 }  // namespace
 
 rtq_status rtq_top_logits(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V, int64_t ld, int64_t k, float temp,
@@ -2359,8 +2511,7 @@ rtq_status rtq_distill(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V
   RTQ_TRY(check_distill(c, z, type, n, V, ld, t, tok, w, hard, kl, logp, dz, ldd));
   if (n == 0) return RTQ_OK;
   RTQ_TRY(check_teacher_ids(t, n, V));
-  for (int64_t i = 0; tok && i < n; i++)
-    if (tok[i] < 0 || tok[i] >= V) return fail(RTQ_ERR_INVALID, "label %d of row %lld out of vocab", tok[i], (long long)i);
+  RTQ_TRY(check_labels(tok, n, V));
   HostCall hc(c);
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = c->stream;
@@ -2428,6 +2579,83 @@ rtq_status rtq_verify_draft(rtq_ctx* c, const void* z, int type, int64_t ld, con
   RTQ_TRY(enqueue_verify(c, zd, type, V, qd, V, b, d, V, xd, nd, ud, temp, ad, kd, p, ar, st));
   RTQ_TRY(d2h(accepted, ad, (size_t)b * 4, st));
   RTQ_TRY(d2h(tokens, kd, (size_t)tr * 4, st));
+  HIP_TRY(hipStreamSynchronize(st));
+  return RTQ_OK;
+}
+
+rtq_status rtq_lm_top_logits(rtq_ctx* c, const rtq_weight* w, const float* norm, float eps, float offset, const float* x,
+                             int64_t t, const int32_t* pos, int64_t n, int64_t k, float temp, float* vals, int32_t* ids,
+                             float* rest) {
+  RTQ_TRY(check_lm_top(c, w, norm, x, t, pos, n, k, temp, vals, ids));
+  RTQ_TRY(check_positions(pos, n, t));
+  if (n == 0) return RTQ_OK;
+  HostCall hc(c);
+  HIP_TRY(hipSetDevice(c->device));
+  hipStream_t st = c->stream;
+  const int64_t d = w->cols;
+  const TopPlan p = top_plan(RTQ_TYPE_F32, n, w->rows, k);
+  RTQ_TRY(ensure_ws(c, lm_bytes(c, w, n, false, p.bytes) + (size_t)(t * d + d + n * (2 * k + 2)) * 4 + 6 * 256));
+  Arena ar{(char*)c->ws, c->ws_bytes, 0};
+  float* xd = ar.take<float>((size_t)(t * d));
+  float* nd = ar.take<float>((size_t)d);
+  int32_t* pd = ar.take<int32_t>((size_t)n);
+  float* vd = ar.take<float>((size_t)(n * k));
+  int32_t* idd = ar.take<int32_t>((size_t)(n * k));
+  float* rd = ar.take<float>((size_t)n);
+  RTQ_TRY(h2d(xd, x, (size_t)(t * d) * 4, st));
+  RTQ_TRY(h2d(nd, norm, (size_t)d * 4, st));
+  RTQ_TRY(h2d(pd, pos, (size_t)n * 4, st));
+  RTQ_TRY(enqueue_lm_top(c, w, nd, eps, offset, xd, t, pd, n, k, temp, vd, idd, rest ? rd : nullptr, p, ar, st));
+  RTQ_TRY(d2h(vals, vd, (size_t)(n * k) * 4, st));
+  RTQ_TRY(d2h(ids, idd, (size_t)(n * k) * 4, st));
+  if (rest) RTQ_TRY(d2h(rest, rd, (size_t)n * 4, st));
+  HIP_TRY(hipStreamSynchronize(st));
+  return RTQ_OK;
+}
+
+rtq_status rtq_lm_distill(rtq_ctx* c, const rtq_weight* w, const float* norm, float eps, float offset, const float* x,
+                          int64_t t, const int32_t* pos, const int32_t* tok, const float* weights, int64_t n,
+                          const rtq_teacher* teacher, float hard, float* kl, float* logp, float* dx) {
+  RTQ_TRY(check_lm_distill(c, w, norm, x, t, pos, tok, weights, n, teacher, hard, kl, logp, dx));
+  RTQ_TRY(check_positions(pos, n, t));
+  if (n > 0) RTQ_TRY(check_teacher_ids(teacher, n, w->rows));
+  RTQ_TRY(check_labels(tok, n, w->rows));
+  const int64_t d = w->cols;
+  if (n == 0) {
+    if (weights && dx) memset(dx, 0, (size_t)(t * d) * 4);
+    return RTQ_OK;
+  }
+  HostCall hc(c);
+  HIP_TRY(hipSetDevice(c->device));
+  hipStream_t st = c->stream;
+  const DistillPlan p = distill_plan(n, w->rows, teacher->k);
+  const int64_t k = teacher->k;
+  RTQ_TRY(ensure_ws(c, lm_bytes(c, w, n, weights != nullptr, p.bytes) + (size_t)(2 * t * d + d + n * (2 * k + 6)) * 4 + 11 * 256));
+  Arena ar{(char*)c->ws, c->ws_bytes, 0};
+  float* xd = ar.take<float>((size_t)(t * d));
+  float* nd = ar.take<float>((size_t)d);
+  int32_t* pd = ar.take<int32_t>((size_t)n);
+  int32_t* kd = tok ? ar.take<int32_t>((size_t)n) : nullptr;
+  float* wd = weights ? ar.take<float>((size_t)n) : nullptr;
+  int32_t* idd = ar.take<int32_t>((size_t)(n * k));
+  float* vd = ar.take<float>((size_t)(n * k));
+  float* rd = teacher->rest ? ar.take<float>((size_t)n) : nullptr;
+  float* kld = ar.take<float>((size_t)n);
+  float* lpd = tok ? ar.take<float>((size_t)n) : nullptr;
+  float* dxd = weights ? ar.take<float>((size_t)(t * d)) : nullptr;
+  RTQ_TRY(h2d(xd, x, (size_t)(t * d) * 4, st));
+  RTQ_TRY(h2d(nd, norm, (size_t)d * 4, st));
+  RTQ_TRY(h2d(pd, pos, (size_t)n * 4, st));
+  if (kd) RTQ_TRY(h2d(kd, tok, (size_t)n * 4, st));
+  if (wd) RTQ_TRY(h2d(wd, weights, (size_t)n * 4, st));
+  RTQ_TRY(h2d(idd, teacher->ids, (size_t)(n * k) * 4, st));
+  RTQ_TRY(h2d(vd, teacher->vals, (size_t)(n * k) * 4, st));
+  if (rd) RTQ_TRY(h2d(rd, teacher->rest, (size_t)n * 4, st));
+  const rtq_teacher td{k, idd, vd, rd, teacher->temperature};
+  RTQ_TRY(enqueue_lm_distill(c, w, nd, eps, offset, xd, t, pd, kd, wd, n, td, hard, kld, lpd, dxd, p, ar, st));
+  RTQ_TRY(d2h(kl, kld, (size_t)n * 4, st));
+  if (lpd) RTQ_TRY(d2h(logp, lpd, (size_t)n * 4, st));
+  if (dxd) RTQ_TRY(d2h(dx, dxd, (size_t)(t * d) * 4, st));
   HIP_TRY(hipStreamSynchronize(st));
   return RTQ_OK;
 }

@@ -79,6 +79,12 @@ __device__ __forceinline__ float exp_scaled(float t, float ch, float cl) {
   return y < -150.0f ? 0.0f : fmaf(e, d * 0.693147181f, e);  // -inf and overflows of t ch among them
 }
 
+// whether row i has logits (rows formed at positions: the position is one of the sequence's)
+template <class Args>
+__device__ __forceinline__ bool row_ok(const Args& a, int i) {
+  return !a.pos || (a.pos[i] >= 0 && a.pos[i] < a.t);
+}
+
 template <class T>
 __device__ __forceinline__ T wave_sum_any(T v) {
 #pragma unroll
@@ -173,6 +179,12 @@ __device__ __forceinline__ float wave_sort(float v) {
 
 constexpr int kTopB = 1024, kTopW = kTopB / 64, kTopCap = 2048;
 
+// the outputs of a row without logits
+__device__ __forceinline__ void top_none(const TopArgs& a, int i) {
+  for (int s = threadIdx.x; s < a.k; s += kTopB) a.vals[(int64_t)i * a.k + s] = __builtin_nanf(""), a.ids[(int64_t)i * a.k + s] = -1;
+  if (threadIdx.x == 0 && a.rest) a.rest[i] = __builtin_nanf("");
+}
+
 // The k largest of slice g of row i, in order, and (max, sum) of the slice's others.  The slice stays
 // in registers (NV vectors a thread).  A bound below the k-th largest comes from the lanes' maxima:
 // with r = ceil(k / waves), every wave has r maxima at or above its own r-th, so the least of those r-ths
@@ -188,6 +200,10 @@ __device__ __forceinline__ void top_slice(const TopArgs& a) {
   __shared__ int hist[256];
   __shared__ int cnt, pick, above;
   const int tid = threadIdx.x, g = blockIdx.x, i = blockIdx.y;
+  if (!row_ok(a, i)) {
+    if (g == 0) top_none(a, i);
+    return;
+  }
   const void* row = static_cast<const char*>(a.z) + (int64_t)i * a.ld * R::ES;
   const int j0 = g * a.L, j1 = min(a.V, j0 + a.L);  // L <= kTopB * NV * E
   const float ninf = -__builtin_inff();
@@ -336,6 +352,7 @@ extern "C" __global__ __launch_bounds__(kTopB) void rtq_top_merge(TopArgs a) {
   __shared__ uint64_t bound;
   const int tid = threadIdx.x, i = blockIdx.x, r = (a.k + a.G - 1) / a.G, total = a.G * a.k;
   const uint64_t* L = a.lists + (int64_t)i * total;
+  if (!row_ok(a, i)) return;  // written by slice 0
   if (tid < 64) {
     uint64_t lo = ~0ull, hi = 0;
     for (int g = tid; g < a.G; g += 64) {
@@ -419,6 +436,7 @@ __device__ __forceinline__ void distill_stats(const DistillArgs& a) {
   __shared__ float redf[kDisW];
   __shared__ double redd[kDisW];
   const int tid = threadIdx.x, g = blockIdx.x, i = blockIdx.y;
+  if (!row_ok(a, i)) return;
   const void* row = static_cast<const char*>(a.z) + (int64_t)i * a.ld * R::ES;
   const int j0 = g * a.L, j1 = min(a.V, j0 + a.L);
   const float ninf = -__builtin_inff();
@@ -472,6 +490,16 @@ __device__ __forceinline__ void distill_grad(const DistillArgs& a) {
   __shared__ double pl[kDisB];
   const int tid = threadIdx.x, g = blockIdx.x, i = blockIdx.y;
   const float ninf = -__builtin_inff();
+  const int j0 = g * a.L, j1 = min(a.V, j0 + a.L);
+  void* out = static_cast<char*>(a.dz) + (int64_t)i * a.ldd * R::ES;
+  if (!row_ok(a, i)) {
+    if (g == 0 && tid == 0) {
+      a.kl[i] = __builtin_nanf("");
+      if (a.logp) a.logp[i] = __builtin_nanf("");
+    }
+    for (int j = j0 + tid; a.w && j < j1; j += kDisB) R::put(out, j, 0.0f);
+    return;
+  }
   const double invt = 1.0 / (double)a.temp;
   // the unlisted
   float mu = ninf;
@@ -549,8 +577,6 @@ __device__ __forceinline__ void distill_grad(const DistillArgs& a) {
   const float D = w == 0.0 || w1 == 0.0 || (empty && Z1 == Z1) ? 0.0f : (float)(w1 * (fu1 / Z1));
   const float ref = empty ? 0.0f : mu;
   const void* row = static_cast<const char*>(a.z) + (int64_t)i * a.ld * R::ES;
-  void* out = static_cast<char*>(a.dz) + (int64_t)i * a.ldd * R::ES;
-  const int j0 = g * a.L, j1 = min(a.V, j0 + a.L);
   for (int j = j0 + tid * R::E; j < j1; j += kDisB * R::E) {
     const u4v r = R::load_upto(row, j, j1, ninf);
     float f[R::E];

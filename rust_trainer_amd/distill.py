@@ -8,7 +8,8 @@ tokens that a draft model (a distilled student, say) proposed, such that what co
 target's samples.
 
 Rows are numpy arrays of float32 or float16 (bfloat16: uint16 arrays with ``type=TYPE_BF16``); a row may be longer
-apart than it is long (a view ``a[:, :vocab]``).  The ``_d`` variants take device addresses and a stream and only enqueue.
+apart than it is long (a view ``a[:, :vocab]``).  ``head_top_logits`` and ``head_distill`` take the rows from an LM head
+(``GpuModel.top_logits``, ``forward_backward_distill`` and ``verify_draft`` from a whole model).  The ``_d`` variants take device addresses and a stream and only enqueue.
 """
 from __future__ import annotations
 
@@ -18,7 +19,7 @@ import dataclasses
 import numpy as np
 
 from . import _ffi
-from .frozen import Context, default_context
+from .frozen import Context, HipFrozen, default_context
 
 
 @dataclasses.dataclass
@@ -55,6 +56,12 @@ def _rows(a, type: int | None, what: str) -> tuple[np.ndarray, int, int]:
     return a, type, a.strides[0] // a.itemsize if a.shape[0] > 1 else a.shape[1]
 
 
+def _per_row(a, dtype, n: int, what: str) -> np.ndarray | None:
+    a = None if a is None else np.ascontiguousarray(a, dtype=dtype).reshape(-1)
+    assert a is None or a.size == n, f"one {what} per row"
+    return a
+
+
 def _addr(a) -> int | None:
     return None if a is None else a.ctypes.data
 
@@ -77,10 +84,7 @@ def distill(logits, teacher: Teacher, labels=None, weights=None, hard: float = 0
     a, ty, ld = _rows(logits, type, "distill")
     n, vocab = a.shape
     view = teacher._view(n)
-    tok = None if labels is None else np.ascontiguousarray(labels, dtype=np.int32).reshape(-1)
-    w = None if weights is None else np.ascontiguousarray(weights, dtype=np.float32).reshape(-1)
-    assert tok is None or tok.size == n, "one label per row"
-    assert w is None or w.size == n, "one weight per row"
+    tok, w = _per_row(labels, np.int32, n, "label"), _per_row(weights, np.float32, n, "weight")
     kl = np.empty(n, np.float32)
     logp = None if tok is None else np.empty(n, np.float32)
     dz = None if w is None else np.empty((n, vocab), a.dtype)
@@ -114,6 +118,43 @@ def verify_draft(logits, drafted, uniforms=None, draft=None, lens=None, temperat
                                            x.ctypes.data, _addr(n), _addr(u), temperature, accepted.ctypes.data,
                                            tokens.ctypes.data), "rtq_verify_draft")
     return accepted, tokens
+
+
+def _head(lm_head: HipFrozen, final_norm, x, positions) -> tuple[np.ndarray, np.ndarray, np.ndarray, int]:
+    d = lm_head.in_dim()
+    x = np.ascontiguousarray(x, dtype=np.float32).reshape(-1)
+    assert x.size % d == 0, "x is not a whole number of rows"
+    norm = np.ascontiguousarray(final_norm, dtype=np.float32)
+    assert norm.size == d, "final_norm length != hidden size"
+    return norm, x, np.ascontiguousarray(positions, dtype=np.int32).reshape(-1), x.size // d
+
+
+def head_top_logits(lm_head: HipFrozen, final_norm, x, positions, k: int, temperature: float = 1.0, eps: float = 1e-6,
+                    offset: float = 0.0) -> Teacher:
+    """``top_logits`` of the LM head's logits at ``positions`` of the [t x d] hidden states ``x`` (as ``head`` forms them)."""
+    norm, x, pos, t = _head(lm_head, final_norm, x, positions)
+    n = pos.size
+    vals, ids, rest = np.empty((n, k), np.float32), np.empty((n, k), np.int32), np.empty(n, np.float32)
+    _ffi.check(_ffi.lib().rtq_lm_top_logits(lm_head.ctx.handle, lm_head.handle, norm.ctypes.data, eps, offset, x.ctypes.data, t,
+                                            pos.ctypes.data, n, k, temperature, vals.ctypes.data, ids.ctypes.data,
+                                            rest.ctypes.data), "rtq_lm_top_logits")
+    return Teacher(ids, vals, rest, temperature)
+
+
+def head_distill(lm_head: HipFrozen, final_norm, x, positions, teacher: Teacher, labels=None, weights=None, hard: float = 0.0,
+                 eps: float = 1e-6, offset: float = 0.0) -> tuple[np.ndarray, np.ndarray, np.ndarray]:
+    """``(kl, logp, dx)``: ``distill`` of the LM head's logits at ``positions``, with ``weights`` the gradient to the
+    hidden states ``x`` (zero rows outside ``positions``; empty without weights)."""
+    norm, x, pos, t = _head(lm_head, final_norm, x, positions)
+    n = pos.size
+    view = teacher._view(n)
+    tok, w = _per_row(labels, np.int32, n, "label"), _per_row(weights, np.float32, n, "weight")
+    kl, logp = np.empty(n, np.float32), None if tok is None else np.empty(n, np.float32)
+    dx = None if w is None else np.empty(x.size, np.float32)
+    _ffi.check(_ffi.lib().rtq_lm_distill(lm_head.ctx.handle, lm_head.handle, norm.ctypes.data, eps, offset, x.ctypes.data, t,
+                                         pos.ctypes.data, _addr(tok), _addr(w), n, ctypes.byref(view), hard, kl.ctypes.data,
+                                         _addr(logp), _addr(dx)), "rtq_lm_distill")
+    return kl, np.empty(0, np.float32) if logp is None else logp, np.empty(0, np.float32) if dx is None else dx
 
 
 # ---- device-pointer variants (ints are device addresses, 0: none; stream 0 = the HIP null stream)

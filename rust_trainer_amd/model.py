@@ -13,6 +13,7 @@ import ctypes
 import numpy as np
 
 from . import _ffi
+from .distill import Teacher, _addr, _per_row
 from .frozen import Context, default_context
 
 LINEARS = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
@@ -199,3 +200,56 @@ class GpuModel:
     def score(self, tokens, targets) -> tuple[np.ndarray, int]:
         """``Model::score`` (src/model.rs:553-557): log-probs and hits, no backward."""
         return self.forward_backward(tokens, targets, None)
+
+    def _layout(self, tokens, packed):
+        """(tokens, positions, segments): of one sequence, or of a ``packing.Packed`` batch."""
+        if packed is None:
+            return np.ascontiguousarray(tokens, dtype=np.int32).reshape(-1), None, None
+        assert tokens is None, "tokens or a packed batch"
+        a = [np.ascontiguousarray(v, dtype=np.int32).reshape(-1) for v in (packed.tokens, packed.positions, packed.segments)]
+        assert a[1].size == a[0].size and a[2].size == a[0].size, "one position and segment per token"
+        return a
+
+    def top_logits(self, tokens, positions, k: int, temperature: float = 1.0, packed=None) -> Teacher:
+        """A teacher's pass: ``distill.top_logits`` of the logits at ``positions`` of ``tokens`` (of ``packed``'s, with
+        ``tokens`` None)."""
+        toks, ps, sg = self._layout(tokens, packed)
+        pos = np.ascontiguousarray(positions, dtype=np.int32).reshape(-1)
+        n = pos.size
+        vals, ids, rest = np.empty((n, k), np.float32), np.empty((n, k), np.int32), np.empty(n, np.float32)
+        _ffi.check(_ffi.lib().rtq_model_top_logits(self._h, toks.ctypes.data, toks.size, _addr(ps), _addr(sg), pos.ctypes.data, n, k,
+                                                   temperature, vals.ctypes.data, ids.ctypes.data, rest.ctypes.data),
+                   "rtq_model_top_logits")
+        self._stepped = True
+        return Teacher(ids, vals, rest, temperature)
+
+    def forward_backward_distill(self, tokens, positions, teacher: Teacher, labels=None, weights=None, hard: float = 0.0,
+                                 packed=None) -> tuple[np.ndarray, np.ndarray]:
+        """``(kl, logp)`` of ``distill.distill`` at ``positions`` of ``tokens`` (of ``packed``'s, with ``tokens`` None); with
+        ``weights`` the adapters' gradients of ``sum w ((1 - hard) T^2 kl - hard logp)`` accumulate."""
+        toks, ps, sg = self._layout(tokens, packed)
+        pos = np.ascontiguousarray(positions, dtype=np.int32).reshape(-1)
+        n = pos.size
+        view = teacher._view(n)
+        tok, w = _per_row(labels, np.int32, n, "label"), _per_row(weights, np.float32, n, "weight")
+        kl, logp = np.empty(n, np.float32), None if tok is None else np.empty(n, np.float32)
+        _ffi.check(_ffi.lib().rtq_model_forward_backward_distill(
+            self._h, toks.ctypes.data, toks.size, _addr(ps), _addr(sg), pos.ctypes.data, _addr(tok), _addr(w), n, ctypes.byref(view), hard,
+            kl.ctypes.data, _addr(logp)), "rtq_model_forward_backward_distill")
+        self._stepped = True
+        return kl, np.empty(0, np.float32) if logp is None else logp
+
+    def verify_draft(self, tokens, drafted: int, uniforms=None, draft: "GpuModel | None" = None,
+                     temperature: float = 1.0) -> tuple[int, np.ndarray]:
+        """``distill.verify_draft`` of the last ``drafted`` of ``tokens`` by this model: how many are accepted, and
+        the accepted ones, the token drawn after them, -1 beyond [drafted + 1].  ``draft``: the model that they were
+        drawn from at this temperature (None: not drawn); ``uniforms`` [drafted + 1]."""
+        toks = np.ascontiguousarray(tokens, dtype=np.int32).reshape(-1)
+        u = None if uniforms is None else np.ascontiguousarray(uniforms, dtype=np.float32).reshape(-1)
+        assert u is None or u.size == drafted + 1, "one uniform number per drafted token, and one more"
+        acc, out = ctypes.c_int32(), np.empty(max(drafted, 0) + 1, np.int32)
+        _ffi.check(_ffi.lib().rtq_model_verify_draft(self._h, None if draft is None else draft._h, toks.ctypes.data, toks.size, drafted,
+                                                     _addr(u), temperature, ctypes.byref(acc), out.ctypes.data),
+                   "rtq_model_verify_draft")
+        self._stepped = True
+        return int(acc.value), out

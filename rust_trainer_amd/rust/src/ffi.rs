@@ -170,6 +170,21 @@ extern "C" {
                               uniforms: *const f32, temperature: f32, accepted: *mut i32, tokens: *mut i32,
                               stream: *mut c_void) -> rtq_status;
 
+    pub fn rtq_lm_top_logits(ctx: *mut rtq_ctx, lm_head: *const rtq_weight, norm_w: *const f32, eps: f32, offset: f32,
+                             x: *const f32, t: i64, pos: *const i32, n: i64, k: i64, temperature: f32, vals: *mut f32,
+                             ids: *mut i32, rest: *mut f32) -> rtq_status;
+    pub fn rtq_lm_top_logits_d(ctx: *mut rtq_ctx, lm_head: *const rtq_weight, norm_w: *const f32, eps: f32,
+                               offset: f32, x: *const f32, t: i64, pos: *const i32, n: i64, k: i64, temperature: f32,
+                               vals: *mut f32, ids: *mut i32, rest: *mut f32, stream: *mut c_void) -> rtq_status;
+    pub fn rtq_lm_distill(ctx: *mut rtq_ctx, lm_head: *const rtq_weight, norm_w: *const f32, eps: f32, offset: f32,
+                          x: *const f32, t: i64, pos: *const i32, tok: *const i32, weights: *const f32, n: i64,
+                          teacher: *const rtq_teacher, hard: f32, kl: *mut f32, logp: *mut f32,
+                          dx: *mut f32) -> rtq_status;
+    pub fn rtq_lm_distill_d(ctx: *mut rtq_ctx, lm_head: *const rtq_weight, norm_w: *const f32, eps: f32, offset: f32,
+                            x: *const f32, t: i64, pos: *const i32, tok: *const i32, weights: *const f32, n: i64,
+                            teacher: *const rtq_teacher, hard: f32, kl: *mut f32, logp: *mut f32, dx: *mut f32,
+                            stream: *mut c_void) -> rtq_status;
+
     // the device-resident training step (Model::forward_backward)
     pub fn rtq_model_from_gguf(ctx: *mut rtq_ctx, g: *const rtq_gguf, out: *mut *mut rtq_model) -> rtq_status;
     pub fn rtq_model_config_from_gguf(g: *const rtq_gguf, out: *mut rtq_model_config) -> rtq_status;
@@ -193,6 +208,16 @@ extern "C" {
                                              segments: *const i32, pos: *const i32, tok: *const i32,
                                              weights: *const f32, n: i64, logp: *mut f32,
                                              hits: *mut i64) -> rtq_status;
+    pub fn rtq_model_top_logits(m: *mut rtq_model, tokens: *const i32, t: i64, positions: *const i32,
+                                segments: *const i32, pos: *const i32, n: i64, k: i64, temperature: f32,
+                                vals: *mut f32, ids: *mut i32, rest: *mut f32) -> rtq_status;
+    pub fn rtq_model_forward_backward_distill(m: *mut rtq_model, tokens: *const i32, t: i64, positions: *const i32,
+                                              segments: *const i32, pos: *const i32, tok: *const i32,
+                                              weights: *const f32, n: i64, teacher: *const rtq_teacher, hard: f32,
+                                              kl: *mut f32, logp: *mut f32) -> rtq_status;
+    pub fn rtq_model_verify_draft(m: *mut rtq_model, draft: *mut rtq_model, tokens: *const i32, t: i64, d: i64,
+                                  uniforms: *const f32, temperature: f32, accepted: *mut i32,
+                                  out: *mut i32) -> rtq_status;
     pub fn rtq_model_set_checkpointing(m: *mut rtq_model, mode: c_int) -> rtq_status;
     pub fn rtq_model_checkpointing(m: *const rtq_model) -> c_int;
     pub fn rtq_model_set_attention(m: *mut rtq_model, mode: c_int) -> rtq_status;
