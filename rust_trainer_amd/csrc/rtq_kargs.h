@@ -353,19 +353,19 @@ struct HeadArgs {
 };
 
 // ---------------------------------------------------------------- rows of vocabulary logits
-// z: rows of V logits (f32, f16 or bf16), stride ld elements; a row is cut into G slices of L
+// z: rows of V logits (f32, f16 or bf16), stride ld elements; where a row is cut, into G slices of L
 // logits.  ch + cl = log2(e) / temp.
 struct TopArgs {
   const void* z;
   int64_t ld;
-  int n, V, k, G, L;
+  int n, V, k;
+  int NG;  // groups per row (32 f32 or 64 16-bit logits each), rounded up to whole chunks of 64
   float temp, ch, cl;
-  uint64_t* lists;  // [n x G x k] each slice's largest, in order (G > 1)
-  float* pm;        // [n x G] maximum of each slice's others
-  double* ps;       // [n x G] their sum of exp((z - pm) / temp)
-  float* vals;      // [n x k]
-  int32_t* ids;     // [n x k]
-  float* rest;      // [n] or null
+  float* gm;     // [n x NG] each group's maximum (NaN if it holds one)
+  float* gs;     // [n x NG] and its sum of exp((z - maximum) / temp)
+  float* vals;   // [n x k]
+  int32_t* ids;  // [n x k]
+  float* rest;   // [n] or null
   const int32_t* pos;  // [n] positions that the rows were formed at, or null: a row whose position is
   int t;               // outside [0, t) has no logits (vals and rest NaN, ids -1)
 };

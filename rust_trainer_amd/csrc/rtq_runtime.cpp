@@ -165,9 +165,9 @@ enum Kid {
   K_HEAD_NORM_BWD,
   K_ACT_PREP8,   // Q8_0 activations of the block norms on 8-token tiles
   K_ACT_PREP4,   // the same on 4-token tiles
-  K_TOP,         // + type + 3 * (the longer slices): top logits of a slice, of a row from its slices
-  K_TOP_MERGE = K_TOP + 6,
-  K_DISTILL_STATS,  // + type
+  K_TOP_SCAN,    // + type (f32, f16, bf16)
+  K_TOP_PICK = K_TOP_SCAN + 3,
+  K_DISTILL_STATS = K_TOP_PICK + 3,
   K_DISTILL_GRAD = K_DISTILL_STATS + 3,
   K_VERIFY_STATS = K_DISTILL_GRAD + 3,
   K_VERIFY_ACCEPT = K_VERIFY_STATS + 3,
@@ -204,8 +204,8 @@ constexpr const char* kKernelNames[] = {
     "rtq_dense_bwd32",      "rtq_dense_bwd32_q8",   "rtq_dense_bwd64",      "rtq_dense_bwd64_q8",
     "rtq_head_norm",        "rtq_head_max",         "rtq_head_sum",         "rtq_head_grad",
     "rtq_head_norm_bwd",    "rtq_act_prep8_q8_0",   "rtq_act_prep4_q8_0",
-    "rtq_top_f32_s",        "rtq_top_f16_s",        "rtq_top_bf16_s",       "rtq_top_f32_l",        "rtq_top_f16_l",
-    "rtq_top_bf16_l",       "rtq_top_merge",
+    "rtq_top_scan_f32",     "rtq_top_scan_f16",     "rtq_top_scan_bf16",
+    "rtq_top_pick_f32",     "rtq_top_pick_f16",     "rtq_top_pick_bf16",
     "rtq_distill_stats_f32", "rtq_distill_stats_f16", "rtq_distill_stats_bf16",
     "rtq_distill_grad_f32", "rtq_distill_grad_f16", "rtq_distill_grad_bf16",
     "rtq_verify_stats_f32", "rtq_verify_stats_f16", "rtq_verify_stats_bf16",
@@ -1870,7 +1870,6 @@ rtq_status rtq_lm_head_d(rtq_ctx* c, const rtq_weight* w, const float* norm, flo
 namespace {
 
 constexpr int64_t kVocabMax = 1 << 20;
-constexpr int64_t kTopMergeMax = 8192;  // list entries that rtq_top_merge sorts at most (64 KiB of LDS)
 
 int logit_type(int type) { return type == RTQ_TYPE_F32 ? 0 : type == RTQ_TYPE_F16 ? 1 : type == RTQ_TYPE_BF16 ? 2 : -1; }
 int64_t logit_bytes(int type) { return type == RTQ_TYPE_F32 ? 4 : 2; }
@@ -1912,18 +1911,14 @@ void exp_scale(float t, float* hi, float* lo) {
 
 // ---- top logits
 struct TopPlan {
-  bool large;  // the longer slices
-  int64_t G, L;
+  int64_t NG;  // groups per row, whole chunks of 64 (rtq_top_scan_*: a wave each)
   size_t bytes;
 };
 
-TopPlan top_plan(int type, int64_t n, int64_t V, int64_t k) {
-  const int64_t per = 1024 * 16 / logit_bytes(type);  // logits a workgroup loads at once
+TopPlan top_plan(int type, int64_t n, int64_t V) {
   TopPlan p{};
-  p.L = 2 * per;
-  if (cdiv(V, p.L) * k > kTopMergeMax) p.large = true, p.L = (type == RTQ_TYPE_F32 ? 8 : 4) * per;
-  p.G = cdiv(V, p.L);
-  if (p.G > 1) p.bytes = (size_t)(n * p.G * k) * 8 + (size_t)(n * p.G) * 12 + 4 * 256;
+  p.NG = cdiv(V, 64 * 8 * 16 / logit_bytes(type)) * 64;
+  p.bytes = (size_t)(n * p.NG) * 8 + 3 * 256;
   return p;
 }
 
@@ -1942,21 +1937,15 @@ rtq_status enqueue_top(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V
                        const int32_t* pos = nullptr, int64_t t = 0) {
   TopArgs a{};
   a.pos = pos, a.t = (int)t;
-  a.z = z, a.ld = ld, a.n = (int)n, a.V = (int)V, a.k = (int)k, a.G = (int)p.G, a.L = (int)p.L;
+  a.z = z, a.ld = ld, a.n = (int)n, a.V = (int)V, a.k = (int)k, a.NG = (int)p.NG;
   a.temp = temp;
   exp_scale(temp, &a.ch, &a.cl);
   a.vals = vals, a.ids = ids, a.rest = rest;
-  if (p.G > 1) {
-    a.lists = ar.take<uint64_t>((size_t)(n * p.G * k));
-    a.ps = ar.take<double>((size_t)(n * p.G));
-    a.pm = ar.take<float>((size_t)(n * p.G));
-    if (ar.off > ar.cap) return fail(RTQ_ERR_INVALID, "internal: workspace too small");
-  }
-  RTQ_TRY(launch(c, K_TOP + logit_type(type) + (p.large ? 3 : 0), dim3((unsigned)p.G, (unsigned)n), dim3(1024), st, a));
-  if (p.G == 1) return RTQ_OK;
-  unsigned P = 2;
-  while (P < p.G * k) P <<= 1;
-  return launch(c, K_TOP_MERGE, dim3((unsigned)n), dim3(1024), st, a, P * 8);
+  a.gm = ar.take<float>((size_t)(n * p.NG));
+  a.gs = ar.take<float>((size_t)(n * p.NG));
+  if (ar.off > ar.cap) return fail(RTQ_ERR_INVALID, "internal: workspace too small");
+  RTQ_TRY(launch(c, K_TOP_SCAN + logit_type(type), dim3((unsigned)cdiv(p.NG, 256), (unsigned)n), dim3(256), st, a));
+  return launch(c, K_TOP_PICK + logit_type(type), dim3((unsigned)n), dim3(512), st, a);
 }
 
 // ---- distillation
@@ -2081,7 +2070,7 @@ rtq_status rtq_top_logits_d(rtq_ctx* c, const void* z, int type, int64_t n, int6
   std::lock_guard<std::mutex> lk(c->mu);
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = (hipStream_t)stream;
-  const TopPlan p = top_plan(type, n, V, k);
+  const TopPlan p = top_plan(type, n, V);
   RTQ_TRY(row_ws(c, p.bytes, st));
   Arena ar{(char*)c->ws, c->ws_bytes, 0};
   return enqueue_top(c, z, type, n, V, ld, k, temp, vals, ids, rest, p, ar, st);
@@ -2218,7 +2207,7 @@ rtq_status rtq_lm_top_logits_d(rtq_ctx* c, const rtq_weight* w, const float* nor
   std::lock_guard<std::mutex> lk(c->mu);
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = (hipStream_t)stream;
-  const TopPlan p = top_plan(RTQ_TYPE_F32, n, w->rows, k);
+  const TopPlan p = top_plan(RTQ_TYPE_F32, n, w->rows);
   RTQ_TRY(row_ws(c, lm_bytes(c, w, n, false, p.bytes), st));
   Arena ar{(char*)c->ws, c->ws_bytes, 0};
   return enqueue_lm_top(c, w, norm, eps, offset, x, t, pos, n, k, temp, vals, ids, rest, p, ar, st);
@@ -2489,7 +2478,7 @@ rtq_status rtq_top_logits(rtq_ctx* c, const void* z, int type, int64_t n, int64_
   HostCall hc(c);
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = c->stream;
-  const TopPlan p = top_plan(type, n, V, k);
+  const TopPlan p = top_plan(type, n, V);
   const int64_t es = logit_bytes(type);
   RTQ_TRY(ensure_ws(c, p.bytes + (size_t)(n * V * es + n * (8 * k + 4)) + 4 * 256));
   Arena ar{(char*)c->ws, c->ws_bytes, 0};
@@ -2593,7 +2582,7 @@ rtq_status rtq_lm_top_logits(rtq_ctx* c, const rtq_weight* w, const float* norm,
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = c->stream;
   const int64_t d = w->cols;
-  const TopPlan p = top_plan(RTQ_TYPE_F32, n, w->rows, k);
+  const TopPlan p = top_plan(RTQ_TYPE_F32, n, w->rows);
   RTQ_TRY(ensure_ws(c, lm_bytes(c, w, n, false, p.bytes) + (size_t)(t * d + d + n * (2 * k + 2)) * 4 + 6 * 256));
   Arena ar{(char*)c->ws, c->ws_bytes, 0};
   float* xd = ar.take<float>((size_t)(t * d));

@@ -85,11 +85,31 @@ __device__ __forceinline__ bool row_ok(const Args& a, int i) {
   return !a.pos || (a.pos[i] >= 0 && a.pos[i] < a.t);
 }
 
+// the value of lane ^ J (J = 1, 2, 4, 8 by DPP controls within rows of 16 lanes)
+template <int J>
+__device__ __forceinline__ float lane_xor(float v) {
+  if constexpr (J == 1) return dpp_f<0xB1>(v);
+  else if constexpr (J == 2) return dpp_f<0x4E>(v);
+  else if constexpr (J == 4) return dpp_f<0x1B>(dpp_f<0x141>(v));  // mirrored in eight, then in four
+  else if constexpr (J == 8) return dpp_f<0x128>(v);               // rotated by eight
+  else return __shfl_xor(v, J);
+}
+template <int J>
+__device__ __forceinline__ double lane_xor(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_bit_cast(uint32_t, lane_xor<J>(__builtin_bit_cast(float, (uint32_t)u)));
+  const uint32_t hi = __builtin_bit_cast(uint32_t, lane_xor<J>(__builtin_bit_cast(float, (uint32_t)(u >> 32))));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
 template <class T>
 __device__ __forceinline__ T wave_sum_any(T v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m);
-  return v;
+  v += lane_xor<1>(v);
+  v += lane_xor<2>(v);
+  v += lane_xor<4>(v);
+  v += lane_xor<8>(v);
+  v += lane_xor<16>(v);
+  return v + lane_xor<32>(v);
 }
 
 // sum / maximum over a workgroup of W waves (red: W values of LDS); every thread gets the result
@@ -104,9 +124,17 @@ __device__ __forceinline__ T group_sum(T v, T* red) {
   for (int w = 1; w < W; w++) s += red[w];
   return s;
 }
+__device__ __forceinline__ float wave_max_any(float v) {
+  v = fmaxf(v, lane_xor<1>(v));
+  v = fmaxf(v, lane_xor<2>(v));
+  v = fmaxf(v, lane_xor<4>(v));
+  v = fmaxf(v, lane_xor<8>(v));
+  v = fmaxf(v, lane_xor<16>(v));
+  return fmaxf(v, lane_xor<32>(v));
+}
 template <int W>
 __device__ __forceinline__ float group_max(float v, float* red) {
-  v = wave_max(v);
+  v = wave_max_any(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -132,293 +160,366 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 }
 __device__ __forceinline__ int key_index(uint64_t k) { return (int)~(uint32_t)k; }
 
-// (max, sum of exp((x - max) / T)) of two sets
-__device__ __forceinline__ void join_sums(float& m, double& s, float m2, double s2, double invt) {
-  if (m2 == -__builtin_inff()) return;
-  if (m == -__builtin_inff()) {
-    m = m2, s = s2;
-    return;
-  }
-  const float mm = fmaxf(m, m2);
-  s = s * exp(((double)m - mm) * invt) + s2 * exp(((double)m2 - mm) * invt);
-  m = mm;
-}
 __device__ __forceinline__ float lse_of(float m, double s, double invt) {
-  if (m == -__builtin_inff() || m == __builtin_inff()) return m;
-  return (float)((double)m * invt + log(s));
+  if (m == -__builtin_inff()) return s != s ? __builtin_nanf("") : m;
+  return m == __builtin_inff() ? m : (float)((double)m * invt + log(s));
 }
 
-// keys[0 .. P) sorted from the largest, P a power of two
-template <int B>
-__device__ __forceinline__ void sort_keys(uint64_t* keys, int P) {
-  for (int k = 2; k <= P; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      __syncthreads();
-      for (int p = threadIdx.x; p < P / 2; p += B) {
-        const int i = 2 * p - (p & (j - 1)), q = i | j;
-        const uint64_t a = keys[i], b = keys[q];
-        if ((a < b) == ((i & k) == 0)) keys[i] = b, keys[q] = a;
+// maximum / sum over each eight neighbouring lanes; every lane gets it
+__device__ __forceinline__ float oct_max(float v) {
+  v = fmaxf(v, dpp_f<0xB1>(v));
+  v = fmaxf(v, dpp_f<0x4E>(v));
+  return fmaxf(v, dpp_f<0x141>(v));
+}
+__device__ __forceinline__ float oct_sum(float v) {
+  v += dpp_f<0xB1>(v);
+  v += dpp_f<0x4E>(v);
+  return v + dpp_f<0x141>(v);
+}
+
+// lane i's value of the wave's 64 sorted from the largest (a bitonic network; K: sorted runs, J: distance)
+template <int K, int J>
+__device__ __forceinline__ float sort_step(float v) {
+  const int l = threadIdx.x & 63;
+  const float o = lane_xor<J>(v);
+  const bool up = ((l & K) == 0) == ((l & J) == 0);  // this lane keeps the larger
+  v = up ? fmaxf(v, o) : fminf(v, o);
+  if constexpr (J > 1) return sort_step<K, J / 2>(v);
+  else if constexpr (K < 64) return sort_step<K * 2, K>(v);
+  else return v;
+}
+__device__ __forceinline__ float wave_sort(float v) { return sort_step<2, 1>(v); }
+
+// The row is read once, by groups of eight lanes' vectors (32 f32 or 64 16-bit logits, contiguous):
+// of each group its maximum and the sum of exp((z - maximum) / T) are kept.  The k largest logits lie
+// in the k groups of the largest maxima, so rtq_top_pick_* reads only those again; every other group
+// enters the rest as a whole, so that nothing is subtracted.  A group that holds a NaN has maximum NaN.
+//
+// grid (chunks / 4, n), a wave per chunk of 64 groups: kTopU vectors a lane, all loaded at once
+constexpr int kTopU = 8;
+
+template <int VT>
+__device__ __forceinline__ void top_scan(const TopArgs& a) {
+  using R = VRow<VT>;
+  constexpr int E = R::E, C = 64 * E * kTopU;
+  const int l = threadIdx.x & 63, i = blockIdx.y;
+  const int q = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (q * 64 >= a.NG || !row_ok(a, i)) return;
+  const void* row = static_cast<const char*>(a.z) + (int64_t)i * a.ld * R::ES;
+  const float ninf = -__builtin_inff();
+  const int j0 = q * C + l * E;
+  u4v raw[kTopU];
+  if ((q + 1) * C <= a.V) {
+#pragma unroll
+    for (int u = 0; u < kTopU; u++) raw[u] = R::load(row, j0 + u * 64 * E);
+  } else {
+#pragma unroll
+    for (int u = 0; u < kTopU; u++) raw[u] = R::load_upto(row, j0 + u * 64 * E, a.V, ninf);
+  }
+  float gm = ninf, gs = 0.0f;
+#pragma unroll
+  for (int u = 0; u < kTopU; u++) {
+    float m = R::get(raw[u], 0);
+#pragma unroll
+    for (int e = 1; e < E; e++) m = fmaxf(m, R::get(raw[u], e));
+    m = oct_max(m);
+    const float ref = m == ninf ? 0.0f : m;
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; e++) s += __builtin_amdgcn_exp2f((R::get(raw[u], e) - ref) * a.ch);
+    s = oct_sum(s);
+    if (__ballot(s != s)) {  // a NaN, or infinity less itself
+      float bad = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; e++) bad = R::get(raw[u], e) != R::get(raw[u], e) ? 1.0f : bad;
+      if (oct_max(bad) > 0.0f) m = __builtin_nanf("");
+    }
+    gm = (l & 7) == u ? m : gm;
+    gs = (l & 7) == u ? s : gs;
+  }
+  const int64_t o = (int64_t)i * a.NG + q * 64 + (l & 7) * 8 + (l >> 3);
+  a.gm[o] = gm;
+  a.gs[o] = gs;
+}
+
+// the K-th largest of the keys f(0) .. f(N - 1) (0: none; the others differ), eight bits at a time
+template <int B, class F>
+__device__ __forceinline__ uint64_t radix_kth(int N, int K, int* hist, int* out, F&& f) {
+  const int tid = threadIdx.x;
+  uint64_t low = 0, mask = 0;
+  int need = K;
+  for (int sh = 56; sh >= 0; sh -= 8) {
+    for (int b = tid; b < 256; b += B) hist[b] = 0;
+    __syncthreads();
+    for (int p = tid; p < (N + 63) / 64 * 64; p += B) {
+      const uint64_t key = p < N ? f(p) : 0;
+      const bool in = key != 0 && (key & mask) == low;
+      const int d = (int)(key >> sh) & 255;
+      // a wave's equal digits (ties, the index's upper digits) are counted with one atomic
+      const uint64_t m = __ballot(in);
+      if (m == 0) continue;
+      const int lead = __builtin_ctzll(m);
+      if (__ballot(in && d != __shfl(d, lead)) == 0) {
+        if ((tid & 63) == lead) atomicAdd(&hist[d], __popcll(m));
+      } else if (in) {
+        atomicAdd(&hist[d], 1);
       }
     }
-  __syncthreads();
-}
-
-// lane i's value of the wave's 64 sorted from the largest
-__device__ __forceinline__ float wave_sort(float v) {
-  const int l = threadIdx.x & 63;
+    __syncthreads();
+    if (tid < 64) {  // lane l: bins 4 l .. 4 l + 3; the bin where the count from the top reaches `need`
+      int h[4], s = 0;
 #pragma unroll
-  for (int k = 2; k <= 64; k <<= 1)
+      for (int b = 0; b < 4; b++) h[b] = hist[4 * tid + b], s += h[b];
+      int above = s;  // of this lane and all above it
 #pragma unroll
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      const float o = __shfl_xor(v, j);
-      const bool up = ((l & k) == 0) == ((l & j) == 0);  // this lane keeps the larger
-      v = up ? fmaxf(v, o) : fminf(v, o);
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_down(above, d);
+        above += tid + d < 64 ? o : 0;
+      }
+      above -= s;
+#pragma unroll
+      for (int b = 3; b >= 0; b--) {
+        if (above < need && need <= above + h[b]) out[0] = 4 * tid + b, out[1] = above, out[2] = h[b];
+        above += h[b];
+      }
     }
-  return v;
+    __syncthreads();
+    need -= out[1];
+    low |= (uint64_t)out[0] << sh;
+    mask |= (uint64_t)255 << sh;
+    if (out[2] == need) return low;  // the whole bin belongs
+  }
+  return low;
 }
 
-constexpr int kTopB = 1024, kTopW = kTopB / 64, kTopCap = 2048;
-
-// the outputs of a row without logits
-__device__ __forceinline__ void top_none(const TopArgs& a, int i) {
-  for (int s = threadIdx.x; s < a.k; s += kTopB) a.vals[(int64_t)i * a.k + s] = __builtin_nanf(""), a.ids[(int64_t)i * a.k + s] = -1;
-  if (threadIdx.x == 0 && a.rest) a.rest[i] = __builtin_nanf("");
+// (m, s) of a set joined by N others: x[e] with exponential sum w[e] (0: no member)
+template <int N>
+__device__ __forceinline__ void join_rest(float& m, double& s, const float* x, const float* w, const TopArgs& a) {
+  float b = m;
+  bool nan = false;
+#pragma unroll
+  for (int e = 0; e < N; e++) {
+    b = fmaxf(b, w[e] != 0.0f ? x[e] : b);
+    nan |= w[e] != 0.0f && x[e] != x[e];
+  }
+  if (nan) s = (double)__builtin_nanf("");
+  if (b == -__builtin_inff()) return;
+  if (b > m) {
+    s *= (double)__builtin_amdgcn_exp2f((m - b) * a.ch);
+    m = b;
+  }
+  float t = 0.0f;
+#pragma unroll
+  for (int e = 0; e < N; e++) t += w[e] != 0.0f ? w[e] * __builtin_amdgcn_exp2f((x[e] - m) * a.ch) : 0.0f;
+  s += (double)t;
 }
 
-// The k largest of slice g of row i, in order, and (max, sum) of the slice's others.  The slice stays
-// in registers (NV vectors a thread).  A bound below the k-th largest comes from the lanes' maxima:
-// with r = ceil(k / waves), every wave has r maxima at or above its own r-th, so the least of those r-ths
-// has k logits at or above it.  What reaches the bound (about 1.5 to 4 k of them in a row without
-// structure) is gathered and sorted.  Where more than kTopCap reach it (ties, masks, sorted rows), the
-// bound is found digit by digit over the whole keys instead.
-template <int VT, int NV>
-__device__ __forceinline__ void top_slice(const TopArgs& a) {
+// grid n: row i's k largest logits and the rest's log-sum-exp, from its groups.  A bound
+// below the k-th largest comes from the threads' maxima over the groups: with r = ceil(k / waves),
+// every wave has r at or above its own r-th, so the least of those r-ths has k logits at or above
+// it.  The groups that reach it (1.5 to 4 k of them in a row without structure) are read again, and what
+// reaches it there is ranked by counting.  Where too many do, a second bound comes from the
+// logits of those groups; where that does not help either (ties, masks, sorted rows), exactly the k
+// groups and then exactly the k logits are found digit by digit.  512 threads: alone on the chip 8.4 us
+// at k = 20 of 151936 f32 logits against 9.5 with 256 and 10.2 with 1024; 1024 rows at k = 128 take 38.8 us
+// against 40.9 and 67.6.
+constexpr int kPickB = 512;
+
+template <int VT>
+__device__ __forceinline__ void top_pick(const TopArgs& a) {
   using R = VRow<VT>;
-  __shared__ uint64_t cand[kTopCap];
-  __shared__ float redf[kTopW];
-  __shared__ double redd[kTopW];
+  constexpr int E = R::E, GS = 8 * E, B = kPickB, W = B / 64, CAP = 4 * B, U = 5120 / B, UE = 4;
+  __shared__ uint64_t cand[CAP];
+  __shared__ uint32_t list[CAP];
+  __shared__ float redf[W];
+  __shared__ double redd[W];
   __shared__ int hist[256];
-  __shared__ int cnt, pick, above;
-  const int tid = threadIdx.x, g = blockIdx.x, i = blockIdx.y;
+  __shared__ int out[3];
+  __shared__ int cnt, groups;
+  const int tid = threadIdx.x, l = tid & 63, i = blockIdx.x;
+  const float ninf = -__builtin_inff(), inf = __builtin_inff();
   if (!row_ok(a, i)) {
-    if (g == 0) top_none(a, i);
+    for (int s = tid; s < a.k; s += B) a.vals[(int64_t)i * a.k + s] = __builtin_nanf(""), a.ids[(int64_t)i * a.k + s] = -1;
+    if (tid == 0 && a.rest) a.rest[i] = __builtin_nanf("");
     return;
   }
   const void* row = static_cast<const char*>(a.z) + (int64_t)i * a.ld * R::ES;
-  const int j0 = g * a.L, j1 = min(a.V, j0 + a.L);  // L <= kTopB * NV * E
-  const float ninf = -__builtin_inff();
-  u4v raw[NV];
-#pragma unroll
-  for (int q = 0; q < NV; q++) {
-    const int j = j0 + (q * kTopB + tid) * R::E;
-    float f[R::E];
-#pragma unroll
-    for (int e = 0; e < R::E; e++) f[e] = ninf;
-    raw[q] = j < j1 ? R::load_upto(row, j, j1, ninf) : R::pack(f);
-  }
-  float lm = ninf;
-#pragma unroll
-  for (int q = 0; q < NV; q++)
-#pragma unroll
-    for (int e = 0; e < R::E; e++) lm = fmaxf(lm, R::get(raw[q], e));
-  if (tid == 0) cnt = 0;
-  const int r = (a.k + kTopW - 1) / kTopW;
-  const float ws = wave_sort(lm);
-  if ((tid & 63) == r - 1) redf[tid >> 6] = ws;
-  __syncthreads();
-  float thr = redf[0];
-#pragma unroll
-  for (int w = 1; w < kTopW; w++) thr = fminf(thr, redf[w]);
-  __syncthreads();
-  // gather what is not below the bound (NaN is not); an index at or past j1 is padding
-  float nm = ninf;
-  auto gather = [&](auto&& in) {
-    nm = ninf;
-#pragma unroll
-    for (int q = 0; q < NV; q++)
-#pragma unroll
-      for (int e = 0; e < R::E; e++) {
-        const int j = j0 + (q * kTopB + tid) * R::E + e;
-        const float x = R::get(raw[q], e);
-        const bool c = j < j1 && in(x, j);
-        if (!c) nm = fmaxf(nm, x);
-        const uint64_t m = __ballot(c);
-        if (m) {
-          int at = 0;
-          if ((tid & 63) == __builtin_ctzll(m)) at = atomicAdd(&cnt, __popcll(m));
-          at = __shfl(at, __builtin_ctzll(m)) + __popcll(m & ((1ull << (tid & 63)) - 1));
-          if (c && at < kTopCap) cand[at] = rank_key(x, j);
-        }
-      }
+  const float* gm = a.gm + (int64_t)i * a.NG;
+  const float* gs = a.gs + (int64_t)i * a.NG;
+  const int held = (a.V + GS - 1) / GS;  // groups with a logit
+  // the least over the first n / 64 waves (those whose lanes all have a maximum) of their r-ths
+  auto bound = [&](float lm, int n) {
+    const int full = min(W, n / 64), r = full ? (a.k + full - 1) / full : 65;
+    const float ws = wave_sort(lm);
+    if (l == r - 1) redf[tid >> 6] = ws;
+    __syncthreads();
+    float t = r > 64 ? ninf : redf[0];
+    for (int w = 1; w < full; w++) t = r > 64 ? ninf : fminf(t, redf[w]);
+    return t;
   };
-  gather([&](float x, int) { return !(x < thr); });
+  if (tid == 0) cnt = 0, groups = 0;
+  // the first U B groups stay in registers (V up to 163840 f32 or 327680 16-bit logits: all of them)
+  float m0[U], s0[U];
+  auto load_groups = [&](int g0, float* m, float* s) {
+#pragma unroll
+    for (int u = 0; u < U; u++) m[u] = g0 + u * B < held ? gm[g0 + u * B] : ninf;
+#pragma unroll
+    for (int u = 0; u < U; u++) s[u] = g0 + u * B < held && a.rest ? gs[g0 + u * B] : 0.0f;
+  };
+  auto largest = [&](const float* m) {
+    float x = ninf;
+#pragma unroll
+    for (int u = 0; u < U; u++) x = fmaxf(x, m[u] != m[u] ? inf : m[u]);
+    return x;
+  };
+  load_groups(tid, m0, s0);
+  float lm = largest(m0);
+  for (int g0 = tid + U * B; g0 < held; g0 += U * B) {
+    float m[U], s[U];
+    load_groups(g0, m, s);
+    lm = fmaxf(lm, largest(m));
+  }
+  float thr = bound(lm, held);
+  float rm = ninf;
+  double rs = 0.0;
+  // the groups in(m, g) takes go to the list, the others to the rest
+  auto choose = [&](bool kept, auto&& in) {
+    auto some = [&](int g0, const float* m, const float* s) {
+      float w[U];
+      uint32_t bits = 0;
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const bool c = g0 + u * B < held && in(m[u], g0 + u * B);
+        bits |= c ? 1u << u : 0u;
+        w[u] = c ? 0.0f : s[u];
+      }
+      if (bits) {
+        int at = atomicAdd(&groups, __popc(bits));
+        for (; bits; bits &= bits - 1, at++)
+          if (at < CAP) list[at] = (uint32_t)(g0 + (__ffs(bits) - 1) * B);
+      }
+      if (a.rest) join_rest<U>(rm, rs, m, w, a);
+    };
+    if (kept) some(tid, m0, s0);
+    for (int g0 = tid + (kept ? U * B : 0); g0 < held; g0 += U * B) {
+      float m[U], s[U];
+      load_groups(g0, m, s);
+      some(g0, m, s);
+    }
+  };
+  choose(true, [&](float m, int) { return !(m < thr); });
   __syncthreads();
-  int n = cnt;
-  uint64_t low = 0;
-  const bool many = n > kTopCap;
-  if (many) {
-    uint64_t mask = 0;
-    int need = a.k;
-    for (int sh = 56; sh >= 0; sh -= 8) {
-      for (int b = tid; b < 256; b += kTopB) hist[b] = 0;
-      __syncthreads();
+  // the listed groups' logits, UE vectors at a time: f(vector, index of its first); past the list's end
+  // the index is V
+  auto each = [&](auto&& f) {
+    const int n = groups * 8;
+    for (int p0 = tid; p0 < n; p0 += B * UE) {
+      u4v v[UE];
+      int j[UE];
 #pragma unroll
-      for (int q = 0; q < NV; q++)
+      for (int u = 0; u < UE; u++) {
+        const int p = p0 + u * B;
+        j[u] = p < n ? (int)list[p >> 3] * GS + (p & 7) * E : a.V;
+      }
 #pragma unroll
-        for (int e = 0; e < R::E; e++) {
-          const int j = j0 + (q * kTopB + tid) * R::E + e;
-          const uint64_t key = rank_key(R::get(raw[q], e), j);
-          const bool in = j < j1 && (key & mask) == low;
-          const int d = (int)(key >> sh) & 255;
-          // equal digits of a wave (ties, the index's upper digits) are counted with one atomic
-          const uint64_t m = __ballot(in);
-          if (m) {
-            const int first = __shfl(d, __builtin_ctzll(m));
-            if (__ballot(in && d != first) == 0) {
-              if ((tid & 63) == __builtin_ctzll(m)) atomicAdd(&hist[d], __popcll(m));
-            } else if (in) {
-              atomicAdd(&hist[d], 1);
-            }
+      for (int u = 0; u < UE; u++) {
+        v[u] = u4v{0, 0, 0, 0};
+        if (j[u] < a.V) v[u] = R::load_upto(row, j[u], a.V, ninf);
+      }
+#pragma unroll
+      for (int u = 0; u < UE; u++)
+        if (j[u] < a.V) f(v[u], j[u]);
+    }
+  };
+  // the logits that in(x, index) takes are the candidates, the others go to the rest
+  auto collect = [&](auto&& in) {
+    each([&](const u4v& v, int j) {
+      float x[E], w[E];
+      uint32_t bits = 0;
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        x[e] = R::get(v, e);
+        const bool c = j + e < a.V && in(x[e], j + e);
+        bits |= c ? 1u << e : 0u;
+        w[e] = j + e < a.V && !c ? 1.0f : 0.0f;
+      }
+      if (bits) {
+        int at = atomicAdd(&cnt, __popc(bits));
+#pragma unroll
+        for (int e = 0; e < E; e++)
+          if ((bits >> e) & 1) {
+            if (at < CAP) cand[at] = rank_key(x[e], j + e);
+            at++;
           }
-        }
-      __syncthreads();
-      if (tid == 0) {
-        int s = 0, b = 255;
-        while (b > 0 && s + hist[b] < need) s += hist[b--];
-        pick = b, above = s;
       }
-      __syncthreads();
-      const int inbin = hist[pick];
-      need -= above;
-      low |= (uint64_t)pick << sh;
-      mask |= (uint64_t)255 << sh;
-      const bool done = a.k - need + inbin <= kTopCap;
-      __syncthreads();
-      if (done) break;
-    }
-    if (tid == 0) cnt = 0;
+      if (a.rest) join_rest<E>(rm, rs, x, w, a);
+    });
     __syncthreads();
-    gather([&](float x, int j) { return rank_key(x, j) >= low; });
+  };
+  const float gm_rest = rm;
+  const double gs_rest = rs;
+  bool many = groups > CAP;
+  if (!many) {
+    collect([&](float x, int) { return !(x < thr); });
+    if (cnt > CAP) {
+      float em = ninf;
+      each([&](const u4v& v, int j) {
+#pragma unroll
+        for (int e = 0; e < E; e++) em = j + e < a.V ? fmaxf(em, R::get(v, e) != R::get(v, e) ? inf : R::get(v, e)) : em;
+      });
+      thr = fmaxf(thr, bound(em, groups * 8));
+      if (tid == 0) cnt = 0;
+      __syncthreads();
+      rm = gm_rest, rs = gs_rest;
+      collect([&](float x, int) { return !(x < thr); });
+    }
+    many = cnt > CAP;
+  }
+  if (many) {
+    auto group_key = [&](float m, int g) { return rank_key(m, g); };
+    const uint64_t gk = radix_kth<B>(held, min(a.k, held), hist, out, [&](int g) { return group_key(gm[g], g); });
     __syncthreads();
-    n = cnt;
+    if (tid == 0) cnt = 0, groups = 0;
+    __syncthreads();
+    rm = ninf, rs = 0.0;
+    choose(false, [&](float m, int g) { return group_key(m, g) >= gk; });  // min(k, held) of them
+    __syncthreads();
+    const uint64_t ek = radix_kth<B>(groups * GS, a.k, hist, out, [&](int p) {
+      const int j = (int)list[p / GS] * GS + p % GS;
+      return j < a.V ? rank_key(R::one(row, j), j) : 0ull;
+    });
+    collect([&](float x, int j) { return rank_key(x, j) >= ek; });  // k of them
   }
-  // others: the maximum and the sum of what was not gathered, then the gathered beyond the k-th
-  nm = group_max<kTopW>(nm, redf);
-  double ns = 0.0;
-  if (nm != ninf && (a.rest || a.G > 1)) {
-#pragma unroll
-    for (int q = 0; q < NV; q++) {
-      float s = 0.0f;
-#pragma unroll
-      for (int e = 0; e < R::E; e++) {
-        const int j = j0 + (q * kTopB + tid) * R::E + e;
-        const float x = R::get(raw[q], e);
-        const bool c = j >= j1 || (many ? rank_key(x, j) >= low : !(x < thr));
-        s += c ? 0.0f : exp_scaled(x - nm, a.ch, a.cl);
-      }
-      ns += (double)s;
-    }
-  }
-  ns = group_sum<kTopW>(ns, redd);
-  int P = 2;
-  while (P < n || P < a.k) P <<= 1;
-  for (int p = n + tid; p < P; p += kTopB) cand[p] = 0;
-  sort_keys<kTopB>(cand, P);
-  const double invt = 1.0 / (double)a.temp;
-  const float cm = a.k < n ? key_value(cand[a.k]) : ninf;
-  double cs = 0.0;
-  for (int p = a.k + tid; p < n; p += kTopB) cs += cm == ninf ? 0.0 : exp(((double)key_value(cand[p]) - cm) * invt);
-  cs = group_sum<kTopW>(cs, redd);
-  join_sums(nm, ns, cm, cs, invt);
-  if (a.G > 1) {
-    for (int s = tid; s < a.k; s += kTopB) a.lists[((int64_t)i * a.G + g) * a.k + s] = cand[s];
-    if (tid == 0) a.pm[(int64_t)i * a.G + g] = nm, a.ps[(int64_t)i * a.G + g] = ns;
-    return;
-  }
-  for (int s = tid; s < a.k; s += kTopB) {
-    a.vals[(int64_t)i * a.k + s] = key_value(cand[s]);
-    a.ids[(int64_t)i * a.k + s] = key_index(cand[s]);
-  }
-  if (tid == 0 && a.rest) a.rest[i] = lse_of(nm, ns, invt);
-}
-
-// row i's k largest of its G slices' sorted lists (lists[g][s], 0 where a slice has fewer), by the
-// same bound: the least of the lists' r-ths, r = ceil(k / G), or the largest of their k-ths
-extern "C" __global__ __launch_bounds__(kTopB) void rtq_top_merge(TopArgs a) {
-  extern __shared__ uint64_t mkeys[];  // G * k rounded up to a power of two
-  __shared__ float redf[kTopW];
-  __shared__ double redd[kTopW];
-  __shared__ int cnt;
-  __shared__ uint64_t bound;
-  const int tid = threadIdx.x, i = blockIdx.x, r = (a.k + a.G - 1) / a.G, total = a.G * a.k;
-  const uint64_t* L = a.lists + (int64_t)i * total;
-  if (!row_ok(a, i)) return;  // written by slice 0
-  if (tid < 64) {
-    uint64_t lo = ~0ull, hi = 0;
-    for (int g = tid; g < a.G; g += 64) {
-      const uint64_t x = L[g * a.k + r - 1], y = L[g * a.k + a.k - 1];
-      lo = x < lo ? x : lo, hi = y > hi ? y : hi;
-    }
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-      const uint64_t x = __shfl_xor(lo, m), y = __shfl_xor(hi, m);
-      lo = x < lo ? x : lo, hi = y > hi ? y : hi;
-    }
-    if (tid == 0) bound = hi > lo ? hi : lo, cnt = 0;
-  }
+  // each candidate's place is the number of larger ones
+  const int n = cnt, n8 = (n + 7) & ~7;
+  if (tid < n8 - n) cand[n + tid] = 0;
   __syncthreads();
-  const uint64_t low = bound > 1 ? bound : 1;
-  for (int p = tid; p < total; p += kTopB) {
-    const uint64_t key = L[p];
-    if (key >= low) mkeys[atomicAdd(&cnt, 1)] = key;
-  }
-  __syncthreads();
-  const int n = cnt;
-  int P = 2;
-  while (P < n || P < a.k) P <<= 1;
-  for (int p = n + tid; p < P; p += kTopB) mkeys[p] = 0;
-  sort_keys<kTopB>(mkeys, P);
-  for (int s = tid; s < a.k; s += kTopB) {
-    a.vals[(int64_t)i * a.k + s] = key_value(mkeys[s]);
-    a.ids[(int64_t)i * a.k + s] = key_index(mkeys[s]);
+  for (int p = tid; p < n; p += B) {
+    const uint64_t key = cand[p];
+    int place = 0;
+    for (int q = 0; q < n8; q += 8)
+#pragma unroll
+      for (int e = 0; e < 8; e++) place += cand[q + e] > key;
+    if (place < a.k) {
+      a.vals[(int64_t)i * a.k + place] = key_value(key);
+      a.ids[(int64_t)i * a.k + place] = key_index(key);
+    } else if (a.rest) {
+      const float x = key_value(key), w = 1.0f;
+      join_rest<1>(rm, rs, &x, &w, a);
+    }
   }
   if (!a.rest) return;
-  // the others: the slices' own, and every list entry after the k-th
-  const double invt = 1.0 / (double)a.temp;
-  const uint64_t kth = mkeys[a.k - 1];
-  float m = -__builtin_inff();
-  bool nan = false;
-  for (int p = tid; p < total; p += kTopB) {
-    const uint64_t key = L[p];
-    if (key == 0 || key >= kth) continue;
-    m = fmaxf(m, key_value(key));
-    nan |= key_value(key) != key_value(key);
-  }
-  for (int g = tid; g < a.G; g += kTopB) m = fmaxf(m, a.pm[(int64_t)i * a.G + g]);
-  m = group_max<kTopW>(m, redf);
-  double s = nan ? (double)__builtin_nanf("") : 0.0;
-  if (m != -__builtin_inff()) {
-    for (int p = tid; p < total; p += kTopB) {
-      const uint64_t key = L[p];
-      if (key != 0 && key < kth) s += exp(((double)key_value(key) - m) * invt);
-    }
-    for (int g = tid; g < a.G; g += kTopB) {
-      const float pm = a.pm[(int64_t)i * a.G + g];
-      if (pm != -__builtin_inff()) s += a.ps[(int64_t)i * a.G + g] * exp(((double)pm - m) * invt);
-    }
-  }
-  s = group_sum<kTopW>(s, redd);
-  if (tid == 0) a.rest[i] = s != s && m != __builtin_inff() ? __builtin_nanf("") : lse_of(m, s, invt);
+  const float m = group_max<W>(rm, redf);
+  rs = group_sum<W>(rm == ninf ? rs : rs * (double)__builtin_amdgcn_exp2f((rm - m) * a.ch), redd);
+  if (tid == 0) a.rest[i] = lse_of(m, rs, 1.0 / (double)a.temp);
 }
 
-#define RTQ_TOP(name, VT, NV) \
-  extern "C" __global__ __launch_bounds__(kTopB) void name(TopArgs a) { top_slice<VT, NV>(a); }
-RTQ_TOP(rtq_top_f32_s, VT_F32, 2)
-RTQ_TOP(rtq_top_f16_s, VT_F16, 2)
-RTQ_TOP(rtq_top_bf16_s, VT_BF16, 2)
-RTQ_TOP(rtq_top_f32_l, VT_F32, 8)
-RTQ_TOP(rtq_top_f16_l, VT_F16, 4)
-RTQ_TOP(rtq_top_bf16_l, VT_BF16, 4)
+#define RTQ_TOP(ty, VT)                                                                                    \
+  extern "C" __global__ __launch_bounds__(256) void rtq_top_scan_##ty(TopArgs a) { top_scan<VT>(a); }      \
+  extern "C" __global__ __launch_bounds__(kPickB, 4) void rtq_top_pick_##ty(TopArgs a) { top_pick<VT>(a); }
+RTQ_TOP(f32, VT_F32)
+RTQ_TOP(f16, VT_F16)
+RTQ_TOP(bf16, VT_BF16)
 
 // ============================================================== distillation
 // Row i: the teacher's distribution p over its listed tokens and the rest (one bucket), the student's
