@@ -355,6 +355,9 @@ struct HeadArgs {
 // ---------------------------------------------------------------- rows of vocabulary logits
 // z: rows of V logits (f32, f16 or bf16), stride ld elements; where a row is cut, into G slices of L
 // logits.  ch + cl = log2(e) / temp.
+#ifndef RTQ_TOP_MAX
+#define RTQ_TOP_MAX 256 /* as in rtq.h */
+#endif
 struct TopArgs {
   const void* z;
   int64_t ld;

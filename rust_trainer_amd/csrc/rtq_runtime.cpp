@@ -167,7 +167,8 @@ enum Kid {
   K_ACT_PREP4,   // the same on 4-token tiles
   K_TOP_SCAN,    // + type (f32, f16, bf16)
   K_TOP_PICK = K_TOP_SCAN + 3,
-  K_DISTILL_STATS = K_TOP_PICK + 3,
+  K_DISTILL = K_TOP_PICK + 3,  // + type + 3 * (256, 512, 1024 threads): a row a workgroup
+  K_DISTILL_STATS = K_DISTILL + 9,
   K_DISTILL_GRAD = K_DISTILL_STATS + 3,
   K_VERIFY_STATS = K_DISTILL_GRAD + 3,
   K_VERIFY_ACCEPT = K_VERIFY_STATS + 3,
@@ -206,6 +207,8 @@ constexpr const char* kKernelNames[] = {
     "rtq_head_norm_bwd",    "rtq_act_prep8_q8_0",   "rtq_act_prep4_q8_0",
     "rtq_top_scan_f32",     "rtq_top_scan_f16",     "rtq_top_scan_bf16",
     "rtq_top_pick_f32",     "rtq_top_pick_f16",     "rtq_top_pick_bf16",
+    "rtq_distill256_f32",   "rtq_distill256_f16",   "rtq_distill256_bf16",  "rtq_distill512_f32",   "rtq_distill512_f16",
+    "rtq_distill512_bf16",  "rtq_distill1024_f32",  "rtq_distill1024_f16",  "rtq_distill1024_bf16",
     "rtq_distill_stats_f32", "rtq_distill_stats_f16", "rtq_distill_stats_bf16",
     "rtq_distill_grad_f32", "rtq_distill_grad_f16", "rtq_distill_grad_bf16",
     "rtq_verify_stats_f32", "rtq_verify_stats_f16", "rtq_verify_stats_bf16",
@@ -270,6 +273,8 @@ struct rtq_ctx {
   int gemvq_wpc = 0;  // its waves per CU (RTQ_GEMVQ_WPC; 0: automatic)
   int fwd_i8 = -1;    // int8-MFMA forwards (rtq_mmi8_*; RTQ_FWD_I8): -1 automatic, 0 never,
                       // 1 every Q4_0 / Q8_0 weight, wherever the 128- or 64-token tiles are chosen
+  int distill_rows = -2;  // distillation: -2 automatic, -1 slices, 0 / 1 / 2 a row a workgroup of 256 / 512 / 1024
+                          // threads (RTQ_DISTILL_ROWS)
   int64_t t_launches[K_COUNT] = {};
   double t_ms[K_COUNT] = {};
   double t_flops[K_COUNT] = {}, t_bytes[K_COUNT] = {};
@@ -1430,6 +1435,7 @@ rtq_status rtq_ctx_create(int device, rtq_ctx** out) {
   if (const char* e = getenv("RTQ_GEMVQ_WPC")) c->gemvq_wpc = std::min(std::max(atoi(e), 0), 32);
   if (const char* e = getenv("RTQ_FWD_RG")) c->fwd_rg = std::min(std::max(atoi(e), 1), 3);
   if (const char* e = getenv("RTQ_ACT_TT")) c->act_tt = atoi(e) <= 4 ? 4 : atoi(e) <= 8 ? 8 : 16;
+  if (const char* e = getenv("RTQ_DISTILL_ROWS")) c->distill_rows = std::min(std::max(atoi(e), -2), 2);
   if (const char* e = getenv("RTQ_G64_MIN")) c->g64_min = atoi(e);
   hipError_t e = hipModuleLoadData(&c->mod, rtq_hsaco_begin);
   if (e != hipSuccess) {
@@ -1950,13 +1956,39 @@ rtq_status enqueue_top(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V
 
 // ---- distillation
 struct DistillPlan {
+  int rows;  // a row a workgroup of 256 << rows threads; -1: slices
   int64_t G, L;
   size_t bytes;
 };
 
-DistillPlan distill_plan(int64_t n, int64_t V, int64_t k) {
+constexpr int64_t kLdsBytes = 160 << 10;          // of a CU, for one workgroup
+constexpr int64_t kDistillStaticLds = 9 << 10;  // at least rtq_distill*_*'s own (the lists of 256 slots)
+// their dynamic LDS: 8 vectors for each thread but the first wave's, a bit per logit
+int64_t distill_lds(int rows, int64_t V) { return ((256 << rows) - 64) * 8 * 16 + (V / 32 + 1) * 4; }
+
+// Which kernels, by times in us fitted to a sweep (V 2048 to 151936, 1 to 2048 rows, both types, with and without
+// a gradient).  A row a workgroup takes about 8 us and 0.2 ns a logit (0.12 without the gradient), whatever the
+// number of rows up to the CUs'; slices of all rows at once take two launches, 14 us, and 2.3 ns a thousand f32
+// logits (1.15 of 16 bits; without the gradient 0.65 and 0.48).  So slices run few rows of a large vocabulary
+// (151936 f32, 16 rows: 17 us against 40; 256 rows: 103 against 68), and many such rows without a gradient (1024:
+// 118 against 134).
+// Of the workgroup sizes, each holds 24 vectors of 16 bytes a thread on the chip.  256 threads let four rows
+// share a CU, 512 two: better where they hold the row and there are enough (8192 f32, 2048 rows: 37 / 44 / 66
+// us; 64000 bf16, 512 rows: 50 / 43 / 48), while one row alone is fastest on the largest that it fills (32000
+// f32: 25 / 15 / 13).
+DistillPlan distill_plan(const rtq_ctx* c, int type, int64_t n, int64_t V, int64_t k, bool grad) {
+  const int64_t E = 16 / logit_bytes(type), cus = c->cu_count;
   DistillPlan p{};
-  p.L = 8192;
+  if (V <= 24 * 192 * E) p.rows = n > 2 * cus ? 0 : 1;
+  else p.rows = n > cus && V <= 36 * 448 * E ? 1 : 2;
+  const double v = (double)V, all = v * (double)n, more = n > cus ? (double)n / (double)cus : 1.0;
+  const double one = 7.5 + more * v * (grad ? 0.2e-3 : n > cus ? 0.2e-3 : 0.12e-3);
+  const double cut = grad ? 14.0 + all * (E == 4 ? 2.3e-6 : 1.15e-6) : 12.5 + all * (E == 4 ? 0.65e-6 : 0.48e-6);
+  if (p.rows == 2 && cut < one && (n <= cus || !grad)) p.rows = -1;
+  if (c->distill_rows >= -1) p.rows = c->distill_rows;
+  if (p.rows >= 0 && distill_lds(p.rows, V) + kDistillStaticLds > kLdsBytes) p.rows = -1;  // a bit per logit does not fit
+  if (p.rows >= 0) return p;
+  p.L = 8 * 256 * E;
   p.G = cdiv(V, p.L);
   p.bytes = (size_t)(n * p.G) * 24 + (size_t)(n * k + n) * 4 + 8 * 256;
   return p;
@@ -1999,6 +2031,9 @@ rtq_status enqueue_distill(rtq_ctx* c, const void* z, int type, int64_t n, int64
   a.temp = t.temperature;
   exp_scale(t.temperature, &a.ch, &a.cl);
   a.hard = hard, a.ids = t.ids, a.tv = t.vals, a.rest = t.rest, a.tok = tok, a.w = w, a.kl = kl, a.logp = logp;
+  const int ty = logit_type(type);
+  if (p.rows >= 0)
+    return launch(c, K_DISTILL + ty + 3 * p.rows, dim3((unsigned)n), dim3(256u << p.rows), st, a, (unsigned)distill_lds(p.rows, V));
   a.psT = ar.take<double>((size_t)(n * p.G));
   a.ps1 = ar.take<double>((size_t)(n * p.G));
   a.pm = ar.take<float>((size_t)(n * p.G));
@@ -2007,8 +2042,8 @@ rtq_status enqueue_distill(rtq_ctx* c, const void* z, int type, int64_t n, int64
   a.zt = ar.take<float>((size_t)n);
   if (ar.off > ar.cap) return fail(RTQ_ERR_INVALID, "internal: workspace too small");
   const dim3 grid((unsigned)p.G, (unsigned)n);
-  RTQ_TRY(launch(c, K_DISTILL_STATS + logit_type(type), grid, dim3(256), st, a, (unsigned)(p.L / 8)));
-  return launch(c, K_DISTILL_GRAD + logit_type(type), w ? grid : dim3(1, (unsigned)n), dim3(256), st, a);
+  RTQ_TRY(launch(c, K_DISTILL_STATS + ty, grid, dim3(320), st, a));
+  return launch(c, K_DISTILL_GRAD + ty, w ? grid : dim3(1, (unsigned)n), dim3(320), st, a);
 }
 
 // ---- drafted tokens
@@ -2084,7 +2119,7 @@ rtq_status rtq_distill_d(rtq_ctx* c, const void* z, int type, int64_t n, int64_t
   std::lock_guard<std::mutex> lk(c->mu);
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = (hipStream_t)stream;
-  const DistillPlan p = distill_plan(n, V, t->k);
+  const DistillPlan p = distill_plan(c, type, n, V, t->k, w != nullptr);
   RTQ_TRY(row_ws(c, p.bytes, st));
   Arena ar{(char*)c->ws, c->ws_bytes, 0};
   return enqueue_distill(c, z, type, n, V, ld, *t, tok, w, hard, kl, logp, dz, ldd, p, ar, st);
@@ -2221,7 +2256,7 @@ rtq_status rtq_lm_distill_d(rtq_ctx* c, const rtq_weight* w, const float* norm, 
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = (hipStream_t)stream;
   if (n == 0) return weights && dx && t > 0 ? fill_zero(c, dx, t * w->cols, st) : RTQ_OK;
-  const DistillPlan p = distill_plan(n, w->rows, teacher->k);
+  const DistillPlan p = distill_plan(c, RTQ_TYPE_F32, n, w->rows, teacher->k, weights != nullptr);
   RTQ_TRY(row_ws(c, lm_bytes(c, w, n, weights != nullptr, p.bytes), st));
   Arena ar{(char*)c->ws, c->ws_bytes, 0};
   return enqueue_lm_distill(c, w, norm, eps, offset, x, t, pos, tok, weights, n, *teacher, hard, kl, logp, dx, p, ar, st);
@@ -2504,7 +2539,7 @@ rtq_status rtq_distill(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V
   HostCall hc(c);
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = c->stream;
-  const DistillPlan p = distill_plan(n, V, t->k);
+  const DistillPlan p = distill_plan(c, type, n, V, t->k, w != nullptr);
   const int64_t es = logit_bytes(type), k = t->k;
   RTQ_TRY(ensure_ws(c, p.bytes + (size_t)(n * V * es + n * (8 * k + 20)) + 8 * 256));
   Arena ar{(char*)c->ws, c->ws_bytes, 0};
@@ -2617,7 +2652,7 @@ rtq_status rtq_lm_distill(rtq_ctx* c, const rtq_weight* w, const float* norm, fl
   HostCall hc(c);
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = c->stream;
-  const DistillPlan p = distill_plan(n, w->rows, teacher->k);
+  const DistillPlan p = distill_plan(c, RTQ_TYPE_F32, n, w->rows, teacher->k, weights != nullptr);
   const int64_t k = teacher->k;
   RTQ_TRY(ensure_ws(c, lm_bytes(c, w, n, weights != nullptr, p.bytes) + (size_t)(2 * t * d + d + n * (2 * k + 6)) * 4 + 11 * 256));
   Arena ar{(char*)c->ws, c->ws_bytes, 0};

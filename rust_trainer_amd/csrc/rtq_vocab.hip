@@ -33,6 +33,11 @@ struct VRow {
     else if constexpr (VT == VT_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)(u >> (16 * (e & 1))));
     else return __builtin_bit_cast(float, (e & 1) ? (u & 0xffff0000u) : (u << 16));
   }
+  __device__ static __forceinline__ float get_at(const u4v& r, int e) {  // e not known to the compiler
+    const int d = VT == VT_F32 ? e : e >> 1;
+    const uint32_t u = d == 0 ? r[0] : d == 1 ? r[1] : d == 2 ? r[2] : r[3];
+    return get(u4v{u, u, u, u}, VT == VT_F32 ? 0 : e & 1);
+  }
   __device__ static __forceinline__ u4v pack(const float* v) {
     u4v r;
     if constexpr (VT == VT_F32) {
@@ -59,13 +64,22 @@ struct VRow {
   __device__ static __forceinline__ void store(void* row, int64_t j, const u4v& r) {
     *reinterpret_cast<u4u*>(static_cast<char*>(row) + j * ES) = r;
   }
-  // elements j .. j + E - 1 of a row of V; those past its end read as `fill`
-  __device__ static __forceinline__ u4v load_upto(const void* row, int64_t j, int64_t V, float fill) {
+  // elements j .. j + E - 1 of a row of V; those past its end read as -inf (the rare path is kept small: it
+  // stands beside unrolled code)
+  __device__ static __forceinline__ u4v load_upto(const void* row, int64_t j, int64_t V) {
     if (j + E <= V) return load(row, j);
-    float v[E];
+    const uint32_t none = VT == VT_F32 ? 0xff800000u : VT == VT_F16 ? 0xfc00fc00u : 0xff80ff80u;
+    u4v r = {none, none, none, none};
+#pragma unroll 1
+    for (int e = 0; j + e < V; e++) {
+      const int d = VT == VT_F32 ? e : e >> 1, sh = VT == VT_F32 ? 0 : 16 * (e & 1);
+      uint32_t u, keep = 0;
+      if constexpr (VT == VT_F32) u = static_cast<const uint32_t*>(row)[j + e];
+      else u = (uint32_t) static_cast<const uint16_t*>(row)[j + e] << sh, keep = 0xffff0000u >> sh;
 #pragma unroll
-    for (int e = 0; e < E; e++) v[e] = j + e < V ? one(row, j + e) : fill;
-    return pack(v);
+      for (int w = 0; w < 4; w++) r[w] = d == w ? (r[w] & keep) | u : r[w];
+    }
+    return r;
   }
 };
 
@@ -100,6 +114,13 @@ __device__ __forceinline__ double lane_xor(double v) {
   const uint32_t lo = __builtin_bit_cast(uint32_t, lane_xor<J>(__builtin_bit_cast(float, (uint32_t)u)));
   const uint32_t hi = __builtin_bit_cast(uint32_t, lane_xor<J>(__builtin_bit_cast(float, (uint32_t)(u >> 32))));
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// a barrier that orders LDS alone: loads and stores of memory stay in flight across it
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 template <class T>
@@ -214,7 +235,7 @@ __device__ __forceinline__ void top_scan(const TopArgs& a) {
     for (int u = 0; u < kTopU; u++) raw[u] = R::load(row, j0 + u * 64 * E);
   } else {
 #pragma unroll
-    for (int u = 0; u < kTopU; u++) raw[u] = R::load_upto(row, j0 + u * 64 * E, a.V, ninf);
+    for (int u = 0; u < kTopU; u++) raw[u] = R::load_upto(row, j0 + u * 64 * E, a.V);
   }
   float gm = ninf, gs = 0.0f;
 #pragma unroll
@@ -424,7 +445,7 @@ __device__ __forceinline__ void top_pick(const TopArgs& a) {
 #pragma unroll
       for (int u = 0; u < UE; u++) {
         v[u] = u4v{0, 0, 0, 0};
-        if (j[u] < a.V) v[u] = R::load_upto(row, j[u], a.V, ninf);
+        if (j[u] < a.V) v[u] = R::load_upto(row, j[u], a.V);
       }
 #pragma unroll
       for (int u = 0; u < UE; u++)
@@ -523,199 +544,602 @@ RTQ_TOP(bf16, VT_BF16)
 
 // ============================================================== distillation
 // Row i: the teacher's distribution p over its listed tokens and the rest (one bucket), the student's
-// q = softmax(z / T) over the same buckets.  The unlisted logits have their own maximum m and sums
-// sT = sum exp((z - m) / T), s1 = sum exp(z - m), so the rest's probability is no difference of two
-// sums.  Gradient at an unlisted token: C exp((z - m) / T) + D exp(z - m) with one C and D a row.
-constexpr int kDisB = 256, kDisW = kDisB / 64;
+// q = softmax(z / T) over the same buckets.  The unlisted logits have their own maximum mu and sums
+// sT = sum exp((z - mu) / T), s1 = sum exp(z - mu), so the rest's probability is no difference of two
+// sums.  Gradient at an unlisted token: C exp((z - mu) / T) + D exp(z - mu) with one C and D a row; the
+// listed tokens and the label are written over it.
+//
+// rtq_distill*_<type>: a row a workgroup, whose first wave does the row's scalars (the teacher's list, the
+// losses, the gradient at the listed tokens) while the others hold their first kDisV vectors a thread in
+// registers and the next kDisL in LDS from the statistics to the gradient: one read and one write of the row
+// (what a longer row has beyond them is read twice).  rtq_distill_stats_* / _grad_* do the two halves for slices of few long rows.
+//
+// Exponentials are exp2(fma(z, c, -K)), one FMA and the instruction: c = log2(e) / T rounded to f32, and a
+// maximum m's reference is f32(m c), so that its rounding cancels between the sums and what is divided by
+// them.  The row's scalars use the same c (the student's temperature is off by 2^-25 of itself at most), in
+// 64 bits.
+constexpr int kDisV = 16, kDisL = 8;
 
-// grid (G, n): the statistics of slice g's unlisted logits; the listed tokens' and the label's logits are
-// kept aside (the gradient may overwrite them)
+struct DisShared {
+  int id[RTQ_TOP_MAX];     // the slots' tokens (-1: empty)
+  float tv[RTQ_TOP_MAX];   // their logits: the teacher's, the student's
+  float zs[RTQ_TOP_MAX];
+  double p[RTQ_TOP_MAX];   // the teacher's probability, and its sum over the slots of the token
+  double pt[RTQ_TOP_MAX];
+  int first[RTQ_TOP_MAX];  // the slot stands for its token
+  float wm[16];            // the waves' maxima and sums
+  double wT[16], w1[16];
+  // the row's scalars: C and D with the unlisted logits' references, log2 of the student's two normalisers
+  float C, D, KT, K1, base;
+  double LT, L1, lu, pr, wgT, wg1;  // lu: log2 of the unlisted sum
+  float zt;
+  int tok, taught;
+};
+
+constexpr float kLog2eF = 1.44269502f;  // the f32 nearest log2(e)
+constexpr double kLn2D = 0.69314718055994530942;
+// a maximum's reference: K = f32(m c) for z c - K, or, where the product could overflow (masks of the type's
+// lowest value), m itself for (z - m) c
+__device__ __forceinline__ bool huge(float m) { return fabsf(m) > 1e30f; }
+__device__ __forceinline__ float ref_base(float m) { return huge(m) && fabsf(m) < __builtin_inff() ? m : 0.0f; }
+__device__ __forceinline__ float ref_of(float m, float c) { return m == -__builtin_inff() || ref_base(m) != 0.0f ? 0.0f : m * c; }
+__device__ __forceinline__ double ref_in(float m, float c) { return (double)ref_base(m) * (double)c + (double)ref_of(m, c); }
+__device__ __forceinline__ float exp_ref(float z, float c, float K) { return __builtin_amdgcn_exp2f(fmaf(z, c, -K)); }
+
+// which logits of a slice are listed: a bit each, and for every wave a bit per vector of its registers that
+// holds one
+template <int ST, int NV, int E>
+struct DisMarks {
+  uint32_t* mask;
+  uint32_t* any;  // [ST / 64]
+  // by all threads; a barrier follows
+  __device__ __forceinline__ void clear(int len) {
+    for (int w = threadIdx.x; w < len / 32 + 1; w += blockDim.x) mask[w] = 0;
+    if (threadIdx.x < ST / 64) any[threadIdx.x] = 0;
+  }
+  __device__ __forceinline__ bool set(int o) {  // whether it was
+    const int v = o / (ST * E);
+    if (v < NV) atomicOr(&any[o % (ST * E) / (64 * E)], 1u << v);
+    const uint32_t bit = 1u << (o & 31);
+    return (atomicOr(&mask[o >> 5], bit) & bit) != 0;
+  }
+  __device__ __forceinline__ bool get(int o) const { return (mask[o >> 5] >> (o & 31)) & 1; }
+  __device__ __forceinline__ uint32_t vec(int o) const { return mask[o >> 5] >> (o & 31); }  // the low E: of vector o / E
+};
+
+// a set of logits: their maximum and their two sums, by the references of that maximum
+struct DisSum {
+  float m = -__builtin_inff();
+  double sT = 0.0, s1 = 0.0;
+  __device__ __forceinline__ void raise(float m2, const DistillArgs& a) {  // to the reference of m2 >= m
+    const bool none = m == -__builtin_inff();  // (a NaN sum stays)
+    sT *= none ? 0.0 : (double)__builtin_amdgcn_exp2f((float)(ref_in(m, a.ch) - ref_in(m2, a.ch)));
+    s1 *= none ? 0.0 : (double)__builtin_amdgcn_exp2f((float)(ref_in(m, kLog2eF) - ref_in(m2, kLog2eF)));
+    m = m2;
+  }
+  // joined over the lanes of a wave; every lane gets it
+  __device__ __forceinline__ void join_wave(const DistillArgs& a) {
+    const float M = wave_max_any(m);
+    if (m != M) raise(M, a);
+    sT = wave_sum_any(sT);
+    s1 = wave_sum_any(s1);
+  }
+};
+
+// A slice [j0, j1) over ST threads (st: 0 .. ST - 1): of the vectors that a whole wave has, the first NV a thread
+// stay in registers and the next NL in LDS; the others are read from memory where they are used.  The code for
+// registers is unrolled, so what is rare goes another way: marked logits become -inf in the registers, and the
+// gradient is written over them afterwards.
+template <int VT, int ST, int NV, int NL>
+struct DisSlice {
+  using R = VRow<VT>;
+  using Marks = DisMarks<ST, NV, R::E>;
+  static constexpr int E = R::E, GV = 2, MV = 4;  // GV: vectors summed together, MV: loaded together from memory
+  static_assert(NV % GV == 0 && MV % GV == 0, "whole groups");
+  u4v raw[NV];
+  u4v* lds;  // [NL][ST]
+  int j0, j1, st, wave, held, kept;  // wave: the wave's first st; its vectors in registers; those and in LDS
+
+  __device__ __forceinline__ void init(int j0_, int j1_, int st_, u4v* lds_) {
+    j0 = j0_, j1 = j1_, st = st_, lds = lds_;
+    wave = __builtin_amdgcn_readfirstlane(st_ & ~63);
+    const int first = (wave + 64) * E, len = j1 - j0;
+    const int full = len >= first ? (len - first) / (ST * E) + 1 : 0;
+    held = min(NV, full);
+    kept = min(NV + NL, full);
+  }
+  __device__ __forceinline__ int place(int v) const { return j0 + (v * ST + st) * E; }
+  __device__ __forceinline__ void load(const void* row) {
+    const void* p = static_cast<const char*>(row) + (int64_t)place(0) * R::ES;
+#pragma unroll
+    for (int v = 0; v < NV; v++)
+      if (v < held) raw[v] = R::load(p, v * ST * E);
+  }
+  // v with its marked elements at -inf
+  __device__ __forceinline__ static u4v unmarked(u4v v, uint32_t bits) {
+#pragma unroll
+    for (int d = 0; d < 4; d++) {
+      const uint32_t none = VT == VT_F32 ? 0xff800000u : VT == VT_F16 ? 0xfc00fc00u : 0xff80ff80u;
+      uint32_t m;
+      if constexpr (VT == VT_F32) m = 0u - ((bits >> d) & 1);
+      else m = ((0u - ((bits >> (2 * d)) & 1)) & 0xffffu) | (0u - ((bits >> (2 * d + 1)) & 1)) << 16;
+      v[d] = (v[d] & ~m) | (none & m);
+    }
+    return v;
+  }
+  __device__ __forceinline__ static void add(DisSum& d, const DistillArgs& a, const u4v* x, bool two) {
+    float f[GV][E], m = d.m;
+#pragma unroll
+    for (int v = 0; v < GV; v++)
+#pragma unroll
+      for (int e = 0; e < E; e++) f[v][e] = R::get(x[v], e), m = fmaxf(m, f[v][e]);
+    const float old = d.m == -__builtin_inff() ? m : d.m;  // without logits so far the reference is m's own
+    const bool odd = __ballot(huge(m) || huge(old)) != 0;
+    if (odd) {
+      const float b = ref_base(m);
+#pragma unroll
+      for (int v = 0; v < GV; v++)
+#pragma unroll
+        for (int e = 0; e < E; e++) f[v][e] -= b;
+    }
+    auto sum = [&](double& s, float c) {
+      const float K = ref_of(m, c);
+      float t[GV];
+#pragma unroll
+      for (int v = 0; v < GV; v++) {
+        float y[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) y[e] = exp_ref(f[v][e], c, K);
+#pragma unroll
+        for (int w = E / 2; w >= 1; w /= 2)
+#pragma unroll
+          for (int e = 0; e < w; e++) y[e] += y[e + w];
+        t[v] = y[0];
+        __builtin_amdgcn_sched_barrier(0);  // a vector at a time: the registers hold the row
+      }
+      float up = ref_of(old, c) - K;
+      if (odd) up = (float)(ref_in(old, c) - ref_in(m, c));
+      s = fma(s, (double)__builtin_amdgcn_exp2f(up), (double)(t[0] + t[1]));
+    };
+    sum(d.sT, a.ch);
+    if (two) sum(d.s1, kLog2eF);
+    d.m = m;
+  }
+  // the statistics of the unmarked logits, into LDS a wave
+  __device__ __forceinline__ void stats(const DistillArgs& a, DisShared& sh, const void* row, const Marks& mk) {
+    const float ninf = -__builtin_inff();
+    const bool two = a.tok && a.temp != 1.0f;  // s1 is a sum of its own
+    const uint32_t any = __builtin_amdgcn_readfirstlane(mk.any[wave >> 6]);
+    float nothing[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) nothing[e] = ninf;
+    const u4v none = R::pack(nothing);
+    DisSum d;
+#pragma unroll
+    for (int g = 0; g < NV; g += GV) {
+      if (g >= held) break;
+#pragma unroll
+      for (int v = g; v < g + GV; v++) {
+        if (v >= held) raw[v] = none;
+        else if ((any >> v) & 1) raw[v] = unmarked(raw[v], mk.vec(place(v) - j0));
+      }
+      add(d, a, &raw[g], two);
+    }
+    for (int j = place(held); j < j1; j += MV * ST * E) {  // beyond the registers
+      u4v x[MV];
+#pragma unroll
+      for (int v = 0; v < MV; v++) {
+        const int o = j + v * ST * E;
+        x[v] = o < j1 ? R::load_upto(row, o, j1) : none;
+      }
+#pragma unroll
+      for (int v = 0; v < MV; v++) {
+        const int o = j + v * ST * E;
+        const uint32_t bits = o < j1 ? mk.vec(o - j0) & ((1u << E) - 1) : 0u;
+        if (bits) x[v] = unmarked(x[v], bits);
+      }
+      if (NL > 0 && j - st * E - j0 < kept * ST * E) {  // (whole waves of vectors: the same for all lanes)
+        const int at = (j - st * E - j0) / (ST * E);
+#pragma unroll
+        for (int v = 0; v < MV; v++)
+          if (at + v < kept) lds[(at + v - held) * ST + st] = x[v];
+      }
+#pragma unroll
+      for (int v = 0; v < MV; v += GV) add(d, a, x + v, two);
+    }
+    if (!two) d.s1 = d.sT;
+    d.join_wave(a);
+    if ((st & 63) == 0) sh.wm[st >> 6] = d.m, sh.wT[st >> 6] = d.sT, sh.w1[st >> 6] = d.s1;
+  }
+  // the row's formula.  MODE 0: zeros, 1: C exp2(c z - K), 2: that and D's
+  template <int MODE>
+  __device__ __forceinline__ void write(void* out, const void* row, float C, float c, float K, float D, float K1, float sub) {
+    auto grad = [&](const u4v& x, float base) {
+      float f[E];
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const float z = base != 0.0f ? R::get(x, e) - base : R::get(x, e);
+        f[e] = MODE == 0 ? 0.0f : C * exp_ref(z, c, K);
+        if constexpr (MODE == 2) f[e] = fmaf(D, exp_ref(z, kLog2eF, K1), f[e]);
+      }
+      return R::pack(f);
+    };
+    if (sub != 0.0f) held = kept = 0;  // from memory
+    void* p = static_cast<char*>(out) + (int64_t)place(0) * R::ES;
+#pragma unroll
+    for (int v = 0; v < NV; v++)
+      if (v < held) R::store(p, v * ST * E, grad(raw[v], 0.0f));
+    for (int v = held; v < kept; v++) R::store(p, v * ST * E, grad(lds[(v - held) * ST + st], 0.0f));
+    for (int j = place(kept); j < j1; j += MV * ST * E) {
+      u4v x[MV];
+#pragma unroll
+      for (int v = 0; v < MV; v++) {
+        const int o = j + v * ST * E;
+        if (o < j1) x[v] = R::load_upto(row, o, j1);
+      }
+#pragma unroll
+      for (int v = 0; v < MV; v++) {
+        const int o = j + v * ST * E;
+        if (o >= j1) break;
+        const u4v y = grad(x[v], sub);
+        if (o + E <= j1) {
+          R::store(out, o, y);
+        } else {
+#pragma unroll 1
+          for (int e = 0; o + e < j1; e++) R::put(out, o + e, R::get_at(y, e));
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void write(const DistillArgs& a, const DisShared& sh, const void* row, void* out) {
+    const float C = sh.C, D = sh.D;
+    if (C == 0.0f && D == 0.0f) return write<0>(out, row, 0, 0, 0, 0, 0, 0);
+    const bool one = D == 0.0f || C == 0.0f || a.temp == 1.0f, label = one && C == 0.0f;
+    if (one) write<1>(out, row, C + D, label ? kLog2eF : a.ch, label ? sh.K1 : sh.KT, 0, 0, sh.base);
+    else write<2>(out, row, C, a.ch, sh.KT, D, sh.K1, sh.base);
+  }
+};
+
+struct DisTeacher {
+  float ml;       // the largest of the student's listed logits
+  double ZT, Z1;  // their sums of exp2((z - ml) c) at the two temperatures, each token once
+  bool nan;       // one of them is
+};
+
+// By one wave, before the statistics are there: the teacher's distribution (sh.p by slots, sh.pt and sh.first by
+// tokens, sh.pr, sh.taught) and the student's listed tokens.
+__device__ __forceinline__ void distill_teacher(const DistillArgs& a, DisShared& sh, int i, bool twice, DisTeacher& st) {
+  const int l = threadIdx.x & 63;
+  const float ninf = -__builtin_inff();
+  const double invt = 1.0 / (double)a.temp, rest = a.rest ? (double)a.rest[i] : -__builtin_inf();
+  float tm = ninf;
+  st.ml = ninf;
+  bool nant = rest != rest;
+  st.nan = false;
+  for (int s = l; s < a.k; s += 64) {
+    const float tv = sh.tv[s], zs = sh.id[s] >= 0 ? sh.zs[s] : ninf;
+    tm = fmaxf(tm, tv);
+    st.ml = fmaxf(st.ml, zs);
+    nant |= tv != tv;
+    st.nan |= zs != zs;
+  }
+  const double tmax = fmax((double)wave_max_any(tm) * invt, rest);
+  st.ml = wave_max_any(st.ml);
+  nant = __ballot(nant) != 0;
+  st.nan = __ballot(st.nan) != 0;
+  const bool taught = tmax != -__builtin_inf() || nant;
+  double sum = 0.0;
+  for (int s = l; s < a.k; s += 64) {
+    const float tv = sh.tv[s];
+    const double pe = tv == ninf ? 0.0 : exp((double)tv * invt - tmax);
+    sh.p[s] = pe;
+    sum += pe;
+  }
+  const double re = rest == -__builtin_inf() ? 0.0 : exp(rest - tmax);
+  sum = wave_sum_any(sum) + re;
+  if (l == 0) sh.taught = taught, sh.pr = taught ? re / sum : 0.0;
+  for (int s = l; s < a.k; s += 64) sh.p[s] = sh.pt[s] = taught ? sh.p[s] / sum : 0.0, sh.first[s] = sh.id[s] >= 0;
+  if (twice) {  // a token's first slot stands for it, with the sum of its slots' probabilities in slot order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int s = l; s < a.k; s += 64) {
+      const int id = sh.id[s];
+      if (id < 0) continue;
+      double pt = 0.0;
+      for (int o = 0; o < a.k; o++)
+        if (sh.id[o] == id) {
+          if (o < s) sh.first[s] = 0;
+          pt += sh.p[o];
+        }
+      sh.pt[s] = pt;
+    }
+  }
+  st.ZT = st.Z1 = 0.0;
+  for (int s = l; s < a.k; s += 64) {
+    const float zs = sh.zs[s];
+    if (!sh.first[s] || zs == ninf) continue;
+    st.ZT += exp2(((double)zs - st.ml) * (double)a.ch);
+    if (a.tok) st.Z1 += exp2(((double)zs - st.ml) * (double)kLog2eF);
+  }
+  st.ZT = wave_sum_any(st.ZT);
+  st.Z1 = wave_sum_any(st.Z1);
+}
+
+// the student's normaliser at scale c: 2^top times what is returned, of the listed sum Z at ml and the unlisted sum
+// s at mu's reference; *share is 2^(that reference - top) over it
+__device__ __forceinline__ double distill_norm(float c, float ml, double Z, float mu, double s, bool bad, double* top, double* share) {
+  const float ninf = -__builtin_inff();
+  const double kl = ml == ninf ? -__builtin_inf() : (double)ml * (double)c, ku = mu == ninf ? -__builtin_inf() : ref_in(mu, c);
+  *top = fmax(kl, ku);
+  const double less = exp2(-fabs(kl - ku));  // (0 where one of them is -inf)
+  const double fl = ml == ninf ? 0.0 : kl < ku ? less : 1.0, fu = mu == ninf ? 0.0 : ku < kl ? less : 1.0;
+  double t = Z * fl + (mu == ninf && s == s ? 0.0 : s * fu);
+  if (bad || (ml == ninf && mu == ninf)) t = (double)__builtin_nanf("");
+  *share = fu / t;
+  return t;
+}
+
+struct DisNorms {
+  double top[2], sum[2];  // of the two temperatures
+};
+
+// with the unlisted logits' statistics: the gradient's constants into sh
+__device__ __forceinline__ void distill_scalars(const DistillArgs& a, DisShared& sh, const DisTeacher& st, const DisSum& d, float w_, DisNorms& nm) {
+  const bool empty = d.m == -__builtin_inff(), label = sh.tok >= 0;
+  double fT, f1 = 0.0;
+  nm.sum[0] = distill_norm(a.ch, st.ml, st.ZT, d.m, d.sT, st.nan, &nm.top[0], &fT);
+  nm.sum[1] = 1.0, nm.top[1] = 0.0;
+  if (a.tok) nm.sum[1] = distill_norm(kLog2eF, st.ml, st.Z1, d.m, d.s1, st.nan, &nm.top[1], &f1);
+  const double w = (double)w_, pr = sh.pr;
+  const double wT = sh.taught && w != 0.0 ? w * (1.0 - (double)a.hard) * (double)a.temp : 0.0;
+  const double w1 = label && w != 0.0 ? w * (double)a.hard : 0.0;
+  if ((threadIdx.x & 63) == 0) {
+    sh.C = wT == 0.0 || (empty && nm.sum[0] == nm.sum[0]) ? 0.0f : (float)(wT * (fT - (pr > 0.0 ? pr / d.sT : 0.0)));
+    sh.D = w1 == 0.0 || (empty && nm.sum[1] == nm.sum[1]) ? 0.0f : (float)(w1 * f1);
+    sh.KT = ref_of(d.m, a.ch), sh.K1 = ref_of(d.m, kLog2eF), sh.base = ref_base(d.m), sh.wgT = wT, sh.wg1 = w1;
+  }
+}
+
+// log2 of the two normalisers and of the unlisted sum, for the losses and the gradient at the listed tokens
+__device__ __forceinline__ void distill_logs(const DistillArgs& a, DisShared& sh, const DisSum& d, const DisNorms& nm) {
+  const double LT = nm.top[0] + log2(nm.sum[0]), L1 = a.tok ? nm.top[1] + log2(nm.sum[1]) : 0.0;
+  const double lu = d.m == -__builtin_inff() ? -__builtin_inf() : ref_in(d.m, a.ch) + log2(d.sT);
+  if ((threadIdx.x & 63) == 0) sh.LT = LT, sh.L1 = L1, sh.lu = lu;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+// the losses, by the wave that formed the scalars
+__device__ __forceinline__ void distill_losses(const DistillArgs& a, const DisShared& sh, int i) {
+  const int l = threadIdx.x & 63;
+  const double c = (double)a.ch, pr = sh.pr;
+  double kl = 0.0;
+  for (int s = l; s < a.k; s += 64) {
+    const double p = sh.p[s];
+    if (p > 0.0 || p != p) kl += p * (log(p) - ((double)sh.zs[s] * c - sh.LT) * kLn2D);
+  }
+  kl = wave_sum_any(kl);
+  if (pr > 0.0 || pr != pr) kl += pr * (log(pr) - (sh.lu - sh.LT) * kLn2D);
+  if (l == 0) {
+    a.kl[i] = sh.taught ? (float)kl : 0.0f;
+    if (a.logp) a.logp[i] = sh.tok >= 0 ? (float)(((double)sh.zt * (double)kLog2eF - sh.L1) * kLn2D) : __builtin_nanf("");
+  }
+}
+
+// the gradient at the listed tokens and the label of [j0, j1), over the row's formula; by one wave
+template <int VT, class Marks>
+__device__ __forceinline__ void distill_marked(const DistillArgs& a, const DisShared& sh, const Marks& mk, void* out, int j0, int j1) {
+  using R = VRow<VT>;
+  const int l = threadIdx.x & 63;
+  const double c = (double)a.ch;
+  for (int s = l; s < a.k; s += 64) {
+    const int id = sh.id[s];
+    if (!sh.first[s] || id < j0 || id >= j1) continue;
+    double v = 0.0;
+    if (sh.wgT != 0.0) v = sh.wgT * (exp2((double)sh.zs[s] * c - sh.LT) - sh.pt[s]);
+    if (sh.wg1 != 0.0) v += sh.wg1 * (exp2((double)sh.zs[s] * (double)kLog2eF - sh.L1) - (id == sh.tok ? 1.0 : 0.0));
+    R::put(out, id, (float)v);
+  }
+  if (l == 0 && sh.tok >= j0 && sh.tok < j1 && !mk.get(sh.tok - j0)) {
+    double v = 0.0;
+    if (sh.wgT != 0.0) v = sh.wgT * (exp2((double)sh.zt * c - sh.LT) - (sh.pr > 0.0 ? sh.pr * exp2((double)sh.zt * c - sh.lu) : 0.0));
+    if (sh.wg1 != 0.0) v += sh.wg1 * (exp2((double)sh.zt * (double)kLog2eF - sh.L1) - 1.0);
+    R::put(out, sh.tok, (float)v);
+  }
+}
+
+// by the row's wave: the slots of row i and its label into LDS
+__device__ __forceinline__ void distill_ids(const DistillArgs& a, DisShared& sh, int i) {
+  for (int s = threadIdx.x & 63; s < a.k; s += 64) {
+    const int id = a.ids[(int64_t)i * a.k + s];
+    const float tv = a.tv[(int64_t)i * a.k + s];
+    const bool held = id >= 0 && id < a.V;
+    sh.id[s] = held ? id : -1;
+    sh.tv[s] = held ? tv : -__builtin_inff();
+  }
+  const int tk = a.tok ? a.tok[i] : -1;
+  sh.tok = tk >= 0 && tk < a.V ? tk : -1;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+// and the marks of those in [j0, j1); whether one was set before
+template <class Marks>
+__device__ __forceinline__ bool distill_marks(const DistillArgs& a, const DisShared& sh, Marks& mk, int j0, int j1) {
+  bool twice = false;
+  for (int s = threadIdx.x & 63; s < a.k; s += 64)
+    if (sh.id[s] >= j0 && sh.id[s] < j1) twice |= mk.set(sh.id[s] - j0);
+  return __ballot(twice) != 0;
+}
+
+// the outputs of a row without logits over [j0, j1)
+template <int VT>
+__device__ __forceinline__ void distill_none(const DistillArgs& a, int i, void* out, int j0, int j1) {
+  if (j0 == 0 && threadIdx.x == 0) {
+    a.kl[i] = __builtin_nanf("");
+    if (a.logp) a.logp[i] = __builtin_nanf("");
+  }
+  for (int j = j0 + (int)threadIdx.x; a.w && j < j1; j += blockDim.x) VRow<VT>::put(out, j, 0.0f);
+}
+
+// grid n, B threads
+template <int VT, int B>
+__device__ __forceinline__ void distill_row(const DistillArgs& a) {
+  using R = VRow<VT>;
+  constexpr int ST = B - 64;
+  using Slice = DisSlice<VT, ST, kDisV, kDisL>;
+  extern __shared__ u4v dyn[];  // [kDisL][ST] vectors, then a bit per logit
+  uint32_t* mask = reinterpret_cast<uint32_t*>(dyn + kDisL * ST);
+  __shared__ uint32_t any[ST / 64];
+  __shared__ DisShared sh;
+  const int tid = threadIdx.x, i = blockIdx.x;
+  const void* row = static_cast<const char*>(a.z) + (int64_t)i * a.ld * R::ES;
+  void* out = static_cast<char*>(a.dz) + (int64_t)i * a.ldd * R::ES;
+  if (!row_ok(a, i)) return distill_none<VT>(a, i, out, 0, a.V);
+  typename Slice::Marks mk{mask, any};
+  if (tid >= 64) {
+    Slice sl;
+    sl.init(0, a.V, tid - 64, dyn);
+    sl.load(row);
+    mk.clear(a.V);
+    lds_barrier();
+    lds_barrier();  // marked
+    sl.stats(a, sh, row, mk);
+    lds_barrier();
+    lds_barrier();  // the scalars are there
+    if (a.w) sl.write(a, sh, row, out);
+    __syncthreads();
+  } else {
+    mk.clear(a.V);
+    distill_ids(a, sh, i);
+    lds_barrier();
+    const bool twice = distill_marks(a, sh, mk, 0, a.V);
+    lds_barrier();
+    for (int s = tid; s < a.k; s += 64)
+      if (sh.id[s] >= 0) sh.zs[s] = R::one(row, sh.id[s]);
+    const float zt = sh.tok >= 0 ? R::one(row, sh.tok) : 0.0f, w = a.w ? a.w[i] : 0.0f;
+    DisTeacher st;
+    distill_teacher(a, sh, i, twice, st);
+    lds_barrier();
+    DisSum d;
+    if (tid < ST / 64) d.m = sh.wm[tid], d.sT = sh.wT[tid], d.s1 = sh.w1[tid];
+    d.join_wave(a);
+    DisNorms nm;
+    distill_scalars(a, sh, st, d, w, nm);
+    lds_barrier();
+    sh.zt = zt;
+    distill_logs(a, sh, d, nm);
+    distill_losses(a, sh, i);
+    __syncthreads();  // the row is written
+    if (a.w) distill_marked<VT>(a, sh, mk, out, 0, a.V);
+  }
+}
+
+// Slices of kSliceB - 64 threads by kSliceV vectors.  grid (G, n): the statistics of slice g; slice 0 keeps the
+// listed tokens' and the label's logits (the gradient may be written over them).
+constexpr int kSliceB = 320, kSliceV = 8;
 template <int VT>
 __device__ __forceinline__ void distill_stats(const DistillArgs& a) {
   using R = VRow<VT>;
-  extern __shared__ uint32_t mask[];  // a bit per logit of the slice: listed
-  __shared__ float redf[kDisW];
-  __shared__ double redd[kDisW];
+  constexpr int ST = kSliceB - 64;
+  using Slice = DisSlice<VT, ST, kSliceV, 0>;
+  __shared__ uint32_t mask[kSliceV * ST * R::E / 32 + 1];
+  __shared__ uint32_t any[ST / 64];
+  __shared__ DisShared sh;
   const int tid = threadIdx.x, g = blockIdx.x, i = blockIdx.y;
   if (!row_ok(a, i)) return;
   const void* row = static_cast<const char*>(a.z) + (int64_t)i * a.ld * R::ES;
-  const int j0 = g * a.L, j1 = min(a.V, j0 + a.L);
-  const float ninf = -__builtin_inff();
-  for (int w = tid; w < a.L / 32; w += kDisB) mask[w] = 0;
-  __syncthreads();
-  int twice = 0;
-  for (int s = tid; s < a.k; s += kDisB) {
-    const int id = a.ids[(int64_t)i * a.k + s];
-    if (id >= j0 && id < j1) {
-      const uint32_t bit = 1u << ((id - j0) & 31);
-      twice |= (atomicOr(&mask[(id - j0) >> 5], bit) & bit) != 0;
-      a.zs[(int64_t)i * a.k + s] = R::one(row, id);
+  const int j0 = g * a.L, j1 = min(a.V, j0 + a.L);  // L = kSliceV ST E
+  typename Slice::Marks mk{mask, any};
+  if (tid >= 64) {
+    Slice sl;
+    sl.init(j0, j1, tid - 64, nullptr);
+    sl.load(row);
+    mk.clear(j1 - j0);
+    lds_barrier();
+    lds_barrier();  // marked
+    sl.stats(a, sh, row, mk);
+    lds_barrier();
+  } else {
+    mk.clear(j1 - j0);
+    distill_ids(a, sh, i);
+    lds_barrier();
+    const bool twice = distill_marks(a, sh, mk, j0, j1);
+    lds_barrier();
+    if (g == 0) {
+      for (int s = tid; s < a.k; s += 64)
+        if (sh.id[s] >= 0) a.zs[(int64_t)i * a.k + s] = R::one(row, sh.id[s]);
+      if (tid == 0 && sh.tok >= 0) a.zt[i] = R::one(row, sh.tok);
     }
-  }
-  if (tid == 0 && a.tok) {
-    const int t = a.tok[i];
-    if (t >= j0 && t < j1) a.zt[i] = R::one(row, t);
-  }
-  twice = __syncthreads_or(twice);
-  auto each = [&](auto&& f) {
-    for (int j = j0 + tid * R::E; j < j1; j += kDisB * R::E) {
-      const u4v r = R::load_upto(row, j, j1, ninf);
-      const uint32_t bits = mask[(j - j0) >> 5] >> ((j - j0) & 31);
-#pragma unroll
-      for (int e = 0; e < R::E; e++) f((bits >> e) & 1 ? ninf : R::get(r, e));
-    }
-  };
-  float m = ninf;
-  each([&](float x) { m = fmaxf(m, x); });
-  m = group_max<kDisW>(m, redf);
-  const float ref = m == ninf ? 0.0f : m;
-  double sT = 0.0, s1 = 0.0;
-  each([&](float x) { sT += (double)exp_scaled(x - ref, a.ch, a.cl); });
-  if (a.tok) each([&](float x) { s1 += (double)exp_scaled(x - ref, 1.44269502f, 1.92596303e-8f); });
-  sT = group_sum<kDisW>(sT, redd);  // NaN if a logit is
-  s1 = group_sum<kDisW>(s1, redd);
-  if (tid == 0) {
+    lds_barrier();
+    DisSum d;
+    if (tid < ST / 64) d.m = sh.wm[tid], d.sT = sh.wT[tid], d.s1 = sh.w1[tid];
+    d.join_wave(a);
     const int64_t o = (int64_t)i * a.G + g;
-    a.pm[o] = m, a.psT[o] = sT, a.ps1[o] = s1, a.twice[o] = twice;
+    if (tid == 0) a.pm[o] = d.m, a.psT[o] = d.sT, a.ps1[o] = d.s1, a.twice[o] = twice;
   }
 }
 
-// grid (G, n): row i's scalars from its slices' statistics and the teacher's list (each workgroup forms
-// them again: k <= 256 = one slot a thread), the losses by slice 0, the gradient over slice g
+// grid (G, n) (n alone without weights): each workgroup joins the row's slices and forms its scalars again, slice 0
+// writes the losses
 template <int VT>
 __device__ __forceinline__ void distill_grad(const DistillArgs& a) {
   using R = VRow<VT>;
-  __shared__ float redf[kDisW];
-  __shared__ double redd[kDisW];
-  __shared__ int idl[kDisB];
-  __shared__ double pl[kDisB];
+  constexpr int ST = kSliceB - 64;
+  using Slice = DisSlice<VT, ST, kSliceV, 0>;
+  __shared__ uint32_t mask[kSliceV * ST * R::E / 32 + 1];
+  __shared__ uint32_t any[ST / 64];
+  __shared__ DisShared sh;
   const int tid = threadIdx.x, g = blockIdx.x, i = blockIdx.y;
-  const float ninf = -__builtin_inff();
   const int j0 = g * a.L, j1 = min(a.V, j0 + a.L);
-  void* out = static_cast<char*>(a.dz) + (int64_t)i * a.ldd * R::ES;
-  if (!row_ok(a, i)) {
-    if (g == 0 && tid == 0) {
-      a.kl[i] = __builtin_nanf("");
-      if (a.logp) a.logp[i] = __builtin_nanf("");
-    }
-    for (int j = j0 + tid; a.w && j < j1; j += kDisB) R::put(out, j, 0.0f);
-    return;
-  }
-  const double invt = 1.0 / (double)a.temp;
-  // the unlisted
-  float mu = ninf;
-  int twice = 0;
-  for (int q = tid; q < a.G; q += kDisB) mu = fmaxf(mu, a.pm[(int64_t)i * a.G + q]), twice |= a.twice[(int64_t)i * a.G + q];
-  mu = group_max<kDisW>(mu, redf);
-  twice = __syncthreads_or(twice);
-  double sT = 0.0, s1 = 0.0;
-  for (int q = tid; q < a.G; q += kDisB) {
-    const int64_t o = (int64_t)i * a.G + q;
-    const float pm = a.pm[o];
-    const double f = pm == ninf ? 1.0 : exp(((double)pm - mu) * invt), f1 = pm == ninf ? 1.0 : exp((double)pm - mu);
-    sT += a.psT[o] * f;
-    s1 += a.ps1[o] * f1;
-  }
-  sT = group_sum<kDisW>(sT, redd);
-  s1 = group_sum<kDisW>(s1, redd);
-  // the teacher's slots
-  const int id = tid < a.k ? a.ids[(int64_t)i * a.k + tid] : -1;
-  const bool held = id >= 0 && id < a.V;
-  const float tv = held ? a.tv[(int64_t)i * a.k + tid] : ninf;
-  const float zs = held ? a.zs[(int64_t)i * a.k + tid] : ninf;
-  const double rest = a.rest ? (double)a.rest[i] : -__builtin_inf();
-  const double tmax = fmax((double)group_max<kDisW>(tv, redf) * invt, rest);
-  const bool nant = __syncthreads_or(tv != tv);
-  const bool taught = tmax != -__builtin_inf() || nant || rest != rest;
-  double pe = tv == ninf ? 0.0 : exp((double)tv * invt - tmax);
-  const double re = rest == -__builtin_inf() ? 0.0 : exp(rest - tmax);
-  const double tsum = group_sum<kDisW>(pe, redd) + re;
-  const double ps = taught ? pe / tsum : 0.0, pr = taught ? re / tsum : 0.0;
-  // tokens listed twice: the first slot stands for the token, with the sum of its slots
-  bool first = held;
-  double pt = ps;
-  if (twice) {
-    idl[tid] = held ? id : -1, pl[tid] = ps;
-    __syncthreads();
-    if (held) {
-      pt = 0.0;
-      for (int s = 0; s < a.k; s++)
-        if (idl[s] == id) {
-          if (s < tid) first = false;
-          pt += pl[s];
-        }
-    }
-  }
-  // the student over all logits
-  const float ml = group_max<kDisW>(zs, redf);
-  const float M = fmaxf(mu, ml);
-  const double fu = mu == ninf ? 0.0 : exp(((double)mu - M) * invt), fu1 = mu == ninf ? 0.0 : exp((double)mu - M);
-  const double es = first && zs != ninf ? exp(((double)zs - M) * invt) : 0.0;
-  const double es1 = first && zs != ninf && a.tok ? exp((double)zs - M) : 0.0;
-  const bool bad = __syncthreads_or(zs != zs);  // a NaN among the listed
-  const double nanv = (double)__builtin_nanf("");
-  double ZT = group_sum<kDisW>(es, redd) + (mu == ninf && sT == sT ? 0.0 : sT * fu);
-  double Z1 = group_sum<kDisW>(es1, redd) + (mu == ninf && s1 == s1 ? 0.0 : s1 * fu1);
-  if (bad || M == ninf) ZT = nanv, Z1 = nanv;
-  const double lT = log(ZT);
-  const int tk = a.tok ? a.tok[i] : -1;
-  const bool label = tk >= 0 && tk < a.V;
-  const float zt = label ? a.zt[i] : ninf;
-  if (g == 0) {
-    double kl = ps > 0.0 || ps != ps ? ps * (log(ps) - ((((double)zs - M) * invt) - lT)) : 0.0;
-    kl = group_sum<kDisW>(kl, redd);
-    if (pr > 0.0 || pr != pr) kl += pr * (log(pr) - ((((double)mu - M) * invt + log(sT)) - lT));
-    if (tid == 0) {
-      a.kl[i] = taught ? (float)kl : 0.0f;
-      if (a.logp) a.logp[i] = label ? (float)((double)zt - M - log(Z1)) : __builtin_nanf("");
-    }
-  }
-  if (!a.w) return;
-  const double w = (double)a.w[i];
-  const double wT = taught ? w * (1.0 - (double)a.hard) * (double)a.temp : 0.0, w1 = label ? w * (double)a.hard : 0.0;
-  const bool empty = mu == ninf;
-  const float C = w == 0.0 || wT == 0.0 || (empty && ZT == ZT) ? 0.0f : (float)(wT * (fu / ZT - (pr > 0.0 ? pr / sT : 0.0)));
-  const float D = w == 0.0 || w1 == 0.0 || (empty && Z1 == Z1) ? 0.0f : (float)(w1 * (fu1 / Z1));
-  const float ref = empty ? 0.0f : mu;
   const void* row = static_cast<const char*>(a.z) + (int64_t)i * a.ld * R::ES;
-  for (int j = j0 + tid * R::E; j < j1; j += kDisB * R::E) {
-    const u4v r = R::load_upto(row, j, j1, ninf);
-    float f[R::E];
-#pragma unroll
-    for (int e = 0; e < R::E; e++) {
-      const float t = R::get(r, e) - ref;
-      float v = 0.0f;
-      if (C != 0.0f) v = C * exp_scaled(t, a.ch, a.cl);
-      if (D != 0.0f) v = fmaf(D, exp_scaled(t, 1.44269502f, 1.92596303e-8f), v);
-      f[e] = v;
+  void* out = static_cast<char*>(a.dz) + (int64_t)i * a.ldd * R::ES;
+  if (!row_ok(a, i)) return distill_none<VT>(a, i, out, j0, j1);
+  typename Slice::Marks mk{mask, any};
+  if (tid >= 64) {
+    Slice sl;
+    sl.init(j0, j1, tid - 64, nullptr);
+    if (a.w) sl.load(row);
+    mk.clear(j1 - j0);
+    lds_barrier();
+    lds_barrier();  // the scalars are there
+    if (a.w) sl.write(a, sh, row, out);
+    __syncthreads();
+  } else {
+    mk.clear(j1 - j0);
+    distill_ids(a, sh, i);
+    for (int s = tid; s < a.k; s += 64)
+      if (sh.id[s] >= 0) sh.zs[s] = a.zs[(int64_t)i * a.k + s];
+    const float zt = sh.tok >= 0 ? a.zt[i] : 0.0f, w = a.w ? a.w[i] : 0.0f;
+    int t2 = 0;
+    DisSum d;
+    for (int q = tid; q < a.G; q += 64) {
+      const int64_t o = (int64_t)i * a.G + q;
+      DisSum e;
+      e.m = a.pm[o], e.sT = a.psT[o], e.s1 = a.ps1[o];
+      t2 |= a.twice[o];
+      if (e.m > d.m) d.raise(e.m, a);
+      if (e.m < d.m) e.raise(d.m, a);
+      d.sT += e.sT, d.s1 += e.s1;
     }
-    if (j + R::E <= j1) {
-      R::store(out, j, R::pack(f));
-    } else {
-#pragma unroll
-      for (int e = 0; e < R::E; e++)
-        if (j + e < j1) R::put(out, j + e, f[e]);
-    }
-  }
-  __syncthreads();  // the listed tokens and the label are written over the rows' formula
-  if (w == 0.0) return;
-  if (first && id >= j0 && id < j1) {
-    double v = 0.0;
-    if (wT != 0.0) v = wT * (exp(((double)zs - M) * invt) / ZT - pt);
-    if (w1 != 0.0) v += w1 * (exp((double)zs - M) / Z1 - (id == tk ? 1.0 : 0.0));
-    R::put(out, id, (float)v);
-  }
-  const bool listed = __syncthreads_or(held && id == tk);
-  if (tid == 0 && label && !listed && w1 != 0.0 && tk >= j0 && tk < j1) {
-    double v = w1 * (exp((double)zt - M) / Z1 - 1.0);
-    if (wT != 0.0) v += wT * exp(((double)zt - M) * invt) / ZT - (pr > 0.0 ? wT * pr * exp(((double)zt - mu) * invt) / sT : 0.0);
-    R::put(out, tk, (float)v);
+    d.join_wave(a);
+    lds_barrier();
+    distill_marks(a, sh, mk, j0, j1);
+    DisTeacher st;
+    distill_teacher(a, sh, i, __ballot(t2) != 0, st);
+    DisNorms nm;
+    distill_scalars(a, sh, st, d, w, nm);
+    lds_barrier();
+    sh.zt = zt;
+    distill_logs(a, sh, d, nm);
+    if (g == 0) distill_losses(a, sh, i);
+    __syncthreads();  // the slice is written
+    if (a.w) distill_marked<VT>(a, sh, mk, out, j0, j1);
   }
 }
 
-#define RTQ_DISTILL(ty, VT)                                                                                     \
-  extern "C" __global__ __launch_bounds__(kDisB) void rtq_distill_stats_##ty(DistillArgs a) { distill_stats<VT>(a); } \
-  extern "C" __global__ __launch_bounds__(kDisB) void rtq_distill_grad_##ty(DistillArgs a) { distill_grad<VT>(a); }
+#define RTQ_DISTILL(ty, VT)                                                                                                \
+  extern "C" __global__ __launch_bounds__(256, 4) void rtq_distill256_##ty(DistillArgs a) { distill_row<VT, 256>(a); }     \
+  extern "C" __global__ __launch_bounds__(512, 4) void rtq_distill512_##ty(DistillArgs a) { distill_row<VT, 512>(a); }     \
+  extern "C" __global__ __launch_bounds__(1024, 4) void rtq_distill1024_##ty(DistillArgs a) { distill_row<VT, 1024>(a); }  \
+  extern "C" __global__ __launch_bounds__(kSliceB) void rtq_distill_stats_##ty(DistillArgs a) { distill_stats<VT>(a); }        \
+  extern "C" __global__ __launch_bounds__(kSliceB) void rtq_distill_grad_##ty(DistillArgs a) { distill_grad<VT>(a); }
 RTQ_DISTILL(f32, VT_F32)
 RTQ_DISTILL(f16, VT_F16)
 RTQ_DISTILL(bf16, VT_BF16)
@@ -753,7 +1177,7 @@ __device__ __forceinline__ void verify_stats(const VerifyArgs& a) {
   const int j0 = g * a.L, j1 = min(a.V, j0 + a.L);
   uint64_t best = 0;
   for (int v = j0 + tid * R::E; v < j1; v += kVdB * R::E) {
-    const u4v r = R::load_upto(z, v, j1, -__builtin_inff());
+    const u4v r = R::load_upto(z, v, j1);
 #pragma unroll
     for (int e = 0; e < R::E; e++) {
       const uint64_t key = v + e < j1 ? rank_key(R::get(r, e), v + e) : 0;
@@ -774,7 +1198,7 @@ __device__ __forceinline__ void verify_stats(const VerifyArgs& a) {
   if (a.temp > 0.0f && m != -__builtin_inf()) {
     const double invt = 1.0 / (double)a.temp;
     for (int v = j0 + tid * R::E; v < j1; v += kVdB * R::E) {
-      const u4v r = R::load_upto(z, v, j1, -__builtin_inff());
+      const u4v r = R::load_upto(z, v, j1);
 #pragma unroll
       for (int e = 0; e < R::E; e++) s += exp(((double)R::get(r, e) - m) * invt);
     }
@@ -873,7 +1297,7 @@ __device__ __forceinline__ void verify_mass(const VerifyArgs& a) {
   const double invt = 1.0 / (double)a.temp;
   double sw = 0.0, sp = 0.0;
   for (int v = j0 + tid * R::E; v < j1; v += kVdB * R::E) {
-    const u4v r = R::load_upto(zp, v, j1, -__builtin_inff()), rq = R::load_upto(zq, v, j1, -__builtin_inff());
+    const u4v r = R::load_upto(zp, v, j1), rq = R::load_upto(zq, v, j1);
 #pragma unroll
     for (int e = 0; e < R::E; e++) {
       double p;

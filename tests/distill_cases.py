@@ -5,9 +5,10 @@ NEG = -np.inf
 EPS = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}  # half a step, relative
 TINY = {"f32": 2.0 ** -126, "f16": 2.0 ** -25, "bf16": 2.0 ** -126}  # half a subnormal step (f16); flushed below (others)
 # Relative error of a sum of f32 exponentials: 2^-22 for an exponential (its instruction and two
-# roundings), 2^-22 for a vector's eight f32 additions, and the rounding of z - max, |z - max| 2^-24 / T
-# averaged over the softmax (at most log of the vocabulary, 12.6, at T = 1; weights below e^-12.6 count less).
-SUM = 2.0 ** -21 + 12.6 * 2.0 ** -24
+# roundings), 2^-22 for a vector's eight f32 additions, the rounding of its argument, |z - max| 2^-24 / T,
+# and of the scale 1 / T, |z - max| 2^-25 / T, averaged over the softmax (|z - max| / T at most log of the
+# vocabulary, 12.6: weights below e^-12.6 count less).
+SUM = 2.0 ** -21 + 12.6 * 1.5 * 2.0 ** -24
 
 
 def lse(x, axis=-1):

@@ -2,8 +2,8 @@
 
 Tolerances: whole numbers and selected logits are equal.  A log-sum-exp is off by D.SUM (a relative error of its
 sum) and half a step; kl by D.SUM for each of the two it holds and half a step; a gradient element by D.SUM and
-one more exponential (2^-22, and |z - max| 2^-24 / T of its argument) of the magnitudes it is a difference of, and half a
-step of its type."""
+one more exponential (2^-22, and its argument's roundings: |z - max| / T of 2^-24 for itself and 2^-25 for the
+scale, doubled for the label's at T = 1) of the magnitudes it is a difference of, and half a step of its type."""
 
 import numpy as np
 import pytest
@@ -70,7 +70,7 @@ def check_lse(got, want, each=1):
 @pytest.mark.parametrize("n,V,k,temp,pad,shift", [
     (1, 1, 1, 1.0, 0, 0), (2, 2, 2, 1.0, 1, 1), (3, 7, 5, 0.5, 0, 3), (5, 63, 63, 1.0, 2, 0), (4, 1000, 256, 2.0, 0, 1),
     (3, 8191, 20, 1.0, 0, 0), (3, 8193, 64, 1.0, 5, 7), (2, 16385, 1, 4.0, 0, 2), (37, 50257, 8, 1.0, 0, 0), (2, 151936, 256, 1.0, 0, 0),
-    (1, 300001, 100, 1.0, 0, 0), (300, 257, 17, 1.0, 0, 1)])
+    (1, 300001, 100, 1.0, 0, 0), (300, 257, 17, 1.0, 0, 1), (1, 1 << 20, 256, 1.0, 0, 0)])
 def test_top_logits(ctx, ty, n, V, k, temp, pad, shift):
     check_top(ctx, D.logits(np.random.default_rng(V + k), n, V), ty, k, temp, pad, shift)
 
@@ -158,7 +158,7 @@ def check_distill(ctx, z, ids, vals, rest, temp, tok=None, w=None, hard=0.0, ty=
         got = host(gview)
         np.testing.assert_array_equal(np.isnan(got), np.isnan(rg))
         with np.errstate(all="ignore"):
-            depth = np.abs(z64 - np.where(np.isfinite(z64), z64, -np.inf).max(1, keepdims=True)) * HALF / min(temp, 1.0)
+            depth = np.abs(z64 - np.where(np.isfinite(z64), z64, -np.inf).max(1, keepdims=True)) * 2 * HALF / min(temp, 1.0)
             bound = np.where(sc > 0, sc * (D.SUM + 2.0 ** -22 + np.minimum(depth, 1.0)), 0.0) + np.abs(rg) * D.EPS[ty] * (1 + 1e-5) + D.TINY[ty]
         bad = ~np.isnan(rg) & ~(np.abs(got - rg) <= bound)
         assert not bad.any(), (np.argwhere(bad)[:5], got[bad][:5], rg[bad][:5], bound[bad][:5])
@@ -198,6 +198,35 @@ def test_distill(ctx, ty, n, V, k, temp, hard, rest, ragged, pad, shift):
     assert torch.equal(g.contiguous().view(torch.uint8), g2.contiguous().view(torch.uint8))
     # losses alone, without labels
     check_distill(ctx, z, ids, vals, r, temp, ty=ty, pad=pad, shift=shift)
+
+
+@pytest.fixture(scope="module", params=["-1", "0", "1", "2"])
+def each_ctx(request):
+    """A context whose distillation runs on slices, or a row a workgroup of 256, 512 or 1024 threads, whatever the size."""
+    import os
+
+    os.environ["RTQ_DISTILL_ROWS"] = request.param
+    c = rt.Context(0)
+    del os.environ["RTQ_DISTILL_ROWS"]
+    yield c
+    c.close()
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("n,V,k,temp,hard", [(1, 3, 2, 1.0, 0.5), (2, 6143, 30, 2.0, 0.25), (3, 40001, 256, 1.0, 0.5), (1, 170003, 20, 0.5, 0.0), (1, 1 << 20, 64, 1.0, 0.5)])
+def test_distill_on_every_kernel(each_ctx, ty, n, V, k, temp, hard):
+    rng = np.random.default_rng(V)
+    z = D.logits(rng, n, V)
+    ids, vals, r = teacher(rng, z, k, temp)
+    tok, w = rng.integers(0, V, n), rng.uniform(0.25, 2.0, n)
+    _, g = check_distill(each_ctx, z, ids, vals, r, temp, tok, w, hard, ty, pad=3, shift=1)
+    _, g2 = check_distill(each_ctx, z, ids, vals, r, temp, tok, w, hard, ty, pad=3, shift=1, in_place=True)
+    assert torch.equal(g.contiguous().view(torch.uint8), g2.contiguous().view(torch.uint8))
+
+
+def test_distill_rows_at_the_edges_on_every_kernel(each_ctx):
+    test_distill_rows_at_the_edges(each_ctx)
+    test_distill_nan_and_infinite_rows(each_ctx)
 
 
 def test_distill_rows_at_the_edges(ctx):
