@@ -397,8 +397,8 @@ struct DistillArgs {
 };
 
 struct VerifyPick {  // the row that sequence i's next token is drawn from
-  double pm, ps, qm, qs;  // maxima and reciprocal sums of the target's and the draft's row
-  int row, not_x, minus_q, pad;
+  double pm, ps, qm, qs;  // the target's and the draft's row: maximum, reciprocal sum
+  int row, not_x, minus_q, best;
 };
 struct VerifyArgs {
   const void* z;  // [b (d + 1)] target rows, stride ld
@@ -411,10 +411,10 @@ struct VerifyArgs {
   const float* u;          // [b x (d + 1)]
   int32_t* accepted;       // [b]
   int32_t* tokens;         // [b x (d + 1)]
-  uint64_t* pk;            // [rows x G] rank key of each slice's maximum
+  uint64_t* pk;            // [rows x G] each slice's maximum (its bits; temp 0: its rank key)
   double* ps;              // [rows x G] sum of exp((z - max) / temp)
   VerifyPick* pick;        // [b]
-  double* mass;            // [b x G x 2] sums of the weights and of p over the row's slices
+  double* mass;            // [b x 4 G x 2] sums of the weights and of p over quarters of the row's slices
 };
 
 // ---------------------------------------------------------------- model-level step

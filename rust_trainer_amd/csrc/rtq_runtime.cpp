@@ -171,8 +171,8 @@ enum Kid {
   K_DISTILL_STATS = K_DISTILL + 9,
   K_DISTILL_GRAD = K_DISTILL_STATS + 3,
   K_VERIFY_STATS = K_DISTILL_GRAD + 3,
-  K_VERIFY_ACCEPT = K_VERIFY_STATS + 3,
-  K_VERIFY_MASS = K_VERIFY_ACCEPT + 3,
+  K_VERIFY_GREEDY = K_VERIFY_STATS + 3,
+  K_VERIFY_MASS = K_VERIFY_GREEDY + 3,
   K_VERIFY_PICK = K_VERIFY_MASS + 3,
   K_ROWS = K_VERIFY_PICK + 3,  // + format
   K_MODEL = K_ROWS + F_COUNT,  // + RtqModelKernel: the decoder block (rtq_model.cpp)
@@ -212,7 +212,7 @@ constexpr const char* kKernelNames[] = {
     "rtq_distill_stats_f32", "rtq_distill_stats_f16", "rtq_distill_stats_bf16",
     "rtq_distill_grad_f32", "rtq_distill_grad_f16", "rtq_distill_grad_bf16",
     "rtq_verify_stats_f32", "rtq_verify_stats_f16", "rtq_verify_stats_bf16",
-    "rtq_verify_accept_f32", "rtq_verify_accept_f16", "rtq_verify_accept_bf16",
+    "rtq_verify_greedy_f32", "rtq_verify_greedy_f16", "rtq_verify_greedy_bf16",
     "rtq_verify_mass_f32",  "rtq_verify_mass_f16",  "rtq_verify_mass_bf16",
     "rtq_verify_pick_f32",  "rtq_verify_pick_f16",  "rtq_verify_pick_bf16",
     "rtq_rows_q4_0",        "rtq_rows_q8_0",        "rtq_rows_q4_k",        "rtq_rows_q6_k",
@@ -2052,12 +2052,12 @@ struct VerifyPlan {
   size_t bytes;
 };
 
-VerifyPlan verify_plan(int64_t b, int64_t d, int64_t V, bool draft) {
+VerifyPlan verify_plan(int type, int64_t b, int64_t d, int64_t V, bool draft) {
   VerifyPlan p{};
-  p.L = 8192;
+  p.L = 256 * 8 * 16 / logit_bytes(type);  // a workgroup's registers
   p.G = cdiv(V, p.L);
   p.rows = b * (d + 1) + (draft ? b * d : 0);
-  p.bytes = (size_t)(p.rows * p.G) * 16 + (size_t)b * sizeof(VerifyPick) + (size_t)(b * p.G) * 16 + 8 * 256;
+  p.bytes = (size_t)(p.rows * p.G) * 16 + (size_t)b * sizeof(VerifyPick) + (size_t)(b * p.G) * 64 + 8 * 256;
   return p;
 }
 
@@ -2085,15 +2085,14 @@ rtq_status enqueue_verify(rtq_ctx* c, const void* z, int type, int64_t ld, const
   a.pk = ar.take<uint64_t>((size_t)(p.rows * p.G));
   a.ps = ar.take<double>((size_t)(p.rows * p.G));
   a.pick = ar.take<VerifyPick>((size_t)b);
-  a.mass = ar.take<double>((size_t)(b * p.G * 2));
+  a.mass = ar.take<double>((size_t)(b * p.G * 8));
   if (ar.off > ar.cap) return fail(RTQ_ERR_INVALID, "internal: workspace too small");
   const int ty = logit_type(type);
   const int64_t gy = std::min<int64_t>(p.rows, 65535);
   RTQ_TRY(launch(c, K_VERIFY_STATS + ty, dim3((unsigned)p.G, (unsigned)gy, (unsigned)cdiv(p.rows, 65535)), dim3(256), st, a));
-  RTQ_TRY(launch(c, K_VERIFY_ACCEPT + ty, dim3((unsigned)b), dim3(64), st, a));
-  if (temp == 0.0f) return RTQ_OK;
+  if (temp == 0.0f) return launch(c, K_VERIFY_GREEDY + ty, dim3((unsigned)b), dim3(256), st, a);
   RTQ_TRY(launch(c, K_VERIFY_MASS + ty, dim3((unsigned)p.G, (unsigned)b), dim3(256), st, a));
-  return launch(c, K_VERIFY_PICK + ty, dim3((unsigned)b), dim3(256), st, a);
+  return launch(c, K_VERIFY_PICK + ty, dim3((unsigned)b), dim3(1024), st, a);
 }
 
 }  // namespace
@@ -2134,7 +2133,7 @@ rtq_status rtq_verify_draft_d(rtq_ctx* c, const void* z, int type, int64_t ld, c
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = (hipStream_t)stream;
   if (temp == 0.0f || d == 0) q = nullptr;
-  const VerifyPlan p = verify_plan(b, d, V, q != nullptr);
+  const VerifyPlan p = verify_plan(type, b, d, V, q != nullptr);
   RTQ_TRY(row_ws(c, p.bytes, st));
   Arena ar{(char*)c->ws, c->ws_bytes, 0};
   return enqueue_verify(c, z, type, ld, q, ldq, b, d, V, drafted, lens, u, temp, accepted, tokens, p, ar, st);
@@ -2584,7 +2583,7 @@ rtq_status rtq_verify_draft(rtq_ctx* c, const void* z, int type, int64_t ld, con
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = c->stream;
   if (temp == 0.0f || d == 0) q = nullptr;
-  const VerifyPlan p = verify_plan(b, d, V, q != nullptr);
+  const VerifyPlan p = verify_plan(type, b, d, V, q != nullptr);
   const int64_t es = logit_bytes(type), tr = b * (d + 1);
   RTQ_TRY(ensure_ws(c, p.bytes + (size_t)(p.rows * V * es + b * (2 + d) * 4 + tr * 8) + 8 * 256));
   Arena ar{(char*)c->ws, c->ws_bytes, 0};

@@ -351,7 +351,7 @@ __device__ __forceinline__ void top_pick(const TopArgs& a) {
   using R = VRow<VT>;
   constexpr int E = R::E, GS = 8 * E, B = kPickB, W = B / 64, CAP = 4 * B, U = 5120 / B, UE = 4;
   __shared__ uint64_t cand[CAP];
-  __shared__ uint32_t list[CAP];
+  __shared__ alignas(16) uint32_t list[CAP];
   __shared__ float redf[W];
   __shared__ double redd[W];
   __shared__ int hist[256];
@@ -481,14 +481,21 @@ __device__ __forceinline__ void top_pick(const TopArgs& a) {
   const double gs_rest = rs;
   bool many = groups > CAP;
   if (!many) {
-    collect([&](float x, int) { return !(x < thr); });
-    if (cnt > CAP) {
+    // a bound from the listed groups' logits, where the groups gave none (few of them hold a row of a small
+    // vocabulary) or too much reaches it: places are found by counting, n of n candidates each
+    auto refine = [&]() {
       float em = ninf;
       each([&](const u4v& v, int j) {
 #pragma unroll
         for (int e = 0; e < E; e++) em = j + e < a.V ? fmaxf(em, R::get(v, e) != R::get(v, e) ? inf : R::get(v, e)) : em;
       });
       thr = fmaxf(thr, bound(em, groups * 8));
+    };
+    const bool none = thr == ninf && groups * GS > 2 * a.k + 128;
+    if (none) refine();
+    collect([&](float x, int) { return !(x < thr); });
+    if (!none && cnt > 4 * a.k + 256) {
+      refine();
       if (tid == 0) cnt = 0;
       __syncthreads();
       rm = gm_rest, rs = gs_rest;
@@ -511,16 +518,38 @@ __device__ __forceinline__ void top_pick(const TopArgs& a) {
     });
     collect([&](float x, int j) { return rank_key(x, j) >= ek; });  // k of them
   }
-  // each candidate's place is the number of larger ones
-  const int n = cnt, n8 = (n + 7) & ~7;
-  if (tid < n8 - n) cand[n + tid] = 0;
+  // Many candidates more than k (a small vocabulary, of which k is a large part): first exactly the k, found digit
+  // by digit (2000 rows of 1000 f32 logits, k = 256: 64 us, 172 by counting all of them).
+  const uint64_t* best = cand;
+  int n = cnt;
+  if (n > 2 * a.k + 128) {
+    const uint64_t kth = radix_kth<B>(n, a.k, hist, out, [&](int p) { return cand[p]; });
+    uint64_t* few = reinterpret_cast<uint64_t*>(list);
+    __syncthreads();
+    if (tid == 0) cnt = 0;
+    __syncthreads();
+    for (int p = tid; p < n; p += B) {
+      const uint64_t key = cand[p];
+      if (key >= kth) {
+        few[atomicAdd(&cnt, 1)] = key;
+      } else if (a.rest) {
+        const float x = key_value(key), w = 1.0f;
+        join_rest<1>(rm, rs, &x, &w, a);
+      }
+    }
+    __syncthreads();
+    best = few, n = a.k;
+  }
+  // a candidate's place is the number of larger ones
+  const int n8 = (n + 7) & ~7;
+  if (tid < n8 - n) const_cast<uint64_t*>(best)[n + tid] = 0;
   __syncthreads();
   for (int p = tid; p < n; p += B) {
-    const uint64_t key = cand[p];
+    const uint64_t key = best[p];
     int place = 0;
     for (int q = 0; q < n8; q += 8)
 #pragma unroll
-      for (int e = 0; e < 8; e++) place += cand[q + e] > key;
+      for (int e = 0; e < 8; e++) place += best[q + e] > key;
     if (place < a.k) {
       a.vals[(int64_t)i * a.k + place] = key_value(key);
       a.ids[(int64_t)i * a.k + place] = key_index(key);
@@ -1150,246 +1179,370 @@ RTQ_DISTILL(bf16, VT_BF16)
 // drawn from max(p - q, 0) at the first rejection, from p after all: the first index whose running sum
 // passes u_d times the total.  T = 0: accept while x_j is the target's largest logit (the lowest index
 // of equals), which is also the token after.  Steps of the running sum over a flat tail lie nearer
-// than 2^-24 of the total, so exponentials and sums are in 64 bits.
-constexpr int kVdB = 256, kVdW = kVdB / 64;
+// than 2^-24 of the total, so exponentials and sums are in 64 bits, whose arithmetic bounds the statistics (384 rows
+// of 151936 bf16 logits in 56 us, 2.1 TB/s).
+constexpr int kVdB = 256, kVdW = kVdB / 64, kVdV = 8;
+
+// 2^(y / 16) for y <= 0: y = 16 n + i + f with |f| <= 1/2, a table of 2^(i / 16), and the series of exp(f ln 2 / 16)
+// to f^5 (2e-13 of it; half the f64 operations of a series over a whole octave).  -inf gives 0; a NaN is not kept.
+struct VdExp {
+  double tab[16];
+  __device__ __forceinline__ void fill() {  // a barrier follows
+    if (threadIdx.x < 16) tab[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
+  }
+  __device__ __forceinline__ double operator()(double y) const {
+    y = fmax(y, -17600.0);
+    const double n = rint(y), f = y - n;
+    const int i = (int)n;
+    double p = 1.271587195055813e-09;  // (ln2 / 16)^5 / 5!
+    p = fma(p, f, 1.467610032291943e-07);
+    p = fma(p, f, 1.3550807779497455e-05);
+    p = fma(p, f, 0.0009383847928089871);
+    p = fma(p, f, 0.04332169878499658);
+    p = fma(p, f, 1.0);
+    return ldexp(p * tab[i & 15], i >> 4);
+  }
+};
+__device__ __forceinline__ double vd_scale(const VerifyArgs& a) { return a.temp > 0.0f ? 23.083120654223414 / (double)a.temp : 0.0; }  // 16 log2(e) / T
 
 template <int VT>
 __device__ __forceinline__ const void* vd_row(const VerifyArgs& a, bool draft, int64_t row) {
   return static_cast<const char*>(draft ? a.q : a.z) + row * (draft ? a.ldq : a.ld) * VRow<VT>::ES;
 }
+__device__ __forceinline__ int vd_len(const VerifyArgs& a, int i) { return a.lens ? min(max(a.lens[i], 0), a.d) : a.d; }
 
-// grid (G, b (d + 1) + b d): maximum (the lowest index of it) and sum exp((z - max) / T) of a slice of a target
+// grid (G, b (d + 1) + b d): maximum and sum exp((z - max) / T) (T = 0: the largest rank key) of a slice of a target
 // row, then of the draft rows; rows past a sequence's length are not read
 template <int VT>
 __device__ __forceinline__ void verify_stats(const VerifyArgs& a) {
   using R = VRow<VT>;
+  constexpr int E = R::E;
   __shared__ uint64_t redk[kVdW];
+  __shared__ float redf[kVdW];
   __shared__ double redd[kVdW];
+  __shared__ VdExp ex;
   const int tid = threadIdx.x, g = blockIdx.x;
   const int64_t rr = blockIdx.y + (int64_t)blockIdx.z * 65535, tr = (int64_t)a.b * (a.d + 1);
   if (rr >= tr + (a.q ? (int64_t)a.b * a.d : 0)) return;
   const bool draft = rr >= tr;
   const int64_t row = draft ? rr - tr : rr;
   const int i = (int)(row / (draft ? a.d : a.d + 1)), j = (int)(row % (draft ? a.d : a.d + 1));
-  const int len = a.lens ? min(max(a.lens[i], 0), a.d) : a.d;
+  const int len = vd_len(a, i);
   if (draft ? j >= len : j > len) return;
   const void* z = vd_row<VT>(a, draft, row);
-  const int j0 = g * a.L, j1 = min(a.V, j0 + a.L);
-  uint64_t best = 0;
-  for (int v = j0 + tid * R::E; v < j1; v += kVdB * R::E) {
-    const u4v r = R::load_upto(z, v, j1);
+  const int j0 = g * a.L, j1 = min(a.V, j0 + a.L);  // L = kVdB kVdV E
+  const float ninf = -__builtin_inff();
+  if (a.temp == 0.0f) {
+    uint64_t best = 0;
+#pragma unroll 1
+    for (int o = j0 + tid * E; o < j1; o += kVdB * E) {
+      const u4v r = R::load_upto(z, o, j1);
 #pragma unroll
-    for (int e = 0; e < R::E; e++) {
-      const uint64_t key = v + e < j1 ? rank_key(R::get(r, e), v + e) : 0;
-      best = key > best ? key : best;
+      for (int e = 0; e < E; e++) {
+        const uint64_t key = o + e < j1 ? rank_key(R::get(r, e), o + e) : 0;
+        best = key > best ? key : best;
+      }
     }
-  }
 #pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) {
-    const uint64_t o = __shfl_xor(best, m);
-    best = o > best ? o : best;
-  }
-  if ((tid & 63) == 0) redk[tid >> 6] = best;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kVdW; w++) best = redk[w] > best ? redk[w] : best;
-  double s = 0.0;
-  const double m = (double)key_value(best);
-  if (a.temp > 0.0f && m != -__builtin_inf()) {
-    const double invt = 1.0 / (double)a.temp;
-    for (int v = j0 + tid * R::E; v < j1; v += kVdB * R::E) {
-      const u4v r = R::load_upto(z, v, j1);
-#pragma unroll
-      for (int e = 0; e < R::E; e++) s += exp(((double)R::get(r, e) - m) * invt);
+    for (int m = 32; m >= 1; m >>= 1) {
+      const uint64_t o = __shfl_xor(best, m);
+      best = o > best ? o : best;
     }
+    if ((tid & 63) == 0) redk[tid >> 6] = best;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kVdW; w++) best = redk[w] > best ? redk[w] : best;
+    if (tid == 0) a.pk[rr * a.G + g] = best;
+    return;
+  }
+  float m = ninf;
+  bool nan = false;
+  auto see = [&](const u4v& r) {
+#pragma unroll
+    for (int e = 0; e < E; e++) m = fmaxf(m, R::get(r, e)), nan |= R::get(r, e) != R::get(r, e);
+  };
+  if (j0 + a.L <= a.V) {
+    u4v raw[kVdV];
+#pragma unroll
+    for (int v = 0; v < kVdV; v++) raw[v] = R::load(z, j0 + (v * kVdB + tid) * E);
+#pragma unroll
+    for (int v = 0; v < kVdV; v++) see(raw[v]);
+  } else {
+#pragma unroll 1
+    for (int o = j0 + tid * E; o < j1; o += kVdB * E) see(R::load_upto(z, o, j1));
+  }
+  ex.fill();
+  m = group_max<kVdW>(m, redf);  // (and its barriers)
+  // (z - m) c and not z c - m c, which is not small where both are the type's lowest value
+  const double c = vd_scale(a), ref = m == ninf ? 0.0 : (double)m;
+  double s = nan || m == __builtin_inff() ? (double)__builtin_nanf("") : 0.0;
+#pragma unroll 1
+  for (int o = j0 + tid * E; o < j1; o += kVdB * E) {  // (again from the cache: in f64 registers go to the exponentials)
+    const u4v r = R::load_upto(z, o, j1);
+#pragma unroll
+    for (int e = 0; e < E; e++) s += ex(((double)R::get(r, e) - ref) * c);
   }
   s = group_sum<kVdW>(s, redd);
-  if (tid == 0) a.pk[rr * a.G + g] = best, a.ps[rr * a.G + g] = s;
+  if (tid == 0) a.pk[rr * a.G + g] = __builtin_bit_cast(uint32_t, m), a.ps[rr * a.G + g] = s;
 }
 
 struct VdRow {
-  double m, s;
-  int best;
+  double m, s;  // maximum, and the sum of exp((z - m) / T); NaN without a distribution
+  int best;     // T = 0
 };
-// a row's maximum and sum from its slices, by one wave
-__device__ __forceinline__ VdRow vd_join(const VerifyArgs& a, int64_t rr) {
+// a row's from its slices, by one wave
+__device__ __forceinline__ VdRow vd_join(const VerifyArgs& a, const VdExp& ex, int64_t rr) {
   const int l = threadIdx.x & 63;
-  const double invt = a.temp > 0.0f ? 1.0 / (double)a.temp : 0.0;
-  uint64_t best = 0;
-  for (int g = l; g < a.G; g += 64) best = a.pk[rr * a.G + g] > best ? a.pk[rr * a.G + g] : best;
+  if (a.temp == 0.0f) {
+    uint64_t best = 0;
+    for (int g = l; g < a.G; g += 64) best = a.pk[rr * a.G + g] > best ? a.pk[rr * a.G + g] : best;
 #pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) {
-    const uint64_t o = __shfl_xor(best, m);
-    best = o > best ? o : best;
+    for (int m = 32; m >= 1; m >>= 1) {
+      const uint64_t o = __shfl_xor(best, m);
+      best = o > best ? o : best;
+    }
+    return VdRow{0.0, 0.0, key_index(best)};
   }
-  const double m = (double)key_value(best);
+  const double c = vd_scale(a);
+  float m = -__builtin_inff();
   double s = 0.0;
   for (int g = l; g < a.G; g += 64) {
-    const double pm = (double)key_value(a.pk[rr * a.G + g]);
-    if (pm != -__builtin_inf()) s += a.ps[rr * a.G + g] * exp((pm - m) * invt);
+    const float m2 = __builtin_bit_cast(float, (uint32_t)a.pk[rr * a.G + g]);
+    const double s2 = a.ps[rr * a.G + g];
+    if (m2 > m) {
+      s = s * (m == -__builtin_inff() ? 0.0 : ex(((double)m - m2) * c)) + s2;
+      m = m2;
+    } else {
+      s += s2 * (m2 == -__builtin_inff() ? 0.0 : ex(((double)m2 - m) * c));
+    }
   }
-  return VdRow{m, wave_sum_any(s), key_index(best)};
+  const float M = wave_max_any(m);
+  if (m != M) s *= m == -__builtin_inff() ? 0.0 : ex(((double)m - M) * c);
+  s = wave_sum_any(s);
+  return VdRow{(double)M, M == -__builtin_inff() ? (double)__builtin_nanf("") : s, -1};
 }
 
-// grid b, one wave: how many of sequence i's drafted tokens are accepted, and the row to draw from
+// How many of sequence i's drafted tokens are accepted, and the row to draw from: the workgroup's waves
+// test a token each, as many at a time as there are waves.  `write`: the outputs too.
 template <int VT>
-__device__ __forceinline__ void verify_accept(const VerifyArgs& a) {
+__device__ __forceinline__ VerifyPick vd_decide(const VerifyArgs& a, const VdExp& ex, int i, VerifyPick* lds, int* stop, bool write) {
   using R = VRow<VT>;
-  const int i = blockIdx.x, l = threadIdx.x;
-  const int len = a.lens ? min(max(a.lens[i], 0), a.d) : a.d;
-  const double invt = a.temp > 0.0f ? 1.0 / (double)a.temp : 0.0;
+  const int tid = threadIdx.x, l = tid & 63, wv = tid >> 6, len = vd_len(a, i);
+  const double c = vd_scale(a);
   const int64_t tr = (int64_t)a.b * (a.d + 1);
-  int acc = 0;
-  VdRow p{}, q{};
-  bool rejected = false;
-  int x = -1;
-  for (; acc <= len; acc++) {
-    const int64_t prow = (int64_t)i * (a.d + 1) + acc, qrow = (int64_t)i * a.d + acc;
-    p = vd_join(a, prow);
-    if (acc == len) break;
-    x = a.drafted[qrow];
-    const bool in = x >= 0 && x < a.V;
-    bool ok;
-    if (a.temp > 0.0f) {
-      const double px = in ? exp(((double)R::one(vd_row<VT>(a, false, prow), x) - p.m) * invt) / p.s : 0.0;
-      double qx = 1.0;
-      if (a.q) {
-        q = vd_join(a, tr + qrow);
-        qx = in ? exp(((double)R::one(vd_row<VT>(a, true, qrow), x) - q.m) * invt) / q.s : 0.0;
+  int at = 0, found = kVdW;
+  for (;; at += kVdW) {
+    const int j = at + wv;
+    bool here = false;  // the accepted end before j
+    if (j <= len) {
+      const int64_t prow = (int64_t)i * (a.d + 1) + j, qrow = (int64_t)i * a.d + j;
+      const int x = j < len ? a.drafted[qrow] : -1;
+      const bool in = x >= 0 && x < a.V;
+      const float zp = in && a.temp > 0.0f ? R::one(vd_row<VT>(a, false, prow), x) : 0.0f;
+      const float zq = in && a.q && j < len ? R::one(vd_row<VT>(a, true, qrow), x) : 0.0f;
+      const VdRow p = vd_join(a, ex, prow);
+      VerifyPick v;
+      v.row = j, v.pm = p.m, v.ps = 1.0 / p.s, v.qm = 0.0, v.qs = 0.0, v.not_x = -1, v.minus_q = 0, v.best = p.best;
+      if (j == len) {
+        here = true;
+      } else if (a.temp > 0.0f) {
+        // (a NaN row gives a NaN probability, which accepts nothing)
+        const double px = in ? (p.s != p.s ? p.s : ex(((double)zp - p.m) * c) / p.s) : 0.0;
+        double qx = 1.0;
+        if (a.q) {
+          const VdRow q = vd_join(a, ex, tr + qrow);
+          qx = in ? (q.s != q.s ? q.s : ex(((double)zq - q.m) * c) / q.s) : 0.0;
+          v.qm = q.m, v.qs = 1.0 / q.s, v.minus_q = 1;
+        } else {
+          v.not_x = x;
+        }
+        here = !((double)a.u[(int64_t)i * (a.d + 1) + j] * qx < px);
+      } else {
+        here = !(in && x == p.best);
       }
-      ok = (double)a.u[(int64_t)i * (a.d + 1) + acc] * qx < px;
-    } else {
-      ok = in && x == p.best;
+      if (here && l == 0) lds[wv] = v;
     }
-    if (!ok) {
-      rejected = true;
-      break;
-    }
+    if (l == 0) stop[wv] = here;
+    __syncthreads();
+    found = kVdW;
+#pragma unroll
+    for (int w = kVdW - 1; w >= 0; w--) found = stop[w] ? w : found;
+    if (found < kVdW) break;  // (the wave of j == len stops at the latest)
+    __syncthreads();
   }
-  for (int j = l; j <= a.d; j += 64)
-    a.tokens[(int64_t)i * (a.d + 1) + j] = j < acc ? a.drafted[(int64_t)i * a.d + j] : (j == acc && a.temp == 0.0f) ? p.best : -1;
-  if (l == 0) {
-    a.accepted[i] = acc;
-    VerifyPick v;
-    v.pm = p.m, v.ps = 1.0 / p.s, v.qm = q.m, v.qs = rejected && a.q ? 1.0 / q.s : 0.0;
-    v.row = acc, v.not_x = rejected && !a.q ? x : -1, v.minus_q = rejected && a.q ? 1 : 0, v.pad = 0;
-    a.pick[i] = v;
+  const VerifyPick v = lds[found];
+  if (write) {
+    for (int j = tid; j <= a.d; j += kVdB)
+      a.tokens[(int64_t)i * (a.d + 1) + j] = j < v.row ? a.drafted[(int64_t)i * a.d + j] : j == v.row && a.temp == 0.0f ? v.best : -1;
+    if (tid == 0) a.accepted[i] = v.row, a.pick[i] = v;
   }
+  return v;
+}
+
+// grid b: T = 0
+template <int VT>
+__device__ __forceinline__ void verify_greedy(const VerifyArgs& a) {
+  __shared__ VerifyPick lds[kVdW];
+  __shared__ int stop[kVdW];
+  VdExp none;
+  vd_decide<VT>(a, none, blockIdx.x, lds, stop, true);
 }
 
 // the weight of token v: max(p - q, 0) after a rejection, or p
-__device__ __forceinline__ double vd_weight(const VerifyPick& k, float zp, float zq, int v, double invt, double& p) {
-  p = exp(((double)zp - k.pm) * invt) * k.ps;
-  if (k.minus_q) return fmax(p - exp(((double)zq - k.qm) * invt) * k.qs, 0.0);
+__device__ __forceinline__ double vd_weight(const VerifyPick& k, const VdExp& ex, double c, float zp, float zq, int v, double& p) {
+  p = ex(((double)zp - k.pm) * c) * k.ps;
+  if (k.minus_q) return fmax(p - ex(((double)zq - k.qm) * c) * k.qs, 0.0);
   return v == k.not_x ? 0.0 : p;
 }
 
-// grid (G, b): the weights' sum over slice g of sequence i's row, and p's
+// grid (G, b): the weights' sums over the quarters of slice g of sequence i's row, a wave each, and p's (each workgroup
+// decides again which row)
 template <int VT>
 __device__ __forceinline__ void verify_mass(const VerifyArgs& a) {
   using R = VRow<VT>;
-  __shared__ double redd[kVdW];
+  constexpr int E = R::E;
+  __shared__ VerifyPick lds[kVdW];
+  __shared__ int stop[kVdW];
+  __shared__ VdExp ex;
   const int tid = threadIdx.x, g = blockIdx.x, i = blockIdx.y;
-  const VerifyPick k = a.pick[i];
+  ex.fill();
+  __syncthreads();
+  const VerifyPick k = vd_decide<VT>(a, ex, i, lds, stop, g == 0);
   const void* zp = vd_row<VT>(a, false, (int64_t)i * (a.d + 1) + k.row);
   const void* zq = k.minus_q ? vd_row<VT>(a, true, (int64_t)i * a.d + k.row) : zp;
-  const int j0 = g * a.L, j1 = min(a.V, j0 + a.L);
-  const double invt = 1.0 / (double)a.temp;
-  double sw = 0.0, sp = 0.0;
-  for (int v = j0 + tid * R::E; v < j1; v += kVdB * R::E) {
-    const u4v r = R::load_upto(zp, v, j1), rq = R::load_upto(zq, v, j1);
+  const int q = g * kVdW + (tid >> 6), j0 = q * (a.L / kVdW), j1 = min(a.V, j0 + a.L / kVdW);
+  const double c = vd_scale(a);
+  double sw = 0.0, sp = k.ps != k.ps ? k.ps : 0.0;
+#pragma unroll 1
+  for (int v = j0 + (tid & 63) * E; v < j1; v += 64 * E) {
+    const u4v r = R::load_upto(zp, v, j1);
+    u4v rq = r;
+    if (k.minus_q) rq = R::load_upto(zq, v, j1);
 #pragma unroll
-    for (int e = 0; e < R::E; e++) {
+    for (int e = 0; e < E; e++) {
       double p;
-      sw += vd_weight(k, R::get(r, e), R::get(rq, e), v + e, invt, p);
+      sw += vd_weight(k, ex, c, R::get(r, e), R::get(rq, e), v + e, p);
       sp += p;
     }
   }
-  sw = group_sum<kVdW>(sw, redd);
-  sp = group_sum<kVdW>(sp, redd);
-  if (tid == 0) a.mass[((int64_t)i * a.G + g) * 2] = sw, a.mass[((int64_t)i * a.G + g) * 2 + 1] = sp;
+  sw = wave_sum_any(sw);
+  sp = wave_sum_any(sp);
+  if ((tid & 63) == 0) {
+    double* out = a.mass + ((int64_t)i * a.G * kVdW + q) * 2;
+    out[0] = sw, out[1] = sp;
+  }
 }
 
-// grid b: the slice that holds u_d times the total, then the token in it
+// the sum over the lanes below this one, and over all
+__device__ __forceinline__ double wave_before(double v, double* all) {
+  const int l = threadIdx.x & 63;
+  double s = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const double o = __shfl_up(s, d);
+    s += l >= d ? o : 0.0;
+  }
+  *all = __shfl(s, 63);
+  const double b = __shfl_up(s, 1);
+  return l ? b : 0.0;
+}
+
+// grid b: the quarter slice that holds u_d times the total, then the token in it (1024 threads, consecutive logits
+// each)
+constexpr int kPickVdB = 1024, kVdMass = 8;  // kVdMass: quarter slices a lane at most (2^20 logits of f32: 512)
 template <int VT>
 __device__ __forceinline__ void verify_pick(const VerifyArgs& a) {
   using R = VRow<VT>;
-  __shared__ double part[kVdB];
-  __shared__ int sslice, sall, token;
+  constexpr int E = R::E, N = E / 2, W = kPickVdB / 64;  // L / 4 = kVdB kVdV E / 4 = kPickVdB N
+  __shared__ double part[W];
+  __shared__ VdExp ex;
+  __shared__ int sslice, sall, first, lastw;
   __shared__ double starget;
-  const int tid = threadIdx.x, i = blockIdx.x;
+  const int tid = threadIdx.x, i = blockIdx.x, Q = a.G * kVdW;
   VerifyPick k = a.pick[i];
-  const double* mass = a.mass + (int64_t)i * a.G * 2;
-  if (tid == 0) {
-    double tot = 0.0;
-    for (int g = 0; g < a.G; g++) tot += mass[2 * g];
+  if (tid < 64) {  // lane l: quarters per l .. per l + per - 1
+    const double* mass = a.mass + (int64_t)i * Q * 2;
+    const int per = (Q + 63) / 64;
+    double w[kVdMass], p[kVdMass], sw = 0.0, sp = 0.0;
+#pragma unroll
+    for (int q = 0; q < kVdMass; q++) {
+      const int at = tid * per + q;
+      const bool in = q < per && at < Q;
+      w[q] = in ? mass[2 * at] : 0.0, p[q] = in ? mass[2 * at + 1] : 0.0;
+    }
+    const float u = a.u[(int64_t)i * (a.d + 1) + a.d];
+#pragma unroll
+    for (int q = 0; q < kVdMass; q++) sw += w[q], sp += p[q];
+    double tot, totp, before = wave_before(sw, &tot), beforep = wave_before(sp, &totp);
     const int all = tot > 0.0 ? 0 : 1;  // p - q is nowhere positive: drawn from p
-    if (all) {
-      tot = 0.0;
-      for (int g = 0; g < a.G; g++) tot += mass[2 * g + 1];
+    if (all) tot = totp, before = beforep;
+    const double t = (double)u * tot;
+    // the first quarter whose running sum passes t, or (rounding) the last that has weight
+    int pass = 1 << 30, has = -1;
+    double lo = 0.0, at_pass = 0.0, at_has = 0.0;
+#pragma unroll
+    for (int q = 0; q < kVdMass; q++) {
+      const double x = all ? p[q] : w[q];
+      if (x > 0.0) {
+        has = tid * per + q, at_has = before + lo;
+        if (pass == 1 << 30 && before + lo + x > t) pass = has, at_pass = at_has;
+      }
+      lo += x;
     }
-    const double t = (double)a.u[(int64_t)i * (a.d + 1) + a.d] * tot;
-    double c = 0.0, before = 0.0;
-    int s = -1;
-    for (int g = 0; g < a.G; g++) {
-      const double w = mass[2 * g + all];
-      if (w > 0.0) s = g, before = c;
-      c += w;
-      if (c > t) break;
-    }
-    sslice = tot > 0.0 ? s : -1, sall = all, starget = t - before, token = -1;  // NaN: no token
+    const uint64_t mp = __ballot(pass < (1 << 30)), mh = __ballot(has >= 0);
+    const int lane = mp ? __builtin_ctzll(mp) : mh ? 63 - __builtin_clzll(mh) : 0;
+    const int slice = __shfl(mp ? pass : has, lane);
+    const double base = __shfl(mp ? at_pass : at_has, lane);
+    if (tid == 0) sslice = tot > 0.0 ? slice : -1, sall = all, starget = t - base, first = 1 << 30, lastw = -1;  // NaN: no token
+  } else if (tid < 64 + 16) {
+    ex.tab[tid - 64] = exp2((double)(tid - 64) / 16.0);
   }
   __syncthreads();
   if (sslice < 0) return;
   if (sall) k.minus_q = 0, k.not_x = -1;
   const void* zp = vd_row<VT>(a, false, (int64_t)i * (a.d + 1) + k.row);
   const void* zq = k.minus_q ? vd_row<VT>(a, true, (int64_t)i * a.d + k.row) : zp;
-  const double invt = 1.0 / (double)a.temp;
-  const int j0 = sslice * a.L, j1 = min(a.V, j0 + a.L), per = (a.L + kVdB - 1) / kVdB;
-  const int v0 = j0 + tid * per, v1 = min(j1, v0 + per);
-  auto weight = [&](int v) {
-    double p;
-    return vd_weight(k, R::one(zp, v), R::one(zq, v), v, invt, p);
-  };
-  double s = 0.0;
+  const double c = vd_scale(a);
+  const int j0 = sslice * (a.L / kVdW), j1 = min(a.V, j0 + a.L / kVdW), v0 = j0 + tid * N;
+  float fp[N], fq[N];
+#pragma unroll
+  for (int e = 0; e < N; e++) fp[e] = v0 + e < j1 ? R::one(zp, v0 + e) : 0.0f, fq[e] = v0 + e < j1 && k.minus_q ? R::one(zq, v0 + e) : 0.0f;
+  double w[N], s = 0.0;
   int last = -1;
-  for (int v = v0; v < v1; v++) {
-    const double w = weight(v);
-    s += w;
-    if (w > 0.0) last = v;
+#pragma unroll
+  for (int e = 0; e < N; e++) {
+    double p;
+    w[e] = v0 + e < j1 ? vd_weight(k, ex, c, fp[e], fq[e], v0 + e, p) : 0.0;
+    s += w[e];
+    last = w[e] > 0.0 ? v0 + e : last;
   }
-  part[tid] = s;
+  double sum;
+  double before = wave_before(s, &sum);
+  if ((tid & 63) == 0) part[tid >> 6] = sum;
   __syncthreads();
-  double before = 0.0;
-  for (int q = 0; q < tid; q++) before += part[q];
-  // the first thread whose running sum passes the target; rounding may leave none: then the last
-  // token of the slice that has weight
-  int mine = 1 << 30;
-  if (before + s > starget && last >= 0) {
-    double c = before;
-    for (int v = v0; v < v1; v++) {
-      c += weight(v);
-      if (c > starget) {
-        mine = v;
-        break;
-      }
+  for (int q = 0; q < (tid >> 6); q++) before += part[q];
+  // the first logit whose running sum passes the target; rounding may leave none: then the last of the
+  // quarter that has weight
+  if (last >= 0) {
+    double t = before;
+    int mine = 1 << 30;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      t += w[e];
+      mine = w[e] > 0.0 && t > starget ? min(mine, v0 + e) : mine;
     }
-    if (mine == 1 << 30) mine = last;
+    if (mine < (1 << 30)) atomicMin(&first, mine);
+    atomicMax(&lastw, last);
   }
-  __shared__ int first, lastw;
-  if (tid == 0) first = 1 << 30, lastw = -1;
-  __syncthreads();
-  atomicMin(&first, mine);
-  atomicMax(&lastw, last);
   __syncthreads();
   if (tid == 0) a.tokens[(int64_t)i * (a.d + 1) + k.row] = first < (1 << 30) ? first : lastw;
 }
 
 #define RTQ_VERIFY(ty, VT)                                                                                              \
   extern "C" __global__ __launch_bounds__(kVdB) void rtq_verify_stats_##ty(VerifyArgs a) { verify_stats<VT>(a); }       \
-  extern "C" __global__ __launch_bounds__(64) void rtq_verify_accept_##ty(VerifyArgs a) { verify_accept<VT>(a); }       \
+  extern "C" __global__ __launch_bounds__(kVdB) void rtq_verify_greedy_##ty(VerifyArgs a) { verify_greedy<VT>(a); }     \
   extern "C" __global__ __launch_bounds__(kVdB) void rtq_verify_mass_##ty(VerifyArgs a) { verify_mass<VT>(a); }         \
-  extern "C" __global__ __launch_bounds__(kVdB) void rtq_verify_pick_##ty(VerifyArgs a) { verify_pick<VT>(a); }
+  extern "C" __global__ __launch_bounds__(kPickVdB) void rtq_verify_pick_##ty(VerifyArgs a) { verify_pick<VT>(a); }
 RTQ_VERIFY(f32, VT_F32)
 RTQ_VERIFY(f16, VT_F16)
 RTQ_VERIFY(bf16, VT_BF16)
