@@ -1972,15 +1972,15 @@ int64_t distill_lds(int rows, int64_t V) { return ((256 << rows) - 64) * 8 * 16 
 // logits (1.15 of 16 bits; without the gradient 0.65 and 0.48).  So slices run few rows of a large vocabulary
 // (151936 f32, 16 rows: 17 us against 40; 256 rows: 103 against 68), and many such rows without a gradient (1024:
 // 118 against 134).
-// Of the workgroup sizes, each holds 24 vectors of 16 bytes a thread on the chip.  256 threads let four rows
-// share a CU, 512 two: better where they hold the row and there are enough (8192 f32, 2048 rows: 37 / 44 / 66
+// Of the workgroup sizes, each holds 24 vectors of 16 bytes a thread on the chip, 22 of 16-bit logits.  256
+// threads let four rows share a CU, 512 two: better where they hold the row and there are enough (8192 f32, 2048 rows: 37 / 44 / 66
 // us; 64000 bf16, 512 rows: 50 / 43 / 48), while one row alone is fastest on the largest that it fills (32000
 // f32: 25 / 15 / 13).
 DistillPlan distill_plan(const rtq_ctx* c, int type, int64_t n, int64_t V, int64_t k, bool grad) {
-  const int64_t E = 16 / logit_bytes(type), cus = c->cu_count;
+  const int64_t E = 16 / logit_bytes(type), per = E == 4 ? 24 : 22, cus = c->cu_count;
   DistillPlan p{};
-  if (V <= 24 * 192 * E) p.rows = n > 2 * cus ? 0 : 1;
-  else p.rows = n > cus && V <= 36 * 448 * E ? 1 : 2;
+  if (V <= per * 192 * E) p.rows = n > 2 * cus ? 0 : 1;
+  else p.rows = n > cus && 2 * V <= 3 * per * 448 * E ? 1 : 2;
   const double v = (double)V, all = v * (double)n, more = n > cus ? (double)n / (double)cus : 1.0;
   const double one = 7.5 + more * v * (grad ? 0.2e-3 : n > cus ? 0.2e-3 : 0.12e-3);
   const double cut = grad ? 14.0 + all * (E == 4 ? 2.3e-6 : 1.15e-6) : 12.5 + all * (E == 4 ? 0.65e-6 : 0.48e-6);
