@@ -354,7 +354,7 @@ struct HeadArgs {
 
 // ---------------------------------------------------------------- rows of vocabulary logits
 // z: rows of V logits (f32, f16 or bf16), stride ld elements; where a row is cut, into G slices of L
-// logits.  ch + cl = log2(e) / temp.
+// logits.  c = log2(e) / temp.
 #ifndef RTQ_TOP_MAX
 #define RTQ_TOP_MAX 256 /* as in rtq.h */
 #endif
@@ -363,7 +363,7 @@ struct TopArgs {
   int64_t ld;
   int n, V, k;
   int NG;  // groups per row (32 f32 or 64 16-bit logits each), rounded up to whole chunks of 64
-  float temp, ch, cl;
+  float temp, c;
   float* gm;     // [n x NG] each group's maximum (NaN if it holds one)
   float* gs;     // [n x NG] and its sum of exp((z - maximum) / temp)
   float* vals;   // [n x k]
@@ -378,7 +378,7 @@ struct DistillArgs {
   void* dz;  // [n x V] gradient, stride ldd (may be z itself)
   int64_t ld, ldd;
   int n, V, k, G, L;
-  float temp, ch, cl, hard;
+  float temp, c, hard;
   const int32_t* ids;  // [n x k] the teacher's tokens (outside [0, V): no token)
   const float* tv;     // [n x k] its logits
   const float* rest;   // [n] log-sum-exp of its other logits / temp, or null

@@ -1908,12 +1908,8 @@ rtq_status check_rows(const void* z, int type, int64_t n, int64_t vocab, int64_t
 
 rtq_status check_ctx(const rtq_ctx* c) { return c ? RTQ_OK : fail(RTQ_ERR_INVALID, "null context"); }
 
-// log2(e) / t as the sum of two floats
-void exp_scale(float t, float* hi, float* lo) {
-  const double e = 1.4426950408889634 / (double)t;
-  *hi = (float)e;
-  *lo = (float)(e - (double)*hi);
-}
+// log2(e) / t: exp(x / t) = exp2(x c)
+float exp_scale(float t) { return (float)(1.4426950408889634 / (double)t); }
 
 // ---- top logits
 struct TopPlan {
@@ -1945,7 +1941,7 @@ rtq_status enqueue_top(rtq_ctx* c, const void* z, int type, int64_t n, int64_t V
   a.pos = pos, a.t = (int)t;
   a.z = z, a.ld = ld, a.n = (int)n, a.V = (int)V, a.k = (int)k, a.NG = (int)p.NG;
   a.temp = temp;
-  exp_scale(temp, &a.ch, &a.cl);
+  a.c = exp_scale(temp);
   a.vals = vals, a.ids = ids, a.rest = rest;
   a.gm = ar.take<float>((size_t)(n * p.NG));
   a.gs = ar.take<float>((size_t)(n * p.NG));
@@ -2029,7 +2025,7 @@ rtq_status enqueue_distill(rtq_ctx* c, const void* z, int type, int64_t n, int64
   a.z = z, a.dz = dz, a.ld = ld, a.ldd = ldd;
   a.n = (int)n, a.V = (int)V, a.k = (int)t.k, a.G = (int)p.G, a.L = (int)p.L;
   a.temp = t.temperature;
-  exp_scale(t.temperature, &a.ch, &a.cl);
+  a.c = exp_scale(t.temperature);
   a.hard = hard, a.ids = t.ids, a.tv = t.vals, a.rest = t.rest, a.tok = tok, a.w = w, a.kl = kl, a.logp = logp;
   const int ty = logit_type(type);
   if (p.rows >= 0)

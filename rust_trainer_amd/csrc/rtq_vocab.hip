@@ -83,16 +83,6 @@ struct VRow {
   }
 };
 
-// exp(t / T) for t <= 0 as exp2(t c), c = log2(e) / T given as ch + cl: the product's rounding and
-// cl enter to first order, so the result is near the exponential instruction's own last place at
-// every t (the plain product is off by |t c| 2^-24, which a small divergence would show)
-__device__ __forceinline__ float exp_scaled(float t, float ch, float cl) {
-  const float y = t * ch;
-  const float d = fmaf(t, cl, fmaf(t, ch, -y));
-  const float e = __builtin_amdgcn_exp2f(y);
-  return y < -150.0f ? 0.0f : fmaf(e, d * 0.693147181f, e);  // -inf and overflows of t ch among them
-}
-
 // whether row i has logits (rows formed at positions: the position is one of the sequence's)
 template <class Args>
 __device__ __forceinline__ bool row_ok(const Args& a, int i) {
@@ -247,7 +237,7 @@ __device__ __forceinline__ void top_scan(const TopArgs& a) {
     const float ref = m == ninf ? 0.0f : m;
     float s = 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; e++) s += __builtin_amdgcn_exp2f((R::get(raw[u], e) - ref) * a.ch);
+    for (int e = 0; e < E; e++) s += __builtin_amdgcn_exp2f((R::get(raw[u], e) - ref) * a.c);
     s = oct_sum(s);
     if (__ballot(s != s)) {  // a NaN, or infinity less itself
       float bad = 0.0f;
@@ -326,12 +316,12 @@ __device__ __forceinline__ void join_rest(float& m, double& s, const float* x, c
   if (nan) s = (double)__builtin_nanf("");
   if (b == -__builtin_inff()) return;
   if (b > m) {
-    s *= (double)__builtin_amdgcn_exp2f((m - b) * a.ch);
+    s *= (double)__builtin_amdgcn_exp2f((m - b) * a.c);
     m = b;
   }
   float t = 0.0f;
 #pragma unroll
-  for (int e = 0; e < N; e++) t += w[e] != 0.0f ? w[e] * __builtin_amdgcn_exp2f((x[e] - m) * a.ch) : 0.0f;
+  for (int e = 0; e < N; e++) t += w[e] != 0.0f ? w[e] * __builtin_amdgcn_exp2f((x[e] - m) * a.c) : 0.0f;
   s += (double)t;
 }
 
@@ -560,7 +550,7 @@ __device__ __forceinline__ void top_pick(const TopArgs& a) {
   }
   if (!a.rest) return;
   const float m = group_max<W>(rm, redf);
-  rs = group_sum<W>(rm == ninf ? rs : rs * (double)__builtin_amdgcn_exp2f((rm - m) * a.ch), redd);
+  rs = group_sum<W>(rm == ninf ? rs : rs * (double)__builtin_amdgcn_exp2f((rm - m) * a.c), redd);
   if (tid == 0) a.rest[i] = lse_of(m, rs, 1.0 / (double)a.temp);
 }
 
@@ -645,7 +635,7 @@ struct DisSum {
   double sT = 0.0, s1 = 0.0;
   __device__ __forceinline__ void raise(float m2, const DistillArgs& a) {  // to the reference of m2 >= m
     const bool none = m == -__builtin_inff();  // (a NaN sum stays)
-    sT *= none ? 0.0 : (double)__builtin_amdgcn_exp2f((float)(ref_in(m, a.ch) - ref_in(m2, a.ch)));
+    sT *= none ? 0.0 : (double)__builtin_amdgcn_exp2f((float)(ref_in(m, a.c) - ref_in(m2, a.c)));
     s1 *= none ? 0.0 : (double)__builtin_amdgcn_exp2f((float)(ref_in(m, kLog2eF) - ref_in(m2, kLog2eF)));
     m = m2;
   }
@@ -735,7 +725,7 @@ struct DisSlice {
       if (odd) up = (float)(ref_in(old, c) - ref_in(m, c));
       s = fma(s, (double)__builtin_amdgcn_exp2f(up), (double)(t[0] + t[1]));
     };
-    sum(d.sT, a.ch);
+    sum(d.sT, a.c);
     if (two) sum(d.s1, kLog2eF);
     d.m = m;
   }
@@ -829,8 +819,8 @@ struct DisSlice {
     const float C = sh.C, D = sh.D;
     if (C == 0.0f && D == 0.0f) return write<0>(out, row, 0, 0, 0, 0, 0, 0);
     const bool one = D == 0.0f || C == 0.0f || a.temp == 1.0f, label = one && C == 0.0f;
-    if (one) write<1>(out, row, C + D, label ? kLog2eF : a.ch, label ? sh.K1 : sh.KT, 0, 0, sh.base);
-    else write<2>(out, row, C, a.ch, sh.KT, D, sh.K1, sh.base);
+    if (one) write<1>(out, row, C + D, label ? kLog2eF : a.c, label ? sh.K1 : sh.KT, 0, 0, sh.base);
+    else write<2>(out, row, C, a.c, sh.KT, D, sh.K1, sh.base);
   }
 };
 
@@ -891,7 +881,7 @@ __device__ __forceinline__ void distill_teacher(const DistillArgs& a, DisShared&
   for (int s = l; s < a.k; s += 64) {
     const float zs = sh.zs[s];
     if (!sh.first[s] || zs == ninf) continue;
-    st.ZT += exp2(((double)zs - st.ml) * (double)a.ch);
+    st.ZT += exp2(((double)zs - st.ml) * (double)a.c);
     if (a.tok) st.Z1 += exp2(((double)zs - st.ml) * (double)kLog2eF);
   }
   st.ZT = wave_sum_any(st.ZT);
@@ -920,7 +910,7 @@ struct DisNorms {
 __device__ __forceinline__ void distill_scalars(const DistillArgs& a, DisShared& sh, const DisTeacher& st, const DisSum& d, float w_, DisNorms& nm) {
   const bool empty = d.m == -__builtin_inff(), label = sh.tok >= 0;
   double fT, f1 = 0.0;
-  nm.sum[0] = distill_norm(a.ch, st.ml, st.ZT, d.m, d.sT, st.nan, &nm.top[0], &fT);
+  nm.sum[0] = distill_norm(a.c, st.ml, st.ZT, d.m, d.sT, st.nan, &nm.top[0], &fT);
   nm.sum[1] = 1.0, nm.top[1] = 0.0;
   if (a.tok) nm.sum[1] = distill_norm(kLog2eF, st.ml, st.Z1, d.m, d.s1, st.nan, &nm.top[1], &f1);
   const double w = (double)w_, pr = sh.pr;
@@ -929,14 +919,14 @@ __device__ __forceinline__ void distill_scalars(const DistillArgs& a, DisShared&
   if ((threadIdx.x & 63) == 0) {
     sh.C = wT == 0.0 || (empty && nm.sum[0] == nm.sum[0]) ? 0.0f : (float)(wT * (fT - (pr > 0.0 ? pr / d.sT : 0.0)));
     sh.D = w1 == 0.0 || (empty && nm.sum[1] == nm.sum[1]) ? 0.0f : (float)(w1 * f1);
-    sh.KT = ref_of(d.m, a.ch), sh.K1 = ref_of(d.m, kLog2eF), sh.base = ref_base(d.m), sh.wgT = wT, sh.wg1 = w1;
+    sh.KT = ref_of(d.m, a.c), sh.K1 = ref_of(d.m, kLog2eF), sh.base = ref_base(d.m), sh.wgT = wT, sh.wg1 = w1;
   }
 }
 
 // log2 of the two normalisers and of the unlisted sum, for the losses and the gradient at the listed tokens
 __device__ __forceinline__ void distill_logs(const DistillArgs& a, DisShared& sh, const DisSum& d, const DisNorms& nm) {
   const double LT = nm.top[0] + log2(nm.sum[0]), L1 = a.tok ? nm.top[1] + log2(nm.sum[1]) : 0.0;
-  const double lu = d.m == -__builtin_inff() ? -__builtin_inf() : ref_in(d.m, a.ch) + log2(d.sT);
+  const double lu = d.m == -__builtin_inff() ? -__builtin_inf() : ref_in(d.m, a.c) + log2(d.sT);
   if ((threadIdx.x & 63) == 0) sh.LT = LT, sh.L1 = L1, sh.lu = lu;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
@@ -944,7 +934,7 @@ __device__ __forceinline__ void distill_logs(const DistillArgs& a, DisShared& sh
 // the losses, by the wave that formed the scalars
 __device__ __forceinline__ void distill_losses(const DistillArgs& a, const DisShared& sh, int i) {
   const int l = threadIdx.x & 63;
-  const double c = (double)a.ch, pr = sh.pr;
+  const double c = (double)a.c, pr = sh.pr;
   double kl = 0.0;
   for (int s = l; s < a.k; s += 64) {
     const double p = sh.p[s];
@@ -963,7 +953,7 @@ template <int VT, class Marks>
 __device__ __forceinline__ void distill_marked(const DistillArgs& a, const DisShared& sh, const Marks& mk, void* out, int j0, int j1) {
   using R = VRow<VT>;
   const int l = threadIdx.x & 63;
-  const double c = (double)a.ch;
+  const double c = (double)a.c;
   for (int s = l; s < a.k; s += 64) {
     const int id = sh.id[s];
     if (!sh.first[s] || id < j0 || id >= j1) continue;
