@@ -194,7 +194,7 @@ rtq_status rtq_top_logits_d(rtq_ctx* ctx, const void* logits, int type, int64_t 
  * With weights (else NULL, and dlogits unused), for L = sum weights[i] ((1 - hard) T^2 kl[i] - hard logp[i]),
  * hard in [0, 1]: dlogits [n x vocab], rows ldd elements apart, = dL/dz in the logits' type, OVERWRITTEN;
  * it may be the logits themselves (same ldd), and must not overlap them otherwise.  A row of weight 0
- * has gradient 0.  A NaN logit, or a row of -inf alone, makes the row's outputs NaN. */
+ * has gradient 0.  A NaN or +inf logit, or a row of -inf alone, makes the row's outputs NaN. */
 rtq_status rtq_distill(rtq_ctx* ctx, const void* logits, int type, int64_t n, int64_t vocab, int64_t ld,
                        const rtq_teacher* teacher, const int32_t* tok, const float* weights, float hard, float* kl,
                        float* logp, void* dlogits, int64_t ldd);
@@ -213,8 +213,9 @@ rtq_status rtq_distill_d(rtq_ctx* ctx, const void* logits, int type, int64_t n, 
  * temperature 0: accepted while x_j is the row's largest logit (the lowest id of equals), which is also the
  * token drawn; draft and uniforms are not read.  accepted [b]; tokens [b x (d + 1)]: the accepted ones,
  * the drawn one, -1 after.  A drafted id outside [0, vocab) is rejected (host version: refused).  Rows
- * past a sequence's length are not read.  A row without a distribution (a NaN, or -inf alone) accepts
- * nothing and draws -1. */
+ * past a sequence's length are not read.  A target row without a distribution (a NaN, +inf or -inf alone; at
+ * temperature 0 a NaN or -inf alone) accepts nothing and draws -1; a draft row without one accepts nothing,
+ * and the token is drawn from p. */
 rtq_status rtq_verify_draft(rtq_ctx* ctx, const void* logits, int type, int64_t ld, const void* draft, int64_t ldq,
                             int64_t b, int64_t d, int64_t vocab, const int32_t* drafted, const int32_t* lens,
                             const float* uniforms, float temperature, int32_t* accepted, int32_t* tokens);

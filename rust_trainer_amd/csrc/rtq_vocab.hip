@@ -1283,7 +1283,7 @@ __device__ __forceinline__ void verify_stats(const VerifyArgs& a) {
 
 struct VdRow {
   double m, s;  // maximum, and the sum of exp((z - m) / T); NaN without a distribution
-  int best;     // T = 0
+  int best;     // T = 0: the largest logit's index, -1 without a distribution
 };
 // a row's from its slices, by one wave
 __device__ __forceinline__ VdRow vd_join(const VerifyArgs& a, const VdExp& ex, int64_t rr) {
@@ -1296,7 +1296,8 @@ __device__ __forceinline__ VdRow vd_join(const VerifyArgs& a, const VdExp& ex, i
       const uint64_t o = __shfl_xor(best, m);
       best = o > best ? o : best;
     }
-    return VdRow{0.0, 0.0, key_index(best)};
+    const float z = key_value(best);  // NaN or -inf: no token
+    return VdRow{0.0, 0.0, z > -__builtin_inff() ? key_index(best) : -1};
   }
   const double c = vd_scale(a);
   float m = -__builtin_inff();

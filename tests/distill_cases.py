@@ -83,7 +83,12 @@ def verify(z, q, drafted, lens, u, temp):
     z = np.asarray(z, np.float64).reshape(b, d + 1, V)
     q = None if q is None else np.asarray(q, np.float64).reshape(b, d, V)
     acc, out = np.zeros(b, np.int32), np.full((b, d + 1), -1, np.int32)
-    soft = lambda x: np.exp(x / temp - lse(x / temp))  # noqa: E731
+    soft = lambda x: np.exp(x / temp - lse(x / temp)) if np.isfinite(x.max()) else np.full(V, np.nan)  # noqa: E731
+
+    def best(row):  # of the logits, -1 without a distribution
+        v, j, _ = top(row[None], 1, 1.0)
+        return j[0, 0] if v[0, 0] > NEG else -1
+
     with np.errstate(all="ignore"):
         for i in range(b):
             n = d if lens is None else min(max(int(lens[i]), 0), d)
@@ -92,7 +97,7 @@ def verify(z, q, drafted, lens, u, temp):
                 x = int(drafted[i, a])
                 ok = 0 <= x < V
                 if temp == 0:
-                    ok = ok and x == top(z[i, a][None], 1, 1.0)[1][0, 0]
+                    ok = ok and x == best(z[i, a])
                 else:
                     p = soft(z[i, a])
                     qa = np.arange(V) == x if q is None else soft(q[i, a])
@@ -107,7 +112,7 @@ def verify(z, q, drafted, lens, u, temp):
                 a += 1
             acc[i] = a
             if temp == 0:
-                out[i, a] = top(z[i, a][None], 1, 1.0)[1][0, 0]
+                out[i, a] = best(z[i, a])
                 continue
             if w is None:
                 w = soft(z[i, a])

@@ -355,6 +355,29 @@ def test_verify_draft_at_the_edges(ctx):
     check_verify(ctx, zp, zq, x, lens, u, 1.0)
 
 
+def test_verify_draft_rows_without_a_distribution(ctx):
+    """A target row of -inf alone, with a NaN or with +inf draws nothing (at temperature 0 the last has a largest
+    logit); a draft row like that accepts nothing and leaves the draw to the target."""
+    b, d, V = 7, 2, 5003
+    rng = np.random.default_rng(14)
+    zp = D.logits(rng, b * (d + 1), V)
+    zq = D.logits(rng, b * d, V, near=zp.reshape(b, d + 1, V)[:, :d].reshape(b * d, V))
+    T, Q = zp.reshape(b, d + 1, V), zq.reshape(b, d, V)
+    x = np.argmax(T[:, :d], 2)
+    u = np.zeros((b, d + 1))
+    u[:, d] = 0.5
+    for i, v in enumerate((np.nan, -np.inf, np.inf)):
+        at = slice(None) if v == -np.inf else 4321
+        T[i, i % d + (i == 2), at] = v  # rows 0, 1 and the last
+        Q[3 + i, 1, at] = v
+    for temp in (1.0, 0.0):
+        for ty in ("f32", "f16", "bf16"):
+            check_verify(ctx, zp, zq, x, None, u, temp, ty)
+            check_verify(ctx, zp, None, x, None, u, temp, ty)
+    acc, out = D.verify(zp, zq, x, None, u, 1.0)
+    assert acc[:6].tolist() == [0, 1, 1, 1, 1, 1] and out[0, 0] == out[1, 1] == out[2, 1] == -1 and (out[3:6, 1] >= 0).all()
+
+
 def test_host_calls_and_their_refusals(ctx):
     rng = np.random.default_rng(6)
     n, V, k = 5, 1003, 7
