@@ -1174,31 +1174,33 @@ RTQ_DISTILL(bf16, VT_BF16)
 // drawn from max(p - q, 0) at the first rejection, from p after all: the first index whose running sum
 // passes u_d times the total.  T = 0: accept while x_j is the target's largest logit (the lowest index
 // of equals), which is also the token after.  Steps of the running sum over a flat tail lie nearer
-// than 2^-24 of the total, so exponentials and sums are in 64 bits, whose arithmetic bounds the statistics (384 rows
-// of 151936 bf16 logits in 56 us, 2.1 TB/s).
+// than 2^-24 of the total, so exponentials and sums are in 64 bits, whose arithmetic bounds the statistics (384
+// rows of 151936 bf16 logits: 51 us, 2.3 TB/s; in one pass with a running maximum, the loads ahead of the sums: 53).
 constexpr int kVdB = 256, kVdW = kVdB / 64, kVdV = 8;
 
-// 2^(y / 16) for y <= 0: y = 16 n + i + f with |f| <= 1/2, a table of 2^(i / 16), and the series of exp(f ln 2 / 16)
-// to f^5 (2e-13 of it; half the f64 operations of a series over a whole octave).  -inf gives 0; a NaN is not kept.
+// 2^(y / 64) for y <= 0: y = 64 n + i + f with |f| <= 1/2, a table of 2^(i / 64), and a cubic for x = f ln 2 / 64: the
+// series of exp(x) with x^4 / 24 replaced by (h^2 x^2 - h^4 / 8) / 24, nearest to it on |x| <= h = ln 2 / 128 (off by
+// 5e-12 of the result; with 16 entries and the series to the fifth power the statistics took 56 us).  -inf
+// gives 0; a NaN is not kept.
 struct VdExp {
-  double tab[16];
+  double tab[64];
   __device__ __forceinline__ void fill() {  // a barrier follows
-    if (threadIdx.x < 16) tab[threadIdx.x] = exp2((double)threadIdx.x / 16.0);
+    if (threadIdx.x < 64) tab[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
   }
   __device__ __forceinline__ double operator()(double y) const {
-    y = fmax(y, -17600.0);
-    const double n = rint(y), f = y - n;
-    const int i = (int)n;
-    double p = 1.271587195055813e-09;  // (ln2 / 16)^5 / 5!
-    p = fma(p, f, 1.467610032291943e-07);
-    p = fma(p, f, 1.3550807779497455e-05);
-    p = fma(p, f, 0.0009383847928089871);
-    p = fma(p, f, 0.04332169878499658);
-    p = fma(p, f, 1.0);
-    return ldexp(p * tab[i & 15], i >> 4);
+    const double whole = 6755399441055744.0;  // 1.5 2^52: a sum with it ends at the ones, in its low bits
+    y = fmax(y, -70400.0);
+    const double n = y + whole, f = y - (n - whole);
+    const int i = (int)(uint32_t)__builtin_bit_cast(uint64_t, n);
+    constexpr double g = 0.6931471805599453 / 64.0, h = g / 2;
+    double p = g * g * g / 6.0;
+    p = fma(p, f, g * g * (0.5 + h * h / 24.0));
+    p = fma(p, f, g);
+    p = fma(p, f, 1.0 - h * h * h * h / 192.0);
+    return ldexp(p * tab[i & 63], i >> 6);
   }
 };
-__device__ __forceinline__ double vd_scale(const VerifyArgs& a) { return a.temp > 0.0f ? 23.083120654223414 / (double)a.temp : 0.0; }  // 16 log2(e) / T
+__device__ __forceinline__ double vd_scale(const VerifyArgs& a) { return a.temp > 0.0f ? 92.33248261689366 / (double)a.temp : 0.0; }  // 64 log2(e) / T
 
 template <int VT>
 __device__ __forceinline__ const void* vd_row(const VerifyArgs& a, bool draft, int64_t row) {
@@ -1490,8 +1492,8 @@ __device__ __forceinline__ void verify_pick(const VerifyArgs& a) {
     const int slice = __shfl(mp ? pass : has, lane);
     const double base = __shfl(mp ? at_pass : at_has, lane);
     if (tid == 0) sslice = tot > 0.0 ? slice : -1, sall = all, starget = t - base, first = 1 << 30, lastw = -1;  // NaN: no token
-  } else if (tid < 64 + 16) {
-    ex.tab[tid - 64] = exp2((double)(tid - 64) / 16.0);
+  } else if (tid < 128) {
+    ex.tab[tid - 64] = exp2((double)(tid - 64) / 64.0);
   }
   __syncthreads();
   if (sslice < 0) return;
