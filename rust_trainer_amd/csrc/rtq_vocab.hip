@@ -582,6 +582,9 @@ constexpr int kDisL = 8;
 template <int VT>
 constexpr int kDisV = VT == VT_F32 ? 16 : 14;  // as many as leave the sums their registers (4 waves a SIMD)
 
+constexpr float kLog2eF = 1.44269502f;  // the f32 nearest log2(e)
+constexpr double kLn2D = 0.69314718055994530942;
+
 struct DisShared {
   int id[RTQ_TOP_MAX];     // the slots' tokens (-1: empty)
   float tv[RTQ_TOP_MAX];   // their logits: the teacher's, the student's
@@ -591,21 +594,23 @@ struct DisShared {
   int first[RTQ_TOP_MAX];  // the slot stands for its token
   float wm[16];            // the waves' maxima and sums
   double wT[16], w1[16];
-  // the row's scalars: C and D with the unlisted logits' references, log2 of the student's two normalisers
+  // the row's scalars: C and D with the unlisted logits' references, the student's two normalisers
+  // (2^tT sum at the list's scale and 2^t1 sum, kept apart: beside a maximum of -1e9 log2 of the sum would be lost)
   float C, D, KT, K1, base;
-  double LT, L1, lu, pr, wgT, wg1;  // lu: log2 of the unlisted sum
+  double tT, LT, t1, L1, lu, pr, wgT, wg1;  // LT, L1: log2 of those sums; lu: log2 of the unlisted one's less tT
   float zt;
   int tok, taught;
+  // log2 of a logit's probability
+  __device__ __forceinline__ double log_qT(float z, double c) const { return ((double)z * c - tT) - LT; }
+  __device__ __forceinline__ double log_q1(float z) const { return ((double)z * (double)kLog2eF - t1) - L1; }
 };
 
-constexpr float kLog2eF = 1.44269502f;  // the f32 nearest log2(e)
-constexpr double kLn2D = 0.69314718055994530942;
-// a maximum's reference: K = f32(m c) for z c - K, or, where the product could overflow (masks of the type's
-// lowest value), m itself for (z - m) c
-__device__ __forceinline__ bool huge(float m) { return fabsf(m) > 1e30f; }
-__device__ __forceinline__ float ref_base(float m) { return huge(m) && fabsf(m) < __builtin_inff() ? m : 0.0f; }
-__device__ __forceinline__ float ref_of(float m, float c) { return m == -__builtin_inff() || ref_base(m) != 0.0f ? 0.0f : m * c; }
-__device__ __forceinline__ double ref_in(float m, float c) { return (double)ref_base(m) * (double)c + (double)ref_of(m, c); }
+// a maximum's reference: K = f32(m c) for z c - K, or, where that product's rounding could overflow an exponential
+// (masks of -1e9 and below: |m| c > 2^26 = big c, its last place 8), m itself for (z - m) c
+__device__ __forceinline__ bool huge(float m, float big) { return fabsf(m) > big; }
+__device__ __forceinline__ float ref_base(float m, float big) { return huge(m, big) && fabsf(m) < __builtin_inff() ? m : 0.0f; }
+__device__ __forceinline__ float ref_of(float m, float c, float big) { return m == -__builtin_inff() || ref_base(m, big) != 0.0f ? 0.0f : m * c; }
+__device__ __forceinline__ double ref_in(float m, float c, float big) { return (double)ref_base(m, big) * (double)c + (double)ref_of(m, c, big); }
 __device__ __forceinline__ float exp_ref(float z, float c, float K) { return __builtin_amdgcn_exp2f(fmaf(z, c, -K)); }
 
 // which logits of a slice are listed: a bit each, and for every wave a bit per vector of its registers that
@@ -635,8 +640,8 @@ struct DisSum {
   double sT = 0.0, s1 = 0.0;
   __device__ __forceinline__ void raise(float m2, const DistillArgs& a) {  // to the reference of m2 >= m
     const bool none = m == -__builtin_inff();  // (a NaN sum stays)
-    sT *= none ? 0.0 : (double)__builtin_amdgcn_exp2f((float)(ref_in(m, a.c) - ref_in(m2, a.c)));
-    s1 *= none ? 0.0 : (double)__builtin_amdgcn_exp2f((float)(ref_in(m, kLog2eF) - ref_in(m2, kLog2eF)));
+    sT *= none ? 0.0 : (double)__builtin_amdgcn_exp2f((float)(ref_in(m, a.c, a.big) - ref_in(m2, a.c, a.big)));
+    s1 *= none ? 0.0 : (double)__builtin_amdgcn_exp2f((float)(ref_in(m, kLog2eF, a.big) - ref_in(m2, kLog2eF, a.big)));
     m = m2;
   }
   // joined over the lanes of a wave; every lane gets it
@@ -698,16 +703,16 @@ struct DisSlice {
 #pragma unroll
       for (int e = 0; e < E; e++) f[v][e] = R::get(x[v], e), m = fmaxf(m, f[v][e]);
     const float old = d.m == -__builtin_inff() ? m : d.m;  // without logits so far the reference is m's own
-    const bool odd = __ballot(huge(m) || huge(old)) != 0;
+    const bool odd = __ballot(huge(m, a.big) || huge(old, a.big)) != 0;
     if (odd) {
-      const float b = ref_base(m);
+      const float b = ref_base(m, a.big);
 #pragma unroll
       for (int v = 0; v < GV; v++)
 #pragma unroll
         for (int e = 0; e < E; e++) f[v][e] -= b;
     }
     auto sum = [&](double& s, float c) {
-      const float K = ref_of(m, c);
+      const float K = ref_of(m, c, a.big);
       float t[GV];
 #pragma unroll
       for (int v = 0; v < GV; v++) {
@@ -721,8 +726,8 @@ struct DisSlice {
         t[v] = y[0];
         __builtin_amdgcn_sched_barrier(0);  // a vector at a time: the registers hold the row
       }
-      float up = ref_of(old, c) - K;
-      if (odd) up = (float)(ref_in(old, c) - ref_in(m, c));
+      float up = ref_of(old, c, a.big) - K;
+      if (odd) up = (float)(ref_in(old, c, a.big) - ref_in(m, c, a.big));
       s = fma(s, (double)__builtin_amdgcn_exp2f(up), (double)(t[0] + t[1]));
     };
     sum(d.sT, a.c);
@@ -890,9 +895,9 @@ __device__ __forceinline__ void distill_teacher(const DistillArgs& a, DisShared&
 
 // the student's normaliser at scale c: 2^top times what is returned, of the listed sum Z at ml and the unlisted sum
 // s at mu's reference; *share is 2^(that reference - top) over it
-__device__ __forceinline__ double distill_norm(float c, float ml, double Z, float mu, double s, bool bad, double* top, double* share) {
+__device__ __forceinline__ double distill_norm(const DistillArgs& a, float c, float ml, double Z, float mu, double s, bool bad, double* top, double* share) {
   const float ninf = -__builtin_inff();
-  const double kl = ml == ninf ? -__builtin_inf() : (double)ml * (double)c, ku = mu == ninf ? -__builtin_inf() : ref_in(mu, c);
+  const double kl = ml == ninf ? -__builtin_inf() : (double)ml * (double)c, ku = mu == ninf ? -__builtin_inf() : ref_in(mu, c, a.big);
   *top = fmax(kl, ku);
   const double less = exp2(-fabs(kl - ku));  // (0 where one of them is -inf)
   const double fl = ml == ninf ? 0.0 : kl < ku ? less : 1.0, fu = mu == ninf ? 0.0 : ku < kl ? less : 1.0;
@@ -910,24 +915,24 @@ struct DisNorms {
 __device__ __forceinline__ void distill_scalars(const DistillArgs& a, DisShared& sh, const DisTeacher& st, const DisSum& d, float w_, DisNorms& nm) {
   const bool empty = d.m == -__builtin_inff(), label = sh.tok >= 0;
   double fT, f1 = 0.0;
-  nm.sum[0] = distill_norm(a.c, st.ml, st.ZT, d.m, d.sT, st.nan, &nm.top[0], &fT);
+  nm.sum[0] = distill_norm(a, a.c, st.ml, st.ZT, d.m, d.sT, st.nan, &nm.top[0], &fT);
   nm.sum[1] = 1.0, nm.top[1] = 0.0;
-  if (a.tok) nm.sum[1] = distill_norm(kLog2eF, st.ml, st.Z1, d.m, d.s1, st.nan, &nm.top[1], &f1);
+  if (a.tok) nm.sum[1] = distill_norm(a, kLog2eF, st.ml, st.Z1, d.m, d.s1, st.nan, &nm.top[1], &f1);
   const double w = (double)w_, pr = sh.pr;
   const double wT = sh.taught && w != 0.0 ? w * (1.0 - (double)a.hard) * (double)a.temp : 0.0;
   const double w1 = label && w != 0.0 ? w * (double)a.hard : 0.0;
   if ((threadIdx.x & 63) == 0) {
     sh.C = wT == 0.0 || (empty && nm.sum[0] == nm.sum[0]) ? 0.0f : (float)(wT * (fT - (pr > 0.0 ? pr / d.sT : 0.0)));
     sh.D = w1 == 0.0 || (empty && nm.sum[1] == nm.sum[1]) ? 0.0f : (float)(w1 * f1);
-    sh.KT = ref_of(d.m, a.c), sh.K1 = ref_of(d.m, kLog2eF), sh.base = ref_base(d.m), sh.wgT = wT, sh.wg1 = w1;
+    sh.KT = ref_of(d.m, a.c, a.big), sh.K1 = ref_of(d.m, kLog2eF, a.big), sh.base = ref_base(d.m, a.big), sh.wgT = wT, sh.wg1 = w1;
   }
 }
 
 // log2 of the two normalisers and of the unlisted sum, for the losses and the gradient at the listed tokens
 __device__ __forceinline__ void distill_logs(const DistillArgs& a, DisShared& sh, const DisSum& d, const DisNorms& nm) {
-  const double LT = nm.top[0] + log2(nm.sum[0]), L1 = a.tok ? nm.top[1] + log2(nm.sum[1]) : 0.0;
-  const double lu = d.m == -__builtin_inff() ? -__builtin_inf() : ref_in(d.m, a.c) + log2(d.sT);
-  if ((threadIdx.x & 63) == 0) sh.LT = LT, sh.L1 = L1, sh.lu = lu;
+  const double LT = log2(nm.sum[0]), L1 = log2(nm.sum[1]);
+  const double lu = d.m == -__builtin_inff() ? -__builtin_inf() : (ref_in(d.m, a.c, a.big) - nm.top[0]) + log2(d.sT);
+  if ((threadIdx.x & 63) == 0) sh.tT = nm.top[0], sh.LT = LT, sh.t1 = nm.top[1], sh.L1 = L1, sh.lu = lu;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
@@ -938,13 +943,13 @@ __device__ __forceinline__ void distill_losses(const DistillArgs& a, const DisSh
   double kl = 0.0;
   for (int s = l; s < a.k; s += 64) {
     const double p = sh.p[s];
-    if (p > 0.0 || p != p) kl += p * (log(p) - ((double)sh.zs[s] * c - sh.LT) * kLn2D);
+    if (p > 0.0 || p != p) kl += p * (log(p) - sh.log_qT(sh.zs[s], c) * kLn2D);
   }
   kl = wave_sum_any(kl);
   if (pr > 0.0 || pr != pr) kl += pr * (log(pr) - (sh.lu - sh.LT) * kLn2D);
   if (l == 0) {
     a.kl[i] = sh.taught ? (float)kl : 0.0f;
-    if (a.logp) a.logp[i] = sh.tok >= 0 ? (float)(((double)sh.zt * (double)kLog2eF - sh.L1) * kLn2D) : __builtin_nanf("");
+    if (a.logp) a.logp[i] = sh.tok >= 0 ? (float)(sh.log_q1(sh.zt) * kLn2D) : __builtin_nanf("");
   }
 }
 
@@ -958,14 +963,14 @@ __device__ __forceinline__ void distill_marked(const DistillArgs& a, const DisSh
     const int id = sh.id[s];
     if (!sh.first[s] || id < j0 || id >= j1) continue;
     double v = 0.0;
-    if (sh.wgT != 0.0) v = sh.wgT * (exp2((double)sh.zs[s] * c - sh.LT) - sh.pt[s]);
-    if (sh.wg1 != 0.0) v += sh.wg1 * (exp2((double)sh.zs[s] * (double)kLog2eF - sh.L1) - (id == sh.tok ? 1.0 : 0.0));
+    if (sh.wgT != 0.0) v = sh.wgT * (exp2(sh.log_qT(sh.zs[s], c)) - sh.pt[s]);
+    if (sh.wg1 != 0.0) v += sh.wg1 * (exp2(sh.log_q1(sh.zs[s])) - (id == sh.tok ? 1.0 : 0.0));
     R::put(out, id, (float)v);
   }
   if (l == 0 && sh.tok >= j0 && sh.tok < j1 && !mk.get(sh.tok - j0)) {
     double v = 0.0;
-    if (sh.wgT != 0.0) v = sh.wgT * (exp2((double)sh.zt * c - sh.LT) - (sh.pr > 0.0 ? sh.pr * exp2((double)sh.zt * c - sh.lu) : 0.0));
-    if (sh.wg1 != 0.0) v += sh.wg1 * (exp2((double)sh.zt * (double)kLog2eF - sh.L1) - 1.0);
+    if (sh.wgT != 0.0) v = sh.wgT * (exp2(sh.log_qT(sh.zt, c)) - (sh.pr > 0.0 ? sh.pr * exp2(((double)sh.zt * c - sh.tT) - sh.lu) : 0.0));
+    if (sh.wg1 != 0.0) v += sh.wg1 * (exp2(sh.log_q1(sh.zt)) - 1.0);
     R::put(out, sh.tok, (float)v);
   }
 }

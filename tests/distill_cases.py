@@ -35,6 +35,9 @@ def distill(z, ids, vals, rest, temp, tok=None, w=None, hard=0.0):
     gradient is a difference of."""
     z = np.asarray(z, np.float64)
     n, V = z.shape
+    with np.errstate(all="ignore"):  # from the maximum: beside one of -1e20 the logarithms would be lost
+        m = z.max(1, keepdims=True)
+        z = z - np.where(np.isfinite(m), m, 0.0)
     kl, logp, g, sc = np.zeros(n), np.full(n, np.nan), np.zeros((n, V)), np.zeros((n, V))
     with np.errstate(all="ignore"):
         for i in range(n):

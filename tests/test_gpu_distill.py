@@ -264,6 +264,28 @@ def test_distill_rows_at_the_edges(ctx):
     check_distill(ctx, z, ids, vals, None, 2.0, tok, w, 0.5)
 
 
+@pytest.mark.parametrize("temp", [1.0, 0.25, 3.0])
+def test_distill_masks_of_any_size(each_ctx, temp):
+    """Masked logits of -1e5 to -1e30 beside live ones, all but the list masked, and whole rows masked: the rest
+    is small or nothing but every sum stays finite."""
+    V, k = 9000, 6
+    sizes = [-1e5, -1e8, -1e9, -1e10, -3e13, -1e20, -1e30]
+    rng = np.random.default_rng(15)
+    n = 3 * len(sizes)
+    z = D.logits(rng, n, V)
+    ids, vals, rest = teacher(rng, z, k, temp)
+    for i, m in enumerate(sizes):
+        z[i, np.setdiff1d(np.arange(100, 8000), ids[i])] = m
+        z[len(sizes) + i, np.setdiff1d(np.arange(V), ids[len(sizes) + i])] = m
+        rest[len(sizes) + i] = -np.inf
+        z[2 * len(sizes) + i] = m
+    tok, w = rng.integers(0, V, n), np.ones(n)
+    tok[len(sizes):2 * len(sizes)] = ids[len(sizes):2 * len(sizes), 0]
+    for ty in ("f32", "bf16"):
+        check_distill(each_ctx, z, ids, vals, rest, temp, tok, w, 0.5, ty)
+        check_distill(each_ctx, z, ids, vals, rest, temp, None, w, 0.0, ty)
+
+
 def test_distill_nan_and_infinite_rows(ctx):
     V, k = 20000, 4
     rng = np.random.default_rng(9)
