@@ -52,7 +52,7 @@ def check_top(ctx, z, ty, k, temp=1.0, pad=0, shift=0):
     a, z64 = D.rounded(z, ty)
     _, view = rows(a, ty, pad, shift)
     vals, ids, rest = run_top(ctx, view, ty, k, temp)
-    v, j, r = D.top(z64, k, temp)
+    v, j, r = D.top(z64, k, float(np.float32(temp)))
     np.testing.assert_array_equal(ids, j)
     np.testing.assert_array_equal(vals.astype(np.float64), v)
     check_lse(rest, r)
@@ -118,7 +118,7 @@ def test_top_logits_nan_and_infinity(ctx):
     assert none is None and np.array_equal(ids2, ids)
 
 
-def check_distill(ctx, z, ids, vals, rest, temp, tok=None, w=None, hard=0.0, ty="f32", pad=0, shift=0, dpad=0, in_place=False):
+def check_distill(ctx, z, ids, vals, rest, temp, tok=None, w=None, hard=0.0, ty="f32", pad=0, shift=0, dpad=0, in_place=False, kl_rel=HALF):
     a, z64 = D.rounded(z, ty)
     n, V = a.shape
     k = ids.shape[1]
@@ -140,11 +140,11 @@ def check_distill(ctx, z, ids, vals, rest, temp, tok=None, w=None, hard=0.0, ty=
               ptr(dw), kl.data_ptr(), ptr(lp), gview.data_ptr() if w is not None else 0, gview.stride(0), hard=hard,
               stream=torch.cuda.current_stream().cuda_stream)
     torch.cuda.synchronize()
-    rk, rl, rg, sc = D.distill(z64, ids, vals.astype(np.float64), rest, temp, tok, w, hard)
+    rk, rl, rg, sc = D.distill(z64, ids, vals.astype(np.float64), rest, float(np.float32(temp)), tok, w, hard)  # (a float in the call)
     got = kl.cpu().numpy().astype(np.float64)
     fin = np.isfinite(rk)
     np.testing.assert_array_equal(got[~fin], rk[~fin])
-    assert np.all(np.abs(got[fin] - rk[fin]) <= 2 * D.SUM + HALF * np.abs(rk[fin])), float(np.abs(got[fin] - rk[fin]).max())
+    assert np.all(np.abs(got[fin] - rk[fin]) <= 2 * D.SUM + kl_rel * np.abs(rk[fin])), float(np.abs(got[fin] - rk[fin]).max())
     if tok is not None:
         got = lp.cpu().numpy().astype(np.float64)
         np.testing.assert_array_equal(np.isnan(got), np.isnan(rl))
@@ -286,6 +286,20 @@ def test_distill_masks_of_any_size(each_ctx, temp):
         check_distill(each_ctx, z, ids, vals, rest, temp, None, w, 0.0, ty)
 
 
+@pytest.mark.parametrize("temp", [1e-4, 1e4])
+def test_the_ends_of_the_temperatures(each_ctx, temp):
+    """The divergence at 1e-4 is some 1e4 and proportional to 1 / T, whose scale log2(e) / T is a float: 2^-25 of it
+    more than its own rounding, 2^-24."""
+    V, k, n = 9000, 6, 5
+    rng = np.random.default_rng(16)
+    z = D.logits(rng, n, V)
+    ids, vals, rest = teacher(rng, z, k, temp)
+    for ty in ("f32", "f16"):
+        check_distill(each_ctx, z, ids, vals, rest, temp, rng.integers(0, V, n), np.ones(n), 0.5, ty, kl_rel=1.5 * HALF)
+        test_top_logits(each_ctx, ty, n, V, k, temp, 0, 0)
+        test_verify_draft(each_ctx, ty, n, 3, V, temp, True, False, 0, 0)
+
+
 def test_distill_nan_and_infinite_rows(ctx):
     V, k = 20000, 4
     rng = np.random.default_rng(9)
@@ -333,7 +347,7 @@ def check_verify(ctx, zp, zq, x, lens, u, temp, ty="f32", pad=0, shift=0):
                    0 if dl is None else dl.data_ptr(), du.data_ptr(), acc.data_ptr(), out.data_ptr(), temperature=temp,
                    stream=torch.cuda.current_stream().cuda_stream)
     torch.cuda.synchronize()
-    want = D.verify(z64, q64, x, lens, u, temp)
+    want = D.verify(z64, q64, x, lens, u, float(np.float32(temp)))
     np.testing.assert_array_equal(acc.cpu().numpy(), want[0])
     np.testing.assert_array_equal(out.cpu().numpy(), want[1])
 
