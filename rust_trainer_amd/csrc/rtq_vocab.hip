@@ -941,8 +941,8 @@ __device__ __forceinline__ void distill_losses(const DistillArgs& a, const DisSh
   const int l = threadIdx.x & 63;
   const double c = (double)a.c, pr = sh.pr;
   double kl = 0.0;
-  for (int s = l; s < a.k; s += 64) {
-    const double p = sh.p[s];
+  for (int s = l; s < a.k; s += 64) {  // a token's slots are one bucket
+    const double p = sh.first[s] ? sh.pt[s] : 0.0;
     if (p > 0.0 || p != p) kl += p * (log(p) - sh.log_qT(sh.zs[s], c) * kLn2D);
   }
   kl = wave_sum_any(kl);

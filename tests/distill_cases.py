@@ -52,9 +52,10 @@ def distill(z, ids, vals, rest, temp, tok=None, w=None, hard=0.0):
             if taught:
                 p = np.exp(t - lse(t))
                 lr = lse(lq[~listed]) if (~listed).any() else NEG
-                for b, s in enumerate(held):
-                    if p[b] > 0 or np.isnan(p[b]):
-                        kl[i] += p[b] * (np.log(p[b]) - lq[ids[i][s]])
+                for j in {ids[i][s] for s in held}:  # slots of one token are one bucket
+                    pj = sum(p[b] for b, s in enumerate(held) if ids[i][s] == j)
+                    if pj > 0 or np.isnan(pj):
+                        kl[i] += pj * (np.log(pj) - lq[j])
                 if p[-1] > 0 or np.isnan(p[-1]):
                     kl[i] += p[-1] * (np.log(p[-1]) - lr)
                 d = q.copy()

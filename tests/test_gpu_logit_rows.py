@@ -1,0 +1,99 @@
+"""Rows of vocabulary logits at places where top logits, distillation and draft verification have gone wrong, each
+against a form of its own in 64 bits or more."""
+import os
+
+import numpy as np
+import pytest
+import torch
+
+import distill_cases as D
+import rust_trainer_amd as rt
+from rust_trainer_amd.distill import distill_d, teacher_d, top_logits_d, verify_draft_d
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": (rt.TYPE_F32, torch.float32), "f16": (rt.TYPE_F16, torch.float16), "bf16": (rt.TYPE_BF16, torch.bfloat16)}
+HALF = 2.0 ** -24
+# a sum of f32 exponentials, relative: 2^-22 each and 2^-22 for the f32 additions among eight; the roundings of an
+# argument and of the scale log2(e) / T, 2^-24 of |z - max| / T each, at most 12.6 on average over a softmax
+SUM = 2.0 ** -21 + 12.6 * 2 * 2.0 ** -24
+
+
+@pytest.fixture(scope="module", params=["-1", "0", "1", "2"])
+def each_ctx(request):
+    """A context whose distillation runs on slices, or a row a workgroup of 256, 512 or 1024 threads, whatever the size."""
+    os.environ["RTQ_DISTILL_ROWS"] = request.param
+    c = rt.Context(0)
+    del os.environ["RTQ_DISTILL_ROWS"]
+    yield c
+    c.close()
+
+
+def dev(a, dtype=None):
+    t = torch.from_numpy(np.ascontiguousarray(a)).cuda()
+    return t if dtype is None else t.to(dtype)
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def losses(ctx, z, ids, vals, rest, temp, tok=None, w=None, hard=0.0, ty="f32"):
+    """(kl, logp, gradient) of device rows, as 64-bit numpy arrays (None where there is none)."""
+    n, V = z.shape
+    z = dev(z.astype(np.float32), TYPES[ty][1])
+    keep = [dev(np.asarray(ids, np.int32)), dev(np.asarray(vals, np.float32))]
+    keep += [None if a is None else dev(np.asarray(a, t)) for a, t in ((rest, np.float32), (tok, np.int32), (w, np.float32))]
+    di, dv, dr, dt, dw = keep
+    kl, lp = torch.full((n,), 7.0, device="cuda"), None if tok is None else torch.full((n,), 7.0, device="cuda")
+    g = None if w is None else torch.full((n, V), 7.0, dtype=TYPES[ty][1], device="cuda")
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    distill_d(ctx, z.data_ptr(), TYPES[ty][0], n, V, V, teacher_d(di.shape[1], di.data_ptr(), dv.data_ptr(), ptr(dr), temp), ptr(dt), ptr(dw),
+              kl.data_ptr(), ptr(lp), ptr(g), V, hard=hard, stream=stream())
+    torch.cuda.synchronize()
+    return [None if t is None else t.double().cpu().numpy() for t in (kl, lp, g)]
+
+
+def divergence(z, ids, vals, rest, temp):
+    """kl of one row from its definition: a bucket for each token that is listed, one for all others."""
+    weights = {}
+    for i, v in zip(ids, vals):
+        if 0 <= i < len(z):
+            weights[int(i)] = np.logaddexp(weights.get(int(i), -np.inf), float(v) / temp)
+    others = np.ones(len(z), bool)
+    others[list(weights)] = False
+    lt = np.array(list(weights.values()) + [-np.inf if rest is None else float(rest)])
+    lq = z / temp - D.lse(z / temp)
+    lq = np.append(lq[list(weights)], D.lse(lq[others]) if others.any() else -np.inf)
+    lp = lt - D.lse(lt)
+    on = lp > -np.inf
+    return float(np.sum(np.exp(lp[on]) * (lp[on] - lq[on])))
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+def test_slots_of_one_token_are_one_bucket(each_ctx, ty):
+    """A token in several slots has the sum of their weights: the divergence is that of the merged list, at least 0."""
+    q = np.repeat(np.log([[0.9, 0.1]]), 3, 0)
+    kl, _, _ = losses(each_ctx, q, [[0, 0], [0, 0], [1, 1]], [[1.0, 1.0]] * 3, [-np.inf, 1.0, -np.inf], 1.0)
+    # p = (1, 0): log(1 / 0.9); p = (2/3, 1/3); p = (1 at the other token, 0): log(1 / 0.1)
+    want = [np.log(1 / 0.9), 2 / 3 * np.log(2 / 2.7) + 1 / 3 * np.log(1 / 0.3), np.log(10)]
+    assert np.all(np.abs(kl - want) <= 2 * SUM + HALF * np.abs(want) + 2.0 ** -23)  # (and the roundings of the logits handed over)
+    V, k, n, temp = 9000, 12, 8, 1.25
+    rng = np.random.default_rng(1)
+    z = D.logits(rng, n, V)
+    vals, ids, rest = D.top(D.logits(rng, n, V, near=z), k, temp)
+    ids[0, 1] = ids[0, 0]
+    ids[1, [2, 5, 11]] = ids[1, 8]
+    ids[2] = ids[2, 0]  # one token alone
+    ids[3, 6:] = ids[3, :6]  # each twice
+    ids[4, 4], ids[4, 5] = ids[4, 0], -1
+    ids[5, 3:] = V - 1
+    vals[6, 2], ids[6, 2] = -np.inf, ids[6, 0]
+    z[7, ids[7, 0]], ids[7, 3] = 11.0, ids[7, 0]
+    _, z64 = D.rounded(z, ty)
+    vals, rest = vals.astype(np.float32), rest.astype(np.float32)
+    for r in (rest, None):
+        for w in (None, np.ones(n)):
+            kl, _, _ = losses(each_ctx, z64, ids, vals, r, temp, w=w, ty=ty)
+            want = np.array([divergence(z64[i], ids[i], vals[i], None if r is None else r[i], temp) for i in range(n)])
+            assert np.all(want >= 0) and np.all(np.abs(kl - want) <= 2 * SUM + HALF * np.abs(want)), kl - want
