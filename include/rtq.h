@@ -181,7 +181,8 @@ typedef struct rtq_teacher {
 } rtq_teacher;
 /* The k largest logits of each of n rows, largest first, equal logits by the lower id (a NaN is above
  * every number): vals [n x k], ids [n x k]; rest [n] (or NULL) = log of the sum of exp(logit /
- * temperature) over the others, -inf where there are none.  1 <= k <= min(vocab, RTQ_TOP_MAX). */
+ * temperature) over the others, -inf where there are none, NaN where one of them is.
+ * 1 <= k <= min(vocab, RTQ_TOP_MAX). */
 rtq_status rtq_top_logits(rtq_ctx* ctx, const void* logits, int type, int64_t n, int64_t vocab, int64_t ld, int64_t k,
                           float temperature, float* vals, int32_t* ids, float* rest);
 rtq_status rtq_top_logits_d(rtq_ctx* ctx, const void* logits, int type, int64_t n, int64_t vocab, int64_t ld, int64_t k,

@@ -171,9 +171,9 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 }
 __device__ __forceinline__ int key_index(uint64_t k) { return (int)~(uint32_t)k; }
 
-__device__ __forceinline__ float lse_of(float m, double s, double invt) {
-  if (m == -__builtin_inff()) return s != s ? __builtin_nanf("") : m;
-  return m == __builtin_inff() ? m : (float)((double)m * invt + log(s));
+__device__ __forceinline__ float lse_of(float m, double s, double invt) {  // s is NaN for a NaN alone
+  if (s != s) return __builtin_nanf("");
+  return fabsf(m) == __builtin_inff() ? m : (float)((double)m * invt + log(s));
 }
 
 // maximum / sum over each eight neighbouring lanes; every lane gets it
@@ -303,7 +303,8 @@ __device__ __forceinline__ uint64_t radix_kth(int N, int K, int* hist, int* out,
   return low;
 }
 
-// (m, s) of a set joined by N others: x[e] with exponential sum w[e] (0: no member)
+// (m, s) of a set joined by N others: x[e] with exponential sum w[e] (0: no member).  A NaN makes s NaN, and
+// nothing else does: beside +inf nothing is summed
 template <int N>
 __device__ __forceinline__ void join_rest(float& m, double& s, const float* x, const float* w, const TopArgs& a) {
   float b = m;
@@ -319,6 +320,7 @@ __device__ __forceinline__ void join_rest(float& m, double& s, const float* x, c
     s *= (double)__builtin_amdgcn_exp2f((m - b) * a.c);
     m = b;
   }
+  if (b == __builtin_inff()) return;
   float t = 0.0f;
 #pragma unroll
   for (int e = 0; e < N; e++) t += w[e] != 0.0f ? w[e] * __builtin_amdgcn_exp2f((x[e] - m) * a.c) : 0.0f;
@@ -550,7 +552,7 @@ __device__ __forceinline__ void top_pick(const TopArgs& a) {
   }
   if (!a.rest) return;
   const float m = group_max<W>(rm, redf);
-  rs = group_sum<W>(rm == ninf ? rs : rs * (double)__builtin_amdgcn_exp2f((rm - m) * a.c), redd);
+  rs = group_sum<W>(rm == m || rm == ninf ? rs : rs * (double)__builtin_amdgcn_exp2f((rm - m) * a.c), redd);
   if (tid == 0) a.rest[i] = lse_of(m, rs, 1.0 / (double)a.temp);
 }
 

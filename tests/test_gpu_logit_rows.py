@@ -97,3 +97,31 @@ def test_slots_of_one_token_are_one_bucket(each_ctx, ty):
             kl, _, _ = losses(each_ctx, z64, ids, vals, r, temp, w=w, ty=ty)
             want = np.array([divergence(z64[i], ids[i], vals[i], None if r is None else r[i], temp) for i in range(n)])
             assert np.all(want >= 0) and np.all(np.abs(kl - want) <= 2 * SUM + HALF * np.abs(want)), kl - want
+
+
+@pytest.mark.parametrize("ty", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("V,k", [(40, 3), (700, 20), (20000, 8), (40000, 256)])
+def test_rest_of_a_nan_beside_infinity_is_nan(ctx, ty, V, k):
+    """More NaNs than are listed, and +inf: the log of the sum of the others is NaN, as it is without the infinity;
+    of +inf alone it is +inf."""
+    rng = np.random.default_rng(V)
+    z = rng.normal(0, 1, (8, V))
+    spots = rng.permutation(V)
+    for i, lead in enumerate((1, 2, V - 2 * k - 2)):
+        z[i, spots[:k + lead]] = np.nan
+        z[i, spots[k + lead]] = np.inf  # anywhere
+    z[3, :k + 1], z[3, k + 1:2 * k + 3] = np.nan, np.inf  # side by side
+    z[4, V - 1 - k:], z[4, 0] = np.nan, np.inf
+    z[5, spots[:k + 1]] = np.inf
+    z[6, spots[:k + 1]] = np.nan
+    z[7, spots[:k]], z[7, spots[k]] = np.nan, np.inf
+    zd = dev(z, TYPES[ty][1])
+    vals, ids = torch.empty(8, k, device="cuda"), torch.empty(8, k, dtype=torch.int32, device="cuda")
+    rest = torch.full((8,), 7.0, device="cuda")
+    top_logits_d(ctx, zd.data_ptr(), TYPES[ty][0], 8, V, V, k, vals.data_ptr(), ids.data_ptr(), rest.data_ptr(), stream=stream())
+    torch.cuda.synchronize()
+    rest = rest.cpu().numpy()
+    assert np.isnan(rest[:5]).all() and rest[5] == np.inf and np.isnan(rest[6]) and rest[7] == np.inf, rest
+    # a NaN is above every number, +inf among them
+    order = np.lexsort((np.broadcast_to(np.arange(V), z.shape), -np.nan_to_num(z, nan=0.0, posinf=np.inf), ~np.isnan(z)), axis=1)
+    np.testing.assert_array_equal(ids.cpu().numpy(), order[:, :k])
