@@ -1185,29 +1185,30 @@ RTQ_DISTILL(bf16, VT_BF16)
 // rows of 151936 bf16 logits: 51 us, 2.3 TB/s; in one pass with a running maximum, the loads ahead of the sums: 53).
 constexpr int kVdB = 256, kVdW = kVdB / 64, kVdV = 8;
 
-// 2^(y / 64) for y <= 0: y = 64 n + i + f with |f| <= 1/2, a table of 2^(i / 64), and a cubic for x = f ln 2 / 64: the
-// series of exp(x) with x^4 / 24 replaced by (h^2 x^2 - h^4 / 8) / 24, nearest to it on |x| <= h = ln 2 / 128 (off by
-// 5e-12 of the result; with 16 entries and the series to the fifth power the statistics took 56 us).  -inf
-// gives 0; a NaN is not kept.
+// 2^(y / 256) for y <= 0: y = 256 n + i + f with |f| <= 1/2, a table of 2^(i / 256), and the series of exp(x) to
+// the fourth power for x = f ln 2 / 256, whose next term is below 4e-17: off by a few 2^-53, as the sums are.
+// (verification of 64 x 5 drafted tokens of 151936 bf16: 88 us; 90 with 128 entries and the quartic nearest to the series,
+// 91 with 64 and the fifth power).  -inf gives 0; a NaN is not kept.
 struct VdExp {
-  double tab[64];
-  __device__ __forceinline__ void fill() {  // a barrier follows
-    if (threadIdx.x < 64) tab[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
+  double tab[256];
+  __device__ __forceinline__ void fill(int t) {  // by t = 0 .. 255; a barrier follows
+    tab[t] = exp2((double)t / 256.0);
   }
   __device__ __forceinline__ double operator()(double y) const {
     const double whole = 6755399441055744.0;  // 1.5 2^52: a sum with it ends at the ones, in its low bits
-    y = fmax(y, -70400.0);
+    y = fmax(y, -281600.0);
     const double n = y + whole, f = y - (n - whole);
     const int i = (int)(uint32_t)__builtin_bit_cast(uint64_t, n);
-    constexpr double g = 0.6931471805599453 / 64.0, h = g / 2;
-    double p = g * g * g / 6.0;
-    p = fma(p, f, g * g * (0.5 + h * h / 24.0));
+    constexpr double g = 0.6931471805599453 / 256.0;
+    double p = g * g * g * g / 24.0;
+    p = fma(p, f, g * g * g / 6.0);
+    p = fma(p, f, g * g / 2.0);
     p = fma(p, f, g);
-    p = fma(p, f, 1.0 - h * h * h * h / 192.0);
-    return ldexp(p * tab[i & 63], i >> 6);
+    p = fma(p, f, 1.0);
+    return ldexp(p * tab[i & 255], i >> 8);
   }
 };
-__device__ __forceinline__ double vd_scale(const VerifyArgs& a) { return a.temp > 0.0f ? 92.33248261689366 / (double)a.temp : 0.0; }  // 64 log2(e) / T
+__device__ __forceinline__ double vd_scale(const VerifyArgs& a) { return a.temp > 0.0f ? 369.3299304675746 / (double)a.temp : 0.0; }  // 256 log2(e) / T
 
 template <int VT>
 __device__ __forceinline__ const void* vd_row(const VerifyArgs& a, bool draft, int64_t row) {
@@ -1275,7 +1276,7 @@ __device__ __forceinline__ void verify_stats(const VerifyArgs& a) {
 #pragma unroll 1
     for (int o = j0 + tid * E; o < j1; o += kVdB * E) see(R::load_upto(z, o, j1));
   }
-  ex.fill();
+  ex.fill(tid);
   m = group_max<kVdW>(m, redf);  // (and its barriers)
   // (z - m) c and not z c - m c, which is not small where both are the type's lowest value
   const double c = vd_scale(a), ref = m == ninf ? 0.0 : (double)m;
@@ -1389,7 +1390,7 @@ template <int VT>
 __device__ __forceinline__ void verify_greedy(const VerifyArgs& a) {
   __shared__ VerifyPick lds[kVdW];
   __shared__ int stop[kVdW];
-  VdExp none;
+  __shared__ VdExp none;  // (not read at T = 0)
   vd_decide<VT>(a, none, blockIdx.x, lds, stop, true);
 }
 
@@ -1410,7 +1411,7 @@ __device__ __forceinline__ void verify_mass(const VerifyArgs& a) {
   __shared__ int stop[kVdW];
   __shared__ VdExp ex;
   const int tid = threadIdx.x, g = blockIdx.x, i = blockIdx.y;
-  ex.fill();
+  ex.fill(tid);
   __syncthreads();
   const VerifyPick k = vd_decide<VT>(a, ex, i, lds, stop, g == 0);
   const void* zp = vd_row<VT>(a, false, (int64_t)i * (a.d + 1) + k.row);
@@ -1499,8 +1500,8 @@ __device__ __forceinline__ void verify_pick(const VerifyArgs& a) {
     const int slice = __shfl(mp ? pass : has, lane);
     const double base = __shfl(mp ? at_pass : at_has, lane);
     if (tid == 0) sslice = tot > 0.0 ? slice : -1, sall = all, starget = t - base, first = 1 << 30, lastw = -1;  // NaN: no token
-  } else if (tid < 128) {
-    ex.tab[tid - 64] = exp2((double)(tid - 64) / 64.0);
+  } else if (tid < 64 + 256) {
+    ex.fill(tid - 64);
   }
   __syncthreads();
   if (sslice < 0) return;

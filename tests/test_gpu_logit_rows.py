@@ -125,3 +125,40 @@ def test_rest_of_a_nan_beside_infinity_is_nan(ctx, ty, V, k):
     # a NaN is above every number, +inf among them
     order = np.lexsort((np.broadcast_to(np.arange(V), z.shape), -np.nan_to_num(z, nan=0.0, posinf=np.inf), ~np.isnan(z)), axis=1)
     np.testing.assert_array_equal(ids.cpu().numpy(), order[:, :k])
+
+
+@pytest.mark.parametrize("temp", [1.0, 0.75, 2.0])
+@pytest.mark.parametrize("V", [2, 20001])
+def test_draws_and_tests_at_the_borders_are_exact_to_64_bits(ctx, V, temp):
+    """Two live tokens whose border w0 / (w0 + w1) lies 2e-14 to 1e-12 of itself beside the uniform number (placed with
+    a logit next to 0, whose float steps are that fine; expected values in extended precision).  A weight's
+    exponential is off by a few 2^-53: of its table and polynomial, and of its argument, 2^-52 |z - max| / T."""
+    L = np.longdouble
+    rng = np.random.default_rng(int(temp * 100) + V)
+    z1 = rng.uniform(-3, 3, 400).astype(np.float32)
+    u = (1 / (1 + np.exp(z1.astype(L) / L(temp)))).astype(np.float32)
+    off = np.tile([2e-14, -2e-14, 1e-13, -1e-13, 5e-13, -5e-13, 1e-12, -1e-12], 50).astype(L)
+    # w0 / w1 = u / (1 - u) (1 + off) (off the border by (1 - u) off of itself)
+    z0 = (z1.astype(L) + L(temp) * (np.log(u.astype(L)) - np.log1p(-u.astype(L)) + off)).astype(np.float32)
+    e = np.exp((z0.astype(L) - z1.astype(L)) / L(temp))
+    border = e / (1 + e)
+    ok = np.abs(border / u.astype(L) - 1) > 4e-15
+    assert ok.sum() > 300
+    z0, z1, u, border = z0[ok], z1[ok], u[ok], border[ok]
+    b = len(u)
+    i, j = (0, 1) if V == 2 else (4321, 17000)
+    z = np.full((b, V), -np.inf, np.float32)
+    z[:, i], z[:, j] = z0, z1
+    zd, ud = dev(z), dev(u)
+    acc, out = torch.empty(b, dtype=torch.int32, device="cuda"), torch.empty(b, 1, dtype=torch.int32, device="cuda")
+    verify_draft_d(ctx, zd.data_ptr(), rt.TYPE_F32, V, 0, 0, b, 0, V, 0, 0, ud.data_ptr(), acc.data_ptr(), out.data_ptr(), temperature=temp, stream=stream())
+    torch.cuda.synchronize()
+    # drawn: the first token whose running sum passes u times the total
+    np.testing.assert_array_equal(out.cpu().numpy()[:, 0], np.where(border > u, i, j))
+    # a looked-up draft of that token is accepted while u < p
+    zz, uu, x = dev(np.repeat(z, 2, 0)), dev(np.stack([u, u], 1)), torch.full((b, 1), i, dtype=torch.int32, device="cuda")
+    out = torch.empty(b, 2, dtype=torch.int32, device="cuda")
+    verify_draft_d(ctx, zz.data_ptr(), rt.TYPE_F32, V, 0, 0, b, 1, V, x.data_ptr(), 0, uu.data_ptr(), acc.data_ptr(), out.data_ptr(), temperature=temp,
+                   stream=stream())
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(acc.cpu().numpy(), (u < border).astype(np.int32))
