@@ -379,6 +379,7 @@ struct DistillArgs {
   int64_t ld, ldd;
   int n, V, k, G, L;
   float temp, c, hard;
+  double scale;  // log2(e) / temp, which c is rounded from
   float big;  // 2^26 over the larger of c and log2(e)
   const int32_t* ids;  // [n x k] the teacher's tokens (outside [0, V): no token)
   const float* tv;     // [n x k] its logits

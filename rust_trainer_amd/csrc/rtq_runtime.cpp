@@ -2026,6 +2026,7 @@ rtq_status enqueue_distill(rtq_ctx* c, const void* z, int type, int64_t n, int64
   a.n = (int)n, a.V = (int)V, a.k = (int)t.k, a.G = (int)p.G, a.L = (int)p.L;
   a.temp = t.temperature;
   a.c = exp_scale(t.temperature);
+  a.scale = 1.4426950408889634 / (double)t.temperature;
   a.big = 67108864.0f / std::max(a.c, exp_scale(1.0f));
   a.hard = hard, a.ids = t.ids, a.tv = t.vals, a.rest = t.rest, a.tok = tok, a.w = w, a.kl = kl, a.logp = logp;
   const int ty = logit_type(type);

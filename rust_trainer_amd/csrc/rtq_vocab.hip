@@ -578,13 +578,14 @@ RTQ_TOP(bf16, VT_BF16)
 //
 // Exponentials are exp2(fma(z, c, -K)), one FMA and the instruction: c = log2(e) / T rounded to f32, and a
 // maximum m's reference is f32(m c), so that its rounding cancels between the sums and what is divided by
-// them.  The row's scalars use the same c (the student's temperature is off by 2^-25 of itself at most), in
-// 64 bits.
+// them; an exponential below the maximum is off by 2^-24 of its argument for c's rounding.  The row's scalars are
+// in 64 bits with log2(e) / T itself, so a large divergence carries none of that.
 constexpr int kDisL = 8;
 template <int VT>
 constexpr int kDisV = VT == VT_F32 ? 16 : 14;  // as many as leave the sums their registers (4 waves a SIMD)
 
 constexpr float kLog2eF = 1.44269502f;  // the f32 nearest log2(e)
+constexpr double kLog2eD = 1.4426950408889634074;
 constexpr double kLn2D = 0.69314718055994530942;
 
 struct DisShared {
@@ -604,7 +605,7 @@ struct DisShared {
   int tok, taught;
   // log2 of a logit's probability
   __device__ __forceinline__ double log_qT(float z, double c) const { return ((double)z * c - tT) - LT; }
-  __device__ __forceinline__ double log_q1(float z) const { return ((double)z * (double)kLog2eF - t1) - L1; }
+  __device__ __forceinline__ double log_q1(float z) const { return ((double)z * kLog2eD - t1) - L1; }
 };
 
 // a maximum's reference: K = f32(m c) for z c - K, or, where that product's rounding could overflow an exponential
@@ -613,6 +614,10 @@ __device__ __forceinline__ bool huge(float m, float big) { return fabsf(m) > big
 __device__ __forceinline__ float ref_base(float m, float big) { return huge(m, big) && fabsf(m) < __builtin_inff() ? m : 0.0f; }
 __device__ __forceinline__ float ref_of(float m, float c, float big) { return m == -__builtin_inff() || ref_base(m, big) != 0.0f ? 0.0f : m * c; }
 __device__ __forceinline__ double ref_in(float m, float c, float big) { return (double)ref_base(m, big) * (double)c + (double)ref_of(m, c, big); }
+// the same for the scale itself, of which c is the float: sums by the reference of m are 2^-(this) of those of exp2(z scale)
+__device__ __forceinline__ double ref_exact(float m, float c, double scale, float big) {
+  return ref_base(m, big) != 0.0f ? (double)m * scale : (double)ref_of(m, c, big) + (double)m * (scale - (double)c);
+}
 __device__ __forceinline__ float exp_ref(float z, float c, float K) { return __builtin_amdgcn_exp2f(fmaf(z, c, -K)); }
 
 // which logits of a slice are listed: a bit each, and for every wave a bit per vector of its registers that
@@ -888,18 +893,18 @@ __device__ __forceinline__ void distill_teacher(const DistillArgs& a, DisShared&
   for (int s = l; s < a.k; s += 64) {
     const float zs = sh.zs[s];
     if (!sh.first[s] || zs == ninf) continue;
-    st.ZT += exp2(((double)zs - st.ml) * (double)a.c);
-    if (a.tok) st.Z1 += exp2(((double)zs - st.ml) * (double)kLog2eF);
+    st.ZT += exp2(((double)zs - st.ml) * a.scale);
+    if (a.tok) st.Z1 += exp2(((double)zs - st.ml) * kLog2eD);
   }
   st.ZT = wave_sum_any(st.ZT);
   st.Z1 = wave_sum_any(st.Z1);
 }
 
-// the student's normaliser at scale c: 2^top times what is returned, of the listed sum Z at ml and the unlisted sum
+// the student's normaliser at a scale and its float c: 2^top times what is returned, of the listed sum Z at ml and the unlisted sum
 // s at mu's reference; *share is 2^(that reference - top) over it
-__device__ __forceinline__ double distill_norm(const DistillArgs& a, float c, float ml, double Z, float mu, double s, bool bad, double* top, double* share) {
+__device__ __forceinline__ double distill_norm(const DistillArgs& a, float c, double scale, float ml, double Z, float mu, double s, bool bad, double* top, double* share) {
   const float ninf = -__builtin_inff();
-  const double kl = ml == ninf ? -__builtin_inf() : (double)ml * (double)c, ku = mu == ninf ? -__builtin_inf() : ref_in(mu, c, a.big);
+  const double kl = ml == ninf ? -__builtin_inf() : (double)ml * scale, ku = mu == ninf ? -__builtin_inf() : ref_exact(mu, c, scale, a.big);
   *top = fmax(kl, ku);
   const double less = exp2(-fabs(kl - ku));  // (0 where one of them is -inf)
   const double fl = ml == ninf ? 0.0 : kl < ku ? less : 1.0, fu = mu == ninf ? 0.0 : ku < kl ? less : 1.0;
@@ -917,9 +922,9 @@ struct DisNorms {
 __device__ __forceinline__ void distill_scalars(const DistillArgs& a, DisShared& sh, const DisTeacher& st, const DisSum& d, float w_, DisNorms& nm) {
   const bool empty = d.m == -__builtin_inff(), label = sh.tok >= 0;
   double fT, f1 = 0.0;
-  nm.sum[0] = distill_norm(a, a.c, st.ml, st.ZT, d.m, d.sT, st.nan, &nm.top[0], &fT);
+  nm.sum[0] = distill_norm(a, a.c, a.scale, st.ml, st.ZT, d.m, d.sT, st.nan, &nm.top[0], &fT);
   nm.sum[1] = 1.0, nm.top[1] = 0.0;
-  if (a.tok) nm.sum[1] = distill_norm(a, kLog2eF, st.ml, st.Z1, d.m, d.s1, st.nan, &nm.top[1], &f1);
+  if (a.tok) nm.sum[1] = distill_norm(a, kLog2eF, kLog2eD, st.ml, st.Z1, d.m, d.s1, st.nan, &nm.top[1], &f1);
   const double w = (double)w_, pr = sh.pr;
   const double wT = sh.taught && w != 0.0 ? w * (1.0 - (double)a.hard) * (double)a.temp : 0.0;
   const double w1 = label && w != 0.0 ? w * (double)a.hard : 0.0;
@@ -933,7 +938,7 @@ __device__ __forceinline__ void distill_scalars(const DistillArgs& a, DisShared&
 // log2 of the two normalisers and of the unlisted sum, for the losses and the gradient at the listed tokens
 __device__ __forceinline__ void distill_logs(const DistillArgs& a, DisShared& sh, const DisSum& d, const DisNorms& nm) {
   const double LT = log2(nm.sum[0]), L1 = log2(nm.sum[1]);
-  const double lu = d.m == -__builtin_inff() ? -__builtin_inf() : (ref_in(d.m, a.c, a.big) - nm.top[0]) + log2(d.sT);
+  const double lu = d.m == -__builtin_inff() ? -__builtin_inf() : (ref_exact(d.m, a.c, a.scale, a.big) - nm.top[0]) + log2(d.sT);
   if ((threadIdx.x & 63) == 0) sh.tT = nm.top[0], sh.LT = LT, sh.t1 = nm.top[1], sh.L1 = L1, sh.lu = lu;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
@@ -941,7 +946,7 @@ __device__ __forceinline__ void distill_logs(const DistillArgs& a, DisShared& sh
 // the losses, by the wave that formed the scalars
 __device__ __forceinline__ void distill_losses(const DistillArgs& a, const DisShared& sh, int i) {
   const int l = threadIdx.x & 63;
-  const double c = (double)a.c, pr = sh.pr;
+  const double c = a.scale, pr = sh.pr;
   double kl = 0.0;
   for (int s = l; s < a.k; s += 64) {  // a token's slots are one bucket
     const double p = sh.first[s] ? sh.pt[s] : 0.0;
@@ -960,7 +965,7 @@ template <int VT, class Marks>
 __device__ __forceinline__ void distill_marked(const DistillArgs& a, const DisShared& sh, const Marks& mk, void* out, int j0, int j1) {
   using R = VRow<VT>;
   const int l = threadIdx.x & 63;
-  const double c = (double)a.c;
+  const double c = a.scale;
   for (int s = l; s < a.k; s += 64) {
     const int id = sh.id[s];
     if (!sh.first[s] || id < j0 || id >= j1) continue;

@@ -162,3 +162,21 @@ def test_draws_and_tests_at_the_borders_are_exact_to_64_bits(ctx, V, temp):
                    stream=stream())
     torch.cuda.synchronize()
     np.testing.assert_array_equal(acc.cpu().numpy(), (u < border).astype(np.int32))
+
+
+@pytest.mark.parametrize("temp", [1.0, 1.25, 1.44, 2.8848, 0.0907])
+def test_large_losses_carry_no_scale_of_32_bits(each_ctx, temp):
+    """A teacher that is certain of a token far below the student's best: kl is (max - z) / T to the rounding of the
+    result, whatever log2(e) / T rounds to as a float; the same for a label's log-probability."""
+    V, n = 3001, 64
+    rng = np.random.default_rng(7)
+    z = rng.normal(0, 1, (n, V)).astype(np.float32)
+    at = rng.integers(0, V, (n, 1))
+    np.put_along_axis(z, at, -rng.uniform(2e3, 6e4, (n, 1)).astype(np.float32), 1)
+    z64, t = z.astype(np.float64), float(np.float32(temp))
+    vals, tok = np.zeros((n, 1)), at[:, 0]
+    kl, lp, _ = losses(each_ctx, z, at, vals, None, temp, tok=tok)
+    want = -(np.take_along_axis(z64, at, 1)[:, 0] / t - D.lse(z64 / t))
+    assert np.all(np.abs(kl - want) <= 2 * SUM + HALF * want), np.abs(kl / want - 1).max() / HALF
+    want = np.take_along_axis(z64, at, 1)[:, 0] - D.lse(z64)
+    assert np.all(np.abs(lp - want) <= SUM + HALF * np.abs(want)), np.abs(lp / want - 1).max() / HALF
