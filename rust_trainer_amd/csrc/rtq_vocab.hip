@@ -348,7 +348,8 @@ __device__ __forceinline__ void top_pick(const TopArgs& a) {
   __shared__ double redd[W];
   __shared__ int hist[256];
   __shared__ int out[3];
-  __shared__ int cnt, groups;
+  __shared__ alignas(16) int wsum[2][W];
+  __shared__ int fewer;
   const int tid = threadIdx.x, l = tid & 63, i = blockIdx.x;
   const float ninf = -__builtin_inff(), inf = __builtin_inff();
   if (!row_ok(a, i)) {
@@ -370,7 +371,28 @@ __device__ __forceinline__ void top_pick(const TopArgs& a) {
     for (int w = 1; w < full; w++) t = r > 64 ? ninf : fminf(t, redf[w]);
     return t;
   };
-  if (tid == 0) cnt = 0, groups = 0;
+  // this thread's first place for n entries of a list that has `all` so far, by thread (not in order of arrival: which
+  // thread joins what to the rest decides its last bits); called by all threads.  Two buffers, so that one barrier will do
+  int cnt = 0, groups = 0, turn = 0;
+  auto places = [&](int n, int& all) {  // n <= 32
+    int at = all, sum = 0;
+#pragma unroll
+    for (int b = 0; b < 6; b++) {  // the lanes below and all, by the digits of n
+      const uint64_t m = __ballot((n >> b) & 1);
+      at += (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0)) << b;
+      sum += __popcll(m) << b;
+    }
+    if (l == 0) wsum[turn][tid >> 6] = sum;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+      const int o = wsum[turn][w];
+      at += w < tid >> 6 ? o : 0;
+      all += o;
+    }
+    turn ^= 1;
+    return at;
+  };
   // the first U B groups stay in registers (V up to 163840 f32 or 327680 16-bit logits: all of them)
   float m0[U], s0[U];
   auto load_groups = [&](int g0, float* m, float* s) {
@@ -406,32 +428,30 @@ __device__ __forceinline__ void top_pick(const TopArgs& a) {
         bits |= c ? 1u << u : 0u;
         w[u] = c ? 0.0f : s[u];
       }
-      if (bits) {
-        int at = atomicAdd(&groups, __popc(bits));
-        for (; bits; bits &= bits - 1, at++)
-          if (at < CAP) list[at] = (uint32_t)(g0 + (__ffs(bits) - 1) * B);
-      }
+      int at = places(__popc(bits), groups);
+      for (; bits; bits &= bits - 1, at++)
+        if (at < CAP) list[at] = (uint32_t)(g0 + (__ffs(bits) - 1) * B);
       if (a.rest) join_rest<U>(rm, rs, m, w, a);
     };
     if (kept) some(tid, m0, s0);
-    for (int g0 = tid + (kept ? U * B : 0); g0 < held; g0 += U * B) {
+    for (int b0 = kept ? U * B : 0; b0 < held; b0 += U * B) {
       float m[U], s[U];
-      load_groups(g0, m, s);
-      some(g0, m, s);
+      load_groups(b0 + tid, m, s);
+      some(b0 + tid, m, s);
     }
   };
   choose(true, [&](float m, int) { return !(m < thr); });
   __syncthreads();
-  // the listed groups' logits, UE vectors at a time: f(vector, index of its first); past the list's end
-  // the index is V
+  // the listed groups' logits, UE vectors a thread at a time, all threads together: f(vectors, indexes of their
+  // first); past the list's end the index is V or above
   auto each = [&](auto&& f) {
     const int n = groups * 8;
-    for (int p0 = tid; p0 < n; p0 += B * UE) {
+    for (int b0 = 0; b0 < n; b0 += B * UE) {
       u4v v[UE];
       int j[UE];
 #pragma unroll
       for (int u = 0; u < UE; u++) {
-        const int p = p0 + u * B;
+        const int p = b0 + tid + u * B;
         j[u] = p < n ? (int)list[p >> 3] * GS + (p & 7) * E : a.V;
       }
 #pragma unroll
@@ -439,33 +459,38 @@ __device__ __forceinline__ void top_pick(const TopArgs& a) {
         v[u] = u4v{0, 0, 0, 0};
         if (j[u] < a.V) v[u] = R::load_upto(row, j[u], a.V);
       }
-#pragma unroll
-      for (int u = 0; u < UE; u++)
-        if (j[u] < a.V) f(v[u], j[u]);
+      f(v, j);
     }
   };
   // the logits that in(x, index) takes are the candidates, the others go to the rest
   auto collect = [&](auto&& in) {
-    each([&](const u4v& v, int j) {
-      float x[E], w[E];
-      uint32_t bits = 0;
+    each([&](const u4v* v, const int* j) {
+      uint32_t bits = 0;  // E for each vector
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        x[e] = R::get(v, e);
-        const bool c = j + e < a.V && in(x[e], j + e);
-        bits |= c ? 1u << e : 0u;
-        w[e] = j + e < a.V && !c ? 1.0f : 0.0f;
+      for (int u = 0; u < UE; u++) {
+        if (j[u] >= a.V) continue;
+        float x[E], w[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          x[e] = R::get(v[u], e);
+          const bool c = j[u] + e < a.V && in(x[e], j[u] + e);
+          bits |= c ? 1u << (u * E + e) : 0u;
+          w[e] = j[u] + e < a.V && !c ? 1.0f : 0.0f;
+        }
+        if (a.rest) join_rest<E>(rm, rs, x, w, a);
       }
-      if (bits) {
-        int at = atomicAdd(&cnt, __popc(bits));
+      int at = places(__popc(bits), cnt);
+#pragma unroll
+      for (int u = 0; u < UE; u++) {
+        const uint32_t mine = bits >> (u * E) & ((1u << E) - 1);
+        if (!mine) continue;
 #pragma unroll
         for (int e = 0; e < E; e++)
-          if ((bits >> e) & 1) {
-            if (at < CAP) cand[at] = rank_key(x[e], j + e);
+          if ((mine >> e) & 1) {
+            if (at < CAP) cand[at] = rank_key(R::get(v[u], e), j[u] + e);
             at++;
           }
       }
-      if (a.rest) join_rest<E>(rm, rs, x, w, a);
     });
     __syncthreads();
   };
@@ -477,9 +502,11 @@ __device__ __forceinline__ void top_pick(const TopArgs& a) {
     // vocabulary) or too much reaches it: places are found by counting, n of n candidates each
     auto refine = [&]() {
       float em = ninf;
-      each([&](const u4v& v, int j) {
+      each([&](const u4v* v, const int* j) {
 #pragma unroll
-        for (int e = 0; e < E; e++) em = j + e < a.V ? fmaxf(em, R::get(v, e) != R::get(v, e) ? inf : R::get(v, e)) : em;
+        for (int u = 0; u < UE; u++)
+#pragma unroll
+          for (int e = 0; e < E; e++) em = j[u] + e < a.V ? fmaxf(em, R::get(v[u], e) != R::get(v[u], e) ? inf : R::get(v[u], e)) : em;
       });
       thr = fmaxf(thr, bound(em, groups * 8));
     };
@@ -488,8 +515,7 @@ __device__ __forceinline__ void top_pick(const TopArgs& a) {
     collect([&](float x, int) { return !(x < thr); });
     if (!none && cnt > 4 * a.k + 256) {
       refine();
-      if (tid == 0) cnt = 0;
-      __syncthreads();
+      cnt = 0;
       rm = gm_rest, rs = gs_rest;
       collect([&](float x, int) { return !(x < thr); });
     }
@@ -498,9 +524,7 @@ __device__ __forceinline__ void top_pick(const TopArgs& a) {
   if (many) {
     auto group_key = [&](float m, int g) { return rank_key(m, g); };
     const uint64_t gk = radix_kth<B>(held, min(a.k, held), hist, out, [&](int g) { return group_key(gm[g], g); });
-    __syncthreads();
-    if (tid == 0) cnt = 0, groups = 0;
-    __syncthreads();
+    cnt = 0, groups = 0;
     rm = ninf, rs = 0.0;
     choose(false, [&](float m, int g) { return group_key(m, g) >= gk; });  // min(k, held) of them
     __syncthreads();
@@ -517,13 +541,12 @@ __device__ __forceinline__ void top_pick(const TopArgs& a) {
   if (n > 2 * a.k + 128) {
     const uint64_t kth = radix_kth<B>(n, a.k, hist, out, [&](int p) { return cand[p]; });
     uint64_t* few = reinterpret_cast<uint64_t*>(list);
-    __syncthreads();
-    if (tid == 0) cnt = 0;
+    if (tid == 0) fewer = 0;
     __syncthreads();
     for (int p = tid; p < n; p += B) {
       const uint64_t key = cand[p];
       if (key >= kth) {
-        few[atomicAdd(&cnt, 1)] = key;
+        few[atomicAdd(&fewer, 1)] = key;  // (their places go by their keys)
       } else if (a.rest) {
         const float x = key_value(key), w = 1.0f;
         join_rest<1>(rm, rs, &x, &w, a);

@@ -180,3 +180,21 @@ def test_large_losses_carry_no_scale_of_32_bits(each_ctx, temp):
     assert np.all(np.abs(kl - want) <= 2 * SUM + HALF * want), np.abs(kl / want - 1).max() / HALF
     want = np.take_along_axis(z64, at, 1)[:, 0] - D.lse(z64)
     assert np.all(np.abs(lp - want) <= SUM + HALF * np.abs(want)), np.abs(lp / want - 1).max() / HALF
+
+
+def test_the_rest_does_not_depend_on_the_order_of_gathering(ctx):
+    """Rows whose rest is next to 0, where a float's steps are finest: the same bits from call to call."""
+    rng = np.random.default_rng(3)
+    for V, k in ((6000, 200), (20000, 200), (60000, 256)):
+        n = 512
+        z = rng.normal(0, 1.0, (n, V))
+        z -= D.top(z, k, 1.0)[2][:, None]
+        zd = dev(z.astype(np.float32))
+        first = None
+        for rep in range(6):
+            vals, ids, rest = torch.empty(n, k, device="cuda"), torch.empty(n, k, dtype=torch.int32, device="cuda"), torch.empty(n, device="cuda")
+            top_logits_d(ctx, zd.data_ptr(), rt.TYPE_F32, n, V, V, k, vals.data_ptr(), ids.data_ptr(), rest.data_ptr(), stream=stream())
+            torch.cuda.synchronize()
+            assert float(rest.abs().max()) < 1e-3
+            first = rest if first is None else first
+            assert torch.equal(first, rest), (V, k, rep, int((first != rest).sum()))
