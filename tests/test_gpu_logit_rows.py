@@ -198,3 +198,31 @@ def test_the_rest_does_not_depend_on_the_order_of_gathering(ctx):
             assert float(rest.abs().max()) < 1e-3
             first = rest if first is None else first
             assert torch.equal(first, rest), (V, k, rep, int((first != rest).sum()))
+
+
+def test_heads_of_an_empty_sequence(ctx):
+    """No hidden states: every position is out of range, so the losses are NaN, the lists empty and dx has no rows."""
+    import ctypes
+
+    V, d, n, k = 700, 64, 3, 4
+    rng = np.random.default_rng(11)
+    f = rt.HipFrozen.f32(rng.normal(0, 0.1, (V, d)), V, d, ctx=ctx)
+    norm, x, pos = torch.ones(d, device="cuda"), torch.ones(d, device="cuda"), dev(np.array([0, 1, -1], np.int32))
+    tok, w, dx = dev(np.array([1, 2, 3], np.int32)), torch.ones(n, device="cuda"), torch.full((d,), 7.0, device="cuda")
+    ids, vals = dev(np.arange(n * k, dtype=np.int32)), torch.zeros(n, k, device="cuda")
+    kl, lp, hit = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda"), torch.ones(n, dtype=torch.int32, device="cuda")
+    te = rt._ffi.RtqTeacher(k, ids.data_ptr(), vals.data_ptr(), None, 1.0)
+    head = (ctx.handle, f.handle, norm.data_ptr(), 1e-6, 0.0, x.data_ptr(), 0, pos.data_ptr())
+    rt._ffi.check(rt.lib().rtq_lm_distill_d(*head, tok.data_ptr(), w.data_ptr(), n, ctypes.byref(te), 0.5, kl.data_ptr(), lp.data_ptr(), dx.data_ptr(),
+                                            stream() or None), "distill")
+    torch.cuda.synchronize()
+    assert torch.isnan(kl).all() and torch.isnan(lp).all()
+    lp.zero_()
+    rt._ffi.check(rt.lib().rtq_lm_head_d(*head, tok.data_ptr(), w.data_ptr(), n, lp.data_ptr(), hit.data_ptr(), dx.data_ptr(), stream() or None), "head")
+    torch.cuda.synchronize()
+    assert torch.isnan(lp).all() and not hit.any()
+    rt._ffi.check(rt.lib().rtq_lm_top_logits_d(*head, n, k, 1.0, vals.data_ptr(), ids.data_ptr(), kl.data_ptr(), stream() or None), "top")
+    torch.cuda.synchronize()
+    assert torch.isnan(vals).all() and (ids == -1).all() and torch.isnan(kl).all()
+    assert torch.equal(dx, torch.full_like(dx, 7.0))
+    f.close()
