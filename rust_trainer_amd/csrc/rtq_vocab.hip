@@ -897,6 +897,7 @@ __device__ __forceinline__ void distill_teacher(const DistillArgs& a, DisShared&
   const double re = rest == -__builtin_inf() ? 0.0 : exp(rest - tmax);
   sum = wave_sum_any(sum) + re;
   if (l == 0) sh.taught = taught, sh.pr = taught ? re / sum : 0.0;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (all lanes read them)
   for (int s = l; s < a.k; s += 64) sh.p[s] = sh.pt[s] = taught ? sh.p[s] / sum : 0.0, sh.first[s] = sh.id[s] >= 0;
   if (twice) {  // a token's first slot stands for it, with the sum of its slots' probabilities in slot order
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
