@@ -194,8 +194,9 @@ rtq_status rtq_top_logits_d(rtq_ctx* ctx, const void* logits, int type, int64_t 
  * A label outside [0, vocab) is none: logp NaN, no gradient from it (host version: refused).
  * With weights (else NULL, and dlogits unused), for L = sum weights[i] ((1 - hard) T^2 kl[i] - hard logp[i]),
  * hard in [0, 1]: dlogits [n x vocab], rows ldd elements apart, = dL/dz in the logits' type, OVERWRITTEN;
- * it may be the logits themselves (same ldd), and must not overlap them otherwise.  A row of weight 0
- * has gradient 0.  A NaN or +inf logit, or a row of -inf alone, makes the row's outputs NaN. */
+ * it may be the logits themselves (same ldd), and must not overlap them otherwise.  A NaN or +inf logit,
+ * or a row of -inf alone, makes NaN what is asked of the row, but not what its inputs set to 0: a row of
+ * weight 0 has gradient 0, one without a teacher kl 0 and no gradient from it (its logp shows the NaN). */
 rtq_status rtq_distill(rtq_ctx* ctx, const void* logits, int type, int64_t n, int64_t vocab, int64_t ld,
                        const rtq_teacher* teacher, const int32_t* tok, const float* weights, float hard, float* kl,
                        float* logp, void* dlogits, int64_t ldd);

@@ -200,6 +200,28 @@ def test_the_rest_does_not_depend_on_the_order_of_gathering(ctx):
             assert torch.equal(first, rest), (V, k, rep, int((first != rest).sum()))
 
 
+@pytest.mark.parametrize("hard", [0.0, 0.5])
+def test_rows_without_a_teacher_or_a_weight_beside_bad_logits(each_ctx, hard):
+    """What is not asked of a row stays 0 whatever its logits: no teacher, no divergence and none of its gradient; weight
+    0, no gradient.  What is asked of it is NaN."""
+    V, n, k = 9000, 6, 3
+    rng = np.random.default_rng(10)
+    z = D.logits(rng, n, V)
+    z[0, 5], z[1, 6], z[3, 5], z[4, 5] = np.nan, np.inf, np.nan, np.nan
+    z[2] = -np.inf
+    ids = np.array([[1, 2, 3]] * n)
+    ids[[0, 1, 2, 4]] = -1
+    rest = np.zeros(n)
+    rest[[0, 1, 2, 4]] = -np.inf
+    w = np.array([1.0, 1, 1, 0, 0, 1])
+    for ty in ("f32", "bf16"):
+        kl, lp, g = losses(each_ctx, z, ids, np.zeros((n, k)), rest, 1.0, rng.integers(0, V, n), w, hard, ty)
+        assert not kl[[0, 1, 2, 4]].any() and np.isnan(kl[3]) and np.isfinite(kl[5])
+        assert np.isnan(lp[:5]).all() and np.isfinite(lp[5])
+        assert np.isnan(g[:3]).all() if hard else not g[:3].any()
+        assert not g[3:5].any() and np.isfinite(g[5]).all() and g[5].any()
+
+
 def test_heads_of_an_empty_sequence(ctx):
     """No hidden states: every position is out of range, so the losses are NaN, the lists empty and dx has no rows."""
     import ctypes
