@@ -200,6 +200,26 @@ def test_the_rest_does_not_depend_on_the_order_of_gathering(ctx):
             assert torch.equal(first, rest), (V, k, rep, int((first != rest).sum()))
 
 
+def test_many_verification_rows(ctx):
+    """More rows than one grid dimension holds."""
+    b, d, V = 300, 130, 5
+    rng = np.random.default_rng(9)
+    zp, zq = rng.normal(0, 1, (b * (d + 1), V)).astype(np.float32), rng.normal(0, 1, (b * d, V)).astype(np.float32)
+    zq.reshape(b, d, V)[150:] = zp.reshape(b, d + 1, V)[150:, :d]  # accepted far
+    x = np.argmax(zq, 1).reshape(b, d).astype(np.int32)
+    u = rng.random((b, d + 1)).astype(np.float32)
+    assert b * (2 * d + 1) > 65535
+    args = [dev(a) for a in (zp, zq, x, u)]
+    for temp, draft in ((1.0, True), (1.0, False), (0.0, False)):
+        acc, out = torch.empty(b, dtype=torch.int32, device="cuda"), torch.empty(b, d + 1, dtype=torch.int32, device="cuda")
+        verify_draft_d(ctx, args[0].data_ptr(), rt.TYPE_F32, V, args[1].data_ptr() if draft else 0, V if draft else 0, b, d, V, args[2].data_ptr(), 0,
+                       args[3].data_ptr(), acc.data_ptr(), out.data_ptr(), temperature=temp, stream=stream())
+        torch.cuda.synchronize()
+        want = D.verify(zp, zq if draft else None, x, None, u, temp)
+        np.testing.assert_array_equal(acc.cpu().numpy(), want[0])
+        np.testing.assert_array_equal(out.cpu().numpy(), want[1])
+
+
 @pytest.mark.parametrize("hard", [0.0, 0.5])
 def test_rows_without_a_teacher_or_a_weight_beside_bad_logits(each_ctx, hard):
     """What is not asked of a row stays 0 whatever its logits: no teacher, no divergence and none of its gradient; weight
