@@ -7,7 +7,7 @@ from the teacher, mixed with the labels' cross-entropy, and its gradient.  ``ver
 tokens that a draft model (a distilled student, say) proposed, such that what comes out is distributed as the
 target's samples.
 
-Rows are numpy arrays of float32 or float16 (bfloat16: uint16 arrays with ``type=TYPE_BF16``); a row may be longer
+Rows are numpy arrays of float32 or float16 (bfloat16: its bits in uint16 arrays, with ``type=TYPE_BF16``); a row may be longer
 apart than it is long (a view ``a[:, :vocab]``).  ``head_top_logits`` and ``head_distill`` take the rows from an LM head
 (``GpuModel.top_logits``, ``forward_backward_distill`` and ``verify_draft`` from a whole model).  The ``_d`` variants take device addresses and a stream and only enqueue.
 """
@@ -50,7 +50,9 @@ def _rows(a, type: int | None, what: str) -> tuple[np.ndarray, int, int]:
     if type is None:
         type = {np.dtype(np.float32): _ffi.TYPE_F32, np.dtype(np.float16): _ffi.TYPE_F16}.get(a.dtype)
         assert type is not None, f"{what}: {a.dtype} logits"
-    assert a.dtype.itemsize == (4 if type == _ffi.TYPE_F32 else 2), f"{what}: {a.dtype} is not of the given type"
+    own = {_ffi.TYPE_F32: np.float32, _ffi.TYPE_F16: np.float16}.get(type)
+    bits = type != _ffi.TYPE_F32 and a.dtype.itemsize == 2 and a.dtype.kind != "f"  # 16-bit types as integers
+    assert a.dtype.isnative and (a.dtype.type is own or bits), f"{what}: {a.dtype} is not of the given type"
     if a.size and (a.strides[1] != a.itemsize or (a.shape[0] > 1 and (a.strides[0] % a.itemsize or a.strides[0] < a.shape[1] * a.itemsize))):
         a = np.ascontiguousarray(a)
     return a, type, a.strides[0] // a.itemsize if a.shape[0] > 1 else a.shape[1]
