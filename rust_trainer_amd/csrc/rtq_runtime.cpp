@@ -1963,15 +1963,16 @@ constexpr int64_t kDistillStaticLds = 9 << 10;  // at least rtq_distill*_*'s own
 int64_t distill_lds(int rows, int64_t V) { return ((256 << rows) - 64) * 8 * 16 + (V / 32 + 1) * 4; }
 
 // Which kernels, by times in us fitted to a sweep (V 2048 to 151936, 1 to 2048 rows, both types, with and without
-// a gradient).  A row a workgroup takes about 8 us and 0.2 ns a logit (0.12 without the gradient), whatever the
-// number of rows up to the CUs'; slices of all rows at once take two launches, 14 us, and 2.3 ns a thousand f32
-// logits (1.15 of 16 bits; without the gradient 0.65 and 0.48).  So slices run few rows of a large vocabulary
-// (151936 f32, 16 rows: 17 us against 40; 256 rows: 103 against 68), and many such rows without a gradient (1024:
-// 118 against 134).
+// a gradient).  A row a workgroup takes about 8 us and 0.2 ns a logit (0.12 without the gradient) up to some 64 rows,
+// and more as memory fills (151936 f32: 39 us at 16 rows, 48 at 128, 83 at 256), in whole rounds of the CUs (257 rows:
+// 114); slices of all rows at once take two launches, 14 us, and 2.3 ns a thousand f32 logits (1.15 of 16 bits;
+// without the gradient 0.65 and 0.48).  So slices run few rows of a large vocabulary (151936 f32, 16 rows: 17 us against
+// 39; 256 rows: 115 against 83), and many such rows without a gradient (1024: 119 against 133).  Just beyond a round
+// slices can be better and are not taken (257 rows of 16 bits: 70 against 81; of f32 the same 115).
 // Of the workgroup sizes, each holds 24 vectors of 16 bytes a thread on the chip, 22 of 16-bit logits.  256
-// threads let four rows share a CU, 512 two: better where they hold the row and there are enough (8192 f32, 2048 rows: 37 / 44 / 66
-// us; 64000 bf16, 512 rows: 50 / 43 / 48), while one row alone is fastest on the largest that it fills (32000
-// f32: 25 / 15 / 13).
+// threads let four rows share a CU, 512 two: better where they hold the row and there are enough (8192 f32, 2048 rows: 37 / 45 / 70
+// us; 64000 bf16, 512 rows: 48 / 38 / 47), while one row alone is fastest on the largest that it fills (32000
+// f32: 23 / 14 / 13).
 DistillPlan distill_plan(const rtq_ctx* c, int type, int64_t n, int64_t V, int64_t k, bool grad) {
   const int64_t E = 16 / logit_bytes(type), per = E == 4 ? 24 : 22, cus = c->cu_count;
   DistillPlan p{};

@@ -333,9 +333,9 @@ __device__ __forceinline__ void join_rest(float& m, double& s, const float* x, c
 // it.  The groups that reach it (1.5 to 4 k of them in a row without structure) are read again, and what
 // reaches it there is ranked by counting.  Where too many do, a second bound comes from the
 // logits of those groups; where that does not help either (ties, masks, sorted rows), exactly the k
-// groups and then exactly the k logits are found digit by digit.  512 threads: alone on the chip 8.4 us
-// at k = 20 of 151936 f32 logits against 9.5 with 256 and 10.2 with 1024; 1024 rows at k = 128 take 38.8 us
-// against 40.9 and 67.6.
+// groups and then exactly the k logits are found digit by digit.  512 threads: alone on the chip 8.9 us
+// at k = 20 of 151936 f32 logits, and 36 us for 1024 rows at k = 128 (lists filled by atomics took 8.4 and 38.8,
+// 9.5 and 40.9 with 256 threads, 10.2 and 67.6 with 1024).
 constexpr int kPickB = 512;
 
 template <int VT>
@@ -535,7 +535,7 @@ __device__ __forceinline__ void top_pick(const TopArgs& a) {
     collect([&](float x, int j) { return rank_key(x, j) >= ek; });  // k of them
   }
   // Many candidates more than k (a small vocabulary, of which k is a large part): first exactly the k, found digit
-  // by digit (2000 rows of 1000 f32 logits, k = 256: 64 us, 172 by counting all of them).
+  // by digit (2000 rows of 1000 f32 logits, k = 256: 61 us, 172 by counting all of them).
   const uint64_t* best = cand;
   int n = cnt;
   if (n > 2 * a.k + 128) {
@@ -596,7 +596,8 @@ RTQ_TOP(bf16, VT_BF16)
 // rtq_distill*_<type>: a row a workgroup, whose first wave does the row's scalars (the teacher's list, the
 // losses, the gradient at the listed tokens) while the others hold their first kDisV vectors a thread in
 // registers and the next kDisL in LDS from the statistics to the gradient: one read and one write of the row
-// (what a longer row has beyond them is read twice).  2048 rows of 151936 bf16 take 295 us, 4.2 TB/s.
+// (what a longer row has beyond them is read twice: of 151936 f32 logits 39%, of 16 bits none).  2048 rows of 151936
+// bf16 take 292 us, 4.3 TB/s; 256 of f32 83 us, 4.5 TB/s with the second read.
 // rtq_distill_stats_* / _grad_* do the two halves for slices, of few long rows or without a gradient.
 //
 // Exponentials are exp2(fma(z, c, -K)), one FMA and the instruction: c = log2(e) / T rounded to f32, and a
@@ -1211,7 +1212,8 @@ RTQ_DISTILL(bf16, VT_BF16)
 // passes u_d times the total.  T = 0: accept while x_j is the target's largest logit (the lowest index
 // of equals), which is also the token after.  Steps of the running sum over a flat tail lie nearer
 // than 2^-24 of the total, so exponentials and sums are in 64 bits, whose arithmetic bounds the statistics (384
-// rows of 151936 bf16 logits: 51 us, 2.3 TB/s; in one pass with a running maximum, the loads ahead of the sums: 53).
+// rows of 151936 bf16 logits: 51 us, 2.3 TB/s, the VALU busy 83% of it; in one pass with a running maximum, the loads
+// ahead of the sums: 53).
 constexpr int kVdB = 256, kVdW = kVdB / 64, kVdV = 8;
 
 // 2^(y / 256) for y <= 0: y = 256 n + i + f with |f| <= 1/2, a table of 2^(i / 256), and the series of exp(x) to
