@@ -33,7 +33,7 @@ def listed():
          "heads": 32, "kv": 8, "d": 128, "rot": 128, "neox": False, "norm": False, "page": 64, "base": 5e5, "gap": 0},
         # prompts of several lengths, an odd head size that is rotated in part, small pages, rows further apart than they are long
         {"name": "append_odd_f16", "op": "append", "dtype": "f16", "cache": "f16", "b": 13, "len": 333, "new": 157, "ragged": True, "tree": False,
-         "heads": 15, "kv": 3, "d": 80, "rot": 32, "neox": True, "norm": False, "page": 16, "base": 1e4, "gap": 37},
+         "heads": 15, "kv": 3, "d": 80, "rot": 32, "neox": True, "norm": False, "page": 32, "base": 1e4, "gap": 37},
         # a long document's prompt in one call
         {"name": "append_prompt_f32", "op": "append", "dtype": "f32", "cache": "f16", "b": 1, "len": 0, "new": 16384, "ragged": False, "tree": False,
          "heads": 16, "kv": 8, "d": 128, "rot": 128, "neox": True, "norm": True, "page": 64, "base": 1e6, "gap": 0},
@@ -48,7 +48,7 @@ def listed():
          "heads": 32, "kv": 8, "d": 128, "page": 64, "gap": 0},
         # small trees of several sizes, sequences without new tokens among them, an odd head size, small pages, strided rows
         {"name": "attend_odd_f32", "op": "attend", "dtype": "f32", "cache": "bf16", "b": 13, "len": 3001, "new": 11, "ragged": True, "tree": True,
-         "heads": 15, "kv": 3, "d": 80, "page": 16, "gap": 37},
+         "heads": 15, "kv": 3, "d": 80, "page": 32, "gap": 37},
         # the next token over one very long document
         {"name": "attend_document_f16", "op": "attend", "dtype": "f16", "cache": "f16", "b": 1, "len": 131072, "new": 1, "ragged": False, "tree": False,
          "heads": 32, "kv": 8, "d": 128, "page": 128, "gap": 0},
@@ -72,7 +72,7 @@ def draw(rng):
     op = rng.choice(("append", "append", "attend", "attend", "attend", "keep"))
     cache = rng.choice(("f16", "bf16"))
     d = rng.choice((64, 80, 96, 128, 128, 256))
-    c = {"op": op, "cache": cache, "ragged": rng.random() < 0.5, "kv": rng.choice((1, 2, 3, 4, 8)), "d": d, "page": rng.choice((16, 32, 64, 128, 256))}
+    c = {"op": op, "cache": cache, "ragged": rng.random() < 0.5, "kv": rng.choice((1, 2, 3, 4, 8)), "d": d, "page": rng.choice((32, 64, 128, 256))}
     if op == "keep":
         c.update(layers=rng.randint(1, 32), tree=True, b=_spread(rng, 1, 32), len=_spread(rng, 1, 200), new=rng.randint(8, 64), kept=rng.randint(1, 8))
         return c
