@@ -244,6 +244,80 @@ rtq_status rtq_lm_distill_d(rtq_ctx* ctx, const rtq_weight* lm_head, const float
                             int64_t n, const rtq_teacher* teacher, float hard, float* kl, float* logp, float* dx,
                             void* stream);
 
+/* ---- paged cache of keys and values: append, attention of runs and trees, keep ----
+ * No counterpart in the reference.  A cache holds `n_pages` pages for each of n_layer layers; a page is page_size
+ * slots (a power of two, 32 .. 1024) of n_head_kv heads of head_dim (a multiple of 16, 16 .. 256) in
+ * RTQ_TYPE_F16 or _BF16: keys [page][head][slot][head_dim], values [page][head][head_dim][slot].  One page id
+ * names a page of every layer.  k and v of rtq_kv_cache_create: device memory of the caller (16-byte aligned,
+ * n_layer n_pages n_head_kv page_size head_dim elements each, alive as long as the cache), or both NULL: allocated
+ * here, zeros.  A cache is destroyed before its context.  (With the caller's pages ctx may be NULL: the calls' arguments
+ * are checked, then the call is refused.) */
+typedef struct rtq_kv_cache rtq_kv_cache;
+rtq_status rtq_kv_cache_create(rtq_ctx* ctx, int type, int64_t n_layer, int64_t n_pages, int64_t page_size,
+                               int64_t n_head_kv, int64_t head_dim, void* k, void* v, rtq_kv_cache** out);
+void rtq_kv_cache_destroy(rtq_kv_cache* kc);
+rtq_status rtq_kv_cache_pages(const rtq_kv_cache* kc, int64_t layer, void** k, void** v); /* device addresses */
+/* The sequences of a call.  Sequence i holds lens[i] tokens, slot s of it in page table[i ld + s / page_size]; its new
+ * tokens are rows starts[i] .. starts[i + 1] - 1 (ascending; NULL: n / b each) and take the slots after the held
+ * ones.  lens is the caller's to advance, after the last layer.  Rows behind starts[b] are neither read nor
+ * written.  No two sequences of a call may write one slot (pages that are only read may be shared). */
+typedef struct rtq_kv_seqs {
+  int64_t b;             /* sequences, 1 .. 65536 */
+  const int32_t* lens;   /* [b] */
+  const int32_t* starts; /* [b + 1] or NULL */
+  const int32_t* table;  /* [b x ld] */
+  int64_t ld;            /* pages of a table row */
+} rtq_kv_seqs;
+/* The rotation of heads' first `dim` elements (even, 0 .. min(head_dim, 256); 0: none) by position x base^(-2 i / dim)
+ * x freq_scale / factors[i] (factors: host memory, n_factors <= dim / 2, a 0 divides by nothing), pairs (i, i + dim / 2)
+ * with neox, else (2 i, 2 i + 1); before it, where q_norm / k_norm [head_dim] are given, each head's RMS norm
+ * x / sqrt(mean x^2 + eps) (norm + offset).  Angles are taken in 64 bits. */
+typedef struct rtq_rope {
+  int64_t dim;
+  float base, freq_scale;
+  int neox;
+  const float* factors;
+  int64_t n_factors;
+  const float* q_norm;
+  const float* k_norm;
+  float eps, offset;
+} rtq_rope;
+/* The calls below take rows of `type` (RTQ_TYPE_F32, or the cache's type), a row's heads one after another, rows `ld..`
+ * elements apart at any alignment of an element.  The host versions take host arrays (the pages stay on the device),
+ * refuse lists and ids that the `_d` versions treat as stated, and are synchronous; `_d` calls may be captured into
+ * a HIP graph as those on rows of logits may.  A page id outside [0, n_pages), and a slot past the table's end, is
+ * not there: it is neither written nor read (host version: refused where a new or held token needs it).
+ *
+ * rtq_kv_append: the keys k [n x n_head_kv head_dim] (normed and rotated) and the values v of n new tokens enter the
+ * cache's layer; with q [n x n_head head_dim] (else NULL), q_out = the queries normed and rotated, in `type` (q itself is
+ * allowed, with its stride).  positions [n] (NULL: each token's slot) are what the rotation takes. */
+rtq_status rtq_kv_append(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* seqs, int64_t n, int type, const rtq_rope* rope,
+                         const int32_t* positions, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                         int64_t n_head, const void* q, int64_t ldq, void* q_out, int64_t ldo);
+rtq_status rtq_kv_append_d(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* seqs, int64_t n, int type,
+                           const rtq_rope* rope, const int32_t* positions, const void* k, int64_t ldk, const void* v,
+                           int64_t ldv, int64_t n_head, const void* q, int64_t ldq, void* q_out, int64_t ldo, void* stream);
+#define RTQ_TREE_MAX 1024 /* most new tokens of a sequence that is a tree */
+/* out [n x n_head head_dim] = attention of q over the cache's layer, whose slots hold the new tokens' keys and values
+ * already; n_head a multiple of n_head_kv, query head h reads KV head h / (n_head / n_head_kv); weights softmax(scale q k) (scale
+ * 0: 1 / sqrt(head_dim)).  A new token sees every held token, itself, and: without parents, the new tokens before it;
+ * with parents [n] (the index of a token's parent among its sequence's new tokens, before its own; -1: the last held
+ * token), its chain of parents.  A token whose chain meets an entry that is neither sees nothing, and of a sequence
+ * of more than RTQ_TREE_MAX new tokens with parents none does (host version: refused; -2 marks an unused node in
+ * both).  A row that sees no key with a score above -inf is 0.  What a token does not see, NaN and infinities included,
+ * does not change its row.  out may be q itself, with its stride. */
+rtq_status rtq_kv_attend(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* seqs, int64_t n, int type, int64_t n_head,
+                         float scale, const int32_t* parents, const void* q, int64_t ldq, void* out, int64_t ldo);
+rtq_status rtq_kv_attend_d(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* seqs, int64_t n, int type, int64_t n_head,
+                           float scale, const int32_t* parents, const void* q, int64_t ldq, void* out, int64_t ldo,
+                           void* stream);
+/* Keeps some of each sequence's new tokens, in every layer: kept [b x ldk] (1 <= ldk <= RTQ_TREE_MAX) lists them in
+ * ascending order of their index, ended by -1 (_d: by the first entry that does not ascend); the j-th moves to slot
+ * lens[i] + j.  lens_out [b] (or NULL; not lens itself) = lens + the number kept.  seqs->starts is not read. */
+rtq_status rtq_kv_keep(rtq_kv_cache* kc, const rtq_kv_seqs* seqs, const int32_t* kept, int64_t ldk, int32_t* lens_out);
+rtq_status rtq_kv_keep_d(rtq_kv_cache* kc, const rtq_kv_seqs* seqs, const int32_t* kept, int64_t ldk, int32_t* lens_out,
+                         void* stream);
+
 /* ---- device-resident training step (Model::forward_backward over the frozen linears) ----
  * A GGUF Qwen / Llama decoder (load_gguf_from, src/rie.rs:164-260) with every frozen tensor, norm
  * and adapter in device memory.  One call runs embed_tokens, the blocks (RMSNorm, q/k/v, QK-norm,

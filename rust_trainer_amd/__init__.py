@@ -11,6 +11,7 @@ from .distill import Teacher, distill, head_distill, head_top_logits, top_logits
 from .frozen import Context, FrozenMatmul, HipFrozen, default_context, pack_trainer_q8_0  # noqa: F401
 from .gguf import GgufFile, GgufWriter, SyntheticSpec, Value  # noqa: F401
 from .head import Target, answer_targets, embed_tokens, head  # noqa: F401
+from .kvcache import KvCache, Rope, Seqs  # noqa: F401
 from .linear import Linear, Lora  # noqa: F401
 from .model import GpuModel  # noqa: F401
 
@@ -18,4 +19,4 @@ __all__ = ["Context", "FrozenMatmul", "HipFrozen", "Linear", "Lora", "RtqError",
            "TYPE_Q4_0", "TYPE_Q8_0", "TYPE_Q4_K", "TYPE_Q6_K", "TYPE_F32", "TYPE_TQ8_0", "pack_trainer_q8_0",
            "GgufFile", "GgufWriter", "SyntheticSpec", "Value", "Target", "answer_targets", "embed_tokens", "head", "GpuModel",
            "TYPE_F16", "TYPE_BF16", "Teacher", "distill", "head_distill", "head_top_logits", "top_logits",
-           "verify_draft"]
+           "verify_draft", "KvCache", "Rope", "Seqs"]

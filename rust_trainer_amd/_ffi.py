@@ -20,6 +20,7 @@ TYPE_F32, TYPE_TQ8_0 = 0, 264
 # element types of rows of logits, beside TYPE_F32
 TYPE_F16, TYPE_BF16 = 1, 30
 TOP_MAX = 256  # most listed tokens a row
+TREE_MAX = 1024  # most new tokens of a sequence that is a tree
 
 # every symbol include/rtq.h declares, with (restype, argtypes)
 _p = ctypes.c_void_p
@@ -43,6 +44,20 @@ class RtqTeacher(ctypes.Structure):
 
 
 _TP = ctypes.POINTER(RtqTeacher)
+
+
+class RtqKvSeqs(ctypes.Structure):
+    _fields_ = [("b", ctypes.c_int64), ("lens", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("ld", ctypes.c_int64)]
+
+
+class RtqRope(ctypes.Structure):
+    _fields_ = [("dim", ctypes.c_int64), ("base", ctypes.c_float), ("freq_scale", ctypes.c_float), ("neox", ctypes.c_int),
+                ("factors", ctypes.c_void_p), ("n_factors", ctypes.c_int64), ("q_norm", ctypes.c_void_p),
+                ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float), ("offset", ctypes.c_float)]
+
+
+_SP, _RP = ctypes.POINTER(RtqKvSeqs), ctypes.POINTER(RtqRope)
 
 
 class RtqModelConfig(ctypes.Structure):
@@ -99,6 +114,16 @@ SIGNATURES = {
     "rtq_lm_top_logits_d": (_i, [_p, _p, _p, _f, _f, _p, _i64, _p, _i64, _i64, _f, _p, _p, _p, _p]),
     "rtq_lm_distill": (_i, [_p, _p, _p, _f, _f, _p, _i64, _p, _p, _p, _i64, _TP, _f, _p, _p, _p]),
     "rtq_lm_distill_d": (_i, [_p, _p, _p, _f, _f, _p, _i64, _p, _p, _p, _i64, _TP, _f, _p, _p, _p, _p]),
+    # paged cache of keys and values
+    "rtq_kv_cache_create": (_i, [_p, _i, _i64, _i64, _i64, _i64, _i64, _p, _p, ctypes.POINTER(_p)]),
+    "rtq_kv_cache_destroy": (None, [_p]),
+    "rtq_kv_cache_pages": (_i, [_p, _i64, ctypes.POINTER(_p), ctypes.POINTER(_p)]),
+    "rtq_kv_append": (_i, [_p, _i64, _SP, _i64, _i, _RP, _p, _p, _i64, _p, _i64, _i64, _p, _i64, _p, _i64]),
+    "rtq_kv_append_d": (_i, [_p, _i64, _SP, _i64, _i, _RP, _p, _p, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _p]),
+    "rtq_kv_attend": (_i, [_p, _i64, _SP, _i64, _i, _i64, _f, _p, _p, _i64, _p, _i64]),
+    "rtq_kv_attend_d": (_i, [_p, _i64, _SP, _i64, _i, _i64, _f, _p, _p, _i64, _p, _i64, _p]),
+    "rtq_kv_keep": (_i, [_p, _SP, _p, _i64, _p]),
+    "rtq_kv_keep_d": (_i, [_p, _SP, _p, _i64, _p, _p]),
     # device-resident training step
     "rtq_linear_forward_noalloc_d": (_i, [_p, _p, _p, _LP, _p, _i64, _p, _p]),
     "rtq_model_from_gguf": (_i, [_p, _p, ctypes.POINTER(_p)]),

@@ -633,3 +633,49 @@ struct MMaskArgs {
   int nm;
   int64_t row0[3], nrow[3], col0[3], r[3];
 };
+
+// ---- paged cache of keys and values (rtq_kv.hip)
+#define RTQ_KV_ROT 256  // most rotated elements of a head
+// the sequences of a call: new tokens are rows starts[i] .. starts[i + 1] - 1 (null: n / b each)
+struct KvSeqs {
+  const int32_t* lens;    // [b] tokens held before the call
+  const int32_t* starts;  // [b + 1] or null
+  const int32_t* table;   // [b x ldt] pages
+  int b, n, ldt;
+};
+struct KvAppendArgs {
+  KvSeqs s;
+  uint16_t *k, *v;  // the layer's pages
+  const void *q, *kx, *vx;  // rows of ldq, ldk, ldv elements (q null: none)
+  void* qo;
+  int64_t ldq, ldk, ldv, ldo;
+  const int32_t* pos;  // [n] or null: the tokens' slots
+  const float *q_norm, *k_norm;  // [d] or null
+  float eps, off;
+  int nh, nkv, d, rot, neox, ps_shift, n_pages;
+  int vt;  // workgroups of values: (tokens / 32) x KV heads, after those of the tokens
+  double freq[RTQ_KV_ROT / 2];  // turns per position of each pair
+};
+struct KvAttendArgs {
+  KvSeqs s;
+  const uint16_t *k, *v;  // the layer's pages
+  const void* q;
+  void* o;
+  int64_t ldq, ldo;
+  const int32_t* parents;  // [n] or null: runs
+  int nh, nkv, d, ps_shift, n_pages;
+  float scale2;     // scale log2(e)
+  int target;       // items that the keys are split into (at most this many, and one per tile beside)
+  int slots, qids;  // partial slots; query tiles (x KV heads) that the plan may name
+  int tm;           // rows of a tile
+  float* part;      // [slots][rows of a tile][D]
+  float* ml;        // [slots][rows of a tile][2]: maximum, sum
+  int32_t* desc;    // [0] query tiles named, then per tile 8: first slot, splits, first row of the tile ...
+};
+struct KvKeepArgs {
+  const int32_t *lens, *table, *kept;
+  int32_t* after;  // [b] or null
+  int b, ldt, ldk, nkv, d, ps_shift, n_pages;
+  uint16_t *k, *v;
+  int64_t layer;  // elements of a layer's keys (and of its values)
+};

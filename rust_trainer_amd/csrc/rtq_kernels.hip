@@ -4603,6 +4603,7 @@ extern "C" __global__ __launch_bounds__(256) void rtq_head_norm_bwd(HeadArgs a) 
 
 // ============================================================== rows of vocabulary logits
 #include "rtq_vocab.hip"
+#include "rtq_kv.hip"
 
 // ============================================================== decoder block (model-level step)
 #include "rtq_dense.hip"

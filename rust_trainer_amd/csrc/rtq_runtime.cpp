@@ -18,6 +18,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -174,7 +175,11 @@ enum Kid {
   K_VERIFY_GREEDY = K_VERIFY_STATS + 3,
   K_VERIFY_MASS = K_VERIFY_GREEDY + 3,
   K_VERIFY_PICK = K_VERIFY_MASS + 3,
-  K_ROWS = K_VERIFY_PICK + 3,  // + format
+  K_KV_APPEND = K_VERIFY_PICK + 3,  // + rows and cache (f32 f16, f32 bf16, f16, bf16)
+  K_KV_KEEP = K_KV_APPEND + 4,
+  K_KV_ATTEND,                            // + 7 x rows and cache + tile and head size (kv_variant)
+  K_KV_MERGE = K_KV_ATTEND + 28,          // + 3 x type + head size (64, 128, 256)
+  K_ROWS = K_KV_MERGE + 9,  // + format
   K_MODEL = K_ROWS + F_COUNT,  // + RtqModelKernel: the decoder block (rtq_model.cpp)
   K_COUNT = K_MODEL + KM_COUNT
 };
@@ -215,6 +220,18 @@ constexpr const char* kKernelNames[] = {
     "rtq_verify_greedy_f32", "rtq_verify_greedy_f16", "rtq_verify_greedy_bf16",
     "rtq_verify_mass_f32",  "rtq_verify_mass_f16",  "rtq_verify_mass_bf16",
     "rtq_verify_pick_f32",  "rtq_verify_pick_f16",  "rtq_verify_pick_bf16",
+    "rtq_kv_append_f32_f16", "rtq_kv_append_f32_bf16", "rtq_kv_append_f16", "rtq_kv_append_bf16", "rtq_kv_keep",
+    "rtq_kv_attend16_64_f32_f16", "rtq_kv_attend16_128_f32_f16", "rtq_kv_attend16_128p_f32_f16", "rtq_kv_attend16_256p_f32_f16",
+    "rtq_kv_attend32_64_f32_f16", "rtq_kv_attend32_128_f32_f16", "rtq_kv_attend32_128p_f32_f16",
+    "rtq_kv_attend16_64_f32_bf16", "rtq_kv_attend16_128_f32_bf16", "rtq_kv_attend16_128p_f32_bf16", "rtq_kv_attend16_256p_f32_bf16",
+    "rtq_kv_attend32_64_f32_bf16", "rtq_kv_attend32_128_f32_bf16", "rtq_kv_attend32_128p_f32_bf16",
+    "rtq_kv_attend16_64_f16", "rtq_kv_attend16_128_f16", "rtq_kv_attend16_128p_f16", "rtq_kv_attend16_256p_f16",
+    "rtq_kv_attend32_64_f16", "rtq_kv_attend32_128_f16", "rtq_kv_attend32_128p_f16",
+    "rtq_kv_attend16_64_bf16", "rtq_kv_attend16_128_bf16", "rtq_kv_attend16_128p_bf16", "rtq_kv_attend16_256p_bf16",
+    "rtq_kv_attend32_64_bf16", "rtq_kv_attend32_128_bf16", "rtq_kv_attend32_128p_bf16",
+    "rtq_kv_merge64_f32", "rtq_kv_merge128_f32", "rtq_kv_merge256_f32",
+    "rtq_kv_merge64_f16", "rtq_kv_merge128_f16", "rtq_kv_merge256_f16",
+    "rtq_kv_merge64_bf16", "rtq_kv_merge128_bf16", "rtq_kv_merge256_bf16",
     "rtq_rows_q4_0",        "rtq_rows_q8_0",        "rtq_rows_q4_k",        "rtq_rows_q6_k",
     "rtq_m_rmsnorm",        "rtq_m_rmsnorm_bwd",    "rtq_m_qk_prep",        "rtq_m_qk_bwd",
     "rtq_m_gemm",           "rtq_m_softmax",        "rtq_m_softmax_bwd",    "rtq_m_group_sum",
@@ -2138,6 +2155,258 @@ rtq_status rtq_verify_draft_d(rtq_ctx* c, const void* z, int type, int64_t ld, c
   return enqueue_verify(c, z, type, ld, q, ldq, b, d, V, drafted, lens, u, temp, accepted, tokens, p, ar, st);
 }
 
+// ------------------------------------------------------------------ paged cache of keys and values
+struct rtq_kv_cache {
+  rtq_ctx* ctx = nullptr;
+  int type = 0, ps_shift = 0;
+  int64_t n_layer = 0, n_pages = 0, ps = 0, nkv = 0, d = 0;
+  int64_t layer = 0;  // elements of a layer's keys (and of its values)
+  uint16_t *k = nullptr, *v = nullptr;
+  bool owned = false;
+};
+
+namespace {
+// rows and cache: f32 f16, f32 bf16, f16, bf16 (-1: not supported)
+int kv_types(const rtq_kv_cache* kc, int type) {
+  const int h = kc->type == RTQ_TYPE_F16 ? 0 : 1;
+  return type == RTQ_TYPE_F32 ? h : type == kc->type ? 2 + h : -1;
+}
+
+rtq_status kv_check_seqs(const rtq_kv_cache* kc, const rtq_kv_seqs* s) {
+  if (!kc) return fail(RTQ_ERR_INVALID, "null cache");
+  if (!s) return fail(RTQ_ERR_INVALID, "null sequences");
+  if (s->b < 1 || s->b > 65536) return fail(RTQ_ERR_INVALID, "%lld sequences", (long long)s->b);
+  if (s->ld < 0 || s->ld > (1LL << 30)) return fail(RTQ_ERR_INVALID, "%lld pages in a table row", (long long)s->ld);
+  if (!s->lens || (s->ld > 0 && !s->table)) return fail(RTQ_ERR_INVALID, "null lens/table");
+  return RTQ_OK;
+}
+
+rtq_status kv_check(const rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s, int64_t n, int type) {
+  RTQ_TRY(kv_check_seqs(kc, s));
+  if (layer < 0 || layer >= kc->n_layer) return fail(RTQ_ERR_INVALID, "layer %lld of %lld", (long long)layer, (long long)kc->n_layer);
+  if (n < 0 || n > (1 << 24)) return fail(RTQ_ERR_INVALID, "%lld new tokens", (long long)n);
+  if (!s->starts && n % s->b) return fail(RTQ_ERR_INVALID, "%lld new tokens for %lld sequences, and no starts", (long long)n, (long long)s->b);
+  if (kv_types(kc, type) < 0) return fail(RTQ_ERR_UNSUPPORTED, "rows of type %d over a cache of type %d", type, kc->type);
+  return RTQ_OK;
+}
+
+rtq_status kv_check_rows(const void* p, int64_t width, int64_t ld, int type, const char* what) {
+  if (!p) return fail(RTQ_ERR_INVALID, "null %s", what);
+  if (ld < width || ld > (1LL << 40)) return fail(RTQ_ERR_INVALID, "%s: row stride %lld of rows of %lld", what, (long long)ld, (long long)width);
+  if ((uintptr_t)p % (uintptr_t)logit_bytes(type)) return fail(RTQ_ERR_INVALID, "%s not aligned to its elements", what);
+  return RTQ_OK;
+}
+
+rtq_status kv_check_heads(const rtq_kv_cache* kc, int64_t n, int64_t nh) {
+  if (nh < 1 || nh % kc->nkv || nh > 65536 || n * nh > 0x7fffffff)
+    return fail(RTQ_ERR_INVALID, "%lld query heads over %lld KV heads", (long long)nh, (long long)kc->nkv);
+  return RTQ_OK;
+}
+
+KvSeqs kv_seqs(const rtq_kv_seqs& s, int64_t n) {
+  return KvSeqs{s.lens, s.starts, s.table, (int)s.b, (int)n, (int)s.ld};
+}
+
+rtq_status kv_check_append(const rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s, int64_t n, int type, const rtq_rope* r,
+                           const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t nh, const void* q, int64_t ldq,
+                           const void* qo, int64_t ldo) {
+  RTQ_TRY(kv_check(kc, layer, s, n, type));
+  if (!r) return fail(RTQ_ERR_INVALID, "null rotation");
+  if (r->dim < 0 || r->dim % 2 || r->dim > kc->d) return fail(RTQ_ERR_INVALID, "rotation of %lld of %lld elements", (long long)r->dim, (long long)kc->d);
+  if (r->dim > 0 && !(r->base > 0.0f && r->base < INFINITY && std::isfinite(r->freq_scale)))
+    return fail(RTQ_ERR_INVALID, "rotation of base %g, scale %g", (double)r->base, (double)r->freq_scale);
+  if (r->n_factors < 0 || r->n_factors > r->dim / 2 || (r->n_factors > 0 && !r->factors))
+    return fail(RTQ_ERR_INVALID, "%lld frequency factors", (long long)r->n_factors);
+  if ((r->q_norm || r->k_norm) && !(r->eps >= 0.0f && std::isfinite(r->offset)))
+    return fail(RTQ_ERR_INVALID, "norm of eps %g, offset %g", (double)r->eps, (double)r->offset);
+  if (n == 0) return RTQ_OK;
+  RTQ_TRY(kv_check_rows(k, kc->nkv * kc->d, ldk, type, "k"));
+  RTQ_TRY(kv_check_rows(v, kc->nkv * kc->d, ldv, type, "v"));
+  if (!q) return RTQ_OK;
+  RTQ_TRY(kv_check_heads(kc, n, nh));
+  RTQ_TRY(kv_check_rows(q, nh * kc->d, ldq, type, "q"));
+  return kv_check_rows(qo, nh * kc->d, ldo, type, "q_out");
+}
+
+rtq_status enqueue_append(rtq_kv_cache* kc, int64_t layer, const KvSeqs& s, int type, const rtq_rope& r, const int32_t* pos,
+                          const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t nh, const void* q, int64_t ldq,
+                          void* qo, int64_t ldo, hipStream_t st) {
+  KvAppendArgs a{};
+  a.s = s;
+  a.k = kc->k + layer * kc->layer, a.v = kc->v + layer * kc->layer;
+  a.q = q, a.kx = k, a.vx = v, a.qo = qo, a.ldq = ldq, a.ldk = ldk, a.ldv = ldv, a.ldo = ldo, a.pos = pos;
+  a.q_norm = r.q_norm, a.k_norm = r.k_norm, a.eps = r.eps, a.off = r.offset;
+  a.nh = (int)nh, a.nkv = (int)kc->nkv, a.d = (int)kc->d, a.rot = (int)r.dim, a.neox = r.neox;
+  a.ps_shift = kc->ps_shift, a.n_pages = (int)kc->n_pages;
+  for (int64_t i = 0; i < r.dim / 2; i++) {
+    double f = std::pow((double)r.base, -2.0 * (double)i / (double)r.dim) * (double)r.freq_scale;
+    if (i < r.n_factors && r.factors[i] != 0.0f) f /= (double)r.factors[i];
+    a.freq[i] = f / 6.283185307179586476925;
+  }
+  a.vt = (int)(cdiv(s.n, 32) * kc->nkv);
+  return launch(kc->ctx, K_KV_APPEND + kv_types(kc, type), dim3((unsigned)(s.n + a.vt)), dim3(256), st, a);
+}
+
+// The attention's tiles and partial parts.  Rows of a sequence and KV head average n group / b: tiles of 16 up to
+// that, else of 32 (whose registers a head size above 128 has not).  `target` items keep every CU's resident workgroups
+// busy; the split tiles' items are at most twice that (each but a tile's last covers C keys).
+struct AttendPlan {
+  int tm, variant, dk;
+  int64_t target, qids;
+  size_t bytes;
+};
+AttendPlan attend_plan(const rtq_kv_cache* kc, int64_t n, int64_t b, int64_t nh) {
+  AttendPlan p{};
+  const int64_t d = kc->d, rows = n * (nh / kc->nkv);
+  p.tm = d <= 128 && rows > 16 * b ? 32 : 16;
+  const int size = d == 64 ? 0 : d == 128 ? 1 : d < 128 ? 2 : 3;
+  p.dk = d == 64 ? 0 : d <= 128 ? 1 : 2;
+  p.variant = (p.tm == 32 ? 4 : 0) + size;
+  p.target = (int64_t)kc->ctx->cu_count * 2;
+  p.qids = (cdiv(rows, p.tm) + b) * kc->nkv;
+  const int64_t D = 64 << p.dk;
+  p.bytes = (size_t)(2 * p.target * p.tm * (D + 2) * 4 + (8 + 8 * p.qids) * 4) + 4 * 256;
+  return p;
+}
+
+rtq_status kv_check_attend(const rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s, int64_t n, int type, int64_t nh, float scale,
+                           const void* q, int64_t ldq, const void* out, int64_t ldo) {
+  RTQ_TRY(kv_check(kc, layer, s, n, type));
+  RTQ_TRY(kv_check_heads(kc, n, nh));
+  if (!(scale >= 0.0f && scale < INFINITY)) return fail(RTQ_ERR_INVALID, "attention scale %g", (double)scale);
+  if (n == 0) return RTQ_OK;
+  RTQ_TRY(kv_check_rows(q, nh * kc->d, ldq, type, "q"));
+  return kv_check_rows(out, nh * kc->d, ldo, type, "out");
+}
+
+rtq_status enqueue_attend(rtq_kv_cache* kc, int64_t layer, const KvSeqs& s, int type, int64_t nh, float scale, const int32_t* parents,
+                          const void* q, int64_t ldq, void* out, int64_t ldo, const AttendPlan& p, Arena& ar, hipStream_t st) {
+  KvAttendArgs a{};
+  a.s = s;
+  a.k = kc->k + layer * kc->layer, a.v = kc->v + layer * kc->layer;
+  a.q = q, a.o = out, a.ldq = ldq, a.ldo = ldo, a.parents = parents;
+  a.nh = (int)nh, a.nkv = (int)kc->nkv, a.d = (int)kc->d, a.ps_shift = kc->ps_shift, a.n_pages = (int)kc->n_pages;
+  a.scale2 = (float)((scale > 0.0f ? (double)scale : 1.0 / std::sqrt((double)kc->d)) * 1.4426950408889634);
+  a.target = (int)p.target, a.slots = (int)(2 * p.target), a.qids = (int)p.qids, a.tm = p.tm;
+  const int64_t D = 64 << p.dk;
+  a.part = ar.take<float>((size_t)(a.slots * p.tm * D));
+  a.ml = ar.take<float>((size_t)(a.slots * p.tm * 2));
+  a.desc = ar.take<int32_t>((size_t)(8 + 8 * p.qids));
+  if (ar.off > ar.cap) return fail(RTQ_ERR_INVALID, "internal: workspace too small");
+  RTQ_TRY(launch(kc->ctx, K_KV_ATTEND + 7 * kv_types(kc, type) + p.variant, dim3((unsigned)(p.target + p.qids)), dim3(256), st, a));
+  return launch(kc->ctx, K_KV_MERGE + 3 * logit_type(type) + p.dk, dim3((unsigned)p.qids, (unsigned)p.tm), dim3(256), st, a);
+}
+
+rtq_status kv_check_keep(const rtq_kv_cache* kc, const rtq_kv_seqs* s, const int32_t* kept, int64_t ldk, const int32_t* after) {
+  RTQ_TRY(kv_check_seqs(kc, s));
+  if (ldk < 1 || ldk > RTQ_TREE_MAX) return fail(RTQ_ERR_INVALID, "%lld kept tokens", (long long)ldk);
+  if (!kept) return fail(RTQ_ERR_INVALID, "null kept");
+  if (after && after < s->lens + s->b && s->lens < after + s->b) return fail(RTQ_ERR_INVALID, "lens_out overlaps lens");
+  return RTQ_OK;
+}
+
+rtq_status enqueue_keep(rtq_kv_cache* kc, const KvSeqs& s, const int32_t* kept, int64_t ldk, int32_t* after, hipStream_t st) {
+  KvKeepArgs a{s.lens, s.table, kept, after, s.b, s.ldt, (int)ldk, (int)kc->nkv, (int)kc->d, kc->ps_shift, (int)kc->n_pages, kc->k, kc->v, kc->layer};
+  return launch(kc->ctx, K_KV_KEEP, dim3((unsigned)(s.b * kc->nkv), (unsigned)kc->n_layer), dim3(320), st, a);
+}
+
+}  // namespace
+
+rtq_status rtq_kv_cache_create(rtq_ctx* c, int type, int64_t n_layer, int64_t n_pages, int64_t ps, int64_t nkv, int64_t d, void* k, void* v,
+                               rtq_kv_cache** out) {
+  if (!out) return fail(RTQ_ERR_INVALID, "null out");
+  *out = nullptr;
+  if (type != RTQ_TYPE_F16 && type != RTQ_TYPE_BF16) return fail(RTQ_ERR_UNSUPPORTED, "cache of type %d (F16 and BF16 are supported)", type);
+  if (n_layer < 1 || n_layer > 65535) return fail(RTQ_ERR_INVALID, "%lld layers out of range [1, 65535]", (long long)n_layer);
+  if (n_pages < 1 || n_pages > 0x7fffffff) return fail(RTQ_ERR_INVALID, "%lld pages", (long long)n_pages);
+  if (ps < 32 || ps > 1024 || (ps & (ps - 1))) return fail(RTQ_ERR_INVALID, "pages of %lld slots (a power of two in [32, 1024])", (long long)ps);
+  if (nkv < 1 || nkv > 1024) return fail(RTQ_ERR_INVALID, "%lld KV heads out of range [1, 1024]", (long long)nkv);
+  if (d < 16 || d > 256 || d % 16) return fail(RTQ_ERR_INVALID, "head size %lld (a multiple of 16 in [16, 256])", (long long)d);
+  if ((k == nullptr) != (v == nullptr)) return fail(RTQ_ERR_INVALID, "k and v go together");
+  if (((uintptr_t)k | (uintptr_t)v) % 16) return fail(RTQ_ERR_INVALID, "pages not 16-byte aligned");
+  const double bytes = 2.0 * (double)n_layer * (double)n_pages * (double)ps * (double)nkv * (double)d;
+  if (bytes > 1e15) return fail(RTQ_ERR_INVALID, "a cache of %g bytes", 2.0 * bytes);
+  if (!k) RTQ_TRY(check_ctx(c));  // (the caller's pages without a context: calls are checked, then refused)
+  rtq_kv_cache* kc = new (std::nothrow) rtq_kv_cache;
+  if (!kc) return fail(RTQ_ERR_INVALID, "out of host memory");
+  kc->ctx = c, kc->type = type, kc->n_layer = n_layer, kc->n_pages = n_pages, kc->ps = ps, kc->nkv = nkv, kc->d = d;
+  kc->layer = n_pages * ps * nkv * d;
+  while ((1 << kc->ps_shift) < ps) kc->ps_shift++;
+  kc->k = (uint16_t*)k, kc->v = (uint16_t*)v, kc->owned = !k;
+  if (kc->owned) {
+    std::lock_guard<std::mutex> lk(c->mu);
+    const size_t each = (size_t)(n_layer * kc->layer) * 2;
+    hipError_t e = hipSetDevice(c->device);
+    if (e == hipSuccess) e = hipMalloc((void**)&kc->k, each);
+    if (e == hipSuccess) e = hipMalloc((void**)&kc->v, each);
+    if (e == hipSuccess) e = hipMemsetAsync(kc->k, 0, each, c->stream);
+    if (e == hipSuccess) e = hipMemsetAsync(kc->v, 0, each, c->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(c->stream);
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      if (kc->k) (void)hipFree(kc->k);
+      if (kc->v) (void)hipFree(kc->v);
+      delete kc;
+      return fail(RTQ_ERR_HIP, "a cache of 2 x %zu bytes: %s", each, hipGetErrorString(e));
+    }
+  }
+  *out = kc;
+  return RTQ_OK;
+}
+
+void rtq_kv_cache_destroy(rtq_kv_cache* kc) {
+  if (!kc) return;
+  if (kc->owned) {
+    (void)hipSetDevice(kc->ctx->device);
+    (void)hipDeviceSynchronize();
+    (void)hipFree(kc->k);
+    (void)hipFree(kc->v);
+  }
+  delete kc;
+}
+
+rtq_status rtq_kv_cache_pages(const rtq_kv_cache* kc, int64_t layer, void** k, void** v) {
+  if (!kc) return fail(RTQ_ERR_INVALID, "null cache");
+  if (layer < 0 || layer >= kc->n_layer) return fail(RTQ_ERR_INVALID, "layer %lld of %lld", (long long)layer, (long long)kc->n_layer);
+  if (k) *k = kc->k + layer * kc->layer;
+  if (v) *v = kc->v + layer * kc->layer;
+  return RTQ_OK;
+}
+
+rtq_status rtq_kv_append_d(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s, int64_t n, int type, const rtq_rope* rope,
+                           const int32_t* pos, const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t nh,
+                           const void* q, int64_t ldq, void* qo, int64_t ldo, void* stream) {
+  RTQ_TRY(kv_check_append(kc, layer, s, n, type, rope, k, ldk, v, ldv, nh, q, ldq, qo, ldo));
+  RTQ_TRY(check_ctx(kc->ctx));
+  if (n == 0) return RTQ_OK;
+  std::lock_guard<std::mutex> lk(kc->ctx->mu);
+  HIP_TRY(hipSetDevice(kc->ctx->device));
+  return enqueue_append(kc, layer, kv_seqs(*s, n), type, *rope, pos, k, ldk, v, ldv, nh, q, ldq, qo, ldo, (hipStream_t)stream);
+}
+
+rtq_status rtq_kv_attend_d(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s, int64_t n, int type, int64_t nh, float scale,
+                           const int32_t* parents, const void* q, int64_t ldq, void* out, int64_t ldo, void* stream) {
+  RTQ_TRY(kv_check_attend(kc, layer, s, n, type, nh, scale, q, ldq, out, ldo));
+  RTQ_TRY(check_ctx(kc->ctx));
+  if (n == 0) return RTQ_OK;
+  rtq_ctx* c = kc->ctx;
+  std::lock_guard<std::mutex> lk(c->mu);
+  HIP_TRY(hipSetDevice(c->device));
+  hipStream_t st = (hipStream_t)stream;
+  const AttendPlan p = attend_plan(kc, n, s->b, nh);
+  RTQ_TRY(row_ws(c, p.bytes, st));
+  Arena ar{(char*)c->ws, c->ws_bytes, 0};
+  return enqueue_attend(kc, layer, kv_seqs(*s, n), type, nh, scale, parents, q, ldq, out, ldo, p, ar, st);
+}
+
+rtq_status rtq_kv_keep_d(rtq_kv_cache* kc, const rtq_kv_seqs* s, const int32_t* kept, int64_t ldk, int32_t* after, void* stream) {
+  RTQ_TRY(kv_check_keep(kc, s, kept, ldk, after));
+  RTQ_TRY(check_ctx(kc->ctx));
+  std::lock_guard<std::mutex> lk(kc->ctx->mu);
+  HIP_TRY(hipSetDevice(kc->ctx->device));
+  return enqueue_keep(kc, kv_seqs(*s, 0), kept, ldk, after, (hipStream_t)stream);
+}
+
 // ------------------------------------------------------------------ the LM head's top logits and distillation
 namespace {
 
@@ -2601,6 +2870,147 @@ rtq_status rtq_verify_draft(rtq_ctx* c, const void* z, int type, int64_t ld, con
   RTQ_TRY(enqueue_verify(c, zd, type, V, qd, V, b, d, V, xd, nd, ud, temp, ad, kd, p, ar, st));
   RTQ_TRY(d2h(accepted, ad, (size_t)b * 4, st));
   RTQ_TRY(d2h(tokens, kd, (size_t)tr * 4, st));
+  HIP_TRY(hipStreamSynchronize(st));
+  return RTQ_OK;
+}
+
+// ---- paged cache: host arrays
+namespace {
+// starts ascend from 0 or later to n or earlier, lens and the tables hold every held and new token (append, attend)
+rtq_status kv_check_lists(const rtq_kv_cache* kc, const rtq_kv_seqs* s, int64_t n) {
+  for (int64_t i = 0; i < s->b; i++) {
+    const int64_t s0 = s->starts ? s->starts[i] : n / s->b * i, s1 = s->starts ? s->starts[i + 1] : n / s->b * (i + 1);
+    if (s0 < 0 || s1 < s0 || s1 > n) return fail(RTQ_ERR_INVALID, "sequence %lld has rows %lld to %lld of %lld", (long long)i, (long long)s0, (long long)s1, (long long)n);
+    if (s->lens[i] < 0) return fail(RTQ_ERR_INVALID, "sequence %lld holds %d tokens", (long long)i, s->lens[i]);
+    const int64_t total = s->lens[i] + (s1 - s0), pages = cdiv(total, kc->ps);
+    if (s1 == s0) continue;
+    if (pages > s->ld || total > 0x7fffffff)
+      return fail(RTQ_ERR_INVALID, "sequence %lld: %lld tokens in a table of %lld pages", (long long)i, (long long)total, (long long)s->ld);
+    for (int64_t p = 0; p < pages; p++)
+      if (s->table[i * s->ld + p] < 0 || s->table[i * s->ld + p] >= kc->n_pages)
+        return fail(RTQ_ERR_INVALID, "page %d of sequence %lld out of range", s->table[i * s->ld + p], (long long)i);
+  }
+  return RTQ_OK;
+}
+size_t kv_seq_bytes(const rtq_kv_seqs& s) { return (size_t)(2 * s.b + 1 + s.b * s.ld) * 4 + 3 * 256; }
+rtq_status kv_seq_put(const rtq_kv_seqs& s, int64_t n, Arena& ar, hipStream_t st, KvSeqs* out) {
+  int32_t* lens = ar.take<int32_t>((size_t)s.b);
+  int32_t* starts = s.starts ? ar.take<int32_t>((size_t)s.b + 1) : nullptr;
+  int32_t* table = ar.take<int32_t>((size_t)(s.b * s.ld));
+  RTQ_TRY(h2d(lens, s.lens, (size_t)s.b * 4, st));
+  if (starts) RTQ_TRY(h2d(starts, s.starts, (size_t)(s.b + 1) * 4, st));
+  RTQ_TRY(h2d(table, s.table, (size_t)(s.b * s.ld) * 4, st));
+  *out = KvSeqs{lens, starts, table, (int)s.b, (int)n, (int)s.ld};
+  return RTQ_OK;
+}
+}  // namespace
+
+rtq_status rtq_kv_append(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s, int64_t n, int type, const rtq_rope* rope,
+                         const int32_t* pos, const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t nh, const void* q,
+                         int64_t ldq, void* qo, int64_t ldo) {
+  RTQ_TRY(kv_check_append(kc, layer, s, n, type, rope, k, ldk, v, ldv, nh, q, ldq, qo, ldo));
+  if (n == 0) return RTQ_OK;
+  RTQ_TRY(kv_check_lists(kc, s, n));
+  for (int64_t i = 0; pos && i < n; i++)
+    if (pos[i] < 0) return fail(RTQ_ERR_INVALID, "position %lld is negative", (long long)i);
+  rtq_ctx* c = kc->ctx;
+  RTQ_TRY(check_ctx(c));
+  HostCall hc(c);
+  HIP_TRY(hipSetDevice(c->device));
+  hipStream_t st = c->stream;
+  const int64_t es = logit_bytes(type), kw = kc->nkv * kc->d, qw = q ? nh * kc->d : 0;
+  RTQ_TRY(ensure_ws(c, (size_t)(n * (2 * kw + qw) * es + n * 4 + 2 * kc->d * 4) + kv_seq_bytes(*s) + 8 * 256));
+  Arena ar{(char*)c->ws, c->ws_bytes, 0};
+  KvSeqs sd;
+  RTQ_TRY(kv_seq_put(*s, n, ar, st, &sd));
+  char* kd = ar.take<char>((size_t)(n * kw * es));
+  char* vd = ar.take<char>((size_t)(n * kw * es));
+  char* qd = q ? ar.take<char>((size_t)(n * qw * es)) : nullptr;
+  int32_t* pd = pos ? ar.take<int32_t>((size_t)n) : nullptr;
+  rtq_rope r = *rope;
+  float* qn = ar.take<float>((size_t)kc->d);
+  float* kn = ar.take<float>((size_t)kc->d);
+  if (ar.off > ar.cap) return fail(RTQ_ERR_INVALID, "internal: workspace too small");
+  RTQ_TRY(h2d_rows(kd, k, n, kw, ldk, es, st));
+  RTQ_TRY(h2d_rows(vd, v, n, kw, ldv, es, st));
+  if (q) RTQ_TRY(h2d_rows(qd, q, n, qw, ldq, es, st));
+  if (pd) RTQ_TRY(h2d(pd, pos, (size_t)n * 4, st));
+  if (r.q_norm) RTQ_TRY(h2d(qn, r.q_norm, (size_t)kc->d * 4, st));
+  if (r.k_norm) RTQ_TRY(h2d(kn, r.k_norm, (size_t)kc->d * 4, st));
+  if (r.q_norm) r.q_norm = qn;
+  if (r.k_norm) r.k_norm = kn;
+  RTQ_TRY(enqueue_append(kc, layer, sd, type, r, pd, kd, kw, vd, kw, nh, qd, qw, qd, qw, st));
+  const int64_t lo = s->starts ? s->starts[0] : 0, hi = s->starts ? s->starts[s->b] : n;
+  if (q && hi > lo) RTQ_TRY(d2h_rows((char*)qo + lo * ldo * es, qd + lo * qw * es, hi - lo, qw, ldo, es, st));
+  HIP_TRY(hipStreamSynchronize(st));
+  return RTQ_OK;
+}
+
+rtq_status rtq_kv_attend(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s, int64_t n, int type, int64_t nh, float scale,
+                         const int32_t* parents, const void* q, int64_t ldq, void* out, int64_t ldo) {
+  RTQ_TRY(kv_check_attend(kc, layer, s, n, type, nh, scale, q, ldq, out, ldo));
+  if (n == 0) return RTQ_OK;
+  RTQ_TRY(kv_check_lists(kc, s, n));
+  for (int64_t i = 0; parents && i < s->b; i++) {
+    const int64_t s0 = s->starts ? s->starts[i] : n / s->b * i, s1 = s->starts ? s->starts[i + 1] : n / s->b * (i + 1);
+    if (s1 - s0 > RTQ_TREE_MAX) return fail(RTQ_ERR_INVALID, "sequence %lld is a tree of %lld tokens", (long long)i, (long long)(s1 - s0));
+    for (int64_t j = s0; j < s1; j++)
+      if (parents[j] < -2 || parents[j] >= j - s0) return fail(RTQ_ERR_INVALID, "parent %d of token %lld of sequence %lld", parents[j], (long long)(j - s0), (long long)i);
+  }
+  rtq_ctx* c = kc->ctx;
+  RTQ_TRY(check_ctx(c));
+  HostCall hc(c);
+  HIP_TRY(hipSetDevice(c->device));
+  hipStream_t st = c->stream;
+  const AttendPlan p = attend_plan(kc, n, s->b, nh);
+  const int64_t es = logit_bytes(type), qw = nh * kc->d;
+  RTQ_TRY(ensure_ws(c, p.bytes + (size_t)(n * qw * es + n * 4) + kv_seq_bytes(*s) + 4 * 256));
+  Arena ar{(char*)c->ws, c->ws_bytes, 0};
+  KvSeqs sd;
+  RTQ_TRY(kv_seq_put(*s, n, ar, st, &sd));
+  char* qd = ar.take<char>((size_t)(n * qw * es));
+  int32_t* pd = parents ? ar.take<int32_t>((size_t)n) : nullptr;
+  RTQ_TRY(h2d_rows(qd, q, n, qw, ldq, es, st));
+  if (pd) RTQ_TRY(h2d(pd, parents, (size_t)n * 4, st));
+  RTQ_TRY(enqueue_attend(kc, layer, sd, type, nh, scale, pd, qd, qw, qd, qw, p, ar, st));
+  const int64_t lo = s->starts ? s->starts[0] : 0, hi = s->starts ? s->starts[s->b] : n;
+  if (hi > lo) RTQ_TRY(d2h_rows((char*)out + lo * ldo * es, qd + lo * qw * es, hi - lo, qw, ldo, es, st));
+  HIP_TRY(hipStreamSynchronize(st));
+  return RTQ_OK;
+}
+
+rtq_status rtq_kv_keep(rtq_kv_cache* kc, const rtq_kv_seqs* s, const int32_t* kept, int64_t ldk, int32_t* after) {
+  RTQ_TRY(kv_check_keep(kc, s, kept, ldk, after));
+  const int64_t slots = s->ld * kc->ps;
+  for (int64_t i = 0; i < s->b; i++) {
+    if (s->lens[i] < 0) return fail(RTQ_ERR_INVALID, "sequence %lld holds %d tokens", (long long)i, s->lens[i]);
+    int64_t last = -1;
+    for (int64_t j = 0; j < ldk && kept[i * ldk + j] != -1; j++) {
+      const int64_t x = kept[i * ldk + j];
+      if (x <= last || s->lens[i] + x >= slots) return fail(RTQ_ERR_INVALID, "kept token %lld of sequence %lld", (long long)x, (long long)i);
+      for (int64_t at : {s->lens[i] + x, s->lens[i] + j}) {
+        const int32_t pg = s->table[i * s->ld + at / kc->ps];
+        if (pg < 0 || pg >= kc->n_pages) return fail(RTQ_ERR_INVALID, "page %d of sequence %lld out of range", pg, (long long)i);
+      }
+      last = x;
+    }
+  }
+  rtq_ctx* c = kc->ctx;
+  RTQ_TRY(check_ctx(c));
+  HostCall hc(c);
+  HIP_TRY(hipSetDevice(c->device));
+  hipStream_t st = c->stream;
+  rtq_kv_seqs q = *s;
+  q.starts = nullptr;
+  RTQ_TRY(ensure_ws(c, kv_seq_bytes(q) + (size_t)(s->b * (ldk + 1)) * 4 + 2 * 256));
+  Arena ar{(char*)c->ws, c->ws_bytes, 0};
+  KvSeqs sd;
+  RTQ_TRY(kv_seq_put(q, 0, ar, st, &sd));
+  int32_t* kd = ar.take<int32_t>((size_t)(s->b * ldk));
+  int32_t* ad = ar.take<int32_t>((size_t)s->b);
+  RTQ_TRY(h2d(kd, kept, (size_t)(s->b * ldk) * 4, st));
+  RTQ_TRY(enqueue_keep(kc, sd, kd, ldk, ad, st));
+  if (after) RTQ_TRY(d2h(after, ad, (size_t)s->b * 4, st));
   HIP_TRY(hipStreamSynchronize(st));
   return RTQ_OK;
 }

@@ -21,6 +21,7 @@ pub const RTQ_TYPE_TQ8_0: c_int = 264;
 pub const RTQ_TYPE_F16: c_int = 1;
 pub const RTQ_TYPE_BF16: c_int = 30;
 pub const RTQ_TOP_MAX: i64 = 256;
+pub const RTQ_TREE_MAX: i64 = 1024;
 
 #[repr(C)]
 pub struct rtq_ctx {
@@ -39,6 +40,10 @@ pub struct rtq_gguf_writer {
     _p: [u8; 0],
 }
 #[repr(C)]
+pub struct rtq_kv_cache {
+    _p: [u8; 0],
+}
+#[repr(C)]
 pub struct rtq_model {
     _p: [u8; 0],
 }
@@ -52,6 +57,33 @@ pub struct rtq_lora {
     pub a: *const f32,
     pub b: *const f32,
     pub enabled: c_int,
+}
+
+/// The sequences of a call on a paged cache (`include/rtq.h`).
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct rtq_kv_seqs {
+    pub b: i64,
+    pub lens: *const i32,
+    pub starts: *const i32,
+    pub table: *const i32,
+    pub ld: i64,
+}
+
+/// The rotation (and norms) of queries and keys on their way into a cache.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct rtq_rope {
+    pub dim: i64,
+    pub base: f32,
+    pub freq_scale: f32,
+    pub neox: c_int,
+    pub factors: *const f32,
+    pub n_factors: i64,
+    pub q_norm: *const f32,
+    pub k_norm: *const f32,
+    pub eps: f32,
+    pub offset: f32,
 }
 
 /// A teacher's top logits: ids and vals [n x k], rest [n] (or null).
@@ -184,6 +216,32 @@ extern "C" {
                             x: *const f32, t: i64, pos: *const i32, tok: *const i32, weights: *const f32, n: i64,
                             teacher: *const rtq_teacher, hard: f32, kl: *mut f32, logp: *mut f32, dx: *mut f32,
                             stream: *mut c_void) -> rtq_status;
+
+    // paged cache of keys and values
+    pub fn rtq_kv_cache_create(ctx: *mut rtq_ctx, type_: c_int, n_layer: i64, n_pages: i64, page_size: i64,
+                               n_head_kv: i64, head_dim: i64, k: *mut c_void, v: *mut c_void,
+                               out: *mut *mut rtq_kv_cache) -> rtq_status;
+    pub fn rtq_kv_cache_destroy(kc: *mut rtq_kv_cache);
+    pub fn rtq_kv_cache_pages(kc: *const rtq_kv_cache, layer: i64, k: *mut *mut c_void,
+                              v: *mut *mut c_void) -> rtq_status;
+    pub fn rtq_kv_append(kc: *mut rtq_kv_cache, layer: i64, seqs: *const rtq_kv_seqs, n: i64, type_: c_int,
+                         rope: *const rtq_rope, positions: *const i32, k: *const c_void, ldk: i64, v: *const c_void,
+                         ldv: i64, n_head: i64, q: *const c_void, ldq: i64, q_out: *mut c_void,
+                         ldo: i64) -> rtq_status;
+    pub fn rtq_kv_append_d(kc: *mut rtq_kv_cache, layer: i64, seqs: *const rtq_kv_seqs, n: i64, type_: c_int,
+                           rope: *const rtq_rope, positions: *const i32, k: *const c_void, ldk: i64, v: *const c_void,
+                           ldv: i64, n_head: i64, q: *const c_void, ldq: i64, q_out: *mut c_void, ldo: i64,
+                           stream: *mut c_void) -> rtq_status;
+    pub fn rtq_kv_attend(kc: *mut rtq_kv_cache, layer: i64, seqs: *const rtq_kv_seqs, n: i64, type_: c_int,
+                         n_head: i64, scale: f32, parents: *const i32, q: *const c_void, ldq: i64, out: *mut c_void,
+                         ldo: i64) -> rtq_status;
+    pub fn rtq_kv_attend_d(kc: *mut rtq_kv_cache, layer: i64, seqs: *const rtq_kv_seqs, n: i64, type_: c_int,
+                           n_head: i64, scale: f32, parents: *const i32, q: *const c_void, ldq: i64, out: *mut c_void,
+                           ldo: i64, stream: *mut c_void) -> rtq_status;
+    pub fn rtq_kv_keep(kc: *mut rtq_kv_cache, seqs: *const rtq_kv_seqs, kept: *const i32, ldk: i64,
+                       lens_out: *mut i32) -> rtq_status;
+    pub fn rtq_kv_keep_d(kc: *mut rtq_kv_cache, seqs: *const rtq_kv_seqs, kept: *const i32, ldk: i64,
+                         lens_out: *mut i32, stream: *mut c_void) -> rtq_status;
 
     // the device-resident training step (Model::forward_backward)
     pub fn rtq_model_from_gguf(ctx: *mut rtq_ctx, g: *const rtq_gguf, out: *mut *mut rtq_model) -> rtq_status;
