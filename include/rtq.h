@@ -394,6 +394,14 @@ rtq_status rtq_model_forward_backward_distill(rtq_model* m, const int32_t* token
  * from the same tokens; NULL: drafts that were not drawn. */
 rtq_status rtq_model_verify_draft(rtq_model* m, rtq_model* draft, const int32_t* tokens, int64_t t, int64_t d,
                                   const float* uniforms, float temperature, int32_t* accepted, int32_t* out);
+/* The step's forward over a cache (no counterpart in the reference): the n tokens of seqs' sequences (host arrays, as
+ * rtq_kv_append takes them; seqs->lens held before the call and the caller's to advance) enter kc in every block and
+ * attend over it, and rtq_top_logits of the rows that `pos` [np] names (0 <= pos < n, each inside a sequence) is
+ * returned.  parents [n] or NULL as rtq_kv_attend's: a token's position is its parent's plus one (the held tokens' number for -1).
+ * kc: of the model's context, layers, KV heads and head size. */
+rtq_status rtq_model_extend(rtq_model* m, rtq_kv_cache* kc, const rtq_kv_seqs* seqs, const int32_t* tokens, int64_t n,
+                            const int32_t* parents, const int32_t* pos, int64_t np, int64_t k, float temperature,
+                            float* vals, int32_t* ids, float* rest);
 /* Model::checkpointing (src/model.rs:299-300; the loader's default true, src/rie.rs:254): 1 keeps
  * only each block's input and recomputes its forward in the backward (src/model.rs:663-665,
  * 678-680); 0 keeps every block's activations; -1 (default) keeps them when they take at most half

@@ -144,6 +144,7 @@ SIGNATURES = {
     "rtq_model_top_logits": (_i, [_p, _p, _i64, _p, _p, _p, _i64, _i64, _f, _p, _p, _p]),
     "rtq_model_forward_backward_distill": (_i, [_p, _p, _i64, _p, _p, _p, _p, _p, _i64, _TP, _f, _p, _p]),
     "rtq_model_verify_draft": (_i, [_p, _p, _p, _i64, _i64, _p, _f, ctypes.POINTER(ctypes.c_int32), _p]),
+    "rtq_model_extend": (_i, [_p, _p, _SP, _p, _i64, _p, _p, _i64, _i64, _f, _p, _p, _p]),
     "rtq_model_set_checkpointing": (_i, [_p, _i]),
     "rtq_model_checkpointing": (_i, [_p]),
     "rtq_model_set_attention": (_i, [_p, _i]),

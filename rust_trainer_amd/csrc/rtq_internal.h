@@ -60,6 +60,10 @@ rtq_status rtq_check_temperature(float t);
 // logits [n x vocab] of the hidden states x [t x d] at pos (final RMSNorm, lm_head.forward)
 extern "C" rtq_status rtq_lm_logits_d(rtq_ctx* c, const rtq_weight* lm_head, const float* norm_w, float eps, float offset,
                                       const float* x, int64_t t, const int32_t* pos, int64_t n, float* out, void* stream);
+// a cache's calls over host lists: refuses what rtq_kv_append and rtq_kv_attend do, and caches of another context or shape
+extern "C" rtq_status rtq_kv_check_step(const rtq_kv_cache* kc, const rtq_ctx* c, int64_t n_layer, int64_t nh, int64_t nkv,
+                                        int64_t d, const rtq_kv_seqs* seqs, int64_t n, const int32_t* parents);
+extern "C" uint64_t rtq_kv_cache_id(const rtq_kv_cache* kc);  // of no other cache of the process
 // floats of the LoRA-down partials a forward of t tokens at rank r can keep for the backward of the
 // same x (0: not kept for this weight - dense, or slicings that differ)
 int64_t rtq_lora_partial_floats(const rtq_weight* w, int64_t t, int64_t r);

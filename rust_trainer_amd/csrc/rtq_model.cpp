@@ -226,10 +226,23 @@ struct rtq_model {
   float *job_vals = nullptr, *job_rest = nullptr, *job_kl = nullptr;
   void* draft_mem = nullptr;  // rtq_model_verify_draft: the logits' rows and the small arrays
   size_t draft_cap = 0;
+  // an extension of a cache (null: a step of its own): the cache, and the sequences' lists on the device
+  struct KvStep* kv = nullptr;
+  void* kv_mem = nullptr;
+  size_t kv_cap = 0;
   // pinned staging of the step's host inputs (tokens, target positions and tokens, weights) and
   // outputs (log-probs, hits)
   void* io_host = nullptr;
   size_t io_cap = 0;
+};
+
+// rtq_model_extend: its sequences on the host and on the device, the tokens' positions and parents
+struct KvStep {
+  rtq_kv_cache* kc;
+  const rtq_kv_seqs* seqs;
+  const int32_t *parents, *positions;  // host (parents may be null)
+  rtq_kv_seqs seqs_d;
+  const int32_t *parents_d, *positions_d;
 };
 
 // a step's head other than cross-entropy: top logits, distillation, or the logits' rows themselves
@@ -1118,6 +1131,27 @@ void gu_view(const rtq_model* m, const Layer& L, float* base, int64_t t, float**
   *ld = L.gu_fused ? 2 * ff : ff;
 }
 
+// a block from its attention's output (in its cache) on: o, the residual, the MLP (add_out: as block_forward's)
+rtq_status block_mlp(rtq_model* m, int l, int64_t t, float* x, float* y, bool add_out) {
+  const Layer& L = m->layers[(size_t)l];
+  Cache& k = m->cache[m->ckpt ? 0 : (size_t)l];
+  const int64_t d = m->cfg.n_embd;
+  M_TRY(lin_fwd(m, L.groups[(size_t)L.gi[LO]], k.o, t, m->mo));
+  float *g, *u;
+  int64_t ldg;
+  gu_view(m, L, k.gu, t, &g, &u, &ldg);
+  // h = x + attn, n2 = rmsnorm(h)
+  if (L.gu_fused) {
+    M_TRY(lin_fwd_norm(m, L.groups[(size_t)L.gi[LGATE]], x, m->mo, k.h, L.ffn_norm, k.n2, k.inv2, t, k.gu));
+  } else {
+    M_TRY(lin_fwd_norm(m, L.groups[(size_t)L.gi[LGATE]], x, m->mo, k.h, L.ffn_norm, k.n2, k.inv2, t, g));
+    M_TRY(lin_fwd(m, L.groups[(size_t)L.gi[LUP]], k.n2, t, u));
+  }
+  M_TRY(lin_fwd_swiglu(m, L.groups[(size_t)L.gi[LDOWN]], g, u, ldg, k.hm, t, m->f));
+  if (!add_out) return RTQ_OK;
+  return k_elt(m, KM_ADD, k.h, m->f, nullptr, y, nullptr, t * d);  // y = h + mlp
+}
+
 // add_in: x is not written yet: it is the previous block's output h + mlp (its h in its cache, mlp
 // in f), summed by this block's first norm kernel (which writes x); add_out: this block writes y,
 // else it leaves h (cache) and mlp (f) for the next block's first norm
@@ -1125,7 +1159,7 @@ rtq_status block_forward(rtq_model* m, int l, int64_t t, float* x, float* y, boo
   const rtq_model_config& c = m->cfg;
   const Layer& L = m->layers[(size_t)l];
   Cache& k = m->cache[m->ckpt ? 0 : (size_t)l];
-  const int64_t d = c.n_embd, nh = c.n_head, nkv = c.n_head_kv, hd = c.head_dim, grp = nh / nkv;
+  const int64_t nh = c.n_head, nkv = c.n_head_kv, hd = c.head_dim, grp = nh / nkv;
   const int64_t qd = nh * hd, kd = nkv * hd;
   // x = h + mlp of block l - 1 (src/model.rs:196), n1 = rmsnorm(x)
   const float* in_a = add_in ? m->cache[m->ckpt ? 0 : (size_t)(l - 1)].h : x;
@@ -1138,6 +1172,16 @@ rtq_status block_forward(rtq_model* m, int l, int64_t t, float* x, float* y, boo
     M_TRY(lin_fwd_norm(m, L.groups[(size_t)L.gi[LQ]], in_a, in_b, in_h, L.attn_norm, k.n1, k.inv1, t, qv.q));
     M_TRY(lin_fwd(m, L.groups[(size_t)L.gi[LK]], k.n1, t, qv.k));
     M_TRY(lin_fwd(m, L.groups[(size_t)L.gi[LV]], k.n1, t, qv.v));
+  }
+  if (m->kv) {  // over a cache: its append norms and rotates, its attention reads every held token
+    const KvStep& kv = *m->kv;
+    const rtq_rope r{c.rope_dim, c.rope_base, c.rope_freq_scale, c.rope_neox, m->rope_factors.data(),
+                     (int64_t)m->rope_factors.size(), L.q_norm, L.k_norm, c.rms_eps, c.norm_offset};
+    M_TRY(rtq_kv_append_d(kv.kc, l, &kv.seqs_d, t, RTQ_TYPE_F32, &r, kv.positions_d, qv.k, qv.ldk, qv.v, qv.ldv, nh, qv.q, qv.ldq,
+                          k.q, qd, stream_of(m)));
+    M_TRY(rtq_kv_attend_d(kv.kc, l, &kv.seqs_d, t, RTQ_TYPE_F32, nh, 1.0f / sqrtf((float)hd), kv.parents_d, k.q, qd, k.o, qd,
+                          stream_of(m)));
+    return block_mlp(m, l, t, x, y, add_out);
   }
   const MQkArgs qa = qk_args(m, L, k, t);
   M_TRY(rtq_model_launch(m->ctx, KM_QK_PREP, dim3(qk_grid(m, t * (nh + 2 * nkv))), dim3(256), stream_of(m),
@@ -1189,20 +1233,7 @@ rtq_status block_forward(rtq_model* m, int l, int64_t t, float* x, float* y, boo
                  SPLIT_HF));
   }
   if (seq) M_TRY(rtq_model_launch(m->ctx, KM_SEQ_SCATTER, dim3((unsigned)t), dim3(256), stream_of(m), &sq));
-  M_TRY(lin_fwd(m, L.groups[(size_t)L.gi[LO]], k.o, t, m->mo));
-  float *g, *u;
-  int64_t ldg;
-  gu_view(m, L, k.gu, t, &g, &u, &ldg);
-  // h = x + attn, n2 = rmsnorm(h)
-  if (L.gu_fused) {
-    M_TRY(lin_fwd_norm(m, L.groups[(size_t)L.gi[LGATE]], x, m->mo, k.h, L.ffn_norm, k.n2, k.inv2, t, k.gu));
-  } else {
-    M_TRY(lin_fwd_norm(m, L.groups[(size_t)L.gi[LGATE]], x, m->mo, k.h, L.ffn_norm, k.n2, k.inv2, t, g));
-    M_TRY(lin_fwd(m, L.groups[(size_t)L.gi[LUP]], k.n2, t, u));
-  }
-  M_TRY(lin_fwd_swiglu(m, L.groups[(size_t)L.gi[LDOWN]], g, u, ldg, k.hm, t, m->f));
-  if (!add_out) return RTQ_OK;
-  return k_elt(m, KM_ADD, k.h, m->f, nullptr, y, nullptr, t * d);  // y = h + mlp
+  return block_mlp(m, l, t, x, y, add_out);
 }
 
 rtq_status block_backward(rtq_model* m, int l, int64_t t, const float* x, const float* dy, float* dx) {
@@ -1655,6 +1686,7 @@ void rtq_model_destroy(rtq_model* m) {
   if (m->seq_mem) (void)hipFree(m->seq_mem);
   if (m->job_mem) (void)hipFree(m->job_mem);
   if (m->draft_mem) (void)hipFree(m->draft_mem);
+  if (m->kv_mem) (void)hipFree(m->kv_mem);
   delete m;
 }
 
@@ -1882,7 +1914,7 @@ rtq_status step_kernels(rtq_model* m, int64_t t, int64_t n, bool weights) {
     const bool out = l == c.n_layer - 1 || l == m->dbg_layer;
     M_TRY(block_forward(m, (int)l, t, x, y, pending, out));
     pending = !out;
-    if (l == m->dbg_layer) M_TRY(dbg_forward(m, (int)l, t, x, y));
+    if (l == m->dbg_layer && !m->kv) M_TRY(dbg_forward(m, (int)l, t, x, y));
   }
   if (n == 0) return RTQ_OK;
   const float* xl = m->X + c.n_layer * t * d;
@@ -1995,11 +2027,39 @@ rtq_status download_job(rtq_model* m, const HeadJob& j, int64_t n, float* logp, 
   return RTQ_OK;
 }
 
+// an extension's lists in one copy: lens [b] | starts [b + 1] | table [b x ld] | positions [t] | parents [t]
+rtq_status upload_kv(rtq_model* m, KvStep& kv, int64_t t, size_t ints, int32_t* io, hipStream_t st) {
+  if (ints * 4 > m->kv_cap) {
+    if (m->kv_mem) {
+      M_HIP(hipStreamSynchronize(st));
+      M_HIP(hipFree(m->kv_mem));
+      m->kv_mem = nullptr;
+      m->kv_cap = 0;
+    }
+    M_HIP(hipMalloc(&m->kv_mem, ints * 4));
+    m->kv_cap = ints * 4;
+    m->gen++;
+  }
+  const rtq_kv_seqs& s = *kv.seqs;
+  const size_t b = (size_t)s.b, tab = (size_t)(s.b * s.ld);
+  std::memcpy(io, s.lens, b * 4);
+  if (s.starts) std::memcpy(io + b, s.starts, (b + 1) * 4);
+  if (tab) std::memcpy(io + 2 * b + 1, s.table, tab * 4);
+  std::memcpy(io + 2 * b + 1 + tab, kv.positions, (size_t)t * 4);
+  if (kv.parents) std::memcpy(io + 2 * b + 1 + tab + t, kv.parents, (size_t)t * 4);
+  M_HIP(hipMemcpyAsync(m->kv_mem, io, ints * 4, hipMemcpyHostToDevice, st));
+  const int32_t* d = (const int32_t*)m->kv_mem;
+  kv.seqs_d = rtq_kv_seqs{s.b, d, s.starts ? d + b : nullptr, d + 2 * b + 1, s.ld};
+  kv.positions_d = d + 2 * b + 1 + tab;
+  kv.parents_d = kv.parents ? kv.positions_d + t : nullptr;
+  return RTQ_OK;
+}
+
 // one step (forward_backward_layout, src/model.rs:644-687): checks, buffers and tables, the
 // inputs' upload, the kernels (eager, captured or replayed), the outputs' download
 rtq_status step(rtq_model* m, const int32_t* tokens, int64_t t, const int32_t* positions, const int32_t* segments,
                 const int32_t* pos, const int32_t* tok, const float* weights, int64_t n, float* logp, int64_t* hits,
-                const HeadJob* job = nullptr) {
+                const HeadJob* job = nullptr, KvStep* kv = nullptr) {
   if (!m || !tokens || t <= 0 || n < 0 || (n > 0 && (!pos || (!job && (!tok || !logp)))))
     return rtq_fail(RTQ_ERR_INVALID, "null model/tokens/targets or empty sequence");
   const rtq_model_config& c = m->cfg;
@@ -2018,20 +2078,30 @@ rtq_status step(rtq_model* m, const int32_t* tokens, int64_t t, const int32_t* p
       if (segments[i] < 0) return rtq_fail(RTQ_ERR_INVALID, "segment %lld is negative", (long long)i);
   M_HIP(hipSetDevice(rtq_ctx_device_id(m->ctx)));
   m->job = job;
-  m->attn_fused = m->attn_hd_ok && m->attn_mode != 0;
-  M_TRY(choose_ckpt(m, t, n));
-  M_TRY(choose_defer(m, t));
+  m->kv = kv;
+  if (!kv) {
+    m->attn_fused = m->attn_hd_ok && m->attn_mode != 0;
+    M_TRY(choose_ckpt(m, t, n));
+    M_TRY(choose_defer(m, t));
+  } else if (m->step_mem && t <= m->t_cap && n <= m->n_cap) {  // any step's buffers do
+    m->attn_fused = m->layout_fused == 1, m->ckpt = m->cache_cap == 1, m->defer_lg = m->layout_defer == 1;
+  } else {  // no backward follows: one block's activations, no probabilities
+    m->attn_fused = m->ckpt = true, m->defer_lg = false;
+  }
   M_TRY(ensure_step(m, t, n));
   M_TRY(ensure_hpk(m, t));
   M_TRY(ensure_lgrad(m, t));
-  M_TRY(ensure_rope(m, t, positions));
-  M_TRY(upload_layout(m, segments, t));
-  if (m->attn_fused) M_TRY(ensure_attn_plan(m, t, segments));
-  M_TRY(ensure_seq_plan(m, t, segments));
+  if (!kv) {
+    M_TRY(ensure_rope(m, t, positions));
+    M_TRY(upload_layout(m, segments, t));
+    if (m->attn_fused) M_TRY(ensure_attn_plan(m, t, segments));
+    M_TRY(ensure_seq_plan(m, t, segments));
+  }
   hipStream_t st = stream_of(m);
   // host inputs and outputs pass through pinned staging, so the copies are asynchronous; the
   // staging is free again once the step's synchronisation below returns
-  const size_t io_need = (size_t)(t + 5 * n) * 4;
+  const size_t kv_ints = kv ? (size_t)(2 * kv->seqs->b + 1 + kv->seqs->b * kv->seqs->ld + 2 * t) : 0;
+  const size_t io_need = ((size_t)(t + 5 * n) + kv_ints) * 4;
   if (io_need > m->io_cap) {
     if (m->io_host) M_HIP(hipHostFree(m->io_host));
     m->io_host = nullptr;
@@ -2055,6 +2125,7 @@ rtq_status step(rtq_model* m, const int32_t* tokens, int64_t t, const int32_t* p
       M_HIP(hipMemcpyAsync(m->wts_d, io + t + 2 * n, (size_t)n * 4, hipMemcpyHostToDevice, st));
     }
   }
+  if (kv) M_TRY(upload_kv(m, *kv, t, kv_ints, io + t + 5 * n, st));
   if (job && n > 0) M_TRY(upload_job(m, *job, n, st));
   // the launch key: everything the step's launches depend on besides gen (bumped by the rest)
   const bool graphable = m->graph_on && m->dbg_layer < 0 && !rtq_ctx_timing_on(m->ctx);
@@ -2073,6 +2144,10 @@ rtq_status step(rtq_model* m, const int32_t* tokens, int64_t t, const int32_t* p
                        (uint64_t)(uintptr_t)job->rows})
       key.push_back(v);
   }
+  if (graphable && kv)
+    for (uint64_t v : {rtq_kv_cache_id(kv->kc), (uint64_t)kv->seqs->b, (uint64_t)kv->seqs->ld, (uint64_t)(kv->seqs->starts ? 1 : 0),
+                       (uint64_t)(kv->parents ? 1 : 0)})
+      key.push_back(v);
   if (graphable && m->gexec && key == m->gkey) {
     M_HIP(hipGraphLaunch(m->gexec, st));
     m->graph_replays++;
@@ -2207,6 +2282,35 @@ rtq_status rtq_model_verify_draft(rtq_model* m, rtq_model* draft, const int32_t*
   M_HIP(hipMemcpyAsync(out, od, (size_t)(d + 1) * 4, hipMemcpyDeviceToHost, st));
   M_HIP(hipStreamSynchronize(st));
   return RTQ_OK;
+}
+
+rtq_status rtq_model_extend(rtq_model* m, rtq_kv_cache* kc, const rtq_kv_seqs* seqs, const int32_t* tokens, int64_t n,
+                            const int32_t* parents, const int32_t* pos, int64_t np, int64_t k, float temperature,
+                            float* vals, int32_t* ids, float* rest) {
+  if (!m) return rtq_fail(RTQ_ERR_INVALID, "null model");
+  const rtq_model_config& c = m->cfg;
+  if (np < 0 || np > 65535) return rtq_fail(RTQ_ERR_INVALID, "row count %lld out of range [0, 65535]", (long long)np);
+  if (n < 1 || n > 65535) return rtq_fail(RTQ_ERR_INVALID, "token count %lld out of range [1, 65535]", (long long)n);
+  if (k < 1 || k > RTQ_TOP_MAX || k > c.n_vocab)
+    return rtq_fail(RTQ_ERR_INVALID, "k = %lld out of range [1, min(%lld, %d)]", (long long)k, (long long)c.n_vocab, RTQ_TOP_MAX);
+  if (np > 0 && (!pos || !vals || !ids)) return rtq_fail(RTQ_ERR_INVALID, "null pos/vals/ids");
+  M_TRY(rtq_check_temperature(temperature));
+  M_TRY(rtq_kv_check_step(kc, m->ctx, c.n_layer, c.n_head, c.n_head_kv, c.head_dim, seqs, n, parents));
+  const int64_t lo = seqs->starts ? seqs->starts[0] : 0, hi = seqs->starts ? seqs->starts[seqs->b] : n;
+  for (int64_t i = 0; i < np; i++)
+    if (pos[i] < lo || pos[i] >= hi) return rtq_fail(RTQ_ERR_INVALID, "row %d of tokens %lld to %lld", pos[i], (long long)lo, (long long)hi);
+  std::vector<int32_t> at((size_t)n, 0);  // rows outside the sequences: none
+  for (int64_t i = 0; i < seqs->b; i++) {
+    const int64_t s0 = seqs->starts ? seqs->starts[i] : n / seqs->b * i, s1 = seqs->starts ? seqs->starts[i + 1] : n / seqs->b * (i + 1);
+    for (int64_t j = s0; j < s1; j++)
+      at[(size_t)j] = !parents ? (int32_t)(seqs->lens[i] + (j - s0)) : parents[j] < 0 ? seqs->lens[i] : at[(size_t)(s0 + parents[j])] + 1;
+  }
+  HeadJob j{HeadJob::TOP};
+  j.k = k, j.temp = temperature, j.vals = vals, j.ids = ids, j.rest = rest;
+  KvStep kv{kc, seqs, parents, at.data(), {}, nullptr, nullptr};
+  const rtq_status st = step(m, tokens, n, nullptr, nullptr, pos, nullptr, nullptr, np, nullptr, nullptr, &j, &kv);
+  m->kv = nullptr;
+  return st;
 }
 
 rtq_status rtq_model_set_checkpointing(rtq_model* m, int mode) {

@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -2163,6 +2164,7 @@ struct rtq_kv_cache {
   int64_t layer = 0;  // elements of a layer's keys (and of its values)
   uint16_t *k = nullptr, *v = nullptr;
   bool owned = false;
+  uint64_t id = 0;
 };
 
 namespace {
@@ -2331,6 +2333,8 @@ rtq_status rtq_kv_cache_create(rtq_ctx* c, int type, int64_t n_layer, int64_t n_
   if (!kc) return fail(RTQ_ERR_INVALID, "out of host memory");
   kc->ctx = c, kc->type = type, kc->n_layer = n_layer, kc->n_pages = n_pages, kc->ps = ps, kc->nkv = nkv, kc->d = d;
   kc->layer = n_pages * ps * nkv * d;
+  static std::atomic<uint64_t> ids{0};
+  kc->id = ++ids;
   while ((1 << kc->ps_shift) < ps) kc->ps_shift++;
   kc->k = (uint16_t*)k, kc->v = (uint16_t*)v, kc->owned = !k;
   if (kc->owned) {
@@ -2892,6 +2896,15 @@ rtq_status kv_check_lists(const rtq_kv_cache* kc, const rtq_kv_seqs* s, int64_t 
   }
   return RTQ_OK;
 }
+rtq_status kv_check_parents(const rtq_kv_seqs* s, int64_t n, const int32_t* parents) {
+  for (int64_t i = 0; parents && i < s->b; i++) {
+    const int64_t s0 = s->starts ? s->starts[i] : n / s->b * i, s1 = s->starts ? s->starts[i + 1] : n / s->b * (i + 1);
+    if (s1 - s0 > RTQ_TREE_MAX) return fail(RTQ_ERR_INVALID, "sequence %lld is a tree of %lld tokens", (long long)i, (long long)(s1 - s0));
+    for (int64_t j = s0; j < s1; j++)
+      if (parents[j] < -2 || parents[j] >= j - s0) return fail(RTQ_ERR_INVALID, "parent %d of token %lld of sequence %lld", parents[j], (long long)(j - s0), (long long)i);
+  }
+  return RTQ_OK;
+}
 size_t kv_seq_bytes(const rtq_kv_seqs& s) { return (size_t)(2 * s.b + 1 + s.b * s.ld) * 4 + 3 * 256; }
 rtq_status kv_seq_put(const rtq_kv_seqs& s, int64_t n, Arena& ar, hipStream_t st, KvSeqs* out) {
   int32_t* lens = ar.take<int32_t>((size_t)s.b);
@@ -2951,12 +2964,7 @@ rtq_status rtq_kv_attend(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s, 
   RTQ_TRY(kv_check_attend(kc, layer, s, n, type, nh, scale, q, ldq, out, ldo));
   if (n == 0) return RTQ_OK;
   RTQ_TRY(kv_check_lists(kc, s, n));
-  for (int64_t i = 0; parents && i < s->b; i++) {
-    const int64_t s0 = s->starts ? s->starts[i] : n / s->b * i, s1 = s->starts ? s->starts[i + 1] : n / s->b * (i + 1);
-    if (s1 - s0 > RTQ_TREE_MAX) return fail(RTQ_ERR_INVALID, "sequence %lld is a tree of %lld tokens", (long long)i, (long long)(s1 - s0));
-    for (int64_t j = s0; j < s1; j++)
-      if (parents[j] < -2 || parents[j] >= j - s0) return fail(RTQ_ERR_INVALID, "parent %d of token %lld of sequence %lld", parents[j], (long long)(j - s0), (long long)i);
-  }
+  RTQ_TRY(kv_check_parents(s, n, parents));
   rtq_ctx* c = kc->ctx;
   RTQ_TRY(check_ctx(c));
   HostCall hc(c);
@@ -3013,6 +3021,20 @@ rtq_status rtq_kv_keep(rtq_kv_cache* kc, const rtq_kv_seqs* s, const int32_t* ke
   if (after) RTQ_TRY(d2h(after, ad, (size_t)s->b * 4, st));
   HIP_TRY(hipStreamSynchronize(st));
   return RTQ_OK;
+}
+
+uint64_t rtq_kv_cache_id(const rtq_kv_cache* kc) { return kc->id; }
+
+rtq_status rtq_kv_check_step(const rtq_kv_cache* kc, const rtq_ctx* c, int64_t n_layer, int64_t nh, int64_t nkv, int64_t d,
+                             const rtq_kv_seqs* s, int64_t n, const int32_t* parents) {
+  RTQ_TRY(kv_check(kc, 0, s, n, RTQ_TYPE_F32));
+  if (kc->n_layer != n_layer || kc->nkv != nkv || kc->d != d)
+    return fail(RTQ_ERR_INVALID, "a cache of %lld layers, %lld KV heads of %lld for a model of %lld, %lld of %lld", (long long)kc->n_layer,
+                (long long)kc->nkv, (long long)kc->d, (long long)n_layer, (long long)nkv, (long long)d);
+  if (kc->ctx != c) return fail(RTQ_ERR_INVALID, "the cache is of another context than the model");
+  RTQ_TRY(kv_check_heads(kc, n, nh));
+  RTQ_TRY(kv_check_lists(kc, s, n));
+  return kv_check_parents(s, n, parents);
 }
 
 rtq_status rtq_lm_top_logits(rtq_ctx* c, const rtq_weight* w, const float* norm, float eps, float offset, const float* x,

@@ -15,6 +15,7 @@ import numpy as np
 from . import _ffi
 from .distill import Teacher, _addr, _per_row
 from .frozen import Context, default_context
+from .kvcache import KvCache, Seqs
 
 LINEARS = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
 GGUF_LINEARS = ("attn_q", "attn_k", "attn_v", "attn_output", "ffn_gate", "ffn_up", "ffn_down")
@@ -253,3 +254,25 @@ class GpuModel:
                    "rtq_model_verify_draft")
         self._stepped = True
         return int(acc.value), out
+
+    def cache(self, n_pages: int, page_size: int = 64, type: int = _ffi.TYPE_F16) -> KvCache:
+        """A paged cache for ``extend``: ``n_pages`` pages of ``page_size`` tokens in every block."""
+        c = self.config
+        return KvCache(c["n_layer"], n_pages, page_size, c["n_head_kv"], c["head_dim"], type=type, ctx=self.ctx)
+
+    def extend(self, cache: KvCache, seqs: Seqs, tokens, k: int, positions=None, parents=None, temperature: float = 1.0) -> Teacher:
+        """The sequences' new ``tokens`` (all of them, in their order) enter ``cache`` and attend over it; returns
+        ``distill.top_logits`` of the rows ``positions`` (indices into ``tokens``; None: every token's).  ``parents`` makes each
+        sequence's tokens a tree (``KvCache.attend``), whose accepted branches ``cache.keep`` continues.  ``seqs.lens``
+        are the caller's to advance."""
+        toks = np.ascontiguousarray(tokens, dtype=np.int32).reshape(-1)
+        pos = np.ascontiguousarray(np.arange(toks.size) if positions is None else positions, dtype=np.int32).reshape(-1)
+        par = None if parents is None else np.ascontiguousarray(parents, dtype=np.int32).reshape(-1)
+        assert par is None or par.size == toks.size, "one parent per new token"
+        n = pos.size
+        vals, ids, rest = np.empty((n, k), np.float32), np.empty((n, k), np.int32), np.empty(n, np.float32)
+        sv = seqs._view()
+        _ffi.check(_ffi.lib().rtq_model_extend(self._h, cache.handle, ctypes.byref(sv), toks.ctypes.data, toks.size, _addr(par), pos.ctypes.data, n, k,
+                                               temperature, vals.ctypes.data, ids.ctypes.data, rest.ctypes.data), "rtq_model_extend")
+        self._stepped = True
+        return Teacher(ids, vals, rest, temperature)

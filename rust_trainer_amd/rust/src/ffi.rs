@@ -276,6 +276,9 @@ extern "C" {
     pub fn rtq_model_verify_draft(m: *mut rtq_model, draft: *mut rtq_model, tokens: *const i32, t: i64, d: i64,
                                   uniforms: *const f32, temperature: f32, accepted: *mut i32,
                                   out: *mut i32) -> rtq_status;
+    pub fn rtq_model_extend(m: *mut rtq_model, kc: *mut rtq_kv_cache, seqs: *const rtq_kv_seqs, tokens: *const i32,
+                            n: i64, parents: *const i32, pos: *const i32, np: i64, k: i64, temperature: f32,
+                            vals: *mut f32, ids: *mut i32, rest: *mut f32) -> rtq_status;
     pub fn rtq_model_set_checkpointing(m: *mut rtq_model, mode: c_int) -> rtq_status;
     pub fn rtq_model_checkpointing(m: *const rtq_model) -> c_int;
     pub fn rtq_model_set_attention(m: *mut rtq_model, mode: c_int) -> rtq_status;
