@@ -653,7 +653,7 @@ struct KvAppendArgs {
   const float *q_norm, *k_norm;  // [d] or null
   float eps, off;
   int nh, nkv, d, rot, neox, ps_shift, n_pages;
-  int vt;  // workgroups of values: (tokens / 32) x KV heads, after those of the tokens
+  int tw, wave_tokens;  // workgroups of tokens (four tokens each, or one); behind them, of values: 32 tokens of a KV head
   double freq[RTQ_KV_ROT / 2];  // turns per position of each pair
 };
 struct KvAttendArgs {
@@ -668,9 +668,11 @@ struct KvAttendArgs {
   int target;       // items that the keys are split into (at most this many, and one per tile beside)
   int slots, qids;  // partial slots; query tiles (x KV heads) that the plan may name
   int tm;           // rows of a tile
+  int cache_bf16;
   float* part;      // [slots][rows of a tile][D]
   float* ml;        // [slots][rows of a tile][2]: maximum, sum
-  int32_t* desc;    // [0] query tiles named, then per tile 8: first slot, splits, first row of the tile ...
+  int32_t* desc;    // [0] query tiles named; from [8] on 8 each: first slot (-1: none), splits, the sequence's first row,
+                    // the tile's first row, its rows, KV head, some row is NaN (tiles without slots), sequence
 };
 struct KvKeepArgs {
   const int32_t *lens, *table, *kept;

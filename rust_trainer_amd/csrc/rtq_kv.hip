@@ -20,52 +20,51 @@ __device__ __forceinline__ int kv_held(const int32_t* lens, int i, int ldt, int 
 }
 
 // ------------------------------------------------------------------ append
-// One token a workgroup (its KV heads' values beside, 32 tokens a workgroup): 16 lanes take a head, a lane
-// eight elements at a time, four pairs of the rotation.  The angles are turns: position x freq in 64 bits,
-// of which the whole turns are dropped before sine and cosine are taken in 32 (at position 10^5 a 32-bit
-// angle is off by 4e-3), once per lane and pair for all of its heads.
-template <int XT, int CT>
-__device__ __forceinline__ void kv_append_rows(const KvAppendArgs& a, int tok, int held, int idx, int seq) {
+// 16 lanes take a head, a lane eight of its elements at a time (a unit: the two sides of four pairs, or eight in a
+// row), a wave four heads.  Few tokens take a workgroup each, its waves sharing the heads; many take a wave
+// each.  The angles are turns: position x freq in 64 bits, of which the whole turns are dropped before sine and cosine
+// are taken in 32 (at position 10^5 a 32-bit angle is off by 4e-3), once per lane and pair for all of its heads.
+__device__ __forceinline__ void kv_turn(double pos, double freq, float& c, float& s) {
+  double t = pos * freq;
+  t -= rint(t);
+  sincospif(2.0f * (float)t, &s, &c);
+}
+
+template <int XT, int CT, int NU>
+__device__ __forceinline__ void kv_append_rows(const KvAppendArgs& a, int tok, int seq, int h0, int step) {
   typedef VRow<XT> X;
   typedef VRow<CT> C;
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, l16 = lane & 15;
+  typedef u2v u2u __attribute__((aligned(2)));
+  const int lane = threadIdx.x & 63, l16 = lane & 15;
   const int half = a.rot / 2, units = a.d / 8;
-  const int64_t slot = (int64_t)held + idx;
+  const int64_t slot = (int64_t)kv_held(a.s.lens, seq, a.s.ldt, a.ps_shift) + (tok - kv_start(a.s, seq));
   const int p = (int)(slot >> a.ps_shift), ps = 1 << a.ps_shift;
   const int pid = p < a.s.ldt ? a.s.table[(int64_t)seq * a.s.ldt + p] : -1;
-  const bool stored = (unsigned)pid < (unsigned)a.n_pages;
+  const bool stored = (unsigned)pid < (unsigned)a.n_pages, whole = a.rot % 8 == 0;
   const double pos = a.pos ? (double)a.pos[tok] : (double)slot;
-  const int heads = (a.q ? a.nh : 0) + a.nkv, nq = a.q ? a.nh : 0;
-  // this lane's units: l16 and l16 + 16 (d <= 256)
-  float cs[2][4], sn[2][4];
-  const bool whole = a.rot % 8 == 0;
+  const int nq = a.q ? a.nh : 0, heads = nq + a.nkv;
+  uint16_t* const kp = a.k + (((int64_t)(stored ? pid : 0) * a.nkv << a.ps_shift) + (slot & (ps - 1))) * a.d;
+  // this lane's units: l16 and, of heads above 128, l16 + 16
+  float cs[NU][4], sn[NU][4];
 #pragma unroll
-  for (int u = 0; u < 2; u++)
+  for (int u = 0; u < NU; u++)
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const int i = 4 * (l16 + 16 * u) + e;
       cs[u][e] = 1.0f, sn[u][e] = 0.0f;
-      if (i < half) {
-        double t = pos * a.freq[i];
-        t -= rint(t);
-        float sv, cv;
-        sincospif(2.0f * (float)t, &sv, &cv);
-        cs[u][e] = cv, sn[u][e] = sv;
-      }
+      if (whole && l16 + 16 * u < a.rot / 8) kv_turn(pos, a.freq[4 * (l16 + 16 * u) + e], cs[u][e], sn[u][e]);
     }
-  for (int h = wv * 4 + (lane >> 4); h < heads; h += 16) {
+  for (int h = h0 + (lane >> 4); h < heads; h += step) {
     const bool isq = h < nq;
     const int hh = isq ? h : h - nq;
     const void* x = isq ? a.q : a.kx;
-    const int64_t at = isq ? (int64_t)tok * a.ldq + (int64_t)hh * a.d : (int64_t)tok * a.ldk + (int64_t)hh * a.d;
+    const int64_t at = (int64_t)tok * (isq ? a.ldq : a.ldk) + (int64_t)hh * a.d, qd = (int64_t)tok * a.ldo + (int64_t)hh * a.d;
     const float* w = isq ? a.q_norm : a.k_norm;
-    uint16_t* kd = a.k + ((((int64_t)(stored ? pid : 0) * a.nkv + hh) << a.ps_shift) + (slot & (ps - 1))) * a.d;
-    const int64_t qd = (int64_t)tok * a.ldo + (int64_t)hh * a.d;
-    const auto put = [&](int j, float y) {
-      if (isq) X::put(a.qo, qd + j, y);
-      else if (stored) C::put(kd, j, y);
-    };
-    if (!whole) {  // a rotation that ends inside a unit of eight: element by element
+    uint16_t* const kd = kp + ((int64_t)hh << a.ps_shift) * a.d;
+    if (!whole) {  // a rotation that ends inside a unit: element by element
+      const auto put = [&](int j, float y) {
+        if (isq) X::put(a.qo, qd + j, y);
+        else if (stored) C::put(kd, j, y);
+      };
       float ir = 1.0f;
       if (w) {
         float s = 0.0f;
@@ -76,22 +75,21 @@ __device__ __forceinline__ void kv_append_rows(const KvAppendArgs& a, int tok, i
       }
       const auto get = [&](int j) { return w ? X::one(x, at + j) * (ir * (w[j] + a.off)) : X::one(x, at + j); };
       for (int j = a.rot + l16; j < a.d; j += 16) put(j, get(j));
+#pragma unroll 1
       for (int i = l16; i < half; i += 16) {
         const int ia = a.neox ? i : 2 * i, ib = a.neox ? i + half : 2 * i + 1;
-        double t = pos * a.freq[i];
-        t -= rint(t);
         float sv, cv;
-        sincospif(2.0f * (float)t, &sv, &cv);
+        kv_turn(pos, a.freq[i], cv, sv);
         const float x1 = get(ia), x2 = get(ib);
         put(ia, x1 * cv - x2 * sv), put(ib, x2 * cv + x1 * sv);
       }
       continue;
     }
-    // unit u covers elements o1 .. o1 + 3 and o2 .. o2 + 3: the two sides of four pairs, or eight in a row
-    float v[2][8];
-    int o1[2], o2[2];
+    // unit u covers elements o1 .. o1 + 3 and o2 .. o2 + 3
+    float v[NU][8];
+    int o1[NU], o2[NU];
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
+    for (int u = 0; u < NU; u++) {
       const int un = l16 + 16 * u;
       if (un >= units) continue;
       const bool split = a.neox && un < a.rot / 8;
@@ -101,19 +99,17 @@ __device__ __forceinline__ void kv_append_rows(const KvAppendArgs& a, int tok, i
         const u4v r1 = X::load(x, at + o1[u]), r2 = X::load(x, at + o2[u]);
 #pragma unroll
         for (int e = 0; e < 4; e++) v[u][e] = X::get(r1, e), v[u][4 + e] = X::get(r2, e);
-      } else if (split) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[u][e] = X::one(x, at + o1[u] + e), v[u][4 + e] = X::one(x, at + o2[u] + e);
       } else {
-        const u4v r = X::load(x, at + o1[u]);
+        const uint16_t* b = static_cast<const uint16_t*>(x) + at;
+        const u2v r1 = *reinterpret_cast<const u2u*>(b + o1[u]), r2 = *reinterpret_cast<const u2u*>(b + o2[u]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[u][e] = X::get(r, e);
+        for (int e = 0; e < 8; e++) v[u][e] = X::get(u4v{r1.x, r1.y, r2.x, r2.y}, e);
       }
     }
     if (w) {  // RMS norm of the head: (x / rms) (w + off)
       float s = 0.0f;
 #pragma unroll
-      for (int u = 0; u < 2; u++)
+      for (int u = 0; u < NU; u++)
         if (l16 + 16 * u < units)
 #pragma unroll
           for (int e = 0; e < 8; e++) s += v[u][e] * v[u][e];
@@ -121,82 +117,67 @@ __device__ __forceinline__ void kv_append_rows(const KvAppendArgs& a, int tok, i
       for (int m = 1; m <= 8; m <<= 1) s += __shfl_xor(s, m);
       const float ir = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(s, (float)a.d) + a.eps));
 #pragma unroll
-      for (int u = 0; u < 2; u++)
+      for (int u = 0; u < NU; u++)
         if (l16 + 16 * u < units)
 #pragma unroll
           for (int e = 0; e < 8; e++) v[u][e] *= ir * (w[(e < 4 ? o1[u] : o2[u] - 4) + e] + a.off);
     }
 #pragma unroll
-    for (int u = 0; u < 2; u++)
+    for (int u = 0; u < NU; u++)
       if (l16 + 16 * u < a.rot / 8) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const int ia = a.neox ? e : 2 * e, ib = a.neox ? 4 + e : 2 * e + 1;
-          const float x1 = v[u][ia], x2 = v[u][ib];
-          v[u][ia] = x1 * cs[u][e] - x2 * sn[u][e];
-          v[u][ib] = x2 * cs[u][e] + x1 * sn[u][e];
+          const float x1 = a.neox ? v[u][e] : v[u][2 * e], x2 = a.neox ? v[u][4 + e] : v[u][2 * e + 1];
+          const float y1 = x1 * cs[u][e] - x2 * sn[u][e], y2 = x2 * cs[u][e] + x1 * sn[u][e];
+          if (a.neox) v[u][e] = y1, v[u][4 + e] = y2;
+          else v[u][2 * e] = y1, v[u][2 * e + 1] = y2;
         }
       }
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
+    for (int u = 0; u < NU; u++) {
       if (l16 + 16 * u >= units) continue;
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        put((e < 4 ? o1[u] : o2[u] - 4) + e, v[u][e]);
+      if (isq) {
+        if constexpr (XT == VT_F32) {
+          X::store(a.qo, qd + o1[u], X::pack(v[u])), X::store(a.qo, qd + o2[u], X::pack(v[u] + 4));
+        } else {
+          uint16_t* b = static_cast<uint16_t*>(a.qo) + qd;
+          const u4v r = X::pack(v[u]);
+          *reinterpret_cast<u2u*>(b + o1[u]) = u2v{r[0], r[1]}, *reinterpret_cast<u2u*>(b + o2[u]) = u2v{r[2], r[3]};
+        }
+      } else if (stored) {  // (rows of the cache are 32-byte aligned)
+        const u4v r = C::pack(v[u]);
+        *reinterpret_cast<u2v*>(kd + o1[u]) = u2v{r[0], r[1]}, *reinterpret_cast<u2v*>(kd + o2[u]) = u2v{r[2], r[3]};
       }
     }
   }
 }
 
-// the sequence that row tok belongs to (-1: none), found by the workgroup's 256 threads
-__device__ __forceinline__ int kv_find(const KvSeqs& s, int tok, int* found) {
-  if (!s.starts) {
-    const int per = s.n / s.b;
-    return tok / per;
+// the sequence that row tok belongs to (-1: none), found by the wave's lanes
+__device__ __forceinline__ int kv_find(const KvSeqs& s, int tok) {
+  if (!s.starts) return tok / (s.n / s.b);
+  for (int i0 = 0; i0 < s.b; i0 += 64) {
+    const int i = i0 + (threadIdx.x & 63);
+    const uint64_t hit = __ballot(i < s.b && kv_start(s, i) <= tok && tok < kv_start(s, i + 1));
+    if (hit) return i0 + __ffsll((unsigned long long)hit) - 1;
   }
-  if (threadIdx.x == 0) *found = -1;
-  __syncthreads();
-  for (int i = threadIdx.x; i < s.b; i += 256)
-    if (kv_start(s, i) <= tok && tok < kv_start(s, i + 1)) *found = i;
-  __syncthreads();
-  return *found;
+  return -1;
 }
 
-template <int XT, int CT>
+template <int XT, int CT, int NU>
 __device__ __forceinline__ void kv_append(const KvAppendArgs& a) {
-  __shared__ int found;
-  if ((int)blockIdx.x < a.s.n) {
-    const int tok = blockIdx.x, seq = kv_find(a.s, tok, &found);
-    if (seq < 0) return;
-    kv_append_rows<XT, CT>(a, tok, kv_held(a.s.lens, seq, a.s.ldt, a.ps_shift), tok - kv_start(a.s, seq), seq);
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if ((int)blockIdx.x < a.tw) {
+    const int tok = a.wave_tokens ? 4 * blockIdx.x + wv : blockIdx.x;
+    if (tok >= a.s.n) return;
+    const int seq = kv_find(a.s, tok);
+    if (seq >= 0) kv_append_rows<XT, CT, NU>(a, tok, seq, a.wave_tokens ? 0 : 4 * wv, a.wave_tokens ? 4 : 16);
     return;
   }
-  // values: 32 tokens of one KV head, through LDS, so that neighbouring tokens are stored together
-  __shared__ float tile[32][257];
+  // values: 32 tokens of one KV head, through LDS, so that neighbouring slots are stored together
+  __shared__ uint16_t tile[256][34];  // [element][token], rows off each other's banks
   __shared__ int64_t dst[32];
-  const int wg = blockIdx.x - a.s.n, hv = wg % a.nkv, t0 = wg / a.nkv * 32;
+  const int wg = blockIdx.x - a.tw, hv = wg % a.nkv, t0 = wg / a.nkv * 32;
   const int nt = min(32, a.s.n - t0), ps = 1 << a.ps_shift;
-  if (threadIdx.x < 32) dst[threadIdx.x] = -1;
-  __syncthreads();
-  if (a.s.starts) {  // each sequence names the tokens of this tile that are its own
-    for (int i = threadIdx.x; i < a.s.b; i += 256) {
-      const int s0 = kv_start(a.s, i), s1 = kv_start(a.s, i + 1);
-      for (int t = max(s0, t0); t < min(s1, t0 + nt); t++) dst[t - t0] = (int64_t)i << 32 | (t - s0);
-    }
-  } else if ((int)threadIdx.x < nt) {
-    const int per = a.s.n / a.s.b, t = t0 + threadIdx.x;
-    dst[threadIdx.x] = (int64_t)(t / per) << 32 | (t % per);
-  }
-  __syncthreads();
-  if (threadIdx.x < 32 && dst[threadIdx.x] >= 0) {
-    const int seq = (int)(dst[threadIdx.x] >> 32), idx = (int)(dst[threadIdx.x] & 0xffffffff);
-    const int64_t slot = (int64_t)kv_held(a.s.lens, seq, a.s.ldt, a.ps_shift) + idx;
-    const int64_t p = slot >> a.ps_shift;
-    const int pid = p < a.s.ldt ? a.s.table[(int64_t)seq * a.s.ldt + p] : -1;
-    dst[threadIdx.x] = (unsigned)pid < (unsigned)a.n_pages
-                           ? (((int64_t)pid * a.nkv + hv) * a.d << a.ps_shift) + (slot & (ps - 1))
-                           : -1;
-  }
   typedef VRow<XT> X;
   constexpr int E = X::E;
   const int vecs = a.d / E;
@@ -204,16 +185,59 @@ __device__ __forceinline__ void kv_append(const KvAppendArgs& a) {
     const int t = i / vecs, c = i % vecs * E;
     const u4v r = X::load(a.vx, (int64_t)(t0 + t) * a.ldv + (int64_t)hv * a.d + c);
 #pragma unroll
-    for (int e = 0; e < E; e++) tile[t][c + e] = X::get(r, e);
+    for (int e = 0; e < E; e++) VRow<CT>::put(tile[c + e], t, X::get(r, e));
+  }
+  if (threadIdx.x < 64) {
+    // where the tile's tokens go: a wave finds their sequences
+    const int lane = threadIdx.x;
+    int seq = -1, idx = 0;
+    if (a.s.starts) {
+      for (int i0 = 0; i0 < a.s.b; i0 += 64) {
+        const int i = i0 + lane, s0 = i < a.s.b ? kv_start(a.s, i) : 0, s1 = i < a.s.b ? kv_start(a.s, i + 1) : 0;
+        uint64_t near = __ballot(s0 < t0 + nt && s1 > t0 && s1 > s0);
+        while (near) {  // (each sequence that meets the tile)
+          const int j = __ffsll((unsigned long long)near) - 1;
+          near &= near - 1;
+          const int b0 = __builtin_amdgcn_readlane(s0, j), b1 = __builtin_amdgcn_readlane(s1, j), t = t0 + lane;
+          if (t >= b0 && t < b1) seq = i0 + j, idx = t - b0;
+        }
+      }
+    } else {
+      const int per = a.s.n / a.s.b;
+      seq = (t0 + lane) / per, idx = (t0 + lane) % per;
+    }
+    if (lane < 32) {
+      int64_t at = -1;
+      if (lane < nt && seq >= 0) {
+        const int64_t slot = (int64_t)kv_held(a.s.lens, seq, a.s.ldt, a.ps_shift) + idx;
+        const int64_t p = slot >> a.ps_shift;
+        const int pid = p < a.s.ldt ? a.s.table[(int64_t)seq * a.s.ldt + p] : -1;
+        if ((unsigned)pid < (unsigned)a.n_pages) at = (((int64_t)pid * a.nkv + hv) * a.d << a.ps_shift) + (slot & (ps - 1));
+      }
+      dst[lane] = at;
+    }
   }
   __syncthreads();
-  const int t = threadIdx.x & 31;
-  if (t >= nt || dst[t] < 0) return;
-  for (int c = threadIdx.x >> 5; c < a.d; c += 8) VRow<CT>::put(a.v, dst[t] + ((int64_t)c << a.ps_shift), tile[t][c]);
+  // eight tokens in neighbouring, aligned slots are one store
+  const int t8 = (threadIdx.x & 3) * 8;
+  bool run = dst[t8] >= 0 && dst[t8] % 8 == 0;
+#pragma unroll
+  for (int j = 1; j < 8; j++) run = run && dst[t8 + j] == dst[t8] + j;
+  for (int c = threadIdx.x >> 2; c < a.d; c += 64) {
+    if (run) {
+      const uint32_t* r = reinterpret_cast<const uint32_t*>(&tile[c][t8]);
+      *reinterpret_cast<u4v*>(a.v + dst[t8] + ((int64_t)c << a.ps_shift)) = u4v{r[0], r[1], r[2], r[3]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if (dst[t8 + j] >= 0) a.v[dst[t8 + j] + ((int64_t)c << a.ps_shift)] = tile[c][t8 + j];
+    }
+  }
 }
 
 #define RTQ_KV_APPEND(NAME, XT, CT) \
-  extern "C" __global__ __launch_bounds__(256) void NAME(KvAppendArgs a) { kv_append<XT, CT>(a); }
+  extern "C" __global__ __launch_bounds__(256) void NAME(KvAppendArgs a) { kv_append<XT, CT, 1>(a); } \
+  extern "C" __global__ __launch_bounds__(256) void NAME##_256(KvAppendArgs a) { kv_append<XT, CT, 2>(a); }
 RTQ_KV_APPEND(rtq_kv_append_f32_f16, VT_F32, VT_F16)
 RTQ_KV_APPEND(rtq_kv_append_f32_bf16, VT_F32, VT_BF16)
 RTQ_KV_APPEND(rtq_kv_append_f16, VT_F16, VT_F16)
@@ -221,57 +245,68 @@ RTQ_KV_APPEND(rtq_kv_append_bf16, VT_BF16, VT_BF16)
 
 // ------------------------------------------------------------------ keep
 // Workgroup: one KV head of one sequence and layer.  Kept tokens ascend, so the j-th comes from a slot no
-// earlier than its own: a thread that moves its elements in order, eight loads before their stores, never
-// writes a slot that it has yet to read, and no two threads touch the same elements.
+// earlier than its own: a wave that moves its elements in batches of eight tokens, in order, each batch's loads before its
+// stores, never writes a slot that it has yet to read, and no two waves touch the same elements.  Values: eight
+// lanes take an element's eight tokens (neighbouring slots of one row), keys: d / 8 lanes a token.
 #define RTQ_KV_KEEP 1024
-extern "C" __global__ __launch_bounds__(320) void rtq_kv_keep(KvKeepArgs a) {
+extern "C" __global__ __launch_bounds__(256) void rtq_kv_keep(KvKeepArgs a) {
   __shared__ int64_t from[RTQ_KV_KEEP], to[RTQ_KV_KEEP];  // page x slots + slot; from -1: not moved
   __shared__ int count;
-  const int hv = blockIdx.x % a.nkv, seq = blockIdx.x / a.nkv;
+  const int hv = blockIdx.x % a.nkv, seq = blockIdx.x / a.nkv, tid = threadIdx.x;
   const int32_t* kept = a.kept + (int64_t)seq * a.ldk;
   const int held = kv_held(a.lens, seq, a.ldt, a.ps_shift), ps = 1 << a.ps_shift;
-  if (threadIdx.x == 0) count = a.ldk;
+  if (tid == 0) count = a.ldk;
   __syncthreads();
-  for (int j = threadIdx.x; j < a.ldk; j += 320)  // the list ends at the first entry that does not ascend
-    if (kept[j] < 0 || (j && kept[j] <= kept[j - 1])) atomicMin(&count, j);
-  __syncthreads();
-  const int n = count;
-  for (int j = threadIdx.x; j < n; j += 320) {
-    const int64_t f = (int64_t)held + kept[j], t = (int64_t)held + j;
+  for (int j = tid; j < a.ldk; j += 256) {  // the list ends at the first entry that does not ascend
+    const int x = kept[j];
+    if (x < 0 || (j && x <= kept[j - 1])) atomicMin(&count, j);
+    const int64_t f = (int64_t)held + max(x, 0), t = (int64_t)held + j;
     const int64_t fp = f >> a.ps_shift, tp = t >> a.ps_shift;
     const int fi = fp < a.ldt ? a.table[(int64_t)seq * a.ldt + fp] : -1, ti = tp < a.ldt ? a.table[(int64_t)seq * a.ldt + tp] : -1;
     const bool ok = (unsigned)fi < (unsigned)a.n_pages && (unsigned)ti < (unsigned)a.n_pages && f != t;
     from[j] = ok ? ((int64_t)fi << 32 | (f & (ps - 1))) : -1;
     to[j] = (int64_t)ti << 32 | (t & (ps - 1));
   }
-  if (blockIdx.y == 0 && hv == 0 && threadIdx.x == 0 && a.after) a.after[seq] = a.lens[seq] + n;
   __syncthreads();
+  const int n = count;
+  if (blockIdx.y == 0 && hv == 0 && tid == 0 && a.after) a.after[seq] = a.lens[seq] + n;
   const int64_t row = (int64_t)a.d << a.ps_shift;  // elements of a head's page
   uint16_t* k = a.k + blockIdx.y * a.layer;
   uint16_t* v = a.v + blockIdx.y * a.layer;
-  const int c = threadIdx.x;
   const auto page = [&](int64_t at) { return ((at >> 32) * a.nkv + hv) * row; };
-  if (c < a.d) {
+  const int lane = tid & 63, wv = tid >> 6, lanes = a.d / 8;
+  if (wv == 0) {  // keys, 16 bytes a lane: 64 / lanes tokens at once (2 .. 32; 5 .. 15 lanes leave some idle)
+    const int per = min(64 / lanes, 8), jl = lane / lanes, e = lane % lanes * 8;
     for (int j0 = 0; j0 < n; j0 += 8) {
-      uint16_t x[8];
+      u4v x[4];
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        if (j0 + j < n && from[j0 + j] >= 0) x[j] = v[page(from[j0 + j]) + ((int64_t)c << a.ps_shift) + (from[j0 + j] & 0xffffffff)];
+      for (int i = 0; i < 4; i++) {
+        const int j = j0 + i * per + jl;
+        if (jl < per && i * per + jl < 8 && j < n && from[j] >= 0) x[i] = *reinterpret_cast<const u4v*>(k + page(from[j]) + (from[j] & 0xffffffff) * a.d + e);
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a lane may write what another has read)
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        if (j0 + j < n && from[j0 + j] >= 0) v[page(to[j0 + j]) + ((int64_t)c << a.ps_shift) + (to[j0 + j] & 0xffffffff)] = x[j];
+      for (int i = 0; i < 4; i++) {
+        const int j = j0 + i * per + jl;
+        if (jl < per && i * per + jl < 8 && j < n && from[j] >= 0) *reinterpret_cast<u4v*>(k + page(to[j]) + (to[j] & 0xffffffff) * a.d + e) = x[i];
+      }
     }
   }
-  const int e = (319 - c) * 8;  // keys: the last threads, 16 bytes each
-  if (e < a.d) {
-    for (int j0 = 0; j0 < n; j0 += 8) {
-      u4v x[8];
+  const int jl = lane & 7;
+  for (int j0 = 0; j0 < n; j0 += 8) {
+    const int j = j0 + jl;
+    if (j >= n || from[j] < 0) continue;
+    const uint16_t* src = v + page(from[j]) + (from[j] & 0xffffffff);
+    uint16_t* dst = v + page(to[j]) + (to[j] & 0xffffffff);
+    for (int c0 = 8 * wv + (lane >> 3); c0 < a.d; c0 += 128) {
+      uint16_t x[4];
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        if (j0 + j < n && from[j0 + j] >= 0) x[j] = *reinterpret_cast<const u4v*>(k + page(from[j0 + j]) + (from[j0 + j] & 0xffffffff) * a.d + e);
+      for (int i = 0; i < 4; i++)
+        if (c0 + 32 * i < a.d) x[i] = src[(int64_t)(c0 + 32 * i) << a.ps_shift];
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        if (j0 + j < n && from[j0 + j] >= 0) *reinterpret_cast<u4v*>(k + page(to[j0 + j]) + (to[j0 + j] & 0xffffffff) * a.d + e) = x[j];
+      for (int i = 0; i < 4; i++)
+        if (c0 + 32 * i < a.d) dst[(int64_t)(c0 + 32 * i) << a.ps_shift] = x[i];
     }
   }
 }
@@ -290,14 +325,27 @@ struct KvItem {
   int seq, row0, cnt, held, total, tile, hv, split, splits, slot, qid, C;
 };
 
-__device__ __forceinline__ int kv_wave_scan(int v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
+// inclusive sums over the wave's lanes (DPP: rows of 16, then across them)
+__device__ __forceinline__ int kv_wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // the lane 1, 2, 4, 8 before, within the row
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row 0's and row 2's last lane to the row behind
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row 1's to rows 2 and 3
   return v;
+}
+__device__ __forceinline__ float kv_wave_total(float v) {
+  const auto dpp = [&](auto c, auto rows) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(c)::value, decltype(rows)::value, 0xf, false));
+  };
+  v += dpp(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});
+  v += dpp(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+  v += dpp(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+  v += dpp(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+  v += dpp(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
+  v += dpp(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 // item `block` of the plan (every wave finds it by itself; a lane looks after b / 64 sequences); false: none.
@@ -314,14 +362,13 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, int block, KvItem
     tiles = (int)(((int64_t)cnt * group + TM - 1) / TM);
   };
   int row0, cnt, held, total, tiles;
-  double w = 0.0;
+  float w = 0.0f;
   for (int i = i0; i < i1; i++) {
     look(i, row0, cnt, held, total, tiles);
-    w += (double)tiles * (double)total;
+    w += (float)tiles * (float)total;
   }
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) w += __shfl_xor(w, m);
-  const int C = (int)min(ceil(w * (double)a.nkv / (double)a.target / 128.0), (double)(RTQ_KV_SLOTS / 128)) * 128;
+  w = kv_wave_total(w);
+  const int C = (int)fminf(ceilf(w * (float)a.nkv / (float)a.target / 128.0f), (float)(RTQ_KV_SLOTS / 128)) * 128;
   it.C = max(C, 128);
   int items = 0, slots = 0, qids = 0;
   for (int i = i0; i < i1; i++) {
@@ -365,6 +412,12 @@ __device__ __forceinline__ f4 kv_mfma(u4v x, u4v y, f4 c) {
   if constexpr (CT == VT_F16) return mfma_f16(__builtin_bit_cast(half8, x), __builtin_bit_cast(half8, y), c);
   else return mfma_bf16(__builtin_bit_cast(bf8, x), __builtin_bit_cast(bf8, y), c);
 }
+template <int CT>
+__device__ __forceinline__ f16v kv_mfma32(u4v x, u4v y, f16v c) {
+  if constexpr (CT == VT_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, x), __builtin_bit_cast(half8, y), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, x), __builtin_bit_cast(bf8, y), c, 0, 0, 0);
+}
 
 // eight floats as N planes of 16 bits, each the rounding of what the ones before it leave: 11 (f16) or 8
 // (bf16) bits of the value a plane: f32 rows take two (f16) or three, one plane of a 16-bit row is the row itself.
@@ -382,45 +435,122 @@ __device__ __forceinline__ void kv_planes(const float* v, u4v* out) {
   }
 }
 
+// the page of slot k of sequence seq (uniform: a scalar load, which no vector load in flight is waited for with)
+__device__ __forceinline__ int kv_page(const KvSeqs& s, int seq, int k, int ps_shift) {
+  typedef const __attribute__((address_space(4))) int32_t* cptr;
+  if (s.ldt <= 0) return -1;
+  return reinterpret_cast<cptr>(reinterpret_cast<uintptr_t>(s.table + (int64_t)seq * s.ldt))[min(k >> ps_shift, s.ldt - 1)];
+}
+
 #define RTQ_KV_TREE 1024  // most new tokens of a sequence that is a tree
 
+// f16 weights are taken times 2^15 (as is their sum): small ones, of which a long context has many, keep their bits
+template <int CT>
+constexpr float kKvUp = CT == VT_F16 ? 15.0f : 0.0f;
+
+// What an item works on, beside the plan's: its rows and slots
+struct KvTile {
+  int row_lo, rows, k_lo, k_hi;
+  bool tail;  // some of its slots hold new tokens
+};
+template <int TM>
+__device__ __forceinline__ KvTile kv_tile(const KvAttendArgs& a, const KvItem& it) {
+  KvTile t;
+  const int group = a.nh / a.nkv;
+  t.row_lo = it.tile * TM, t.rows = min((int)((int64_t)it.cnt * group - t.row_lo), TM);
+  t.k_lo = it.split * it.C;
+  // no row of the tile sees a new token after its own
+  const int64_t last = (int64_t)it.held + (t.row_lo + t.rows - 1) / group + 1;
+  t.k_hi = (int)min(min((int64_t)t.k_lo + it.C, (int64_t)it.total), last);
+  t.tail = t.k_hi > it.held;
+  return t;
+}
+
+// The tile's tokens' chains as bits, seen[token - the tile's first] (none, not even the token's own, where the chain meets
+// what is no parent: nothing is seen).  up: room for RTQ_KV_TREE parents.  Ends with a barrier.
+typedef uint32_t KvSeen[RTQ_KV_TREE / 32];
+template <int TOK, int THREADS>
+__device__ __forceinline__ void kv_tree(const KvAttendArgs& a, const KvItem& it, const KvTile& t, KvSeen* seen, uint16_t* up) {
+  const int group = a.nh / a.nkv, n = min(it.cnt, RTQ_KV_TREE);
+  const int first = t.row_lo / group, toks = (t.row_lo + t.rows - 1) / group - first + 1;
+  for (int i = threadIdx.x; i < TOK * (RTQ_KV_TREE / 32); i += THREADS) (&seen[0][0])[i] = 0;
+  for (int i = threadIdx.x; i < n; i += THREADS) {  // 0: the cache, else the parent + 1; 65535: none
+    const int p = a.parents[it.row0 + i];
+    up[i] = p < -1 || p >= i ? 65535 : p + 1;
+  }
+  __syncthreads();
+  for (int r = threadIdx.x; r < toks; r += THREADS) {
+    int node = first + r, dead = it.cnt > RTQ_KV_TREE;
+    while (!dead && node >= 0) {
+      seen[r][node >> 5] |= 1u << (node & 31);
+      const int p = up[node];
+      dead = p == 65535;
+      node = p - 1;
+    }
+    if (dead)
+      for (int w = 0; w < RTQ_KV_TREE / 32; w++) seen[r][w] = 0;
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ bool kv_dead(const uint32_t* seen, int tok) { return !(seen[(tok & (RTQ_KV_TREE - 1)) >> 5] >> (tok & 31) & 1); }
+// 32 bits from new token nw0 on (held tokens before it are seen): what token tok sees of them
+__device__ __forceinline__ uint32_t kv_run_bits(int nw0, int tok) {
+  const int n = tok - nw0 + 1;
+  return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
+}
+__device__ __forceinline__ uint32_t kv_tree_bits(int nw0, const uint32_t* seen) {
+  const int w = nw0 >> 5, sh = nw0 & 31;
+  const auto word = [&](int i) { return i < 0 ? 0xffffffffu : i < RTQ_KV_TREE / 32 ? seen[i] : 0u; };
+  return (uint32_t)(((uint64_t)word(w + 1) << 32 | word(w)) >> sh);
+}
+
+// eight 16-bit elements, of which those from element n on are cleared
+__device__ __forceinline__ u4v kv_clear(u4v x, int n) {
+#pragma unroll
+  for (int w = 0; w < 4; w++) x[w] = 2 * w >= n ? 0u : 2 * w + 1 >= n ? x[w] & 0xffffu : x[w];
+  return x;
+}
+
+// a tile's entry in the plan that the joining kernel reads
+__device__ __forceinline__ void kv_describe(const KvAttendArgs& a, const KvItem& it, const KvTile& t) {
+  if (it.split == 0 && threadIdx.x == 0) {
+    int32_t* q = a.desc + 8 + 8 * it.qid;
+    q[0] = it.slot, q[1] = it.splits, q[2] = it.row0, q[3] = t.row_lo, q[4] = t.rows, q[5] = it.hv, q[6] = 0, q[7] = it.seq;
+  }
+}
+
+// f32 rows over an f16 cache are scaled by a power of two (whose exponent is returned) that brings the row's
+// largest element, of which the caller has mx, to [2^13, 2^14): its planes then neither overflow nor lose bits
+__device__ __forceinline__ int kv_row_shift(float mx) {
+  const int ex = (int)(__builtin_bit_cast(uint32_t, mx) >> 23);
+  return ex == 255 || ex == 0 ? 0 : min(max(140 - ex, -120), 120);
+}
+
+// ---- small tiles: 16 or 32 rows, four waves that share the tile's slots, operands straight from the cache
 template <int CT, bool QF, int D, bool FULL, int NQ>
 __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
   constexpr int DC = D / 32, DT = D / 16, TM = 16 * NQ, LDR = D + 4;
   constexpr int NS = QF ? (CT == VT_F16 ? 2 : 3) : 1, NP = QF ? NS : 2;
-  constexpr uint32_t EXP = CT == VT_F16 ? 0x7c00u : 0x7f80u;  // infinity and NaN
-  // f16 weights are taken times 2^15 (as is their sum): small ones, of which a long context has many, keep their bits
-  constexpr float UP = CT == VT_F16 ? 15.0f : 0.0f;
   typedef VRow<QF ? VT_F32 : CT> Q;
   struct Shared {
     float o[4][TM][LDR];
     float ml[4][TM][2];
-    float w[4][TM][33];
-    uint32_t seen[TM][RTQ_KV_TREE / 32];  // ancestors of each row's token
+    KvSeen seen[TM];
     uint16_t up[RTQ_KV_TREE];
-    int dead[TM];
   };
   __shared__ Shared sh;
-  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, g = lane >> 4;
-  const int group = a.nh / a.nkv, d = FULL ? D : a.d, ps = 1 << a.ps_shift;
   KvItem it;
   if (!kv_plan<TM>(a, blockIdx.x, it)) return;
-  const int row_lo = it.tile * TM, rows = min((int)((int64_t)it.cnt * group - row_lo), TM);
-  const int k_lo = it.split * it.C;
-  // no row of the tile sees a new token after its own
-  const int64_t last = (int64_t)it.held + (row_lo + rows - 1) / group + 1;
-  const int k_hi = (int)min(min((int64_t)k_lo + it.C, (int64_t)it.total), last);
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, g = lane >> 4;
+  const int group = a.nh / a.nkv, d = FULL ? D : a.d, ps = 1 << a.ps_shift;
+  const KvTile tl = kv_tile<TM>(a, it);
+  const int row_lo = tl.row_lo, rows = tl.rows, k_hi = tl.k_hi;
   const bool tree = a.parents != nullptr;
-  if (it.split == 0 && threadIdx.x == 0) {
-    int32_t* q = a.desc + 8 + 8 * it.qid;
-    q[0] = it.slot, q[1] = it.splits, q[2] = it.row0, q[3] = row_lo, q[4] = rows, q[5] = it.hv;
-  }
-  // the rows' tokens (index among the sequence's new ones) of this lane's columns
+  kv_describe(a, it, tl);
+  // the token (index among the sequence's new ones) of each of this lane's columns
   int tok[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; n++) tok[n] = (row_lo + min(16 * n + li, rows - 1)) / group;
-  // f32 rows over an f16 cache are scaled by a power of two that brings the row's largest element to [2^13, 2^14): its
-  // planes then neither overflow nor lose bits below f16's range
   constexpr bool SCALED = QF && CT == VT_F16;
   u4v qf[NS][NQ][DC];
   float sc[NQ];
@@ -454,8 +584,7 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
           for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[c][e]));
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const int ex = (int)(__builtin_bit_cast(uint32_t, mx) >> 23);
-        up = ex == 255 || ex == 0 ? 0 : min(max(140 - ex, -120), 120);
+        up = kv_row_shift(mx);
         sc[n] = ldexpf(a.scale2, -up);
       }
 #pragma unroll
@@ -470,41 +599,24 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
       }
     }
   }
-  const bool tail = k_hi > it.held;  // some of the item's keys are new tokens
-  if (tree && tail) {
-    const int words = (min(it.cnt, RTQ_KV_TREE) + 31) / 32;
-    for (int i = threadIdx.x; i < TM * (RTQ_KV_TREE / 32); i += 256) (&sh.seen[0][0])[i] = 0;
-    for (int i = threadIdx.x; i < min(it.cnt, RTQ_KV_TREE); i += 256) {  // 0: the cache, else the parent + 1; 65535: none
-      const int p = a.parents[it.row0 + i];
-      sh.up[i] = p < -1 || p >= i ? 65535 : p + 1;
-    }
-    __syncthreads();
-    if (threadIdx.x < TM) {
-      const int r = threadIdx.x;
-      int node = r < rows ? (row_lo + r) / group : -1, dead = it.cnt > RTQ_KV_TREE;
-      while (!dead && node >= 0) {
-        sh.seen[r][node >> 5] |= 1u << (node & 31);
-        const int p = sh.up[node];
-        dead = p == 65535;
-        node = p - 1;
-      }
-      sh.dead[r] = dead;
-      if (dead)
-        for (int w = 0; w < words; w++) sh.seen[r][w] = 0;
-    }
-    __syncthreads();
-  }
+  if (tree && tl.tail) kv_tree<TM, 256>(a, it, tl, sh.seen, sh.up);
+  const int tok0 = row_lo / group;
 
   f4 acc[NQ][DT];
   float m[NQ], l[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; n++) {
+    m[n] = -INFINITY, l[n] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < DT; t++) acc[n][t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
   const int64_t head = (int64_t)d << a.ps_shift, pstride = head * a.nkv;
-  const int32_t* table = a.s.table + (int64_t)it.seq * a.s.ldt;
-  const auto page_of = [&](int k0) { return a.s.ldt > 0 ? table[min(k0 >> a.ps_shift, a.s.ldt - 1)] : -1; };
-  const auto base_of = [&](int k0, int pg) { return ((unsigned)pg < (unsigned)a.n_pages ? pg : 0) * pstride + it.hv * head; };
+  const auto page_of = [&](int k0) { return kv_page(a.s, it.seq, k0, a.ps_shift); };
+  const auto base_of = [&](int pg) { return ((unsigned)pg < (unsigned)a.n_pages ? pg : 0) * pstride + it.hv * head; };
   u4v kf[2][DC], vf[DT];
   const uint32_t k_at = (uint32_t)((8 * (li >> 2) + (li & 3)) * d + 8 * g) * 2, v_at = (uint32_t)((li << a.ps_shift) + 8 * g) * 2;
   const auto load_k = [&](int k0, int pg) {
-    const char* base = reinterpret_cast<const char*>(a.k + base_of(k0, pg) + (int64_t)(k0 & (ps - 1)) * d);
+    const char* base = reinterpret_cast<const char*>(a.k + base_of(pg) + (int64_t)(k0 & (ps - 1)) * d);
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -514,22 +626,12 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
       }
   };
   const auto load_v = [&](int k0, int pg) {
-    const char* base = reinterpret_cast<const char*>(a.v + base_of(k0, pg) + (k0 & (ps - 1)));
+    const char* base = reinterpret_cast<const char*>(a.v + base_of(pg) + (k0 & (ps - 1)));
 #pragma unroll
     for (int t = 0; t < DT; t++)
       if (FULL || 16 * t < d) vf[t] = *reinterpret_cast<const u4v*>(base + ((int64_t)(32 * t) << a.ps_shift) + v_at);
   };
-  // A wave whose sums come out NaN takes its slots once more with care: keys and values that are not finite meet the
-  // first plane of queries and weights alone (infinity times a lower plane, which may be 0 or of the other sign, is not
-  // infinity times the whole)
-  for (bool careful = false;; careful = true) {
-#pragma unroll
-  for (int n = 0; n < NQ; n++) {
-    m[n] = -INFINITY, l[n] = 0.0f;
-#pragma unroll
-    for (int t = 0; t < DT; t++) acc[n][t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  int k0 = k_lo + 32 * wv;
+  int k0 = tl.k_lo + 32 * wv;
   int pg = 0, pn = 0;
   if (k0 < k_hi) {
     pg = page_of(k0);
@@ -548,64 +650,33 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
         for (int c = 0; c < DC; c++)
 #pragma unroll
           for (int p = 0; p < NS; p++) s[n][t] = kv_mfma<CT>(kf[t][c], qf[p][n][c], s[n][t]);
-        if constexpr (NS > 1)
-          if (careful) {
-            f4 hi = f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int c = 0; c < DC; c++) hi = kv_mfma<CT>(kf[t][c], qf[0][n][c], hi);
-#pragma unroll
-            for (int r = 0; r < 4; r++) s[n][t][r] = s[n][t][r] != s[n][t][r] ? hi[r] : s[n][t][r];
-          }
       }
     const int kn = k0 + 128 < k_hi ? k0 + 128 : k0;  // (the last step loads its own slots again)
     const int pgn = k0 + 128 < k_hi ? pn : pg;
     load_k(kn, pgn);
     pn = page_of(kn + 128);
     const bool there = (unsigned)pg < (unsigned)a.n_pages;
-    const bool masked = k0 + 32 > it.held || k0 + 32 > k_hi || !there || careful;
-    uint32_t bits[NQ];  // which of the lane's eight slots each row sees
-    bool any_odd = false;  // values that are not finite, taken out of the product (masked steps)
-    if (masked) {
+    if (k0 + 32 > it.held || k0 + 32 > k_hi || !there) {
+      const int here = there ? min(max(k_hi - k0 - 8 * g, 0), 8) : 0;  // of the lane's eight slots
 #pragma unroll
       for (int n = 0; n < NQ; n++) {
-        bits[n] = 0;
         const int r = 16 * n + li;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const int key = k0 + 8 * g + e, nw = key - it.held;
-          bool v = there && key < k_hi && r < rows;
-          if (nw >= 0) v = v && (tree ? (nw < RTQ_KV_TREE && (sh.seen[r][(nw & (RTQ_KV_TREE - 1)) >> 5] >> (nw & 31) & 1)) : nw <= tok[n]);
-          bits[n] |= v ? 1u << e : 0u;
-        }
+        uint32_t bits = tree && tl.tail ? kv_tree_bits(k0 - it.held, sh.seen[tok[n] - tok0]) : kv_run_bits(k0 - it.held, tok[n]);
+        bits = bits >> (8 * g) & ((1u << here) - 1);
+        if (r >= rows) bits = 0;
 #pragma unroll
         for (int e = 0; e < 8; e++)
-          if (!(bits[n] >> e & 1)) s[n][e >> 2][e & 3] = -INFINITY;
+          if (!(bits >> e & 1)) s[n][e >> 2][e & 3] = -INFINITY;
       }
-      // slots that no row may see hold anything: zeros in their place, so that nothing x 0 is not NaN; a value of a
-      // new token that is not finite may be seen by some of the rows, and is added to those alone
+      // what lies behind the last token may be anything, NaN too: zeros, so that its weight 0 makes 0 of it
 #pragma unroll
       for (int t = 0; t < DT; t++)
-        if (FULL || 16 * t < d) {
-#pragma unroll
-          for (int w = 0; w < 4; w++) {
-            const int key = k0 + 8 * g + 2 * w;
-            uint32_t x = vf[t][w];
-            if (!there || key >= k_hi) x = 0;
-            else if (key + 1 >= k_hi) x &= 0xffffu;
-            uint32_t o = 0;
-            if ((x & EXP) == EXP) o |= 0xffffu;
-            if ((x >> 16 & EXP) == EXP) o |= 0xffff0000u;
-            vf[t][w] = x & ~o;
-            any_odd = any_odd || o;
-          }
-        }
-      any_odd = __any(any_odd);
+        if (FULL || 16 * t < d) vf[t] = kv_clear(vf[t], here);
     }
     u4v pf[NQ][NP];
-    float p[NQ][8];
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
-      float mx = s[n][0][0];
+      float mx = s[n][0][0], p[8];
 #pragma unroll
       for (int e = 1; e < 8; e++) mx = fmaxf(mx, s[n][e >> 2][e & 3]);
       mx = fmaxf(mx, __shfl_xor(mx, 16));
@@ -616,15 +687,15 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
       float sum = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        p[n][e] = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][e & 3], sc[n], UP - mu));
-        sum += p[n][e];
+        p[e] = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][e & 3], sc[n], kKvUp<CT> - mu));
+        sum += p[e];
       }
       l[n] = l[n] * al + sum;
       if (__any(al != 1.0f)) {
 #pragma unroll
         for (int t = 0; t < DT; t++) acc[n][t] *= al;
       }
-      kv_planes<CT, NP>(p[n], pf[n]);
+      kv_planes<CT, NP>(p, pf[n]);
     }
 #pragma unroll
     for (int t = 0; t < DT; t++)
@@ -633,54 +704,22 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
         for (int n = 0; n < NQ; n++)
 #pragma unroll
           for (int q = 0; q < NP; q++) acc[n][t] = kv_mfma<CT>(vf[t], pf[n][q], acc[n][t]);
-    if (masked && any_odd) {  // rare: those values are read again, one by one (sums and weights in LDS and the loops
-                              // rolled, so that this path costs the others no registers)
-#pragma unroll
-      for (int n = 0; n < NQ; n++) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) sh.w[wv][16 * n + li][8 * g + e] = bits[n] >> e & 1 ? p[n][e] : -1.0f;
-#pragma unroll
-        for (int t = 0; t < DT; t++) *reinterpret_cast<f4*>(&sh.o[wv][16 * n + li][16 * t + 4 * g]) = acc[n][t];
-      }
-      __builtin_amdgcn_wave_barrier();
-      const uint16_t* base = a.v + base_of(k0, pg) + (k0 & (ps - 1));
-#pragma unroll 1
-      for (int e = 0; e < 32 && k0 + e < k_hi; e++)
-#pragma unroll 1
-        for (int c = 4 * g; c < d; c += (c & 3) < 3 ? 1 : 13) {
-          const uint32_t x = base[((int64_t)c << a.ps_shift) + e];
-          if ((x & EXP) == EXP)
-#pragma unroll 1
-            for (int r = li; r < TM; r += 16)
-              if (sh.w[wv][r][e] != -1.0f) sh.o[wv][r][c] += sh.w[wv][r][e] * VRow<CT>::get(u4v{x, x, x, x}, 0);
-        }
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int n = 0; n < NQ; n++)
-#pragma unroll
-        for (int t = 0; t < DT; t++) acc[n][t] = *reinterpret_cast<const f4*>(&sh.o[wv][16 * n + li][16 * t + 4 * g]);
-    }
     load_v(kn, pgn);
     pg = pgn;
-  }
-  bool nan = false;
-#pragma unroll
-  for (int n = 0; n < NQ; n++) {
-    bool x = l[n] != l[n];
-#pragma unroll
-    for (int t = 0; t < DT; t++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) x = x || acc[n][t][r] != acc[n][t][r];
-    nan = nan || __any(x);
-  }
-  if (careful || !nan) break;
   }
   // the four waves' parts
 #pragma unroll
   for (int n = 0; n < NQ; n++) {
     l[n] += __shfl_xor(l[n], 16);
     l[n] += __shfl_xor(l[n], 32);
-    if (g == 0) sh.ml[wv][16 * n + li][0] = m[n], sh.ml[wv][16 * n + li][1] = l[n];
+    int nan = 0;
+#pragma unroll
+    for (int t = 0; t < DT; t++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) nan |= (FULL || 16 * t < d) && acc[n][t][r] != acc[n][t][r];
+    nan |= __shfl_xor(nan, 16);
+    nan |= __shfl_xor(nan, 32);
+    if (g == 0) sh.ml[wv][16 * n + li][0] = m[n], sh.ml[wv][16 * n + li][1] = nan ? NAN : l[n];
   }
   __syncthreads();
 #pragma unroll
@@ -705,7 +744,7 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
     f4 o = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < 4; w++) o += *reinterpret_cast<const f4*>(&sh.o[w][r][c]);
-    const bool dead = tree && tail && sh.dead[r];
+    const bool dead = tree && tl.tail && kv_dead(sh.seen[(row_lo + r) / group - tok0], (row_lo + r) / group);
     if (it.slot >= 0) {
       *reinterpret_cast<f4*>(a.part + ((int64_t)it.slot * TM + r) * D + c) = o;
       if (c == 0) a.ml[((int64_t)it.slot * TM + r) * 2] = mx, a.ml[((int64_t)it.slot * TM + r) * 2 + 1] = dead ? -1.0f : ls;
@@ -715,70 +754,458 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
       const float inv = 1.0f / ls;
 #pragma unroll
       for (int e = 0; e < 4; e++) Q::put(a.o, at + e, dead || ls == 0.0f ? 0.0f : o[e] * inv);
+      if (c == 0 && !dead && ls != ls) a.desc[8 + 8 * it.qid + 6] = 1;  // (after kv_describe: barriers lie between)
     }
   }
 }
 
-// joins the parts of a tile's row: workgroup (tile, row)
+// ---- large tiles: 32 rows a wave, 64 slots at a time through LDS for all of them
+//
+// The tile's keys and values reach LDS by buffer loads with the LDS destination, two buffers: the next 64 slots
+// are on their way while these are multiplied.  A unit is 32 slots (of one page): keys [slot][d / 8] and values
+// [d][4] of 16-byte chunks, a chunk's place swapped by the low bits of its row so that eight lanes' reads fall on
+// different banks; loads past a head's page (rows of a smaller head size, pages that are not there) give zeros.
+// MFMA 32x32x16, again S^T = K q^T and o^T = V^T p^T: key row m of a unit is slot 16 (m / 16) + 8 (m / 4 % 2) +
+// 4 (m / 8 % 2) + m % 4, so a lane's 16 scores are its operands of the second product in order.
+template <int CT, bool QF, int D, bool FULL, int NW, int R>
+__device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
+  constexpr int DK = D / 16, DT = D / 32, CH = D / 8, TM = 32 * NW, T = 64 * NW;
+  constexpr int NS = QF ? (CT == VT_F16 ? 2 : 3) : 1, NP = NS;
+  constexpr int UK = 32 * CH, UV = D * 4, UNIT = UK + UV;  // chunks
+  typedef VRow<QF ? VT_F32 : CT> Q;
+  struct Shared {
+    u4v st[R][2][UNIT];
+    KvSeen seen[TM];
+  };
+  __shared__ Shared sh;
+  KvItem it;
+  if (!kv_plan<TM>(a, blockIdx.x, it)) return;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q32 = lane & 31, h = lane >> 5;
+  const int group = a.nh / a.nkv, d = FULL ? D : a.d, ps = 1 << a.ps_shift;
+  const KvTile tl = kv_tile<TM>(a, it);
+  const int row_lo = tl.row_lo, rows = tl.rows, k_hi = tl.k_hi;
+  const bool tree = a.parents != nullptr;
+  kv_describe(a, it, tl);
+  const int row = 32 * wv + q32, rc = row_lo + min(row, rows - 1), tok = rc / group, tok0 = row_lo / group;
+  const bool busy = 32 * wv < rows;  // (waves without rows only help with the loads)
+
+  const int64_t head = (int64_t)d << a.ps_shift, pstride = head * a.nkv;
+  // this wave's loads of a unit: chunk places (i NW + wv) 64 + lane of the keys, then of the values
+  constexpr int LK = UK / T, LV = UV / T;
+  static_assert(UK % T == 0 && UV % T == 0, "whole loads");
+  uint32_t ko[LK], vo[LV];
+#pragma unroll
+  for (int i = 0; i < LK; i++) {
+    const int p = (i * NW + wv) * 64 + lane, slot = p / CH, c = (p % CH) ^ ((slot & 3) | (slot >> 1 & 4));
+    ko[i] = FULL || 8 * c < d ? (uint32_t)(slot * d + 8 * c) * 2 : 0x80000000u;
+  }
+#pragma unroll
+  for (int i = 0; i < LV; i++) {
+    const int p = (i * NW + wv) * 64 + lane, r = p / 4, c = (p % 4) ^ (r >> 1 & 3);
+    vo[i] = FULL || r < d ? (uint32_t)((r << a.ps_shift) + 8 * c) * 2 : 0x80000000u;
+  }
+  uint32_t ahead = 0;  // of the slots under way: bit u, unit u's page is not there
+  int page[2];         // of the slots to load next
+  const auto pages = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) page[u] = kv_page(a.s, it.seq, k0 + 32 * u, a.ps_shift);
+  };
+  const auto issue = [&](int buf, int k0) {
+    ahead = 0;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const int at = k0 + 32 * u, pg = page[u];
+      const bool there = (unsigned)pg < (unsigned)a.n_pages;
+      const int64_t base = (there ? pg : 0) * pstride + it.hv * head;
+      const uint32_t bytes = there ? (uint32_t)head * 2 : 0u, in = there ? (uint32_t)(at & (ps - 1)) : 0u;
+      ahead |= there ? 0u : 1u << u;
+      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.k + base), (short)0, bytes, 0x00020000);
+      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.v + base), (short)0, bytes, 0x00020000);
+      u4v* s = sh.st[buf][u];
+#pragma unroll
+      for (int i = 0; i < LK; i++)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, RTQ_LDSP(s + (i * NW + wv) * 64), 16, ko[i], in * (uint32_t)d * 2, 0, 0);
+#pragma unroll
+      for (int i = 0; i < LV; i++)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, RTQ_LDSP(s + UK + (i * NW + wv) * 64), 16, vo[i], in * 2, 0, 0);
+    }
+  };
+  pages(tl.k_lo);
+  if (tl.k_lo < k_hi) issue(0, tl.k_lo);
+  uint32_t missing[R];  // ahead of the slots in turn
+  missing[0] = ahead;
+  pages(tl.k_lo + 64);
+
+  constexpr bool SCALED = QF && CT == VT_F16;
+  u4v qf[NS][DK];
+  float sc = a.scale2;
+  {
+    const int64_t at = (int64_t)(it.row0 + tok) * a.ldq + (int64_t)(it.hv * group + rc % group) * d + 8 * h;
+    int up = 0;
+    if constexpr (SCALED) {
+      float mx = 0.0f;
+#pragma unroll
+      for (int c = 0; c < DK; c++)
+        if (FULL || 16 * c < d) {
+          const u4v r1 = Q::load(a.q, at + 16 * c), r2 = Q::load(a.q, at + 16 * c + 4);
+#pragma unroll
+          for (int e = 0; e < 4; e++) mx = fmaxf(mx, fmaxf(fabsf(Q::get(r1, e)), fabsf(Q::get(r2, e))));
+        }
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      up = kv_row_shift(mx);
+      sc = ldexpf(a.scale2, -up);
+    }
+#pragma unroll
+    for (int c = 0; c < DK; c++) {
+      if constexpr (QF) {
+        float x[8] = {};
+        if (FULL || 16 * c < d) {
+          const u4v r1 = Q::load(a.q, at + 16 * c), r2 = Q::load(a.q, at + 16 * c + 4);
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[e] = Q::get(r1, e), x[4 + e] = Q::get(r2, e);
+        }
+        if constexpr (SCALED)
+#pragma unroll
+          for (int e = 0; e < 8; e++) x[e] = ldexpf(x[e], up);
+        u4v pl[NS];
+        kv_planes<CT, NS>(x, pl);
+#pragma unroll
+        for (int i = 0; i < NS; i++) qf[i][c] = pl[i];
+      } else {
+        qf[0][c] = u4v{0, 0, 0, 0};
+        if (FULL || 16 * c < d) qf[0][c] = Q::load(a.q, at + 16 * c);
+      }
+    }
+  }
+  if (tree && tl.tail) kv_tree<TM, T>(a, it, tl, sh.seen, reinterpret_cast<uint16_t*>(sh.st[R - 1]));  // (not loaded into yet)
+
+  f16v acc[DT];
+  float m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int t = 0; t < DT; t++) acc[t] = f16v{};
+  // this lane's chunks: key row q32's slot, elements 16 c + 8 h; value row 32 t + q32, slots 16 s + 8 h
+  const int kslot = 16 * (q32 >> 4) + 8 * (q32 >> 2 & 1) + 4 * (q32 >> 3 & 1) + (q32 & 3), kx = (kslot & 3) | (kslot >> 1 & 4), vx = q32 >> 1 & 3;
+  if constexpr (R == 3) {
+    if (tl.k_lo + 64 < k_hi) issue(1, tl.k_lo + 64);
+    missing[1] = ahead;
+    pages(tl.k_lo + 128);
+  }
+  // (the waves of a SIMD take turns: one's softmax beside the other's products)
+  if (wv < 4) __builtin_amdgcn_s_setprio(1);
+  int buf = 0;
+  for (int k0 = tl.k_lo; k0 < k_hi; k0 += 64, buf = buf + 1 == R ? 0 : buf + 1) {
+    asm volatile("" ::: "memory");
+    if (R == 3 && k0 + 64 < k_hi) __builtin_amdgcn_s_waitcnt(vm_wait_imm(2 * (LK + LV)));
+    else __builtin_amdgcn_s_waitcnt(vm_wait_imm(0));
+    lds_barrier();  // these 64 slots have landed, and every wave is done with the buffer before them
+    asm volatile("" ::: "memory");
+    const uint32_t lost = missing[0];
+    constexpr int A = R - 1;
+    if (k0 + 64 * A < k_hi) issue(buf == 0 ? A : buf - 1, k0 + 64 * A);
+#pragma unroll
+    for (int i = 0; i + 1 < A; i++) missing[i] = missing[i + 1];
+    missing[A - 1] = ahead;
+    pages(k0 + 64 * A + 64);
+    if (!busy) continue;
+    const auto step = [&](auto some) {  // some: not every row sees all of the 64 slots
+      constexpr bool MASKED = decltype(some)::value;
+      f16v s[2];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const u4v* kt = sh.st[buf][u] + kslot * CH;
+        s[u] = f16v{};
+#pragma unroll
+        for (int c = 0; c < DK; c++) {
+          const u4v kf = kt[(2 * c + h) ^ kx];
+#pragma unroll
+          for (int p = 0; p < NS; p++) s[u] = kv_mfma32<CT>(kf, qf[p][c], s[u]);
+        }
+      }
+      const int here = min(k_hi - k0, 64);  // slots that hold tokens
+      if constexpr (MASKED) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const int nw = k0 + 32 * u - it.held, left = min(max(here - 32 * u, 0), 32);
+          uint32_t bits = tree && tl.tail ? kv_tree_bits(nw, sh.seen[tok - tok0]) : kv_run_bits(nw, tok);
+          if (left < 32) bits &= (1u << left) - 1;
+          if (lost >> u & 1) bits = 0;
+#pragma unroll
+          for (int e = 0; e < 16; e++)
+            if (!(bits >> (16 * (e >> 3) + (e & 7)) >> (8 * h) & 1)) s[u][e] = -INFINITY;
+        }
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int e = 1; e < 32; e++) mx = fmaxf(mx, s[e >> 4][e & 15]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float mn = fmaxf(m, mx * sc), mu = mn == -INFINITY ? 0.0f : mn;
+      if (__any(mn > m)) {
+        const float al = __builtin_amdgcn_exp2f(m - mu);
+        l *= al;
+#pragma unroll
+        for (int t = 0; t < DT; t++) acc[t] *= al;
+      }
+      m = mn;
+      const float off = kKvUp<CT> - mu;
+      u4v pf[4][NP];
+      float sum = 0.0f;
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          p[e] = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + e], sc, off));
+          sum += p[e];
+        }
+        kv_planes<CT, NP>(p, pf[g]);
+      }
+      l += sum;
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const u4v* vt = sh.st[buf][g >> 1] + UK + q32 * 4;
+#pragma unroll
+        for (int t = 0; t < DT; t++) {
+          u4v vf = vt[128 * t + ((2 * (g & 1) + h) ^ vx)];
+          if constexpr (MASKED) vf = kv_clear(vf, min(max(here - 16 * g - 8 * h, 0), 8));
+#pragma unroll
+          for (int p = 0; p < NP; p++) acc[t] = kv_mfma32<CT>(vf, pf[g][p], acc[t]);
+        }
+      }
+    };
+    if (k0 + 64 > it.held || k0 + 64 > k_hi || lost) step(std::true_type{});
+    else step(std::false_type{});
+  }
+  l += __shfl_xor(l, 32);
+  int nan = 0;
+#pragma unroll
+  for (int t = 0; t < DT; t++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) nan |= (FULL || 32 * t + 8 * (e >> 2) + 4 * h < d) && acc[t][e] != acc[t][e];
+  nan |= __shfl_xor(nan, 32);
+  if (nan) l = NAN;
+  __syncthreads();
+  if (row >= rows) return;
+  const bool dead = tree && tl.tail && kv_dead(sh.seen[tok - tok0], tok);
+  if (it.slot >= 0) {
+    float* out = a.part + ((int64_t)it.slot * TM + row) * D;
+#pragma unroll
+    for (int t = 0; t < DT; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        *reinterpret_cast<f4*>(out + 32 * t + 8 * i + 4 * h) = f4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
+    if (h == 0) a.ml[((int64_t)it.slot * TM + row) * 2] = m, a.ml[((int64_t)it.slot * TM + row) * 2 + 1] = dead ? -1.0f : l;
+    return;
+  }
+  const int64_t at = (int64_t)(it.row0 + tok) * a.ldo + (int64_t)(it.hv * group + rc % group) * d + 4 * h;
+  const float inv = dead || l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int t = 0; t < DT; t++)
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (FULL || 32 * t + 8 * i < d)
+#pragma unroll
+        for (int e = 0; e < 4; e++) Q::put(a.o, at + 32 * t + 8 * i + e, inv == 0.0f ? 0.0f : acc[t][4 * i + e] * inv);
+  if (h == 0 && !dead && l != l) a.desc[8 + 8 * it.qid + 6] = 1;  // (after kv_describe: barriers lie between)
+}
+
+// ---- joining
+// A row whose products met infinity or NaN, by the formula: in the matrix instructions a value that the row does not see
+// still meets its weight 0, and the lower planes of queries and weights, which may be 0 or of the other sign,
+// meet infinities.  Here only what is seen is multiplied, in 32 bits; slow, and rare.
+template <int QT>
+__device__ __forceinline__ void kv_row_again(const KvAttendArgs& a, int ct_bf16, const int32_t* q, int row, int64_t out) {
+  __shared__ float qs[256], sc[256], mx[256];
+  __shared__ uint32_t seen[RTQ_KV_TREE / 32];
+  __shared__ int dead;
+  const int tid = threadIdx.x, group = a.nh / a.nkv, tok = row / group, seq = q[7], hv = q[5], d = a.d;
+  const int held = kv_held(a.s.lens, seq, a.s.ldt, a.ps_shift);
+  const int last = (int)min((int64_t)held + tok + 1, min((int64_t)a.s.ldt << a.ps_shift, (int64_t)RTQ_KV_SLOTS));
+  __syncthreads();
+  if (tid < d) qs[tid] = VRow<QT>::one(a.q, (int64_t)(q[2] + tok) * a.ldq + (int64_t)(hv * group + row % group) * d + tid);
+  if (tid < RTQ_KV_TREE / 32) seen[tid] = 0;
+  if (tid == 0) dead = a.parents && tok >= RTQ_KV_TREE;
+  __syncthreads();
+  if (tid == 0 && a.parents)
+    for (int node = tok; node >= 0 && !dead;) {
+      seen[node >> 5] |= 1u << (node & 31);
+      const int p = a.parents[q[2] + node];
+      if (p < -1 || p >= node) dead = 1;
+      node = p;
+    }
+  __syncthreads();
+  const int64_t head = (int64_t)d << a.ps_shift;
+  const int ps = 1 << a.ps_shift;
+  const auto conv = [&](uint16_t x) { return ct_bf16 ? __builtin_bit_cast(float, (uint32_t)x << 16) : (float)__builtin_bit_cast(_Float16, x); };
+  const auto page = [&](int key) {
+    const int pg = a.s.table[(int64_t)seq * a.s.ldt + (key >> a.ps_shift)];
+    return (unsigned)pg < (unsigned)a.n_pages ? ((int64_t)pg * a.nkv + hv) * head : -1;
+  };
+  float m = -INFINITY, l = 0.0f, o = 0.0f;
+  for (int k0 = 0; k0 < last && !dead; k0 += 256) {
+    const int key = k0 + tid, nw = key - held;
+    float s = -INFINITY;
+    bool vis = key < last && (nw < 0 || !a.parents || (seen[(nw & (RTQ_KV_TREE - 1)) >> 5] >> (nw & 31) & 1));
+    if (vis) {
+      const int64_t at = page(key);
+      vis = at >= 0;
+      if (vis) {
+        const uint16_t* k = a.k + at + (int64_t)(key & (ps - 1)) * d;
+        s = 0.0f;
+        for (int c = 0; c < d; c++) s = fmaf(qs[c], conv(k[c]), s);
+        s *= a.scale2;
+      }
+    }
+    mx[tid] = s;
+    __syncthreads();
+    for (int n = 128; n > 0; n >>= 1) {
+      if (tid < n) mx[tid] = fmaxf(mx[tid], mx[tid + n]);
+      __syncthreads();
+    }
+    const float mn = fmaxf(m, mx[0]), mu = mn == -INFINITY ? 0.0f : mn, al = __builtin_amdgcn_exp2f(m - mu);
+    m = mn;
+    sc[tid] = vis ? __builtin_amdgcn_exp2f(s - mu) : -1.0f;
+    __syncthreads();
+    l *= al, o *= al;
+    for (int j = 0; j < 256; j++) {
+      const float p = sc[j];
+      if (p == -1.0f) continue;
+      l += p;
+      if (tid < d) o = fmaf(p, conv(a.v[page(k0 + j) + ((int64_t)tid << a.ps_shift) + ((k0 + j) & (ps - 1))]), o);
+    }
+    __syncthreads();
+  }
+  if (tid < d) VRow<QT>::put(a.o, out + tid, l == 0.0f ? 0.0f : o / l);
+}
+
+// joins the parts of a tile's rows: workgroup (tile, some of its rows)
 template <int QT, int D>
-__device__ __forceinline__ void kv_merge(const KvAttendArgs& a, int TM) {
+__device__ __forceinline__ void kv_merge(const KvAttendArgs& a) {
   constexpr int V = D / 4, G = 256 / V;
   __shared__ float red[256];
   __shared__ f4 ro[256];
   if ((int)blockIdx.x >= a.desc[0]) return;
   const int32_t* q = a.desc + 8 + 8 * blockIdx.x;
-  const int slot = q[0], ns = q[1], r = blockIdx.y;
-  if (slot < 0 || r >= q[4]) return;
-  const float* ml = a.ml + ((int64_t)slot * TM + r) * 2;
-  const int tid = threadIdx.x;
-  float mx = -INFINITY;
-  int dead = 0;
-  for (int i = tid; i < ns; i += 256) mx = fmaxf(mx, ml[(int64_t)i * TM * 2]), dead |= ml[(int64_t)i * TM * 2 + 1] == -1.0f;
-  red[tid] = mx;
-  dead = __syncthreads_or(dead);
-  for (int s = 128; s > 0; s >>= 1) {
-    if (tid < s) red[tid] = fmaxf(red[tid], red[tid + s]);
-    __syncthreads();
-  }
-  mx = red[0];
-  __syncthreads();
-  const int c = tid % V * 4, gr = tid / V;
-  float ls = 0.0f;
-  f4 o = f4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int i = gr; i < ns; i += G) {
-    const float f = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[(int64_t)i * TM * 2] - mx);
-    ls += f * ml[(int64_t)i * TM * 2 + 1];
-    if (c < a.d) o += f * *reinterpret_cast<const f4*>(a.part + ((int64_t)(slot + i) * TM + r) * D + c);
-  }
-  ro[tid] = o, red[tid] = ls;
-  __syncthreads();
-  if (gr == 0 && c < a.d) {
-    for (int i = 1; i < G; i++) o += ro[i * V + tid], ls += red[i * V + tid];
-    const int group = a.nh / a.nkv, row = q[3] + r;
-    const int64_t at = (int64_t)(q[2] + row / group) * a.ldo + (int64_t)(q[5] * group + row % group) * a.d + c;
-    const float inv = 1.0f / ls;
+  const int slot = q[0], ns = q[1], tid = threadIdx.x, TM = a.tm, group = a.nh / a.nkv;
+  if (slot < 0 && !q[6]) return;
+  if (slot >= 0 && ns <= 16) {  // few parts: a wave a row, two parts (of four, of one) at once
+    constexpr int VL = V < 64 ? V : 64, GW = 64 / VL;
+    const int lane = tid & 63, c = lane % VL * 4, gr = lane / VL;
+    for (int r = 4 * blockIdx.y + (tid >> 6); r < q[4]; r += 4 * gridDim.y) {
+      const float* ml = a.ml + ((int64_t)slot * TM + r) * 2;
+      const float mi = lane < ns ? ml[(int64_t)lane * TM * 2] : -INFINITY, li = lane < ns ? ml[(int64_t)lane * TM * 2 + 1] : 0.0f;
+      float mx = mi;
 #pragma unroll
-    for (int e = 0; e < 4; e++) VRow<QT>::put(a.o, at + e, dead || ls == 0.0f ? 0.0f : o[e] * inv);
+      for (int d = 1; d < 16; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
+      mx = __shfl(mx, 0);
+      const bool dead = __any(li == -1.0f);
+      if (!dead && __any(li != li)) continue;  // (below)
+      const float f = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - mx);
+      float ls = f * li;
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) ls += __shfl_xor(ls, d);
+      ls = __shfl(ls, 0);
+      f4 o = f4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int i = 0; i < ns; i += GW) {
+        const float fi = __shfl(f, min(i + gr, ns - 1));
+        if (i + gr < ns && c < a.d) o += fi * *reinterpret_cast<const f4*>(a.part + ((int64_t)(slot + i + gr) * TM + r) * D + c);
+      }
+#pragma unroll
+      for (int d = VL; d < 64; d <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] += __shfl_xor(o[e], d);
+      if (gr == 0 && c < a.d) {
+        const int row = q[3] + r;
+        const int64_t out = (int64_t)(q[2] + row / group) * a.ldo + (int64_t)(q[5] * group + row % group) * a.d + c;
+        const float inv = 1.0f / ls;
+#pragma unroll
+        for (int e = 0; e < 4; e++) VRow<QT>::put(a.o, out + e, dead || ls == 0.0f ? 0.0f : o[e] * inv);
+      }
+    }
+    // rows whose sums are not numbers
+    for (int r0 = 4 * blockIdx.y; r0 < q[4]; r0 += 4 * gridDim.y)
+      for (int r = r0; r < min(r0 + 4, q[4]); r++) {
+        const float* ml = a.ml + ((int64_t)slot * TM + r) * 2;
+        int odd = 0;
+        for (int i = 0; i < ns; i++) {
+          const float li = ml[(int64_t)i * TM * 2 + 1];
+          odd |= li == -1.0f ? 1 : li != li ? 2 : 0;
+        }
+        const int row = q[3] + r;
+        if (odd == 2)
+          kv_row_again<QT>(a, a.cache_bf16, q, row, (int64_t)(q[2] + row / group) * a.ldo + (int64_t)(q[5] * group + row % group) * a.d);
+      }
+    return;
+  }
+  for (int r = blockIdx.y; r < q[4]; r += gridDim.y) {
+    const int row = q[3] + r;
+    const int64_t out = (int64_t)(q[2] + row / group) * a.ldo + (int64_t)(q[5] * group + row % group) * a.d;
+    if (slot < 0) {  // (some row of the tile)
+      kv_row_again<QT>(a, a.cache_bf16, q, row, out);
+      continue;
+    }
+    const float* ml = a.ml + ((int64_t)slot * TM + r) * 2;
+    float mx = -INFINITY;
+    int odd = 0;  // 1: dead, 2: not a number
+    for (int i = tid; i < ns; i += 256) {
+      const float li = ml[(int64_t)i * TM * 2 + 1];
+      mx = fmaxf(mx, ml[(int64_t)i * TM * 2]), odd |= li == -1.0f ? 1 : li != li ? 2 : 0;
+    }
+    red[tid] = mx;
+    const int dead = __syncthreads_or(odd & 1), again = __syncthreads_or(odd & 2);
+    if (again && !dead) {
+      kv_row_again<QT>(a, a.cache_bf16, q, row, out);
+      __syncthreads();
+      continue;
+    }
+    for (int s = 128; s > 0; s >>= 1) {
+      if (tid < s) red[tid] = fmaxf(red[tid], red[tid + s]);
+      __syncthreads();
+    }
+    mx = red[0];
+    __syncthreads();
+    const int c = tid % V * 4, gr = tid / V;
+    float ls = 0.0f;
+    f4 o = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = gr; i < ns; i += G) {
+      const float f = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[(int64_t)i * TM * 2] - mx);
+      ls += f * ml[(int64_t)i * TM * 2 + 1];
+      if (c < a.d) o += f * *reinterpret_cast<const f4*>(a.part + ((int64_t)(slot + i) * TM + r) * D + c);
+    }
+    ro[tid] = o, red[tid] = ls;
+    __syncthreads();
+    if (gr == 0 && c < a.d) {
+      for (int i = 1; i < G; i++) o += ro[i * V + tid], ls += red[i * V + tid];
+      const float inv = 1.0f / ls;
+#pragma unroll
+      for (int e = 0; e < 4; e++) VRow<QT>::put(a.o, out + c + e, dead || ls == 0.0f ? 0.0f : o[e] * inv);
+    }
+    __syncthreads();
   }
 }
 
 #define RTQ_KV_ATTEND(SUF, CT, QF, D, FULL, NQ) \
   extern "C" __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void rtq_kv_attend##SUF(KvAttendArgs a) { kv_attend<CT, QF, D, FULL, NQ>(a); }
-#define RTQ_KV_ATTENDS(SUF, CT, QF)             \
+#define RTQ_KV_BIG(SUF, CT, QF, D, FULL, NW, R) \
+  extern "C" __global__ __launch_bounds__(64 * NW, NW / 4) void rtq_kv_attend##SUF(KvAttendArgs a) { kv_attend_big<CT, QF, D, FULL, NW, R>(a); }
+#define RTQ_KV_ATTENDS(SUF, CT, QF, NW)              \
   RTQ_KV_ATTEND(16_64_##SUF, CT, QF, 64, true, 1)    \
   RTQ_KV_ATTEND(16_128_##SUF, CT, QF, 128, true, 1)  \
   RTQ_KV_ATTEND(16_128p_##SUF, CT, QF, 128, false, 1) \
   RTQ_KV_ATTEND(16_256p_##SUF, CT, QF, 256, false, 1) \
   RTQ_KV_ATTEND(32_64_##SUF, CT, QF, 64, true, 2)    \
   RTQ_KV_ATTEND(32_128_##SUF, CT, QF, 128, true, 2)  \
-  RTQ_KV_ATTEND(32_128p_##SUF, CT, QF, 128, false, 2)
-RTQ_KV_ATTENDS(f32_f16, VT_F16, true)
-RTQ_KV_ATTENDS(f32_bf16, VT_BF16, true)
-RTQ_KV_ATTENDS(f16, VT_F16, false)
-RTQ_KV_ATTENDS(bf16, VT_BF16, false)
+  RTQ_KV_ATTEND(32_128p_##SUF, CT, QF, 128, false, 2) \
+  RTQ_KV_BIG(_big_64_##SUF, CT, QF, 64, true, 4, 3)    \
+  RTQ_KV_BIG(_big_128_##SUF, CT, QF, 128, true, NW, QF ? 2 : 3)  \
+  RTQ_KV_BIG(_big_128p_##SUF, CT, QF, 128, false, NW, QF ? 2 : 3) \
+  RTQ_KV_BIG(_big_256p_##SUF, CT, QF, 256, false, 4, 2)
+RTQ_KV_ATTENDS(f32_f16, VT_F16, true, 4)
+RTQ_KV_ATTENDS(f32_bf16, VT_BF16, true, 4)
+RTQ_KV_ATTENDS(f16, VT_F16, false, 8)
+RTQ_KV_ATTENDS(bf16, VT_BF16, false, 8)
 
 #define RTQ_KV_MERGE(NAME, QT, D) \
-  extern "C" __global__ __launch_bounds__(256) void NAME(KvAttendArgs a) { kv_merge<QT, D>(a, a.tm); }
+  extern "C" __global__ __launch_bounds__(256) void NAME(KvAttendArgs a) { kv_merge<QT, D>(a); }
 RTQ_KV_MERGE(rtq_kv_merge64_f32, VT_F32, 64)
 RTQ_KV_MERGE(rtq_kv_merge128_f32, VT_F32, 128)
 RTQ_KV_MERGE(rtq_kv_merge256_f32, VT_F32, 256)

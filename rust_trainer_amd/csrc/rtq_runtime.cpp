@@ -176,10 +176,10 @@ enum Kid {
   K_VERIFY_GREEDY = K_VERIFY_STATS + 3,
   K_VERIFY_MASS = K_VERIFY_GREEDY + 3,
   K_VERIFY_PICK = K_VERIFY_MASS + 3,
-  K_KV_APPEND = K_VERIFY_PICK + 3,  // + rows and cache (f32 f16, f32 bf16, f16, bf16)
-  K_KV_KEEP = K_KV_APPEND + 4,
-  K_KV_ATTEND,                            // + 7 x rows and cache + tile and head size (kv_variant)
-  K_KV_MERGE = K_KV_ATTEND + 28,          // + 3 x type + head size (64, 128, 256)
+  K_KV_APPEND = K_VERIFY_PICK + 3,  // + 2 x rows and cache (f32 f16, f32 bf16, f16, bf16) + heads above 128
+  K_KV_KEEP = K_KV_APPEND + 8,
+  K_KV_ATTEND,                    // + 11 x rows and cache + tile and head size (attend_plan)
+  K_KV_MERGE = K_KV_ATTEND + 44,  // + 3 x type + head size (64, 128, 256)
   K_ROWS = K_KV_MERGE + 9,  // + format
   K_MODEL = K_ROWS + F_COUNT,  // + RtqModelKernel: the decoder block (rtq_model.cpp)
   K_COUNT = K_MODEL + KM_COUNT
@@ -221,15 +221,20 @@ constexpr const char* kKernelNames[] = {
     "rtq_verify_greedy_f32", "rtq_verify_greedy_f16", "rtq_verify_greedy_bf16",
     "rtq_verify_mass_f32",  "rtq_verify_mass_f16",  "rtq_verify_mass_bf16",
     "rtq_verify_pick_f32",  "rtq_verify_pick_f16",  "rtq_verify_pick_bf16",
-    "rtq_kv_append_f32_f16", "rtq_kv_append_f32_bf16", "rtq_kv_append_f16", "rtq_kv_append_bf16", "rtq_kv_keep",
+    "rtq_kv_append_f32_f16", "rtq_kv_append_f32_f16_256", "rtq_kv_append_f32_bf16", "rtq_kv_append_f32_bf16_256",
+    "rtq_kv_append_f16", "rtq_kv_append_f16_256", "rtq_kv_append_bf16", "rtq_kv_append_bf16_256", "rtq_kv_keep",
     "rtq_kv_attend16_64_f32_f16", "rtq_kv_attend16_128_f32_f16", "rtq_kv_attend16_128p_f32_f16", "rtq_kv_attend16_256p_f32_f16",
     "rtq_kv_attend32_64_f32_f16", "rtq_kv_attend32_128_f32_f16", "rtq_kv_attend32_128p_f32_f16",
+    "rtq_kv_attend_big_64_f32_f16", "rtq_kv_attend_big_128_f32_f16", "rtq_kv_attend_big_128p_f32_f16", "rtq_kv_attend_big_256p_f32_f16",
     "rtq_kv_attend16_64_f32_bf16", "rtq_kv_attend16_128_f32_bf16", "rtq_kv_attend16_128p_f32_bf16", "rtq_kv_attend16_256p_f32_bf16",
     "rtq_kv_attend32_64_f32_bf16", "rtq_kv_attend32_128_f32_bf16", "rtq_kv_attend32_128p_f32_bf16",
+    "rtq_kv_attend_big_64_f32_bf16", "rtq_kv_attend_big_128_f32_bf16", "rtq_kv_attend_big_128p_f32_bf16", "rtq_kv_attend_big_256p_f32_bf16",
     "rtq_kv_attend16_64_f16", "rtq_kv_attend16_128_f16", "rtq_kv_attend16_128p_f16", "rtq_kv_attend16_256p_f16",
     "rtq_kv_attend32_64_f16", "rtq_kv_attend32_128_f16", "rtq_kv_attend32_128p_f16",
+    "rtq_kv_attend_big_64_f16", "rtq_kv_attend_big_128_f16", "rtq_kv_attend_big_128p_f16", "rtq_kv_attend_big_256p_f16",
     "rtq_kv_attend16_64_bf16", "rtq_kv_attend16_128_bf16", "rtq_kv_attend16_128p_bf16", "rtq_kv_attend16_256p_bf16",
     "rtq_kv_attend32_64_bf16", "rtq_kv_attend32_128_bf16", "rtq_kv_attend32_128p_bf16",
+    "rtq_kv_attend_big_64_bf16", "rtq_kv_attend_big_128_bf16", "rtq_kv_attend_big_128p_bf16", "rtq_kv_attend_big_256p_bf16",
     "rtq_kv_merge64_f32", "rtq_kv_merge128_f32", "rtq_kv_merge256_f32",
     "rtq_kv_merge64_f16", "rtq_kv_merge128_f16", "rtq_kv_merge256_f16",
     "rtq_kv_merge64_bf16", "rtq_kv_merge128_bf16", "rtq_kv_merge256_bf16",
@@ -2240,31 +2245,41 @@ rtq_status enqueue_append(rtq_kv_cache* kc, int64_t layer, const KvSeqs& s, int 
   a.q_norm = r.q_norm, a.k_norm = r.k_norm, a.eps = r.eps, a.off = r.offset;
   a.nh = (int)nh, a.nkv = (int)kc->nkv, a.d = (int)kc->d, a.rot = (int)r.dim, a.neox = r.neox;
   a.ps_shift = kc->ps_shift, a.n_pages = (int)kc->n_pages;
+  const double lb = std::log2((double)r.base);
   for (int64_t i = 0; i < r.dim / 2; i++) {
-    double f = std::pow((double)r.base, -2.0 * (double)i / (double)r.dim) * (double)r.freq_scale;
+    double f = std::exp2(-2.0 * (double)i / (double)r.dim * lb) * (double)r.freq_scale;
     if (i < r.n_factors && r.factors[i] != 0.0f) f /= (double)r.factors[i];
     a.freq[i] = f / 6.283185307179586476925;
   }
-  a.vt = (int)(cdiv(s.n, 32) * kc->nkv);
-  return launch(kc->ctx, K_KV_APPEND + kv_types(kc, type), dim3((unsigned)(s.n + a.vt)), dim3(256), st, a);
+  // a token a wave once that fills every CU's waves twice over
+  a.wave_tokens = s.n >= 8 * kc->ctx->cu_count;
+  a.tw = a.wave_tokens ? (int)cdiv(s.n, 4) : s.n;
+  const int64_t vt = cdiv(s.n, 32) * kc->nkv;
+  return launch(kc->ctx, K_KV_APPEND + 2 * kv_types(kc, type) + (kc->d > 128 ? 1 : 0), dim3((unsigned)(a.tw + vt)), dim3(256), st, a);
 }
 
 // The attention's tiles and partial parts.  Rows of a sequence and KV head average n group / b: tiles of 16 up to
-// that, else of 32 (whose registers a head size above 128 has not).  `target` items keep every CU's resident workgroups
-// busy; the split tiles' items are at most twice that (each but a tile's last covers C keys).
+// that, of 32 (whose registers a head size above 128 has not), else large ones.  `target` items keep every
+// CU's resident workgroups busy; the split tiles' items are at most twice that (each but a tile's last covers C keys).
 struct AttendPlan {
-  int tm, variant, dk;
+  int tm, threads, variant, dk;
   int64_t target, qids;
   size_t bytes;
 };
-AttendPlan attend_plan(const rtq_kv_cache* kc, int64_t n, int64_t b, int64_t nh) {
+AttendPlan attend_plan(const rtq_kv_cache* kc, int type, int64_t n, int64_t b, int64_t nh) {
   AttendPlan p{};
   const int64_t d = kc->d, rows = n * (nh / kc->nkv);
-  p.tm = d <= 128 && rows > 16 * b ? 32 : 16;
   const int size = d == 64 ? 0 : d == 128 ? 1 : d < 128 ? 2 : 3;
   p.dk = d == 64 ? 0 : d <= 128 ? 1 : 2;
-  p.variant = (p.tm == 32 ? 4 : 0) + size;
-  p.target = (int64_t)kc->ctx->cu_count * 2;
+  if (rows <= 16 * b) {
+    p.tm = 16, p.variant = size;
+  } else if (rows <= 32 * b && d <= 128) {
+    p.tm = 32, p.variant = 4 + size;
+  } else {
+    p.tm = (size == 1 || size == 2) && type != RTQ_TYPE_F32 ? 256 : 128, p.variant = 7 + size;
+  }
+  p.threads = p.tm > 32 ? 2 * p.tm : 256;
+  p.target = (int64_t)kc->ctx->cu_count * (p.tm > 32 ? 1 : 2);
   p.qids = (cdiv(rows, p.tm) + b) * kc->nkv;
   const int64_t D = 64 << p.dk;
   p.bytes = (size_t)(2 * p.target * p.tm * (D + 2) * 4 + (8 + 8 * p.qids) * 4) + 4 * 256;
@@ -2289,14 +2304,14 @@ rtq_status enqueue_attend(rtq_kv_cache* kc, int64_t layer, const KvSeqs& s, int 
   a.q = q, a.o = out, a.ldq = ldq, a.ldo = ldo, a.parents = parents;
   a.nh = (int)nh, a.nkv = (int)kc->nkv, a.d = (int)kc->d, a.ps_shift = kc->ps_shift, a.n_pages = (int)kc->n_pages;
   a.scale2 = (float)((scale > 0.0f ? (double)scale : 1.0 / std::sqrt((double)kc->d)) * 1.4426950408889634);
-  a.target = (int)p.target, a.slots = (int)(2 * p.target), a.qids = (int)p.qids, a.tm = p.tm;
+  a.target = (int)p.target, a.slots = (int)(2 * p.target), a.qids = (int)p.qids, a.tm = p.tm, a.cache_bf16 = kc->type == RTQ_TYPE_BF16;
   const int64_t D = 64 << p.dk;
-  a.part = ar.take<float>((size_t)(a.slots * p.tm * D));
-  a.ml = ar.take<float>((size_t)(a.slots * p.tm * 2));
+  a.part = ar.take<float>((size_t)(2 * p.target * p.tm * D));
+  a.ml = ar.take<float>((size_t)(2 * p.target * p.tm * 2));
   a.desc = ar.take<int32_t>((size_t)(8 + 8 * p.qids));
   if (ar.off > ar.cap) return fail(RTQ_ERR_INVALID, "internal: workspace too small");
-  RTQ_TRY(launch(kc->ctx, K_KV_ATTEND + 7 * kv_types(kc, type) + p.variant, dim3((unsigned)(p.target + p.qids)), dim3(256), st, a));
-  return launch(kc->ctx, K_KV_MERGE + 3 * logit_type(type) + p.dk, dim3((unsigned)p.qids, (unsigned)p.tm), dim3(256), st, a);
+  RTQ_TRY(launch(kc->ctx, K_KV_ATTEND + 11 * kv_types(kc, type) + p.variant, dim3((unsigned)(p.target + p.qids)), dim3((unsigned)p.threads), st, a));
+  return launch(kc->ctx, K_KV_MERGE + 3 * logit_type(type) + p.dk, dim3((unsigned)p.qids, (unsigned)std::min(p.tm, 16)), dim3(256), st, a);
 }
 
 rtq_status kv_check_keep(const rtq_kv_cache* kc, const rtq_kv_seqs* s, const int32_t* kept, int64_t ldk, const int32_t* after) {
@@ -2309,7 +2324,7 @@ rtq_status kv_check_keep(const rtq_kv_cache* kc, const rtq_kv_seqs* s, const int
 
 rtq_status enqueue_keep(rtq_kv_cache* kc, const KvSeqs& s, const int32_t* kept, int64_t ldk, int32_t* after, hipStream_t st) {
   KvKeepArgs a{s.lens, s.table, kept, after, s.b, s.ldt, (int)ldk, (int)kc->nkv, (int)kc->d, kc->ps_shift, (int)kc->n_pages, kc->k, kc->v, kc->layer};
-  return launch(kc->ctx, K_KV_KEEP, dim3((unsigned)(s.b * kc->nkv), (unsigned)kc->n_layer), dim3(320), st, a);
+  return launch(kc->ctx, K_KV_KEEP, dim3((unsigned)(s.b * kc->nkv), (unsigned)kc->n_layer), dim3(256), st, a);
 }
 
 }  // namespace
@@ -2397,7 +2412,7 @@ rtq_status rtq_kv_attend_d(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s
   std::lock_guard<std::mutex> lk(c->mu);
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = (hipStream_t)stream;
-  const AttendPlan p = attend_plan(kc, n, s->b, nh);
+  const AttendPlan p = attend_plan(kc, type, n, s->b, nh);
   RTQ_TRY(row_ws(c, p.bytes, st));
   Arena ar{(char*)c->ws, c->ws_bytes, 0};
   return enqueue_attend(kc, layer, kv_seqs(*s, n), type, nh, scale, parents, q, ldq, out, ldo, p, ar, st);
@@ -2970,7 +2985,7 @@ rtq_status rtq_kv_attend(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s, 
   HostCall hc(c);
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = c->stream;
-  const AttendPlan p = attend_plan(kc, n, s->b, nh);
+  const AttendPlan p = attend_plan(kc, type, n, s->b, nh);
   const int64_t es = logit_bytes(type), qw = nh * kc->d;
   RTQ_TRY(ensure_ws(c, p.bytes + (size_t)(n * qw * es + n * 4) + kv_seq_bytes(*s) + 4 * 256));
   Arena ar{(char*)c->ws, c->ws_bytes, 0};

@@ -83,9 +83,18 @@ def visible(m, parents=None):
     return seen, alive
 
 
-def attend(q, k, v, held, heads, parents=None, scale=0.0):
+def one_plane(xt, n, b, heads, kv, d):
+    """The half step by which the weights of a call are rounded: large tiles (calls of more than 32 rows a sequence and KV
+    head, of 16 where a head is larger than 128) of 16-bit rows hold each weight in one number of that type; the others'
+    planes are counted with the scores' below."""
+    large = n * (heads // kv) > (32 if d <= 128 else 16) * b
+    return EPS[xt] if large and xt != "f32" else 0.0
+
+
+def attend(q, k, v, held, heads, parents=None, scale=0.0, weights=0.0):
     """(out, bound): attention of one sequence in 64 bits, and what rounding may make of it in the kernels' 32.
-    q [m x heads d], k and v [slots x kv x d]."""
+    q [m x heads d], k and v [slots x kv x d]; weights: what each weight may be off by (``one_plane``): the weights' sum is
+    of the unrounded ones, so a row's error is at most that share of its weighted values' sizes."""
     m, kv, d = q.shape[0], k.shape[1], k.shape[2]
     scale = float(np.float32(scale)) or 1.0 / np.sqrt(d)
     seen, alive = visible(m, parents)
@@ -109,7 +118,7 @@ def attend(q, k, v, held, heads, parents=None, scale=0.0):
         es = (np.abs(qh) @ kabs.T * d * 2.0 ** -24 + np.abs(qh).max(1, keepdims=True) * kabs.sum(1) * 2.0 ** -22) * scale
         size = np.where(vis, np.abs(np.where(vis, s, 0.0)), 0.0).max(1, keepdims=True)
         e = (es * vis).max(1, keepdims=True) + 2.0 ** -22 * size
-        bound[:, h] = (2 * e + 2.0 ** -21 + (k.shape[0] / 32 + 64) * 2.0 ** -24) * (p @ np.abs(fin))
+        bound[:, h] = (2 * e + 2.0 ** -21 + (k.shape[0] / 32 + 64) * 2.0 ** -24 + weights) * (p @ np.abs(fin))
     return out.reshape(m, -1), bound.reshape(m, -1)
 
 

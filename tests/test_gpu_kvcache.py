@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import rust_trainer_amd as rt
-from kv_cases import EPS, TINY, TYPES, Layout, attend, norm, rotate, to_type, tree, value, visible
+from kv_cases import EPS, TINY, TYPES, Layout, attend, norm, one_plane, rotate, to_type, tree, value, visible
 from rust_trainer_amd.kvcache import KvCache, Rope, Seqs, rope_d, seqs_d
 
 torch = pytest.importorskip("torch")
@@ -186,13 +186,14 @@ ATTEND = [  # lens, counts, heads, kv, d, page, tree, gap, off
 ]
 
 
-def check_attend(pg, lay, got, q, xt, heads, parents, scale=0.0, width=None):
+def check_attend(pg, lay, got, q, xt, heads, parents, scale=0.0):
+    weights = one_plane(xt, q.shape[0], lay.b, heads, pg.kv, pg.d)
     for i in range(lay.b):
         a, z = lay.starts[i], lay.starts[i + 1]
         if a == z:
             continue
         k, v = pg.rows(i)
-        want, bound = attend(value(q[a:z], xt), k, v, int(lay.lens[i]), heads, None if parents is None else parents[a:z], scale)
+        want, bound = attend(value(q[a:z], xt), k, v, int(lay.lens[i]), heads, None if parents is None else parents[a:z], scale, weights)
         err = np.abs(value(got[a:z], xt) - want)
         lim = bound + EPS[xt] * (np.abs(want) + bound) + TINY[xt]
         assert np.all(err <= lim), (i, (err / lim).max())
@@ -251,7 +252,8 @@ def test_what_is_not_seen_does_not_matter(ctx, xt, ct):
             hit = seen[:, bad[i]].any(1)
             assert not np.isfinite(got[a:a + m][hit]).all(1).any(), "a row that sees NaN is NaN"
             k, v = pg.rows(i)
-            want, bound = attend(value(q[a:a + m], xt), k, v, lens[i], heads, None if par is None else par[a:a + m])
+            want, bound = attend(value(q[a:a + m], xt), k, v, lens[i], heads, None if par is None else par[a:a + m],
+                                 weights=one_plane(xt, lay.n, 3, heads, kv, d))
             err = np.abs(got[a:a + m] - want)[~hit]
             assert np.all(err <= (bound + EPS[xt] * (np.abs(want) + bound) + TINY[xt])[~hit])
 
@@ -424,7 +426,7 @@ def test_offsets_past_32_bits(ctx):
     assert torch.equal(v[n_pages - 2, :, :, :16].cpu(), torch.from_numpy(rows[8][::-1][24:].reshape(16, kv, d).transpose(1, 2, 0).copy()))
     kk = np.concatenate((held[0], rows[8].reshape(40, kv, d))).astype(np.float64)
     vv = np.concatenate((held[1], rows[8][::-1].reshape(40, kv, d))).astype(np.float64)
-    want, bound = attend(rows[16].astype(np.float64), kk, vv, 1000, 16)
+    want, bound = attend(rows[16].astype(np.float64), kk, vv, 1000, 16, weights=one_plane("f16", 40, 1, 16, 8, 128))
     assert np.all(np.abs(got - want) <= bound + EPS["f16"] * (np.abs(want) + bound) + TINY["f16"])
     cache.close()
 
@@ -501,7 +503,7 @@ def test_drafting_with_a_tree(ctx, xt, ct):
                 allk = np.array([t[layer][0] for t in tokens[i]] + [t[layer][0] for t in new[i]])
                 allv = np.array([t[layer][1] for t in tokens[i]] + [t[layer][1] for t in new[i]])
                 qq = rotate(value(q[a:a + m], xt).reshape(m, heads, d), at, d, 1e4, False).reshape(m, -1)
-                want, bound = attend(qq, allk, allv, int(lens[i]), heads, None if parents is None else parents[i])
+                want, bound = attend(qq, allk, allv, int(lens[i]), heads, None if parents is None else parents[i], weights=one_plane(xt, n, b, heads, kv, d))
                 # the keys and queries that the cache's call rounds (and, once in a thousand, to the other side of a
                 # border than these) leave the scores within 2 half steps of both: weights and rows within that
                 qmax = np.abs(qq.reshape(m, heads, d)).sum(2).max()
