@@ -419,6 +419,7 @@ __device__ __forceinline__ f16v kv_mfma32(u4v x, u4v y, f16v c) {
   else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, x), __builtin_bit_cast(bf8, y), c, 0, 0, 0);
 }
 
+typedef float f8v __attribute__((ext_vector_type(8)));
 // eight floats as N planes of 16 bits, each the rounding of what the ones before it leave: 11 (f16) or 8
 // (bf16) bits of the value a plane: f32 rows take two (f16) or three, one plane of a 16-bit row is the row itself.
 template <int CT, int N>
@@ -428,7 +429,9 @@ __device__ __forceinline__ void kv_planes(const float* v, u4v* out) {
   for (int e = 0; e < 8; e++) r[e] = v[e];
 #pragma unroll
   for (int n = 0; n < N; n++) {
-    out[n] = VRow<CT>::pack(r);
+    const f8v x = {r[0], r[1], r[2], r[3], r[4], r[5], r[6], r[7]};  // (converted in pairs)
+    if constexpr (CT == VT_F16) out[n] = __builtin_bit_cast(u4v, __builtin_convertvector(x, half8));
+    else out[n] = __builtin_bit_cast(u4v, __builtin_convertvector(x, bf8));
     if (n + 1 < N)
 #pragma unroll
       for (int e = 0; e < 8; e++) r[e] -= VRow<CT>::get(out[n], e);
@@ -444,9 +447,12 @@ __device__ __forceinline__ int kv_page(const KvSeqs& s, int seq, int k, int ps_s
 
 #define RTQ_KV_TREE 1024  // most new tokens of a sequence that is a tree
 
-// f16 weights are taken times 2^15 (as is their sum): small ones, of which a long context has many, keep their bits
+// f16 weights are taken times 2^9 (as is their sum): small ones, of which a long context has many, keep their bits.
+// Large tiles follow a row's maximum only once it has risen by kKvLag (a factor 2^6 of the weights, which f16 still
+// holds): with the maxima of 32 rows some rises in most steps, and each rise costs a product per accumulator.
 template <int CT>
-constexpr float kKvUp = CT == VT_F16 ? 15.0f : 0.0f;
+constexpr float kKvUp = CT == VT_F16 ? 9.0f : 0.0f;
+constexpr float kKvLag = 6.0f;
 
 // What an item works on, beside the plan's: its rows and slots
 struct KvTile {
@@ -761,12 +767,20 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
 
 // ---- large tiles: 32 rows a wave, 64 slots at a time through LDS for all of them
 //
-// The tile's keys and values reach LDS by buffer loads with the LDS destination, two buffers: the next 64 slots
-// are on their way while these are multiplied.  A unit is 32 slots (of one page): keys [slot][d / 8] and values
-// [d][4] of 16-byte chunks, a chunk's place swapped by the low bits of its row so that eight lanes' reads fall on
-// different banks; loads past a head's page (rows of a smaller head size, pages that are not there) give zeros.
+// The tile's keys and values reach LDS by buffer loads with the LDS destination, into a ring of R buffers: the next
+// 64 or 128 slots are on their way while these are multiplied.  A unit is 32 slots (of one page): keys [slot][d / 8] and
+// values [d][4] of 16-byte chunks, a chunk's place swapped by its row so that 16 lanes' reads fall on different
+// banks (64 of 4 bytes); loads past a head's page (rows of a smaller head size, pages that are not there) give zeros.
 // MFMA 32x32x16, again S^T = K q^T and o^T = V^T p^T: key row m of a unit is slot 16 (m / 16) + 8 (m / 4 % 2) +
 // 4 (m / 8 % 2) + m % 4, so a lane's 16 scores are its operands of the second product in order.
+// the key rows of lanes 0 .. 15 (and 16 .. 31), by their slots, get 16 places of a row of 16 chunks or more, or eight of each
+// of two neighbouring rows
+template <int CH>
+__device__ __forceinline__ int kv_swap(int slot) {
+  const int row = (slot & 3) | (slot >> 1 & 4) | (slot << 1 & 8);  // the MFMA row of the slot, modulo 16
+  return CH >= 16 ? row : row >> 1;
+}
+
 template <int CT, bool QF, int D, bool FULL, int NW, int R>
 __device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
   constexpr int DK = D / 16, DT = D / 32, CH = D / 8, TM = 32 * NW, T = 64 * NW;
@@ -796,12 +810,12 @@ __device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
   uint32_t ko[LK], vo[LV];
 #pragma unroll
   for (int i = 0; i < LK; i++) {
-    const int p = (i * NW + wv) * 64 + lane, slot = p / CH, c = (p % CH) ^ ((slot & 3) | (slot >> 1 & 4));
+    const int p = (i * NW + wv) * 64 + lane, slot = p / CH, c = (p % CH) ^ kv_swap<CH>(slot);
     ko[i] = FULL || 8 * c < d ? (uint32_t)(slot * d + 8 * c) * 2 : 0x80000000u;
   }
 #pragma unroll
   for (int i = 0; i < LV; i++) {
-    const int p = (i * NW + wv) * 64 + lane, r = p / 4, c = (p % 4) ^ (r >> 1 & 3);
+    const int p = (i * NW + wv) * 64 + lane, r = p / 4, c = (p % 4) ^ (r >> 2 & 3);
     vo[i] = FULL || r < d ? (uint32_t)((r << a.ps_shift) + 8 * c) * 2 : 0x80000000u;
   }
   uint32_t ahead = 0;  // of the slots under way: bit u, unit u's page is not there
@@ -884,7 +898,7 @@ __device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
 #pragma unroll
   for (int t = 0; t < DT; t++) acc[t] = f16v{};
   // this lane's chunks: key row q32's slot, elements 16 c + 8 h; value row 32 t + q32, slots 16 s + 8 h
-  const int kslot = 16 * (q32 >> 4) + 8 * (q32 >> 2 & 1) + 4 * (q32 >> 3 & 1) + (q32 & 3), kx = (kslot & 3) | (kslot >> 1 & 4), vx = q32 >> 1 & 3;
+  const int kslot = 16 * (q32 >> 4) + 8 * (q32 >> 2 & 1) + 4 * (q32 >> 3 & 1) + (q32 & 3), kx = kv_swap<CH>(kslot), vx = q32 >> 2 & 3;
   if constexpr (R == 3) {
     if (tl.k_lo + 64 < k_hi) issue(1, tl.k_lo + 64);
     missing[1] = ahead;
@@ -892,88 +906,96 @@ __device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
   }
   // (the waves of a SIMD take turns: one's softmax beside the other's products)
   if (wv < 4) __builtin_amdgcn_s_setprio(1);
-  int buf = 0;
-  for (int k0 = tl.k_lo; k0 < k_hi; k0 += 64, buf = buf + 1 == R ? 0 : buf + 1) {
+  int buf = 0, k0 = tl.k_lo;
+  uint32_t lost = 0;
+  const auto advance = [&] {
     asm volatile("" ::: "memory");
     if (R == 3 && k0 + 64 < k_hi) __builtin_amdgcn_s_waitcnt(vm_wait_imm(2 * (LK + LV)));
     else __builtin_amdgcn_s_waitcnt(vm_wait_imm(0));
     lds_barrier();  // these 64 slots have landed, and every wave is done with the buffer before them
     asm volatile("" ::: "memory");
-    const uint32_t lost = missing[0];
+    lost = missing[0];
     constexpr int A = R - 1;
     if (k0 + 64 * A < k_hi) issue(buf == 0 ? A : buf - 1, k0 + 64 * A);
 #pragma unroll
     for (int i = 0; i + 1 < A; i++) missing[i] = missing[i + 1];
     missing[A - 1] = ahead;
     pages(k0 + 64 * A + 64);
-    if (!busy) continue;
-    const auto step = [&](auto some) {  // some: not every row sees all of the 64 slots
-      constexpr bool MASKED = decltype(some)::value;
-      f16v s[2];
+  };
+  const auto step = [&](auto some) {  // some: not every row sees all of the 64 slots
+    constexpr bool MASKED = decltype(some)::value;
+    f16v s[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const u4v* kt = sh.st[buf][u] + kslot * CH;
+      s[u] = f16v{};
+#pragma unroll
+      for (int c = 0; c < DK; c++) {
+        const u4v kf = kt[(2 * c + h) ^ kx];
+#pragma unroll
+        for (int p = 0; p < NS; p++) s[u] = kv_mfma32<CT>(kf, qf[p][c], s[u]);
+      }
+    }
+    const int here = min(k_hi - k0, 64);  // slots that hold tokens
+    if constexpr (MASKED) {
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        const u4v* kt = sh.st[buf][u] + kslot * CH;
-        s[u] = f16v{};
+        const int nw = k0 + 32 * u - it.held, left = min(max(here - 32 * u, 0), 32);
+        uint32_t bits = tree && tl.tail ? kv_tree_bits(nw, sh.seen[tok - tok0]) : kv_run_bits(nw, tok);
+        if (left < 32) bits &= (1u << left) - 1;
+        if (lost >> u & 1) bits = 0;
 #pragma unroll
-        for (int c = 0; c < DK; c++) {
-          const u4v kf = kt[(2 * c + h) ^ kx];
-#pragma unroll
-          for (int p = 0; p < NS; p++) s[u] = kv_mfma32<CT>(kf, qf[p][c], s[u]);
-        }
+        for (int e = 0; e < 16; e++)
+          if (!(bits >> (16 * (e >> 3) + (e & 7)) >> (8 * h) & 1)) s[u][e] = -INFINITY;
       }
-      const int here = min(k_hi - k0, 64);  // slots that hold tokens
-      if constexpr (MASKED) {
+    }
+    float mx = s[0][0];
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-          const int nw = k0 + 32 * u - it.held, left = min(max(here - 32 * u, 0), 32);
-          uint32_t bits = tree && tl.tail ? kv_tree_bits(nw, sh.seen[tok - tok0]) : kv_run_bits(nw, tok);
-          if (left < 32) bits &= (1u << left) - 1;
-          if (lost >> u & 1) bits = 0;
+    for (int e = 1; e < 32; e++) mx = fmaxf(mx, s[e >> 4][e & 15]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const float mn = fmaxf(m, mx * sc);
+    if (__any(mn > m + kKvLag)) {
+      const float al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+      l *= al;
 #pragma unroll
-          for (int e = 0; e < 16; e++)
-            if (!(bits >> (16 * (e >> 3) + (e & 7)) >> (8 * h) & 1)) s[u][e] = -INFINITY;
-        }
-      }
-      float mx = s[0][0];
-#pragma unroll
-      for (int e = 1; e < 32; e++) mx = fmaxf(mx, s[e >> 4][e & 15]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      const float mn = fmaxf(m, mx * sc), mu = mn == -INFINITY ? 0.0f : mn;
-      if (__any(mn > m)) {
-        const float al = __builtin_amdgcn_exp2f(m - mu);
-        l *= al;
-#pragma unroll
-        for (int t = 0; t < DT; t++) acc[t] *= al;
-      }
+      for (int t = 0; t < DT; t++) acc[t] *= al;
       m = mn;
-      const float off = kKvUp<CT> - mu;
-      u4v pf[4][NP];
-      float sum = 0.0f;
+    }
+    const float off = kKvUp<CT> - (m == -INFINITY ? 0.0f : m);
+    u4v pf[4][NP];
+    float sum = 0.0f;
 #pragma unroll
-      for (int g = 0; g < 4; g++) {
-        float p[8];
+    for (int g = 0; g < 4; g++) {
+      float p[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          p[e] = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + e], sc, off));
-          sum += p[e];
-        }
-        kv_planes<CT, NP>(p, pf[g]);
+      for (int e = 0; e < 8; e++) {
+        p[e] = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + e], sc, off));
+        sum += p[e];
       }
-      l += sum;
+      kv_planes<CT, NP>(p, pf[g]);
+    }
+    l += sum;
 #pragma unroll
-      for (int g = 0; g < 4; g++) {
-        const u4v* vt = sh.st[buf][g >> 1] + UK + q32 * 4;
+    for (int g = 0; g < 4; g++) {
+      const u4v* vt = sh.st[buf][g >> 1] + UK + q32 * 4;
 #pragma unroll
-        for (int t = 0; t < DT; t++) {
-          u4v vf = vt[128 * t + ((2 * (g & 1) + h) ^ vx)];
-          if constexpr (MASKED) vf = kv_clear(vf, min(max(here - 16 * g - 8 * h, 0), 8));
+      for (int t = 0; t < DT; t++) {
+        u4v vf = vt[128 * t + ((2 * (g & 1) + h) ^ vx)];
+        if constexpr (MASKED) vf = kv_clear(vf, min(max(here - 16 * g - 8 * h, 0), 8));
 #pragma unroll
-          for (int p = 0; p < NP; p++) acc[t] = kv_mfma32<CT>(vf, pf[g][p], acc[t]);
-        }
+        for (int p = 0; p < NP; p++) acc[t] = kv_mfma32<CT>(vf, pf[g][p], acc[t]);
       }
-    };
-    if (k0 + 64 > it.held || k0 + 64 > k_hi || lost) step(std::true_type{});
-    else step(std::false_type{});
+    }
+  };
+  // the slots that every row sees whole, then the others (and what lies behind a page that is not there)
+  const int plain = min(tree ? it.held : it.held + tok0 + 1, k_hi);
+  for (; k0 + 64 <= plain && !missing[0]; k0 += 64, buf = buf + 1 == R ? 0 : buf + 1) {
+    advance();
+    if (busy) step(std::false_type{});
+  }
+  for (; k0 < k_hi; k0 += 64, buf = buf + 1 == R ? 0 : buf + 1) {
+    advance();
+    if (busy) step(std::true_type{});
   }
   l += __shfl_xor(l, 32);
   int nan = 0;
