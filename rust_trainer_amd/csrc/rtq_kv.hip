@@ -905,7 +905,7 @@ __device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
     pages(tl.k_lo + 128);
   }
   // (the waves of a SIMD take turns: one's softmax beside the other's products)
-  if (wv < 4) __builtin_amdgcn_s_setprio(1);
+  if (CT == VT_BF16 && wv < 4) __builtin_amdgcn_s_setprio(1);
   int buf = 0, k0 = tl.k_lo;
   uint32_t lost = 0;
   const auto advance = [&] {
@@ -1208,7 +1208,7 @@ __device__ __forceinline__ void kv_merge(const KvAttendArgs& a) {
 #define RTQ_KV_ATTEND(SUF, CT, QF, D, FULL, NQ) \
   extern "C" __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void rtq_kv_attend##SUF(KvAttendArgs a) { kv_attend<CT, QF, D, FULL, NQ>(a); }
 #define RTQ_KV_BIG(SUF, CT, QF, D, FULL, NW, R) \
-  extern "C" __global__ __launch_bounds__(64 * NW, NW / 4) void rtq_kv_attend##SUF(KvAttendArgs a) { kv_attend_big<CT, QF, D, FULL, NW, R>(a); }
+  extern "C" __global__ __launch_bounds__(64 * NW, 2) void rtq_kv_attend##SUF(KvAttendArgs a) { kv_attend_big<CT, QF, D, FULL, NW, R>(a); }
 #define RTQ_KV_ATTENDS(SUF, CT, QF, NW)              \
   RTQ_KV_ATTEND(16_64_##SUF, CT, QF, 64, true, 1)    \
   RTQ_KV_ATTEND(16_128_##SUF, CT, QF, 128, true, 1)  \
@@ -1218,13 +1218,13 @@ __device__ __forceinline__ void kv_merge(const KvAttendArgs& a) {
   RTQ_KV_ATTEND(32_128_##SUF, CT, QF, 128, true, 2)  \
   RTQ_KV_ATTEND(32_128p_##SUF, CT, QF, 128, false, 2) \
   RTQ_KV_BIG(_big_64_##SUF, CT, QF, 64, true, 4, 3)    \
-  RTQ_KV_BIG(_big_128_##SUF, CT, QF, 128, true, NW, QF ? 2 : 3)  \
-  RTQ_KV_BIG(_big_128p_##SUF, CT, QF, 128, false, NW, QF ? 2 : 3) \
+  RTQ_KV_BIG(_big_128_##SUF, CT, QF, 128, true, NW, NW == 4 ? 2 : 3)  \
+  RTQ_KV_BIG(_big_128p_##SUF, CT, QF, 128, false, NW, NW == 4 ? 2 : 3) \
   RTQ_KV_BIG(_big_256p_##SUF, CT, QF, 256, false, 4, 2)
 RTQ_KV_ATTENDS(f32_f16, VT_F16, true, 4)
 RTQ_KV_ATTENDS(f32_bf16, VT_BF16, true, 4)
-RTQ_KV_ATTENDS(f16, VT_F16, false, 8)
-RTQ_KV_ATTENDS(bf16, VT_BF16, false, 8)
+RTQ_KV_ATTENDS(f16, VT_F16, false, 4)
+RTQ_KV_ATTENDS(bf16, VT_BF16, false, 4)
 
 #define RTQ_KV_MERGE(NAME, QT, D) \
   extern "C" __global__ __launch_bounds__(256) void NAME(KvAttendArgs a) { kv_merge<QT, D>(a); }

@@ -2276,10 +2276,10 @@ AttendPlan attend_plan(const rtq_kv_cache* kc, int type, int64_t n, int64_t b, i
   } else if (rows <= 32 * b && d <= 128) {
     p.tm = 32, p.variant = 4 + size;
   } else {
-    p.tm = (size == 1 || size == 2) && type != RTQ_TYPE_F32 ? 256 : 128, p.variant = 7 + size;
+    p.tm = 128, p.variant = 7 + size;
   }
   p.threads = p.tm > 32 ? 2 * p.tm : 256;
-  p.target = (int64_t)kc->ctx->cu_count * (p.tm > 32 ? 1 : 2);
+  p.target = (int64_t)kc->ctx->cu_count * 2;
   p.qids = (cdiv(rows, p.tm) + b) * kc->nkv;
   const int64_t D = 64 << p.dk;
   p.bytes = (size_t)(2 * p.target * p.tm * (D + 2) * 4 + (8 + 8 * p.qids) * 4) + 4 * 256;
