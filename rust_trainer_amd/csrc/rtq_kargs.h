@@ -636,6 +636,7 @@ struct MMaskArgs {
 
 // ---- paged cache of keys and values (rtq_kv.hip)
 #define RTQ_KV_ROT 256  // most rotated elements of a head
+#define RTQ_KV_TARGET 4096  // most items that an attention call is split for
 // the sequences of a call: new tokens are rows starts[i] .. starts[i + 1] - 1 (null: n / b each)
 struct KvSeqs {
   const int32_t* lens;    // [b] tokens held before the call
@@ -666,13 +667,11 @@ struct KvAttendArgs {
   int nh, nkv, d, ps_shift, n_pages;
   float scale2;     // scale log2(e)
   int target;       // items that the keys are split into (at most this many, and one per tile beside)
-  int slots, qids;  // partial slots; query tiles (x KV heads) that the plan may name
-  int tm;           // rows of a tile
-  int cache_bf16;
+  int slots;        // partial slots
+  int tm, D;        // rows of a tile, elements of a part's row
+  int fused;        // split tiles are joined by their last workgroup, not by a kernel behind it
   float* part;      // [slots][rows of a tile][D]
-  float* ml;        // [slots][rows of a tile][2]: maximum, sum
-  int32_t* desc;    // [0] query tiles named; from [8] on 8 each: first slot (-1: none), splits, the sequence's first row,
-                    // the tile's first row, its rows, KV head, some row is NaN (tiles without slots), sequence
+  float* ml;        // [slots][rows of a tile][2]: maximum, sum (-1: the row sees nothing, NaN: to be done again)
 };
 struct KvKeepArgs {
   const int32_t *lens, *table, *kept;

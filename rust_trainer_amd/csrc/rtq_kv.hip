@@ -322,8 +322,12 @@ extern "C" __global__ __launch_bounds__(256) void rtq_kv_keep(KvKeepArgs a) {
 // key row m of tile t is slot 8 (m / 4) + 4 t + m % 4, and the lane that gets the scores of slots 8 g .. 8 g + 7
 // holds them in the order in which it feeds them to the second product: the weights never leave their lane.
 struct KvItem {
-  int seq, row0, cnt, held, total, tile, hv, split, splits, slot, qid, C;
+  int seq, row0, cnt, held, total, tile, hv, split, splits, slot, C;  // slot: of the tile's first part (-1: one part)
 };
+// workgroups of a split tile that have left their part, at half the tile's first slot (a tile has two or more); zero
+// between launches: the last one clears it
+constexpr int kKvCounters = RTQ_KV_TARGET;  // (slots are twice the items)
+__device__ int kv_arrived[kKvCounters];
 
 // inclusive sums over the wave's lanes (DPP: rows of 16, then across them)
 __device__ __forceinline__ int kv_wave_scan(int v) {
@@ -349,62 +353,65 @@ __device__ __forceinline__ float kv_wave_total(float v) {
 }
 
 // item `block` of the plan (every wave finds it by itself; a lane looks after b / 64 sequences); false: none.
-// Sequences that overlap in `starts` can name more than the host counted: then nothing is joined.
-template <int TM>
-__device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, int block, KvItem& it) {
+// A tile that is joined by its last workgroup has at most kKvJoin / rows parts, one joined by a kernel of its own at most
+// kKvJoin.  Sequences that overlap in `starts` can name more than the host counted: then whole tiles are left out.
+constexpr int kKvJoin = 1024;
+__device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, int TM, int block, KvItem& it) {
   const int lane = threadIdx.x & 63, group = a.nh / a.nkv;
-  const int per = (a.s.b + 63) / 64, i0 = lane * per, i1 = min(i0 + per, a.s.b);
-  const auto look = [&](int i, int& row0, int& cnt, int& held, int& total, int& tiles) {
+  const int per = (a.s.b + 63) / 64, i0 = min(lane * per, a.s.b), i1 = min(i0 + per, a.s.b);
+  int row0 = 0, cnt = 0, held = 0, total = 0, tiles = 0;
+  const auto look = [&](int i) {
     row0 = kv_start(a.s, i);
     cnt = max(kv_start(a.s, i + 1) - row0, 0);
     held = kv_held(a.s.lens, i, a.s.ldt, a.ps_shift);
     total = (int)min((int64_t)held + cnt, min((int64_t)a.s.ldt << a.ps_shift, (int64_t)RTQ_KV_SLOTS));
     tiles = (int)(((int64_t)cnt * group + TM - 1) / TM);
   };
-  int row0, cnt, held, total, tiles;
   float w = 0.0f;
   for (int i = i0; i < i1; i++) {
-    look(i, row0, cnt, held, total, tiles);
+    look(i);
     w += (float)tiles * (float)total;
   }
   w = kv_wave_total(w);
-  const int C = (int)fminf(ceilf(w * (float)a.nkv / (float)a.target / 128.0f), (float)(RTQ_KV_SLOTS / 128)) * 128;
-  it.C = max(C, 128);
-  int items = 0, slots = 0, qids = 0;
+  const int C = max((int)fminf(ceilf(w * (float)a.nkv / (float)a.target / 128.0f), (float)(RTQ_KV_SLOTS / 128)) * 128, 128);
+  // a sequence's slots a part, parts
+  const auto cut = [&](int& c, int& ns) {
+    const int most = a.fused ? kKvJoin / min(max(cnt, 1) * group, TM) : kKvJoin;
+    c = max(C, ((total + most - 1) / most + 127) & ~127);
+    ns = max((total + c - 1) / c, 1);
+  };
+  int items = 0, slots = 0, c, ns;
   for (int i = i0; i < i1; i++) {
-    look(i, row0, cnt, held, total, tiles);
-    const int ns = max((total + it.C - 1) / it.C, 1), n = tiles * a.nkv;
-    items += n * ns, qids += n, slots += ns > 1 ? n * ns : 0;
+    if (per > 1) look(i);
+    cut(c, ns);
+    items += tiles * a.nkv * ns, slots += ns > 1 ? tiles * a.nkv * ns : 0;
   }
-  int ei = kv_wave_scan(items), es = kv_wave_scan(slots), eq = kv_wave_scan(qids);
-  if (block == 0 && threadIdx.x == 63) a.desc[0] = eq <= a.qids && es <= a.slots && ei <= (int)gridDim.x ? eq : 0;
-  ei -= items, es -= slots, eq -= qids;
+  int ei = kv_wave_scan(items) - items, es = kv_wave_scan(slots) - slots;
   const uint64_t mine = __ballot(block >= ei && block < ei + items);
   if (!mine) return false;
   int ok = 0;
   if (block >= ei && block < ei + items) {
     for (int i = i0; i < i1; i++) {
-      look(i, row0, cnt, held, total, tiles);
-      const int ns = max((total + it.C - 1) / it.C, 1), n = tiles * a.nkv;
-      if (block < ei + n * ns) {
+      if (per > 1) look(i);
+      cut(c, ns);
+      const int n = tiles * a.nkv * ns;
+      if (block < ei + n) {
         const int at = block - ei;  // tile by tile, so that a range's tiles are a multiple of the XCDs apart
-        it.seq = i, it.row0 = row0, it.cnt = cnt, it.held = held, it.total = total, it.splits = ns;
+        it.seq = i, it.row0 = row0, it.cnt = cnt, it.held = held, it.total = total, it.splits = ns, it.C = c;
         it.tile = at / (a.nkv * ns), it.hv = at / ns % a.nkv, it.split = at % ns;
-        it.qid = eq + it.tile * a.nkv + it.hv;
-        it.slot = ns > 1 ? es + at : -1;
-        ok = 1;
+        it.slot = ns > 1 ? es + at - it.split : -1;
+        ok = ns == 1 || (it.slot + ns <= a.slots && block - it.split + ns <= (int)gridDim.x);
         break;
       }
-      ei += n * ns, eq += n, es += ns > 1 ? n * ns : 0;
+      ei += n, es += ns > 1 ? n : 0;
     }
   }
   const int src = __ffsll((unsigned long long)mine) - 1;
 #define RTQ_KV_GIVE(F) it.F = __builtin_amdgcn_readlane(it.F, src)
   RTQ_KV_GIVE(seq), RTQ_KV_GIVE(row0), RTQ_KV_GIVE(cnt), RTQ_KV_GIVE(held), RTQ_KV_GIVE(total), RTQ_KV_GIVE(tile);
-  RTQ_KV_GIVE(hv), RTQ_KV_GIVE(split), RTQ_KV_GIVE(splits), RTQ_KV_GIVE(slot), RTQ_KV_GIVE(qid);
+  RTQ_KV_GIVE(hv), RTQ_KV_GIVE(split), RTQ_KV_GIVE(splits), RTQ_KV_GIVE(slot), RTQ_KV_GIVE(C);
 #undef RTQ_KV_GIVE
-  ok = __builtin_amdgcn_readlane(ok, src);
-  return ok && (unsigned)it.qid < (unsigned)a.qids && it.slot < a.slots;
+  return __builtin_amdgcn_readlane(ok, src);
 }
 
 template <int CT>
@@ -459,8 +466,7 @@ struct KvTile {
   int row_lo, rows, k_lo, k_hi;
   bool tail;  // some of its slots hold new tokens
 };
-template <int TM>
-__device__ __forceinline__ KvTile kv_tile(const KvAttendArgs& a, const KvItem& it) {
+__device__ __forceinline__ KvTile kv_tile(const KvAttendArgs& a, int TM, const KvItem& it) {
   KvTile t;
   const int group = a.nh / a.nkv;
   t.row_lo = it.tile * TM, t.rows = min((int)((int64_t)it.cnt * group - t.row_lo), TM);
@@ -517,19 +523,226 @@ __device__ __forceinline__ u4v kv_clear(u4v x, int n) {
   return x;
 }
 
-// a tile's entry in the plan that the joining kernel reads
-__device__ __forceinline__ void kv_describe(const KvAttendArgs& a, const KvItem& it, const KvTile& t) {
-  if (it.split == 0 && threadIdx.x == 0) {
-    int32_t* q = a.desc + 8 + 8 * it.qid;
-    q[0] = it.slot, q[1] = it.splits, q[2] = it.row0, q[3] = t.row_lo, q[4] = t.rows, q[5] = it.hv, q[6] = 0, q[7] = it.seq;
-  }
-}
-
 // f32 rows over an f16 cache are scaled by a power of two (whose exponent is returned) that brings the row's
 // largest element, of which the caller has mx, to [2^13, 2^14): its planes then neither overflow nor lose bits
 __device__ __forceinline__ int kv_row_shift(float mx) {
   const int ex = (int)(__builtin_bit_cast(uint32_t, mx) >> 23);
   return ex == 255 || ex == 0 ? 0 : min(max(140 - ex, -120), 120);
+}
+
+// ---- the end of an item
+// A row whose products met infinity or NaN, by the formula: in the matrix instructions a value that the row does not see
+// still meets its weight 0, and the lower planes of queries and weights, which may be 0 or of the other sign,
+// meet infinities.  Here only what is seen is multiplied, in 32 bits; slow, and rare.
+// (A row is read again as its call was given it: out may be q itself, whose rows no other workgroup writes.)
+struct KvAgain {
+  float qs[256], sc[256], mx[256];
+  uint32_t seen[RTQ_KV_TREE / 32];
+  int dead;
+};
+template <int QT, int CT>
+__device__ __forceinline__ void kv_row_again(const KvAttendArgs& a, const KvItem& it, int row, KvAgain& sh) {
+  float *qs = sh.qs, *sc = sh.sc, *mx = sh.mx;
+  uint32_t* seen = sh.seen;
+  int& dead = sh.dead;
+  const int tid = threadIdx.x, group = a.nh / a.nkv, tok = row / group, seq = it.seq, hv = it.hv, d = a.d, held = it.held;
+  const int last = min(held + tok + 1, it.total);
+  __syncthreads();
+  if (tid < d) qs[tid] = VRow<QT>::one(a.q, (int64_t)(it.row0 + tok) * a.ldq + (int64_t)(hv * group + row % group) * d + tid);
+  if (tid < RTQ_KV_TREE / 32) seen[tid] = 0;
+  if (tid == 0) dead = a.parents && tok >= RTQ_KV_TREE;
+  __syncthreads();
+  if (tid == 0 && a.parents)
+    for (int node = tok; node >= 0 && !dead;) {
+      seen[node >> 5] |= 1u << (node & 31);
+      const int p = a.parents[it.row0 + node];
+      if (p < -1 || p >= node) dead = 1;
+      node = p;
+    }
+  __syncthreads();
+  const int64_t head = (int64_t)d << a.ps_shift;
+  const int ps = 1 << a.ps_shift;
+  const auto conv = [&](uint16_t x) { return VRow<CT>::get(u4v{x, x, x, x}, 0); };
+  const auto page = [&](int key) {
+    const int pg = a.s.table[(int64_t)seq * a.s.ldt + (key >> a.ps_shift)];
+    return (unsigned)pg < (unsigned)a.n_pages ? ((int64_t)pg * a.nkv + hv) * head : -1;
+  };
+  float m = -INFINITY, l = 0.0f, o = 0.0f;
+  for (int k0 = 0; k0 < last && !dead; k0 += 256) {
+    const int key = k0 + tid, nw = key - held;
+    float s = -INFINITY;
+    bool vis = key < last && (nw < 0 || !a.parents || (seen[(nw & (RTQ_KV_TREE - 1)) >> 5] >> (nw & 31) & 1));
+    if (vis) {
+      const int64_t at = page(key);
+      vis = at >= 0;
+      if (vis) {
+        const uint16_t* k = a.k + at + (int64_t)(key & (ps - 1)) * d;
+        s = 0.0f;
+        for (int c = 0; c < d; c++) s = fmaf(qs[c], conv(k[c]), s);
+        s *= a.scale2;
+      }
+    }
+    mx[tid] = s;
+    __syncthreads();
+    for (int n = 128; n > 0; n >>= 1) {
+      if (tid < n) mx[tid] = fmaxf(mx[tid], mx[tid + n]);
+      __syncthreads();
+    }
+    const float mn = fmaxf(m, mx[0]), mu = mn == -INFINITY ? 0.0f : mn, al = __builtin_amdgcn_exp2f(m - mu);
+    m = mn;
+    sc[tid] = vis ? __builtin_amdgcn_exp2f(s - mu) : -1.0f;
+    __syncthreads();
+    l *= al, o *= al;
+    for (int j = 0; j < 256; j++) {
+      const float p = sc[j];
+      if (p == -1.0f) continue;
+      l += p;
+      if (tid < d) o = fmaf(p, conv(a.v[page(k0 + j) + ((int64_t)tid << a.ps_shift) + ((k0 + j) & (ps - 1))]), o);
+    }
+    __syncthreads();
+  }
+  if (tid < d)
+    VRow<QT>::put(a.o, (int64_t)(it.row0 + tok) * a.ldo + (int64_t)(hv * group + row % group) * d + tid, l == 0.0f ? 0.0f : o / l);
+}
+
+
+union KvEnd {
+  struct {
+    float m[kKvJoin], w[kKvJoin];  // [row][part]: maxima, sums; then weights
+    f4 o[256];
+    int odd;
+  } j;
+  KvAgain again;
+};
+// a part's values: through to memory where another workgroup of the launch reads them (through: kv_end)
+__device__ __forceinline__ void kv_part_put(bool through, float* p, float x, float y) {
+  const float2 v = {x, y};
+  if (through) __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  else *reinterpret_cast<float2*>(p) = v;
+}
+__device__ __forceinline__ void kv_part_put(bool through, float* p, f4 v) {
+  if (through) kv_part_put(true, p, v[0], v[1]), kv_part_put(true, p + 2, v[2], v[3]);
+  else *reinterpret_cast<f4*>(p) = v;
+}
+
+// Joins the parts of a tile's rows first, first + step, ... (with 256 threads): what counts is how many loads are under way.
+template <int QT, int CT>
+__device__ __forceinline__ void kv_join(const KvAttendArgs& a, const KvItem& it, const KvTile& t, int TM, int D, int from, int step, KvEnd& sh) {
+  const int tid = threadIdx.x, lane = tid & 63, group = a.nh / a.nkv, ns = it.splits, V = D / 4, G = 256 / V;
+  const int rows = (t.rows - from + step - 1) / step;
+  if (rows <= 0) return;
+  __syncthreads();
+  if (tid == 0) sh.j.odd = 0;
+  // the parts' weights: every maximum and sum at once, then a thread a row of few parts or a wave a row of many
+  for (int i = tid; i < rows * ns; i += 256) {
+    const float* ml = a.ml + ((int64_t)(it.slot + i % ns) * TM + from + i / ns * step) * 2;
+    sh.j.m[i] = ml[0], sh.j.w[i] = ml[1];
+  }
+  __syncthreads();
+  const bool few = ns <= 8;
+  const int part0 = few ? 0 : lane, parts = few ? 1 : 64;
+  for (int r = few ? tid : tid >> 6; r < rows; r += few ? 256 : 4) {
+    float *m = sh.j.m + r * ns, *w = sh.j.w + r * ns;
+    float mx = -INFINITY, ls = 0.0f;
+    int dead = 0;
+    for (int i = part0; i < ns; i += parts) mx = fmaxf(mx, m[i]), dead |= w[i] == -1.0f;
+    if (!few) {
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d)), dead |= __shfl_xor(dead, d);
+    }
+    for (int i = part0; i < ns; i += parts) {
+      const float f = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[i] - mx);
+      ls += f * w[i];
+      m[i] = f;
+    }
+    if (!few) {
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) ls += __shfl_xor(ls, d);
+    }
+    const bool bad = !dead && ls != ls;  // not a number: done again below
+    if (bad) sh.j.odd = 1;
+    const float inv = dead || ls == 0.0f ? 0.0f : 1.0f / ls;
+    for (int i = part0; i < ns; i += parts) w[i] = bad ? NAN : m[i] * inv;
+  }
+  __syncthreads();
+  // then a thread four elements of a row; of few rows some threads share a row's parts
+  int share = 1;
+  while (2 * share * rows <= G) share *= 2;
+  const int c = tid % V * 4, gr = tid / V, first = gr % share;
+  for (int r0 = 0; r0 < rows; r0 += G / share) {
+    const int r = r0 + gr / share;
+    const float* w = sh.j.w + min(r, rows - 1) * ns;
+    f4 o = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (r < rows && c < a.d) {
+      const float* x0 = a.part + ((int64_t)it.slot * TM + from + r * step) * D + c;
+      for (int i = first; i < ns; i += 16 * share) {
+        f4 x[16];
+#pragma unroll
+        for (int u = 0; u < 16; u++) {
+          x[u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+          if (i + u * share < ns) x[u] = *reinterpret_cast<const f4*>(x0 + (int64_t)(i + u * share) * TM * D);
+        }
+#pragma unroll
+        for (int u = 0; u < 16; u++)
+          if (i + u * share < ns && w[i + u * share] != 0.0f) o += w[i + u * share] * x[u];
+      }
+    }
+    if (share > 1) {
+      __syncthreads();
+      sh.j.o[tid] = o;
+      __syncthreads();
+      if (first == 0)
+        for (int i = 1; i < share; i++) o += sh.j.o[tid + i * V];
+    }
+    if (first == 0 && r < rows && c < a.d && w[0] == w[0]) {
+      const int row = t.row_lo + from + r * step;
+      const int64_t out = (int64_t)(it.row0 + row / group) * a.ldo + (int64_t)(it.hv * group + row % group) * a.d + c;
+#pragma unroll
+      for (int e = 0; e < 4; e++) VRow<QT>::put(a.o, out + e, o[e]);
+    }
+  }
+  if (!sh.j.odd) return;
+  for (int r = from; r < t.rows; r += step) {
+    const float* ml = a.ml + ((int64_t)it.slot * TM + r) * 2;
+    int mark = 0;
+    for (int i = 0; i < ns; i++) {
+      const float li = ml[(int64_t)i * TM * 2 + 1];
+      mark |= li == -1.0f ? 1 : li != li ? 2 : 0;
+    }
+    if (mark == 2) kv_row_again<QT, CT>(a, it, t.row_lo + r, sh.again);
+  }
+}
+
+// After a workgroup's item (of 256 threads): nan[r] marks rows of a tile of one part that are to be done again; a part of
+// a split tile is counted, and the last joins the parts.  sh: the workgroup's shared memory, free by now.
+template <int QT, int CT, int D, int TM>
+__device__ __forceinline__ void kv_end(const KvAttendArgs& a, const KvItem& it, const KvTile& t, const int* nan, int* last, KvEnd& sh) {
+  const int tid = threadIdx.x;
+  if (it.slot < 0) {
+    __syncthreads();
+    uint32_t any = 0;
+    for (int r = tid & 63; r < t.rows; r += 64) any |= nan[r];
+    if (!__any(any)) return;
+    for (int r = 0; r < t.rows; r++)
+      if (nan[r]) kv_row_again<QT, CT>(a, it, t.row_lo + r, sh.again);
+    return;
+  }
+  if (!a.fused) return;
+  // The part's stores go through to memory (kv_part_put): once a wave has none under way they are there for every XCD, and
+  // the part may be counted.  (Ordinary stores and a release would write back all that the XCD's L2 holds, in every
+  // workgroup: 30 us of a call of 512.)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  int* count = kv_arrived + (it.slot >> 1);
+  if (tid == 0) {
+    const int n = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (n == it.splits - 1) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *last = n == it.splits - 1;
+  }
+  __syncthreads();
+  if (!*last) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  kv_join<QT, CT>(a, it, t, TM, D, 0, 1, sh);
 }
 
 // ---- small tiles: 16 or 32 rows, four waves that share the tile's slots, operands straight from the cache
@@ -538,25 +751,59 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
   constexpr int DC = D / 32, DT = D / 16, TM = 16 * NQ, LDR = D + 4;
   constexpr int NS = QF ? (CT == VT_F16 ? 2 : 3) : 1, NP = QF ? NS : 2;
   typedef VRow<QF ? VT_F32 : CT> Q;
-  struct Shared {
+  struct Main {
     float o[4][TM][LDR];
     float ml[4][TM][2];
     KvSeen seen[TM];
     uint16_t up[RTQ_KV_TREE];
   };
-  __shared__ Shared sh;
+  union Shared {
+    Main m;
+    KvEnd end;
+  };
+  __shared__ Shared all;
+  __shared__ int nan_row[TM], is_last;
+  Main& sh = all.m;
   KvItem it;
-  if (!kv_plan<TM>(a, blockIdx.x, it)) return;
+  if (!kv_plan(a, TM, blockIdx.x, it)) return;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, g = lane >> 4;
   const int group = a.nh / a.nkv, d = FULL ? D : a.d, ps = 1 << a.ps_shift;
-  const KvTile tl = kv_tile<TM>(a, it);
+  const KvTile tl = kv_tile(a, TM, it);
   const int row_lo = tl.row_lo, rows = tl.rows, k_hi = tl.k_hi;
   const bool tree = a.parents != nullptr;
-  kv_describe(a, it, tl);
   // the token (index among the sequence's new ones) of each of this lane's columns
   int tok[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; n++) tok[n] = (row_lo + min(16 * n + li, rows - 1)) / group;
+  const int64_t head = (int64_t)d << a.ps_shift, pstride = head * a.nkv;
+  const auto page_of = [&](int k0) { return kv_page(a.s, it.seq, k0, a.ps_shift); };
+  const auto base_of = [&](int pg) { return ((unsigned)pg < (unsigned)a.n_pages ? pg : 0) * pstride + it.hv * head; };
+  u4v kf[2][DC], vf[DT];
+  const uint32_t k_at = (uint32_t)((8 * (li >> 2) + (li & 3)) * d + 8 * g) * 2, v_at = (uint32_t)((li << a.ps_shift) + 8 * g) * 2;
+  const auto load_k = [&](int k0, int pg) {
+    const char* base = reinterpret_cast<const char*>(a.k + base_of(pg) + (int64_t)(k0 & (ps - 1)) * d);
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int c = 0; c < DC; c++) {
+        kf[t][c] = u4v{0, 0, 0, 0};
+        if (FULL || 32 * c + 8 * g < d) kf[t][c] = *reinterpret_cast<const u4v*>(base + k_at + (4 * t * d + 32 * c) * 2);
+      }
+  };
+  const auto load_v = [&](int k0, int pg) {
+    const char* base = reinterpret_cast<const char*>(a.v + base_of(pg) + (k0 & (ps - 1)));
+#pragma unroll
+    for (int t = 0; t < DT; t++)
+      if (FULL || 16 * t < d) vf[t] = *reinterpret_cast<const u4v*>(base + ((int64_t)(32 * t) << a.ps_shift) + v_at);
+  };
+  int k0 = tl.k_lo + 32 * wv;
+  int pg = 0, pn = 0;
+  if (k0 < k_hi) {
+    pg = page_of(k0);
+    pn = page_of(k0 + 128);
+    load_k(k0, pg);
+    load_v(k0, pg);
+  }
   constexpr bool SCALED = QF && CT == VT_F16;
   u4v qf[NS][NQ][DC];
   float sc[NQ];
@@ -615,35 +862,6 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
     m[n] = -INFINITY, l[n] = 0.0f;
 #pragma unroll
     for (int t = 0; t < DT; t++) acc[n][t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  const int64_t head = (int64_t)d << a.ps_shift, pstride = head * a.nkv;
-  const auto page_of = [&](int k0) { return kv_page(a.s, it.seq, k0, a.ps_shift); };
-  const auto base_of = [&](int pg) { return ((unsigned)pg < (unsigned)a.n_pages ? pg : 0) * pstride + it.hv * head; };
-  u4v kf[2][DC], vf[DT];
-  const uint32_t k_at = (uint32_t)((8 * (li >> 2) + (li & 3)) * d + 8 * g) * 2, v_at = (uint32_t)((li << a.ps_shift) + 8 * g) * 2;
-  const auto load_k = [&](int k0, int pg) {
-    const char* base = reinterpret_cast<const char*>(a.k + base_of(pg) + (int64_t)(k0 & (ps - 1)) * d);
-#pragma unroll
-    for (int t = 0; t < 2; t++)
-#pragma unroll
-      for (int c = 0; c < DC; c++) {
-        kf[t][c] = u4v{0, 0, 0, 0};
-        if (FULL || 32 * c + 8 * g < d) kf[t][c] = *reinterpret_cast<const u4v*>(base + k_at + (4 * t * d + 32 * c) * 2);
-      }
-  };
-  const auto load_v = [&](int k0, int pg) {
-    const char* base = reinterpret_cast<const char*>(a.v + base_of(pg) + (k0 & (ps - 1)));
-#pragma unroll
-    for (int t = 0; t < DT; t++)
-      if (FULL || 16 * t < d) vf[t] = *reinterpret_cast<const u4v*>(base + ((int64_t)(32 * t) << a.ps_shift) + v_at);
-  };
-  int k0 = tl.k_lo + 32 * wv;
-  int pg = 0, pn = 0;
-  if (k0 < k_hi) {
-    pg = page_of(k0);
-    pn = page_of(k0 + 128);
-    load_k(k0, pg);
-    load_v(k0, pg);
   }
   for (; k0 < k_hi; k0 += 128) {
     f4 s[NQ][2];
@@ -739,7 +957,7 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
       if (FULL || 16 * t < d) *reinterpret_cast<f4*>(&sh.o[wv][16 * n + li][16 * t + 4 * g]) = acc[n][t] * f;
   }
   __syncthreads();
-  const int vecs = d / 4;
+  const int vecs = d / 4, slot = it.slot + it.split;
   for (int i = threadIdx.x; i < rows * vecs; i += 256) {
     const int r = i / vecs, c = i % vecs * 4;
     float mx = -INFINITY, ls = 0.0f;
@@ -752,17 +970,20 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
     for (int w = 0; w < 4; w++) o += *reinterpret_cast<const f4*>(&sh.o[w][r][c]);
     const bool dead = tree && tl.tail && kv_dead(sh.seen[(row_lo + r) / group - tok0], (row_lo + r) / group);
     if (it.slot >= 0) {
-      *reinterpret_cast<f4*>(a.part + ((int64_t)it.slot * TM + r) * D + c) = o;
-      if (c == 0) a.ml[((int64_t)it.slot * TM + r) * 2] = mx, a.ml[((int64_t)it.slot * TM + r) * 2 + 1] = dead ? -1.0f : ls;
+      kv_part_put(a.fused, a.part + ((int64_t)slot * TM + r) * D + c, o);
+      if (c == 0) kv_part_put(a.fused, a.ml + ((int64_t)slot * TM + r) * 2, mx, dead ? -1.0f : ls);
     } else {
+      const bool again = !dead && ls != ls;
+      if (c == 0) nan_row[r] = again;
+      if (again) continue;
       const int tk = (row_lo + r) / group;
       const int64_t at = (int64_t)(it.row0 + tk) * a.ldo + (int64_t)(it.hv * group + (row_lo + r) % group) * d + c;
-      const float inv = 1.0f / ls;
+      const float inv = dead || ls == 0.0f ? 0.0f : 1.0f / ls;
 #pragma unroll
-      for (int e = 0; e < 4; e++) Q::put(a.o, at + e, dead || ls == 0.0f ? 0.0f : o[e] * inv);
-      if (c == 0 && !dead && ls != ls) a.desc[8 + 8 * it.qid + 6] = 1;  // (after kv_describe: barriers lie between)
+      for (int e = 0; e < 4; e++) Q::put(a.o, at + e, inv == 0.0f ? 0.0f : o[e] * inv);
     }
   }
+  kv_end<QF ? VT_F32 : CT, CT, D, TM>(a, it, tl, nan_row, &is_last, all.end);
 }
 
 // ---- large tiles: 32 rows a wave, 64 slots at a time through LDS for all of them
@@ -787,19 +1008,27 @@ __device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
   constexpr int NS = QF ? (CT == VT_F16 ? 2 : 3) : 1, NP = NS;
   constexpr int UK = 32 * CH, UV = D * 4, UNIT = UK + UV;  // chunks
   typedef VRow<QF ? VT_F32 : CT> Q;
-  struct Shared {
+  static_assert(NW == 4, "kv_end");
+  struct Main {
     u4v st[R][2][UNIT];
     KvSeen seen[TM];
   };
-  __shared__ Shared sh;
+  union Shared {
+    Main m;
+    struct {
+      KvEnd e;
+      int nan_row[TM], is_last;
+    } end;
+  };
+  __shared__ Shared all;
+  Main& sh = all.m;
   KvItem it;
-  if (!kv_plan<TM>(a, blockIdx.x, it)) return;
+  if (!kv_plan(a, TM, blockIdx.x, it)) return;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q32 = lane & 31, h = lane >> 5;
   const int group = a.nh / a.nkv, d = FULL ? D : a.d, ps = 1 << a.ps_shift;
-  const KvTile tl = kv_tile<TM>(a, it);
+  const KvTile tl = kv_tile(a, TM, it);
   const int row_lo = tl.row_lo, rows = tl.rows, k_hi = tl.k_hi;
   const bool tree = a.parents != nullptr;
-  kv_describe(a, it, tl);
   const int row = 32 * wv + q32, rc = row_lo + min(row, rows - 1), tok = rc / group, tok0 = row_lo / group;
   const bool busy = 32 * wv < rows;  // (waves without rows only help with the loads)
 
@@ -1005,204 +1234,33 @@ __device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
     for (int e = 0; e < 16; e++) nan |= (FULL || 32 * t + 8 * (e >> 2) + 4 * h < d) && acc[t][e] != acc[t][e];
   nan |= __shfl_xor(nan, 32);
   if (nan) l = NAN;
-  __syncthreads();
-  if (row >= rows) return;
   const bool dead = tree && tl.tail && kv_dead(sh.seen[tok - tok0], tok);
-  if (it.slot >= 0) {
-    float* out = a.part + ((int64_t)it.slot * TM + row) * D;
+  __syncthreads();  // (the end's shared memory lies over the blocks')
+  if (row < rows) {
+    const int64_t slot = it.slot + it.split;
+    const bool again = !dead && l != l;
+    if (it.slot >= 0) {
+      float* out = a.part + (slot * TM + row) * D;
 #pragma unroll
-    for (int t = 0; t < DT; t++)
+      for (int t = 0; t < DT; t++)
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        *reinterpret_cast<f4*>(out + 32 * t + 8 * i + 4 * h) = f4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
-    if (h == 0) a.ml[((int64_t)it.slot * TM + row) * 2] = m, a.ml[((int64_t)it.slot * TM + row) * 2 + 1] = dead ? -1.0f : l;
-    return;
+        for (int i = 0; i < 4; i++)
+          kv_part_put(a.fused, out + 32 * t + 8 * i + 4 * h, f4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]});
+      if (h == 0) kv_part_put(a.fused, a.ml + (slot * TM + row) * 2, m, dead ? -1.0f : l);
+    } else if (!again) {
+      const int64_t at = (int64_t)(it.row0 + tok) * a.ldo + (int64_t)(it.hv * group + rc % group) * d + 4 * h;
+      const float inv = dead || l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+      for (int t = 0; t < DT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (FULL || 32 * t + 8 * i < d)
+#pragma unroll
+            for (int e = 0; e < 4; e++) Q::put(a.o, at + 32 * t + 8 * i + e, inv == 0.0f ? 0.0f : acc[t][4 * i + e] * inv);
+    }
+    if (h == 0) all.end.nan_row[row] = again;
   }
-  const int64_t at = (int64_t)(it.row0 + tok) * a.ldo + (int64_t)(it.hv * group + rc % group) * d + 4 * h;
-  const float inv = dead || l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int t = 0; t < DT; t++)
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (FULL || 32 * t + 8 * i < d)
-#pragma unroll
-        for (int e = 0; e < 4; e++) Q::put(a.o, at + 32 * t + 8 * i + e, inv == 0.0f ? 0.0f : acc[t][4 * i + e] * inv);
-  if (h == 0 && !dead && l != l) a.desc[8 + 8 * it.qid + 6] = 1;  // (after kv_describe: barriers lie between)
-}
-
-// ---- joining
-// A row whose products met infinity or NaN, by the formula: in the matrix instructions a value that the row does not see
-// still meets its weight 0, and the lower planes of queries and weights, which may be 0 or of the other sign,
-// meet infinities.  Here only what is seen is multiplied, in 32 bits; slow, and rare.
-template <int QT>
-__device__ __forceinline__ void kv_row_again(const KvAttendArgs& a, int ct_bf16, const int32_t* q, int row, int64_t out) {
-  __shared__ float qs[256], sc[256], mx[256];
-  __shared__ uint32_t seen[RTQ_KV_TREE / 32];
-  __shared__ int dead;
-  const int tid = threadIdx.x, group = a.nh / a.nkv, tok = row / group, seq = q[7], hv = q[5], d = a.d;
-  const int held = kv_held(a.s.lens, seq, a.s.ldt, a.ps_shift);
-  const int last = (int)min((int64_t)held + tok + 1, min((int64_t)a.s.ldt << a.ps_shift, (int64_t)RTQ_KV_SLOTS));
-  __syncthreads();
-  if (tid < d) qs[tid] = VRow<QT>::one(a.q, (int64_t)(q[2] + tok) * a.ldq + (int64_t)(hv * group + row % group) * d + tid);
-  if (tid < RTQ_KV_TREE / 32) seen[tid] = 0;
-  if (tid == 0) dead = a.parents && tok >= RTQ_KV_TREE;
-  __syncthreads();
-  if (tid == 0 && a.parents)
-    for (int node = tok; node >= 0 && !dead;) {
-      seen[node >> 5] |= 1u << (node & 31);
-      const int p = a.parents[q[2] + node];
-      if (p < -1 || p >= node) dead = 1;
-      node = p;
-    }
-  __syncthreads();
-  const int64_t head = (int64_t)d << a.ps_shift;
-  const int ps = 1 << a.ps_shift;
-  const auto conv = [&](uint16_t x) { return ct_bf16 ? __builtin_bit_cast(float, (uint32_t)x << 16) : (float)__builtin_bit_cast(_Float16, x); };
-  const auto page = [&](int key) {
-    const int pg = a.s.table[(int64_t)seq * a.s.ldt + (key >> a.ps_shift)];
-    return (unsigned)pg < (unsigned)a.n_pages ? ((int64_t)pg * a.nkv + hv) * head : -1;
-  };
-  float m = -INFINITY, l = 0.0f, o = 0.0f;
-  for (int k0 = 0; k0 < last && !dead; k0 += 256) {
-    const int key = k0 + tid, nw = key - held;
-    float s = -INFINITY;
-    bool vis = key < last && (nw < 0 || !a.parents || (seen[(nw & (RTQ_KV_TREE - 1)) >> 5] >> (nw & 31) & 1));
-    if (vis) {
-      const int64_t at = page(key);
-      vis = at >= 0;
-      if (vis) {
-        const uint16_t* k = a.k + at + (int64_t)(key & (ps - 1)) * d;
-        s = 0.0f;
-        for (int c = 0; c < d; c++) s = fmaf(qs[c], conv(k[c]), s);
-        s *= a.scale2;
-      }
-    }
-    mx[tid] = s;
-    __syncthreads();
-    for (int n = 128; n > 0; n >>= 1) {
-      if (tid < n) mx[tid] = fmaxf(mx[tid], mx[tid + n]);
-      __syncthreads();
-    }
-    const float mn = fmaxf(m, mx[0]), mu = mn == -INFINITY ? 0.0f : mn, al = __builtin_amdgcn_exp2f(m - mu);
-    m = mn;
-    sc[tid] = vis ? __builtin_amdgcn_exp2f(s - mu) : -1.0f;
-    __syncthreads();
-    l *= al, o *= al;
-    for (int j = 0; j < 256; j++) {
-      const float p = sc[j];
-      if (p == -1.0f) continue;
-      l += p;
-      if (tid < d) o = fmaf(p, conv(a.v[page(k0 + j) + ((int64_t)tid << a.ps_shift) + ((k0 + j) & (ps - 1))]), o);
-    }
-    __syncthreads();
-  }
-  if (tid < d) VRow<QT>::put(a.o, out + tid, l == 0.0f ? 0.0f : o / l);
-}
-
-// joins the parts of a tile's rows: workgroup (tile, some of its rows)
-template <int QT, int D>
-__device__ __forceinline__ void kv_merge(const KvAttendArgs& a) {
-  constexpr int V = D / 4, G = 256 / V;
-  __shared__ float red[256];
-  __shared__ f4 ro[256];
-  if ((int)blockIdx.x >= a.desc[0]) return;
-  const int32_t* q = a.desc + 8 + 8 * blockIdx.x;
-  const int slot = q[0], ns = q[1], tid = threadIdx.x, TM = a.tm, group = a.nh / a.nkv;
-  if (slot < 0 && !q[6]) return;
-  if (slot >= 0 && ns <= 16) {  // few parts: a wave a row, two parts (of four, of one) at once
-    constexpr int VL = V < 64 ? V : 64, GW = 64 / VL;
-    const int lane = tid & 63, c = lane % VL * 4, gr = lane / VL;
-    for (int r = 4 * blockIdx.y + (tid >> 6); r < q[4]; r += 4 * gridDim.y) {
-      const float* ml = a.ml + ((int64_t)slot * TM + r) * 2;
-      const float mi = lane < ns ? ml[(int64_t)lane * TM * 2] : -INFINITY, li = lane < ns ? ml[(int64_t)lane * TM * 2 + 1] : 0.0f;
-      float mx = mi;
-#pragma unroll
-      for (int d = 1; d < 16; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
-      mx = __shfl(mx, 0);
-      const bool dead = __any(li == -1.0f);
-      if (!dead && __any(li != li)) continue;  // (below)
-      const float f = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - mx);
-      float ls = f * li;
-#pragma unroll
-      for (int d = 1; d < 16; d <<= 1) ls += __shfl_xor(ls, d);
-      ls = __shfl(ls, 0);
-      f4 o = f4{0.0f, 0.0f, 0.0f, 0.0f};
-      for (int i = 0; i < ns; i += GW) {
-        const float fi = __shfl(f, min(i + gr, ns - 1));
-        if (i + gr < ns && c < a.d) o += fi * *reinterpret_cast<const f4*>(a.part + ((int64_t)(slot + i + gr) * TM + r) * D + c);
-      }
-#pragma unroll
-      for (int d = VL; d < 64; d <<= 1)
-#pragma unroll
-        for (int e = 0; e < 4; e++) o[e] += __shfl_xor(o[e], d);
-      if (gr == 0 && c < a.d) {
-        const int row = q[3] + r;
-        const int64_t out = (int64_t)(q[2] + row / group) * a.ldo + (int64_t)(q[5] * group + row % group) * a.d + c;
-        const float inv = 1.0f / ls;
-#pragma unroll
-        for (int e = 0; e < 4; e++) VRow<QT>::put(a.o, out + e, dead || ls == 0.0f ? 0.0f : o[e] * inv);
-      }
-    }
-    // rows whose sums are not numbers
-    for (int r0 = 4 * blockIdx.y; r0 < q[4]; r0 += 4 * gridDim.y)
-      for (int r = r0; r < min(r0 + 4, q[4]); r++) {
-        const float* ml = a.ml + ((int64_t)slot * TM + r) * 2;
-        int odd = 0;
-        for (int i = 0; i < ns; i++) {
-          const float li = ml[(int64_t)i * TM * 2 + 1];
-          odd |= li == -1.0f ? 1 : li != li ? 2 : 0;
-        }
-        const int row = q[3] + r;
-        if (odd == 2)
-          kv_row_again<QT>(a, a.cache_bf16, q, row, (int64_t)(q[2] + row / group) * a.ldo + (int64_t)(q[5] * group + row % group) * a.d);
-      }
-    return;
-  }
-  for (int r = blockIdx.y; r < q[4]; r += gridDim.y) {
-    const int row = q[3] + r;
-    const int64_t out = (int64_t)(q[2] + row / group) * a.ldo + (int64_t)(q[5] * group + row % group) * a.d;
-    if (slot < 0) {  // (some row of the tile)
-      kv_row_again<QT>(a, a.cache_bf16, q, row, out);
-      continue;
-    }
-    const float* ml = a.ml + ((int64_t)slot * TM + r) * 2;
-    float mx = -INFINITY;
-    int odd = 0;  // 1: dead, 2: not a number
-    for (int i = tid; i < ns; i += 256) {
-      const float li = ml[(int64_t)i * TM * 2 + 1];
-      mx = fmaxf(mx, ml[(int64_t)i * TM * 2]), odd |= li == -1.0f ? 1 : li != li ? 2 : 0;
-    }
-    red[tid] = mx;
-    const int dead = __syncthreads_or(odd & 1), again = __syncthreads_or(odd & 2);
-    if (again && !dead) {
-      kv_row_again<QT>(a, a.cache_bf16, q, row, out);
-      __syncthreads();
-      continue;
-    }
-    for (int s = 128; s > 0; s >>= 1) {
-      if (tid < s) red[tid] = fmaxf(red[tid], red[tid + s]);
-      __syncthreads();
-    }
-    mx = red[0];
-    __syncthreads();
-    const int c = tid % V * 4, gr = tid / V;
-    float ls = 0.0f;
-    f4 o = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = gr; i < ns; i += G) {
-      const float f = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[(int64_t)i * TM * 2] - mx);
-      ls += f * ml[(int64_t)i * TM * 2 + 1];
-      if (c < a.d) o += f * *reinterpret_cast<const f4*>(a.part + ((int64_t)(slot + i) * TM + r) * D + c);
-    }
-    ro[tid] = o, red[tid] = ls;
-    __syncthreads();
-    if (gr == 0 && c < a.d) {
-      for (int i = 1; i < G; i++) o += ro[i * V + tid], ls += red[i * V + tid];
-      const float inv = 1.0f / ls;
-#pragma unroll
-      for (int e = 0; e < 4; e++) VRow<QT>::put(a.o, out + c + e, dead || ls == 0.0f ? 0.0f : o[e] * inv);
-    }
-    __syncthreads();
-  }
+  kv_end<QF ? VT_F32 : CT, CT, D, TM>(a, it, tl, all.end.nan_row, &all.end.is_last, all.end.e);
 }
 
 #define RTQ_KV_ATTEND(SUF, CT, QF, D, FULL, NQ) \
@@ -1226,14 +1284,15 @@ RTQ_KV_ATTENDS(f32_bf16, VT_BF16, true, 4)
 RTQ_KV_ATTENDS(f16, VT_F16, false, 4)
 RTQ_KV_ATTENDS(bf16, VT_BF16, false, 4)
 
-#define RTQ_KV_MERGE(NAME, QT, D) \
-  extern "C" __global__ __launch_bounds__(256) void NAME(KvAttendArgs a) { kv_merge<QT, D>(a); }
-RTQ_KV_MERGE(rtq_kv_merge64_f32, VT_F32, 64)
-RTQ_KV_MERGE(rtq_kv_merge128_f32, VT_F32, 128)
-RTQ_KV_MERGE(rtq_kv_merge256_f32, VT_F32, 256)
-RTQ_KV_MERGE(rtq_kv_merge64_f16, VT_F16, 64)
-RTQ_KV_MERGE(rtq_kv_merge128_f16, VT_F16, 128)
-RTQ_KV_MERGE(rtq_kv_merge256_f16, VT_F16, 256)
-RTQ_KV_MERGE(rtq_kv_merge64_bf16, VT_BF16, 64)
-RTQ_KV_MERGE(rtq_kv_merge128_bf16, VT_BF16, 128)
-RTQ_KV_MERGE(rtq_kv_merge256_bf16, VT_BF16, 256)
+// the joining kernel: the workgroup of part i of n joins its tile's rows i, i + n, ...
+template <int QT, int CT>
+__device__ __forceinline__ void kv_join_rows(const KvAttendArgs& a) {
+  __shared__ KvEnd sh;
+  KvItem it;
+  if (!kv_plan(a, a.tm, blockIdx.x, it) || it.slot < 0) return;
+  kv_join<QT, CT>(a, it, kv_tile(a, a.tm, it), a.tm, a.D, it.split, it.splits, sh);
+}
+extern "C" __global__ __launch_bounds__(256) void rtq_kv_join_f32_f16(KvAttendArgs a) { kv_join_rows<VT_F32, VT_F16>(a); }
+extern "C" __global__ __launch_bounds__(256) void rtq_kv_join_f32_bf16(KvAttendArgs a) { kv_join_rows<VT_F32, VT_BF16>(a); }
+extern "C" __global__ __launch_bounds__(256) void rtq_kv_join_f16(KvAttendArgs a) { kv_join_rows<VT_F16, VT_F16>(a); }
+extern "C" __global__ __launch_bounds__(256) void rtq_kv_join_bf16(KvAttendArgs a) { kv_join_rows<VT_BF16, VT_BF16>(a); }

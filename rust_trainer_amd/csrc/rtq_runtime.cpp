@@ -179,8 +179,8 @@ enum Kid {
   K_KV_APPEND = K_VERIFY_PICK + 3,  // + 2 x rows and cache (f32 f16, f32 bf16, f16, bf16) + heads above 128
   K_KV_KEEP = K_KV_APPEND + 8,
   K_KV_ATTEND,                    // + 11 x rows and cache + tile and head size (attend_plan)
-  K_KV_MERGE = K_KV_ATTEND + 44,  // + 3 x type + head size (64, 128, 256)
-  K_ROWS = K_KV_MERGE + 9,  // + format
+  K_KV_JOIN = K_KV_ATTEND + 44,  // + rows and cache
+  K_ROWS = K_KV_JOIN + 4,  // + format
   K_MODEL = K_ROWS + F_COUNT,  // + RtqModelKernel: the decoder block (rtq_model.cpp)
   K_COUNT = K_MODEL + KM_COUNT
 };
@@ -235,9 +235,7 @@ constexpr const char* kKernelNames[] = {
     "rtq_kv_attend16_64_bf16", "rtq_kv_attend16_128_bf16", "rtq_kv_attend16_128p_bf16", "rtq_kv_attend16_256p_bf16",
     "rtq_kv_attend32_64_bf16", "rtq_kv_attend32_128_bf16", "rtq_kv_attend32_128p_bf16",
     "rtq_kv_attend_big_64_bf16", "rtq_kv_attend_big_128_bf16", "rtq_kv_attend_big_128p_bf16", "rtq_kv_attend_big_256p_bf16",
-    "rtq_kv_merge64_f32", "rtq_kv_merge128_f32", "rtq_kv_merge256_f32",
-    "rtq_kv_merge64_f16", "rtq_kv_merge128_f16", "rtq_kv_merge256_f16",
-    "rtq_kv_merge64_bf16", "rtq_kv_merge128_bf16", "rtq_kv_merge256_bf16",
+    "rtq_kv_join_f32_f16", "rtq_kv_join_f32_bf16", "rtq_kv_join_f16", "rtq_kv_join_bf16",
     "rtq_rows_q4_0",        "rtq_rows_q8_0",        "rtq_rows_q4_k",        "rtq_rows_q6_k",
     "rtq_m_rmsnorm",        "rtq_m_rmsnorm_bwd",    "rtq_m_qk_prep",        "rtq_m_qk_bwd",
     "rtq_m_gemm",           "rtq_m_softmax",        "rtq_m_softmax_bwd",    "rtq_m_group_sum",
@@ -2262,15 +2260,16 @@ rtq_status enqueue_append(rtq_kv_cache* kc, int64_t layer, const KvSeqs& s, int 
 // that, of 32 (whose registers a head size above 128 has not), else large ones.  `target` items keep every
 // CU's resident workgroups busy; the split tiles' items are at most twice that (each but a tile's last covers C keys).
 struct AttendPlan {
-  int tm, threads, variant, dk;
-  int64_t target, qids;
+  int tm, variant, D;
+  bool fused;
+  int64_t target, tiles;
   size_t bytes;
 };
-AttendPlan attend_plan(const rtq_kv_cache* kc, int type, int64_t n, int64_t b, int64_t nh) {
+AttendPlan attend_plan(const rtq_kv_cache* kc, int64_t n, int64_t b, int64_t ld, int64_t nh) {
   AttendPlan p{};
   const int64_t d = kc->d, rows = n * (nh / kc->nkv);
   const int size = d == 64 ? 0 : d == 128 ? 1 : d < 128 ? 2 : 3;
-  p.dk = d == 64 ? 0 : d <= 128 ? 1 : 2;
+  p.D = d == 64 ? 64 : d <= 128 ? 128 : 256;
   if (rows <= 16 * b) {
     p.tm = 16, p.variant = size;
   } else if (rows <= 32 * b && d <= 128) {
@@ -2278,11 +2277,12 @@ AttendPlan attend_plan(const rtq_kv_cache* kc, int type, int64_t n, int64_t b, i
   } else {
     p.tm = 128, p.variant = 7 + size;
   }
-  p.threads = p.tm > 32 ? 2 * p.tm : 256;
-  p.target = (int64_t)kc->ctx->cu_count * 2;
-  p.qids = (cdiv(rows, p.tm) + b) * kc->nkv;
-  const int64_t D = 64 << p.dk;
-  p.bytes = (size_t)(2 * p.target * p.tm * (D + 2) * 4 + (8 + 8 * p.qids) * 4) + 4 * 256;
+  p.target = std::min(kc->ctx->cu_count * 2, RTQ_KV_TARGET);
+  p.tiles = (cdiv(rows, p.tm) + b) * kc->nkv;
+  // a tile's rows times its parts, at most: what one workgroup reads again (up to 256 rows in the time that another kernel takes)
+  const int64_t parts = std::min(cdiv(ld * kc->ps, 128), p.target / kc->nkv + 1);
+  p.fused = std::min<int64_t>(p.tm, rows) * parts <= 256;
+  p.bytes = (size_t)(2 * p.target * p.tm * (p.D + 2) * 4) + 4 * 256;
   return p;
 }
 
@@ -2304,14 +2304,14 @@ rtq_status enqueue_attend(rtq_kv_cache* kc, int64_t layer, const KvSeqs& s, int 
   a.q = q, a.o = out, a.ldq = ldq, a.ldo = ldo, a.parents = parents;
   a.nh = (int)nh, a.nkv = (int)kc->nkv, a.d = (int)kc->d, a.ps_shift = kc->ps_shift, a.n_pages = (int)kc->n_pages;
   a.scale2 = (float)((scale > 0.0f ? (double)scale : 1.0 / std::sqrt((double)kc->d)) * 1.4426950408889634);
-  a.target = (int)p.target, a.slots = (int)(2 * p.target), a.qids = (int)p.qids, a.tm = p.tm, a.cache_bf16 = kc->type == RTQ_TYPE_BF16;
-  const int64_t D = 64 << p.dk;
-  a.part = ar.take<float>((size_t)(2 * p.target * p.tm * D));
+  a.target = (int)p.target, a.slots = (int)(2 * p.target);
+  a.part = ar.take<float>((size_t)(2 * p.target * p.tm * p.D));
   a.ml = ar.take<float>((size_t)(2 * p.target * p.tm * 2));
-  a.desc = ar.take<int32_t>((size_t)(8 + 8 * p.qids));
+  a.tm = p.tm, a.D = p.D, a.fused = p.fused;
   if (ar.off > ar.cap) return fail(RTQ_ERR_INVALID, "internal: workspace too small");
-  RTQ_TRY(launch(kc->ctx, K_KV_ATTEND + 11 * kv_types(kc, type) + p.variant, dim3((unsigned)(p.target + p.qids)), dim3((unsigned)p.threads), st, a));
-  return launch(kc->ctx, K_KV_MERGE + 3 * logit_type(type) + p.dk, dim3((unsigned)p.qids, (unsigned)std::min(p.tm, 16)), dim3(256), st, a);
+  const dim3 grid((unsigned)(p.target + p.tiles));
+  RTQ_TRY(launch(kc->ctx, K_KV_ATTEND + 11 * kv_types(kc, type) + p.variant, grid, dim3(256), st, a));
+  return p.fused ? RTQ_OK : launch(kc->ctx, K_KV_JOIN + kv_types(kc, type), grid, dim3(256), st, a);
 }
 
 rtq_status kv_check_keep(const rtq_kv_cache* kc, const rtq_kv_seqs* s, const int32_t* kept, int64_t ldk, const int32_t* after) {
@@ -2412,7 +2412,7 @@ rtq_status rtq_kv_attend_d(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s
   std::lock_guard<std::mutex> lk(c->mu);
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = (hipStream_t)stream;
-  const AttendPlan p = attend_plan(kc, type, n, s->b, nh);
+  const AttendPlan p = attend_plan(kc, n, s->b, s->ld, nh);
   RTQ_TRY(row_ws(c, p.bytes, st));
   Arena ar{(char*)c->ws, c->ws_bytes, 0};
   return enqueue_attend(kc, layer, kv_seqs(*s, n), type, nh, scale, parents, q, ldq, out, ldo, p, ar, st);
@@ -2985,7 +2985,7 @@ rtq_status rtq_kv_attend(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s, 
   HostCall hc(c);
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = c->stream;
-  const AttendPlan p = attend_plan(kc, type, n, s->b, nh);
+  const AttendPlan p = attend_plan(kc, n, s->b, s->ld, nh);
   const int64_t es = logit_bytes(type), qw = nh * kc->d;
   RTQ_TRY(ensure_ws(c, p.bytes + (size_t)(n * qw * es + n * 4) + kv_seq_bytes(*s) + 4 * 256));
   Arena ar{(char*)c->ws, c->ws_bytes, 0};
