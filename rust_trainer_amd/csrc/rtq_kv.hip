@@ -399,6 +399,9 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, int TM, int block
         const int at = block - ei;  // tile by tile, so that a range's tiles are a multiple of the XCDs apart
         it.seq = i, it.row0 = row0, it.cnt = cnt, it.held = held, it.total = total, it.splits = ns, it.C = c;
         it.tile = at / (a.nkv * ns), it.hv = at / ns % a.nkv, it.split = at % ns;
+        // A run's later tiles have more slots: they start first, and where two workgroups a CU take all of them at once, the
+        // n-th longest shares its CU with the n-th shortest.
+        if (!a.parents) it.tile = n > a.target || 2 * it.tile < tiles ? tiles - 1 - it.tile : it.tile - (tiles + 1) / 2;
         it.slot = ns > 1 ? es + at - it.split : -1;
         ok = ns == 1 || (it.slot + ns <= a.slots && block - it.split + ns <= (int)gridDim.x);
         break;
@@ -610,7 +613,6 @@ union KvEnd {
   struct {
     float m[kKvJoin], w[kKvJoin];  // [row][part]: maxima, sums; then weights
     f4 o[256];
-    int odd;
   } j;
   KvAgain again;
 };
@@ -626,13 +628,13 @@ __device__ __forceinline__ void kv_part_put(bool through, float* p, f4 v) {
 }
 
 // Joins the parts of a tile's rows first, first + step, ... (with 256 threads): what counts is how many loads are under way.
-template <int QT, int CT>
-__device__ __forceinline__ void kv_join(const KvAttendArgs& a, const KvItem& it, const KvTile& t, int TM, int D, int from, int step, KvEnd& sh) {
+// nan: room for the tile's rows: those that are not numbers are marked, and left.
+template <int QT>
+__device__ __forceinline__ void kv_join(const KvAttendArgs& a, const KvItem& it, const KvTile& t, int TM, int D, int from, int step, int* nan, KvEnd& sh) {
   const int tid = threadIdx.x, lane = tid & 63, group = a.nh / a.nkv, ns = it.splits, V = D / 4, G = 256 / V;
   const int rows = (t.rows - from + step - 1) / step;
   if (rows <= 0) return;
   __syncthreads();
-  if (tid == 0) sh.j.odd = 0;
   // the parts' weights: every maximum and sum at once, then a thread a row of few parts or a wave a row of many
   for (int i = tid; i < rows * ns; i += 256) {
     const float* ml = a.ml + ((int64_t)(it.slot + i % ns) * TM + from + i / ns * step) * 2;
@@ -659,8 +661,8 @@ __device__ __forceinline__ void kv_join(const KvAttendArgs& a, const KvItem& it,
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) ls += __shfl_xor(ls, d);
     }
-    const bool bad = !dead && ls != ls;  // not a number: done again below
-    if (bad) sh.j.odd = 1;
+    const bool bad = !dead && ls != ls;
+    nan[from + r * step] = bad;
     const float inv = dead || ls == 0.0f ? 0.0f : 1.0f / ls;
     for (int i = part0; i < ns; i += parts) w[i] = bad ? NAN : m[i] * inv;
   }
@@ -701,48 +703,42 @@ __device__ __forceinline__ void kv_join(const KvAttendArgs& a, const KvItem& it,
       for (int e = 0; e < 4; e++) VRow<QT>::put(a.o, out + e, o[e]);
     }
   }
-  if (!sh.j.odd) return;
-  for (int r = from; r < t.rows; r += step) {
-    const float* ml = a.ml + ((int64_t)it.slot * TM + r) * 2;
-    int mark = 0;
-    for (int i = 0; i < ns; i++) {
-      const float li = ml[(int64_t)i * TM * 2 + 1];
-      mark |= li == -1.0f ? 1 : li != li ? 2 : 0;
-    }
-    if (mark == 2) kv_row_again<QT, CT>(a, it, t.row_lo + r, sh.again);
-  }
+}
+
+// the marked rows of a tile (first, first + step, ...) by the formula
+template <int QT, int CT>
+__device__ __forceinline__ void kv_rows_again(const KvAttendArgs& a, const KvItem& it, const KvTile& t, int from, int step, const int* nan, KvAgain& sh) {
+  __syncthreads();
+  uint32_t any = 0;
+  for (int r = threadIdx.x & 63; r < t.rows; r += 64) any |= r % step == from && nan[r];
+  if (!__any(any)) return;
+  for (int r = from; r < t.rows; r += step)
+    if (nan[r]) kv_row_again<QT, CT>(a, it, t.row_lo + r, sh);
 }
 
 // After a workgroup's item (of 256 threads): nan[r] marks rows of a tile of one part that are to be done again; a part of
 // a split tile is counted, and the last joins the parts.  sh: the workgroup's shared memory, free by now.
 template <int QT, int CT, int D, int TM>
-__device__ __forceinline__ void kv_end(const KvAttendArgs& a, const KvItem& it, const KvTile& t, const int* nan, int* last, KvEnd& sh) {
-  const int tid = threadIdx.x;
-  if (it.slot < 0) {
+__device__ __forceinline__ void kv_end(const KvAttendArgs& a, const KvItem& it, const KvTile& t, int* nan, int* last, KvEnd& sh) {
+  if (it.slot >= 0) {
+    if (!a.fused) return;
+    // The part's stores go through to memory (kv_part_put): once a wave has none under way they are there for every XCD, and
+    // the part may be counted.  (Ordinary stores and a release would write back all that the XCD's L2 holds, in every
+    // workgroup: 30 us of a call of 512.)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    uint32_t any = 0;
-    for (int r = tid & 63; r < t.rows; r += 64) any |= nan[r];
-    if (!__any(any)) return;
-    for (int r = 0; r < t.rows; r++)
-      if (nan[r]) kv_row_again<QT, CT>(a, it, t.row_lo + r, sh.again);
-    return;
+    int* count = kv_arrived + (it.slot >> 1);
+    if (threadIdx.x == 0) {
+      const int n = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (n == it.splits - 1) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      *last = n == it.splits - 1;
+    }
+    __syncthreads();
+    if (!*last) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    kv_join<QT>(a, it, t, TM, D, 0, 1, nan, sh);
   }
-  if (!a.fused) return;
-  // The part's stores go through to memory (kv_part_put): once a wave has none under way they are there for every XCD, and
-  // the part may be counted.  (Ordinary stores and a release would write back all that the XCD's L2 holds, in every
-  // workgroup: 30 us of a call of 512.)
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  int* count = kv_arrived + (it.slot >> 1);
-  if (tid == 0) {
-    const int n = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (n == it.splits - 1) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    *last = n == it.splits - 1;
-  }
-  __syncthreads();
-  if (!*last) return;
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-  kv_join<QT, CT>(a, it, t, TM, D, 0, 1, sh);
+  kv_rows_again<QT, CT>(a, it, t, 0, 1, nan, sh.again);
 }
 
 // ---- small tiles: 16 or 32 rows, four waves that share the tile's slots, operands straight from the cache
@@ -1288,9 +1284,13 @@ RTQ_KV_ATTENDS(bf16, VT_BF16, false, 4)
 template <int QT, int CT>
 __device__ __forceinline__ void kv_join_rows(const KvAttendArgs& a) {
   __shared__ KvEnd sh;
+  __shared__ int nan[128];
   KvItem it;
   if (!kv_plan(a, a.tm, blockIdx.x, it) || it.slot < 0) return;
-  kv_join<QT, CT>(a, it, kv_tile(a, a.tm, it), a.tm, a.D, it.split, it.splits, sh);
+  const KvTile t = kv_tile(a, a.tm, it);
+  if (it.split >= t.rows) return;
+  kv_join<QT>(a, it, t, a.tm, a.D, it.split, it.splits, nan, sh);
+  kv_rows_again<QT, CT>(a, it, t, it.split, it.splits, nan, sh.again);
 }
 extern "C" __global__ __launch_bounds__(256) void rtq_kv_join_f32_f16(KvAttendArgs a) { kv_join_rows<VT_F32, VT_F16>(a); }
 extern "C" __global__ __launch_bounds__(256) void rtq_kv_join_f32_bf16(KvAttendArgs a) { kv_join_rows<VT_F32, VT_BF16>(a); }
