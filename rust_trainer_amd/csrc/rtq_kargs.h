@@ -664,7 +664,7 @@ struct KvAttendArgs {
   void* o;
   int64_t ldq, ldo;
   const int32_t* parents;  // [n] or null: runs
-  int nh, nkv, d, ps_shift, n_pages;
+  int nkv, group, d, ps_shift, n_pages;  // group: query heads a KV head
   float scale2;     // scale log2(e)
   int target;       // items that the keys are split into (at most this many, and one per tile beside)
   int slots;        // partial slots

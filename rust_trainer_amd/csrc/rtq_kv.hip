@@ -357,7 +357,7 @@ __device__ __forceinline__ float kv_wave_total(float v) {
 // kKvJoin.  Sequences that overlap in `starts` can name more than the host counted: then whole tiles are left out.
 constexpr int kKvJoin = 1024;
 __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, int TM, int block, KvItem& it) {
-  const int lane = threadIdx.x & 63, group = a.nh / a.nkv;
+  const int lane = threadIdx.x & 63, group = a.group;
   const int per = (a.s.b + 63) / 64, i0 = min(lane * per, a.s.b), i1 = min(i0 + per, a.s.b);
   int row0 = 0, cnt = 0, held = 0, total = 0, tiles = 0;
   const auto look = [&](int i) {
@@ -376,8 +376,8 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, int TM, int block
   const int C = max((int)fminf(ceilf(w * (float)a.nkv / (float)a.target / 128.0f), (float)(RTQ_KV_SLOTS / 128)) * 128, 128);
   // a sequence's slots a part, parts
   const auto cut = [&](int& c, int& ns) {
-    const int most = a.fused ? kKvJoin / min(max(cnt, 1) * group, TM) : kKvJoin;
-    c = max(C, ((total + most - 1) / most + 127) & ~127);
+    const int64_t least = a.fused ? (int64_t)total * min(max(cnt, 1) * a.group, TM) : total;
+    c = max(C, (int)(((least + kKvJoin - 1) / kKvJoin + 127) & ~127));
     ns = max((total + c - 1) / c, 1);
   };
   int items = 0, slots = 0, c, ns;
@@ -398,7 +398,8 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, int TM, int block
       if (block < ei + n) {
         const int at = block - ei;  // tile by tile, so that a range's tiles are a multiple of the XCDs apart
         it.seq = i, it.row0 = row0, it.cnt = cnt, it.held = held, it.total = total, it.splits = ns, it.C = c;
-        it.tile = at / (a.nkv * ns), it.hv = at / ns % a.nkv, it.split = at % ns;
+        it.tile = at / (a.nkv * ns);
+        it.hv = (at - it.tile * a.nkv * ns) / ns, it.split = at - (it.tile * a.nkv + it.hv) * ns;
         // A run's later tiles have more slots: they start first, and where two workgroups a CU take all of them at once, the
         // n-th longest shares its CU with the n-th shortest.
         if (!a.parents) it.tile = n > a.target || 2 * it.tile < tiles ? tiles - 1 - it.tile : it.tile - (tiles + 1) / 2;
@@ -471,7 +472,7 @@ struct KvTile {
 };
 __device__ __forceinline__ KvTile kv_tile(const KvAttendArgs& a, int TM, const KvItem& it) {
   KvTile t;
-  const int group = a.nh / a.nkv;
+  const int group = a.group;
   t.row_lo = it.tile * TM, t.rows = min((int)((int64_t)it.cnt * group - t.row_lo), TM);
   t.k_lo = it.split * it.C;
   // no row of the tile sees a new token after its own
@@ -486,7 +487,7 @@ __device__ __forceinline__ KvTile kv_tile(const KvAttendArgs& a, int TM, const K
 typedef uint32_t KvSeen[RTQ_KV_TREE / 32];
 template <int TOK, int THREADS>
 __device__ __forceinline__ void kv_tree(const KvAttendArgs& a, const KvItem& it, const KvTile& t, KvSeen* seen, uint16_t* up) {
-  const int group = a.nh / a.nkv, n = min(it.cnt, RTQ_KV_TREE);
+  const int group = a.group, n = min(it.cnt, RTQ_KV_TREE);
   const int first = t.row_lo / group, toks = (t.row_lo + t.rows - 1) / group - first + 1;
   for (int i = threadIdx.x; i < TOK * (RTQ_KV_TREE / 32); i += THREADS) (&seen[0][0])[i] = 0;
   for (int i = threadIdx.x; i < n; i += THREADS) {  // 0: the cache, else the parent + 1; 65535: none
@@ -548,7 +549,7 @@ __device__ __forceinline__ void kv_row_again(const KvAttendArgs& a, const KvItem
   float *qs = sh.qs, *sc = sh.sc, *mx = sh.mx;
   uint32_t* seen = sh.seen;
   int& dead = sh.dead;
-  const int tid = threadIdx.x, group = a.nh / a.nkv, tok = row / group, seq = it.seq, hv = it.hv, d = a.d, held = it.held;
+  const int tid = threadIdx.x, group = a.group, tok = row / group, seq = it.seq, hv = it.hv, d = a.d, held = it.held;
   const int last = min(held + tok + 1, it.total);
   __syncthreads();
   if (tid < d) qs[tid] = VRow<QT>::one(a.q, (int64_t)(it.row0 + tok) * a.ldq + (int64_t)(hv * group + row % group) * d + tid);
@@ -631,10 +632,24 @@ __device__ __forceinline__ void kv_part_put(bool through, float* p, f4 v) {
 // nan: room for the tile's rows: those that are not numbers are marked, and left.
 template <int QT>
 __device__ __forceinline__ void kv_join(const KvAttendArgs& a, const KvItem& it, const KvTile& t, int TM, int D, int from, int step, int* nan, KvEnd& sh) {
-  const int tid = threadIdx.x, lane = tid & 63, group = a.nh / a.nkv, ns = it.splits, V = D / 4, G = 256 / V;
+  const int tid = threadIdx.x, lane = tid & 63, group = a.group, ns = it.splits, V = D / 4, G = 256 / V;
   const int rows = (t.rows - from + step - 1) / step;
   if (rows <= 0) return;
   __syncthreads();
+  // A thread takes four elements of a row; of few rows some threads share a row's parts.
+  int share = 1;
+  while (2 * share * rows <= G) share *= 2;
+  const int c = tid % V * 4, gr = tid / V, first = gr % share;
+  f4 x[16];
+  const auto fetch = [&](int r, int i) {
+#pragma unroll
+    for (int u = 0; u < 16; u++) {
+      x[u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (r < rows && c < a.d && i + u * share < ns)
+        x[u] = *reinterpret_cast<const f4*>(a.part + ((int64_t)(it.slot + i + u * share) * TM + from + r * step) * D + c);
+    }
+  };
+  fetch(gr / share, first);  // (under way beside the weights)
   // the parts' weights: every maximum and sum at once, then a thread a row of few parts or a wave a row of many
   for (int i = tid; i < rows * ns; i += 256) {
     const float* ml = a.ml + ((int64_t)(it.slot + i % ns) * TM + from + i / ns * step) * 2;
@@ -667,27 +682,15 @@ __device__ __forceinline__ void kv_join(const KvAttendArgs& a, const KvItem& it,
     for (int i = part0; i < ns; i += parts) w[i] = bad ? NAN : m[i] * inv;
   }
   __syncthreads();
-  // then a thread four elements of a row; of few rows some threads share a row's parts
-  int share = 1;
-  while (2 * share * rows <= G) share *= 2;
-  const int c = tid % V * 4, gr = tid / V, first = gr % share;
   for (int r0 = 0; r0 < rows; r0 += G / share) {
     const int r = r0 + gr / share;
     const float* w = sh.j.w + min(r, rows - 1) * ns;
     f4 o = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (r < rows && c < a.d) {
-      const float* x0 = a.part + ((int64_t)it.slot * TM + from + r * step) * D + c;
-      for (int i = first; i < ns; i += 16 * share) {
-        f4 x[16];
+    for (int i = first; i < ns; i += 16 * share) {
+      if (r0 > 0 || i > first) fetch(r, i);
 #pragma unroll
-        for (int u = 0; u < 16; u++) {
-          x[u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-          if (i + u * share < ns) x[u] = *reinterpret_cast<const f4*>(x0 + (int64_t)(i + u * share) * TM * D);
-        }
-#pragma unroll
-        for (int u = 0; u < 16; u++)
-          if (i + u * share < ns && w[i + u * share] != 0.0f) o += w[i + u * share] * x[u];
-      }
+      for (int u = 0; u < 16; u++)
+        if (i + u * share < ns && w[i + u * share] != 0.0f) o += w[i + u * share] * x[u];
     }
     if (share > 1) {
       __syncthreads();
@@ -763,7 +766,7 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
   KvItem it;
   if (!kv_plan(a, TM, blockIdx.x, it)) return;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, g = lane >> 4;
-  const int group = a.nh / a.nkv, d = FULL ? D : a.d, ps = 1 << a.ps_shift;
+  const int group = a.group, d = FULL ? D : a.d, ps = 1 << a.ps_shift;
   const KvTile tl = kv_tile(a, TM, it);
   const int row_lo = tl.row_lo, rows = tl.rows, k_hi = tl.k_hi;
   const bool tree = a.parents != nullptr;
@@ -1021,7 +1024,7 @@ __device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
   KvItem it;
   if (!kv_plan(a, TM, blockIdx.x, it)) return;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q32 = lane & 31, h = lane >> 5;
-  const int group = a.nh / a.nkv, d = FULL ? D : a.d, ps = 1 << a.ps_shift;
+  const int group = a.group, d = FULL ? D : a.d, ps = 1 << a.ps_shift;
   const KvTile tl = kv_tile(a, TM, it);
   const int row_lo = tl.row_lo, rows = tl.rows, k_hi = tl.k_hi;
   const bool tree = a.parents != nullptr;

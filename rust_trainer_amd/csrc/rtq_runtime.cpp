@@ -2302,7 +2302,7 @@ rtq_status enqueue_attend(rtq_kv_cache* kc, int64_t layer, const KvSeqs& s, int 
   a.s = s;
   a.k = kc->k + layer * kc->layer, a.v = kc->v + layer * kc->layer;
   a.q = q, a.o = out, a.ldq = ldq, a.ldo = ldo, a.parents = parents;
-  a.nh = (int)nh, a.nkv = (int)kc->nkv, a.d = (int)kc->d, a.ps_shift = kc->ps_shift, a.n_pages = (int)kc->n_pages;
+  a.nkv = (int)kc->nkv, a.group = (int)(nh / kc->nkv), a.d = (int)kc->d, a.ps_shift = kc->ps_shift, a.n_pages = (int)kc->n_pages;
   a.scale2 = (float)((scale > 0.0f ? (double)scale : 1.0 / std::sqrt((double)kc->d)) * 1.4426950408889634);
   a.target = (int)p.target, a.slots = (int)(2 * p.target);
   a.part = ar.take<float>((size_t)(2 * p.target * p.tm * p.D));
