@@ -378,6 +378,8 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, int TM, int block
   const auto cut = [&](int& c, int& ns) {
     const int64_t least = a.fused ? (int64_t)total * min(max(cnt, 1) * a.group, TM) : total;
     c = max(C, (int)(((least + kKvJoin - 1) / kKvJoin + 127) & ~127));
+    // joining costs a small tile as much as four more turns of its waves (token over 250: 12.8 us in two parts, 9.9 in one)
+    if (TM <= 32 && total <= 512) c = max(c, 512);
     ns = max((total + c - 1) / c, 1);
   };
   int items = 0, slots = 0, c, ns;
