@@ -14,7 +14,7 @@ __device__ __forceinline__ int kv_start(const KvSeqs& s, int i) {
   return min(max(s.starts[i], 0), s.n);
 }
 #define RTQ_KV_SLOTS (1 << 30)  // most slots of a sequence that are looked at
-// tokens held by sequence i, no more than its table's slots
+// tokens held by sequence i, as far as its table's slots go
 __device__ __forceinline__ int kv_held(const int32_t* lens, int i, int ldt, int ps_shift) {
   return (int)min((int64_t)max(lens[i], 0), min((int64_t)ldt << ps_shift, (int64_t)RTQ_KV_SLOTS));
 }
@@ -37,8 +37,8 @@ __device__ __forceinline__ void kv_append_rows(const KvAppendArgs& a, int tok, i
   typedef u2v u2u __attribute__((aligned(2)));
   const int lane = threadIdx.x & 63, l16 = lane & 15;
   const int half = a.rot / 2, units = a.d / 8;
-  const int64_t slot = (int64_t)kv_held(a.s.lens, seq, a.s.ldt, a.ps_shift) + (tok - kv_start(a.s, seq));
-  const int p = (int)(slot >> a.ps_shift), ps = 1 << a.ps_shift;
+  const int64_t slot = (int64_t)max(a.s.lens[seq], 0) + (tok - kv_start(a.s, seq)), p = slot >> a.ps_shift;
+  const int ps = 1 << a.ps_shift;
   const int pid = p < a.s.ldt ? a.s.table[(int64_t)seq * a.s.ldt + p] : -1;
   const bool stored = (unsigned)pid < (unsigned)a.n_pages, whole = a.rot % 8 == 0;
   const double pos = a.pos ? (double)a.pos[tok] : (double)slot;
@@ -209,7 +209,7 @@ __device__ __forceinline__ void kv_append(const KvAppendArgs& a) {
     if (lane < 32) {
       int64_t at = -1;
       if (lane < nt && seq >= 0) {
-        const int64_t slot = (int64_t)kv_held(a.s.lens, seq, a.s.ldt, a.ps_shift) + idx;
+        const int64_t slot = (int64_t)max(a.s.lens[seq], 0) + idx;
         const int64_t p = slot >> a.ps_shift;
         const int pid = p < a.s.ldt ? a.s.table[(int64_t)seq * a.s.ldt + p] : -1;
         if ((unsigned)pid < (unsigned)a.n_pages) at = (((int64_t)pid * a.nkv + hv) * a.d << a.ps_shift) + (slot & (ps - 1));
@@ -254,7 +254,7 @@ extern "C" __global__ __launch_bounds__(256) void rtq_kv_keep(KvKeepArgs a) {
   __shared__ int count;
   const int hv = blockIdx.x % a.nkv, seq = blockIdx.x / a.nkv, tid = threadIdx.x;
   const int32_t* kept = a.kept + (int64_t)seq * a.ldk;
-  const int held = kv_held(a.lens, seq, a.ldt, a.ps_shift), ps = 1 << a.ps_shift;
+  const int held = max(a.lens[seq], 0), ps = 1 << a.ps_shift;
   if (tid == 0) count = a.ldk;
   __syncthreads();
   for (int j = tid; j < a.ldk; j += 256) {  // the list ends at the first entry that does not ascend

@@ -2290,7 +2290,7 @@ rtq_status kv_check_attend(const rtq_kv_cache* kc, int64_t layer, const rtq_kv_s
                            const void* q, int64_t ldq, const void* out, int64_t ldo) {
   RTQ_TRY(kv_check(kc, layer, s, n, type));
   RTQ_TRY(kv_check_heads(kc, n, nh));
-  if (!(scale >= 0.0f && scale < INFINITY)) return fail(RTQ_ERR_INVALID, "attention scale %g", (double)scale);
+  if (!(scale >= 0.0f && scale <= 1e38f)) return fail(RTQ_ERR_INVALID, "attention scale %g", (double)scale);
   if (n == 0) return RTQ_OK;
   RTQ_TRY(kv_check_rows(q, nh * kc->d, ldq, type, "q"));
   return kv_check_rows(out, nh * kc->d, ldo, type, "out");

@@ -183,6 +183,14 @@ ATTEND = [  # lens, counts, heads, kv, d, page, tree, gap, off
     ([5] * 130, [1] * 130, 2, 2, 32, 32, False, 0, 0),
     ([40] * 66 + [700], [2] * 66 + [5], 2, 1, 16, 32, True, 0, 0),
     ([3000], [1], 32, 8, 128, 128, False, 0, 0),
+    ([20, 5], [3, 1], 200, 1, 64, 32, False, 0, 0),  # more query heads a KV head than a tile has rows
+    ([50], [60], 6, 2, 16, 32, False, 0, 0),
+    ([50, 0], [60, 33], 6, 2, 48, 1024, True, 0, 0),
+    ([33], [45], 4, 1, 112, 32, True, 2, 1),
+    ([700, 900], [40, 40], 8, 1, 64, 32, True, 0, 0),
+    ([1500], [50], 8, 2, 256, 64, False, 0, 0),
+    ([3] * 3000, [1] * 3000, 1, 1, 16, 32, False, 0, 0),
+    ([515, 130, 511, 512, 513], [1] * 5, 5, 1, 128, 32, False, 0, 0),
 ]
 
 
@@ -220,15 +228,17 @@ def test_attend(ctx, case, xt, ct):
     check_attend(pg, lay, got, q, xt, heads, parents, scale)
 
 
+@pytest.mark.parametrize("first, counts", [(70, [20, 6, 40]), (2500, [20, 6, 40]), (1500, [6, 6, 5])])
 @pytest.mark.parametrize("xt, ct", PAIRS)
-def test_what_is_not_seen_does_not_matter(ctx, xt, ct):
-    """NaN in every slot that holds no token, and NaN and infinities in the keys and values of tokens that others do not see."""
-    lens, counts, heads, kv, d = [70, 3, 0], [20, 6, 40], 4, 2, 128
+def test_what_is_not_seen_does_not_matter(ctx, xt, ct, first, counts):
+    """NaN in every slot that holds no token, and NaN and infinities in the keys and values of tokens that others do not see:
+    in tiles of one part and of several."""
+    lens, heads, kv, d = [first, 3, 0], 4, 2, 128
     lay = Layout(lens, counts, 32, seed=5)
     rng = np.random.default_rng(6)
     pg = Pages(ctx, lay, kv, d, ct, fill=np.nan)
     parents = np.array([p for m in counts for p in tree(rng, m)[0]], np.int32)
-    bad = {0: [4, 19], 1: [5], 2: [39, 17]}
+    bad = {0: [4, counts[0] - 1], 1: [5], 2: [counts[2] - 1, counts[2] // 2]}
     for i in range(3):
         p, s = lay.slots(i)
         pg.k0[0][p, :, s] = to_type(rng.standard_normal((p.size, kv, d)), ct)
@@ -431,6 +441,61 @@ def test_offsets_past_32_bits(ctx):
     cache.close()
 
 
+def test_rows_of_no_sequence(ctx):
+    """Rows before the first sequence, behind the last, and a call whose sequences have none."""
+    lay = Layout([40, 7], [3, 2], 32)
+    kv, d, heads = 2, 64, 4
+    rng = np.random.default_rng(1)
+    q, k, v = [rng.standard_normal((9, h * d)).astype(np.float32) for h in (heads, kv, kv)]
+    a, b = Pages(ctx, lay, kv, d, "f16"), Pages(ctx, lay, kv, d, "f16")
+    shifted = dev(lay.starts + 2)
+    sa = seqs_d(2, a.lens.data_ptr(), a.table.data_ptr(), lay.table.shape[1], shifted.data_ptr())
+    qd, kd, vd = rows_d(q), rows_d(k), rows_d(v)
+    out, o2 = [torch.full((9, heads * d), 7.0, device="cuda") for _ in range(2)]
+    a.cache.append_d(0, sa, 9, 0, rope_d(64), kd.data_ptr(), kv * d, vd.data_ptr(), kv * d, heads, qd.data_ptr(), heads * d, out.data_ptr(), heads * d, stream=stream())
+    a.cache.attend_d(0, sa, 9, 0, heads, out.data_ptr(), heads * d, o2.data_ptr(), heads * d, 0, 0.0, stream())
+    s = Seqs(lay.lens, lay.table, lay.starts)
+    want = b.cache.append(0, s, k[2:7], v[2:7], Rope(64), q=q[2:7])
+    assert np.array_equal(out[2:7].cpu().numpy(), want) and torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
+    assert np.array_equal(o2[2:7].cpu().numpy(), b.cache.attend(0, s, want))
+    for t in (out, o2):
+        assert (t[:2] == 7).all() and (t[7:] == 7).all()
+    host_out = b.cache.attend(0, Seqs(lay.lens, lay.table, lay.starts + 2), np.concatenate((q[:2], want, q[7:])))
+    assert np.array_equal(host_out[2:7], o2[2:7].cpu().numpy()) and not host_out[:2].any()
+    k0, v0 = a.k.clone(), a.v.clone()
+    none = torch.zeros(3, dtype=torch.int32, device="cuda")
+    sn = seqs_d(2, a.lens.data_ptr(), a.table.data_ptr(), lay.table.shape[1], none.data_ptr())
+    out.fill_(7.0)
+    a.cache.append_d(0, sn, 9, 0, rope_d(64), kd.data_ptr(), kv * d, vd.data_ptr(), kv * d, heads, qd.data_ptr(), heads * d, out.data_ptr(), heads * d, stream=stream())
+    a.cache.attend_d(0, sn, 9, 0, heads, qd.data_ptr(), heads * d, out.data_ptr(), heads * d, 0, 0.0, stream())
+    torch.cuda.synchronize()
+    assert torch.equal(a.k, k0) and torch.equal(a.v, v0) and (out == 7).all()
+
+
+def test_more_tokens_than_the_table_holds(ctx):
+    """A held length past the table's end: new tokens are not stored, their queries turn by their own positions, and see what
+    the table holds."""
+    lay = Layout([64], [0], 32, wide=0)
+    pg = Pages(ctx, lay, 1, 64, "f16")
+    pg.lens.fill_(1000)
+    starts = torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+    s = seqs_d(1, pg.lens.data_ptr(), pg.table.data_ptr(), 2, starts.data_ptr())
+    q = np.random.default_rng(0).standard_normal((2, 64)).astype(np.float32)
+    qd, out, after = rows_d(q), torch.zeros(2, 64, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    kept = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda")
+    pg.cache.append_d(0, s, 2, 0, rope_d(64), qd.data_ptr(), 64, qd.data_ptr(), 64, 1, qd.data_ptr(), 64, out.data_ptr(), 64, stream=stream())
+    pg.cache.keep_d(s, kept.data_ptr(), 2, after.data_ptr(), stream())
+    torch.cuda.synchronize()
+    want = rotate(q.astype(np.float64)[:, None], [1000, 1001], 64, 1e4, True)[:, 0]
+    assert np.abs(out.cpu().numpy() - want).max() <= 2 * np.abs(q).max() * (6.3 * 2.0 ** -26 + 5 * 2.0 ** -24)
+    assert np.array_equal(host(pg.k, "f16"), pg.k0) and np.array_equal(host(pg.v, "f16"), pg.v0) and after.item() == 1002
+    pg.cache.attend_d(0, s, 2, 0, 1, qd.data_ptr(), 64, out.data_ptr(), 64, 0, 0.0, stream())
+    k, v = pg.rows(0, 64)
+    for i in range(2):  # (the last held token as the one new token of its row: the row sees all 64)
+        want, bound = attend(q[i:i + 1].astype(np.float64), k, v, 63, 1)
+        assert np.all(np.abs(out[i:i + 1].cpu().numpy() - want) <= bound + EPS["f32"] * (np.abs(want) + bound))
+
+
 # ------------------------------------------------------------------ keep
 @pytest.mark.parametrize("ct", ["f16", "bf16"])
 @pytest.mark.parametrize("d, page, kv, layers", [(128, 32, 2, 3), (80, 64, 3, 1), (256, 32, 1, 2), (16, 32, 2, 2)])
@@ -570,6 +635,70 @@ def test_a_captured_step_replays(ctx):
         assert torch.equal(pg.k, ref.k) and torch.equal(pg.v, ref.v)
         assert all(torch.equal(a, b) for a, b in zip(*bufs))
         assert torch.isfinite(bufs[0][0]).all() and (x.sum() * 0 == 0).item()  # the program's own work between the replays
+
+
+def test_two_graphs_share_the_workspace(ctx):
+    """Calls whose parts are joined by the last workgroup, and by a kernel, captured apart and replayed in turn."""
+    lay = Layout([900, 2000, 700], [1, 1, 1], 32)
+    pg = Pages(ctx, lay, 2, 64, "f16")
+    big = Layout([3000], [40], 32, seed=3)
+    pb = Pages(ctx, big, 2, 64, "f16", seed=3)
+    q = [torch.randn(n, 256, device="cuda") for n in (3, 40)]
+    out = [torch.zeros_like(x) for x in q]
+    side = torch.cuda.Stream()
+
+    def call(i, st):
+        p, n = ((pg, 3), (pb, 40))[i]
+        p.cache.attend_d(0, p.seqs, n, 0, 4, q[i].data_ptr(), 256, out[i].data_ptr(), 256, 0, 0.0, st)
+
+    torch.cuda.synchronize()
+    graphs = []
+    with torch.cuda.stream(side):
+        for i in (1, 0):
+            call(i, side.cuda_stream)
+        side.synchronize()
+        for i in (0, 1):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=side):
+                call(i, torch.cuda.current_stream().cuda_stream)
+    for turn in range(4):
+        for x in q:
+            x.normal_()
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            out[i].fill_(7.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for i in ((0, 1), (1, 0), (0, 0, 1), (1, 1, 0))[turn]:
+                graphs[i].replay()
+        side.synchronize()
+        got = [x.clone() for x in out]
+        with torch.cuda.stream(side):
+            for i in (0, 1):
+                call(i, side.cuda_stream)
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, out)) and torch.isfinite(got[0]).all()
+
+
+def test_calls_from_two_threads(ctx):
+    """Host calls on one cache from two threads: each as it is alone."""
+    import threading
+
+    lay = Layout([700, 90], [2, 2], 32)
+    pg = Pages(ctx, lay, 2, 64, "f16")
+    q = [np.random.default_rng(i).standard_normal((4, 256)).astype(np.float32) for i in range(2)]
+    s = [Seqs(lay.lens, lay.table, lay.starts) for _ in range(2)]
+    want = [pg.cache.attend(0, s[i], q[i]) for i in range(2)]
+    ok = [True, True]
+
+    def work(i):
+        for _ in range(20):
+            ok[i] = ok[i] and np.array_equal(pg.cache.attend(0, s[i], q[i]), want[i])
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert all(ok)
 
 
 def test_growing_under_capture_is_refused():

@@ -139,7 +139,7 @@ def test_append_refuses_negative_positions_on_the_host(cache):
     assert st == INVALID and "position" in msg
 
 
-@pytest.mark.parametrize("scale", [-1.0, float("nan"), float("inf")])
+@pytest.mark.parametrize("scale", [-1.0, float("nan"), float("inf"), 3e38])
 def test_attend_refuses_scales(cache, scale):
     for d in (False, True):
         st, msg = attend(cache, seqs(), scale=scale, d=d)
