@@ -144,7 +144,7 @@ __device__ __forceinline__ void kv_append_rows(const KvAppendArgs& a, int tok, i
           const u4v r = X::pack(v[u]);
           *reinterpret_cast<u2u*>(b + o1[u]) = u2v{r[0], r[1]}, *reinterpret_cast<u2u*>(b + o2[u]) = u2v{r[2], r[3]};
         }
-      } else if (stored) {  // (rows of the cache are 32-byte aligned)
+      } else if (stored) {  // (rows of the cache are 16-byte aligned)
         const u4v r = C::pack(v[u]);
         *reinterpret_cast<u2v*>(kd + o1[u]) = u2v{r[0], r[1]}, *reinterpret_cast<u2v*>(kd + o2[u]) = u2v{r[2], r[3]};
       }
@@ -269,7 +269,7 @@ extern "C" __global__ __launch_bounds__(256) void rtq_kv_keep(KvKeepArgs a) {
   }
   __syncthreads();
   const int n = count;
-  if (blockIdx.y == 0 && hv == 0 && tid == 0 && a.after) a.after[seq] = a.lens[seq] + n;
+  if (blockIdx.y == 0 && hv == 0 && tid == 0 && a.after) a.after[seq] = held + n;
   const int64_t row = (int64_t)a.d << a.ps_shift;  // elements of a head's page
   uint16_t* k = a.k + blockIdx.y * a.layer;
   uint16_t* v = a.v + blockIdx.y * a.layer;
@@ -402,11 +402,12 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, int TM, int block
         it.seq = i, it.row0 = row0, it.cnt = cnt, it.held = held, it.total = total, it.splits = ns, it.C = c;
         it.tile = at / (a.nkv * ns);
         it.hv = (at - it.tile * a.nkv * ns) / ns, it.split = at - (it.tile * a.nkv + it.hv) * ns;
+        const bool found = at >= 0 && it.tile < tiles;  // (sums of sequences that overlap may pass 32 bits)
         // A run's later tiles have more slots: they start first, and where two workgroups a CU take all of them at once, the
         // n-th longest shares its CU with the n-th shortest.
         if (!a.parents) it.tile = n > a.target || 2 * it.tile < tiles ? tiles - 1 - it.tile : it.tile - (tiles + 1) / 2;
         it.slot = ns > 1 ? es + at - it.split : -1;
-        ok = ns == 1 || (it.slot + ns <= a.slots && block - it.split + ns <= (int)gridDim.x);
+        ok = found && (ns == 1 || (it.slot >= 0 && it.slot + ns <= a.slots && block - it.split + ns <= (int)gridDim.x));
         break;
       }
       ei += n, es += ns > 1 ? n : 0;
@@ -470,17 +471,17 @@ constexpr float kKvLag = 6.0f;
 // What an item works on, beside the plan's: its rows and slots
 struct KvTile {
   int row_lo, rows, k_lo, k_hi;
-  bool tail;  // some of its slots hold new tokens
+  bool tail;  // some of its slots hold new tokens (or are the last of a table that has none for them)
 };
 __device__ __forceinline__ KvTile kv_tile(const KvAttendArgs& a, int TM, const KvItem& it) {
   KvTile t;
   const int group = a.group;
   t.row_lo = it.tile * TM, t.rows = min((int)((int64_t)it.cnt * group - t.row_lo), TM);
   t.k_lo = it.split * it.C;
-  // no row of the tile sees a new token after its own
+  // (no row of the tile sees a new token after its own)
   const int64_t last = (int64_t)it.held + (t.row_lo + t.rows - 1) / group + 1;
   t.k_hi = (int)min(min((int64_t)t.k_lo + it.C, (int64_t)it.total), last);
-  t.tail = t.k_hi > it.held;
+  t.tail = t.k_hi >= min(it.held + 1, it.total);
   return t;
 }
 
@@ -543,6 +544,7 @@ __device__ __forceinline__ int kv_row_shift(float mx) {
 // (A row is read again as its call was given it: out may be q itself, whose rows no other workgroup writes.)
 struct KvAgain {
   float qs[256], sc[256], mx[256];
+  int64_t at[256];  // the keys' pages (-1: not seen), looked up once
   uint32_t seen[RTQ_KV_TREE / 32];
   int dead;
 };
@@ -577,18 +579,18 @@ __device__ __forceinline__ void kv_row_again(const KvAttendArgs& a, const KvItem
   for (int k0 = 0; k0 < last && !dead; k0 += 256) {
     const int key = k0 + tid, nw = key - held;
     float s = -INFINITY;
-    bool vis = key < last && (nw < 0 || !a.parents || (seen[(nw & (RTQ_KV_TREE - 1)) >> 5] >> (nw & 31) & 1));
+    int64_t at = -1;
+    const bool vis = key < last && (nw < 0 || !a.parents || (seen[(nw & (RTQ_KV_TREE - 1)) >> 5] >> (nw & 31) & 1));
     if (vis) {
-      const int64_t at = page(key);
-      vis = at >= 0;
-      if (vis) {
+      at = page(key);
+      if (at >= 0) {
         const uint16_t* k = a.k + at + (int64_t)(key & (ps - 1)) * d;
         s = 0.0f;
         for (int c = 0; c < d; c++) s = fmaf(qs[c], conv(k[c]), s);
         s *= a.scale2;
       }
     }
-    mx[tid] = s;
+    mx[tid] = s, sh.at[tid] = at;
     __syncthreads();
     for (int n = 128; n > 0; n >>= 1) {
       if (tid < n) mx[tid] = fmaxf(mx[tid], mx[tid + n]);
@@ -596,14 +598,14 @@ __device__ __forceinline__ void kv_row_again(const KvAttendArgs& a, const KvItem
     }
     const float mn = fmaxf(m, mx[0]), mu = mn == -INFINITY ? 0.0f : mn, al = __builtin_amdgcn_exp2f(m - mu);
     m = mn;
-    sc[tid] = vis ? __builtin_amdgcn_exp2f(s - mu) : -1.0f;
+    sc[tid] = __builtin_amdgcn_exp2f(s - mu);
     __syncthreads();
     l *= al, o *= al;
     for (int j = 0; j < 256; j++) {
       const float p = sc[j];
-      if (p == -1.0f) continue;
+      if (sh.at[j] < 0) continue;
       l += p;
-      if (tid < d) o = fmaf(p, conv(a.v[page(k0 + j) + ((int64_t)tid << a.ps_shift) + ((k0 + j) & (ps - 1))]), o);
+      if (tid < d) o = fmaf(p, conv(a.v[sh.at[j] + ((int64_t)tid << a.ps_shift) + ((k0 + j) & (ps - 1))]), o);
     }
     __syncthreads();
   }
@@ -1003,13 +1005,12 @@ __device__ __forceinline__ int kv_swap(int slot) {
   return CH >= 16 ? row : row >> 1;
 }
 
-template <int CT, bool QF, int D, bool FULL, int NW, int R>
+template <int CT, bool QF, int D, bool FULL, int R>
 __device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
-  constexpr int DK = D / 16, DT = D / 32, CH = D / 8, TM = 32 * NW, T = 64 * NW;
+  constexpr int NW = 4, DK = D / 16, DT = D / 32, CH = D / 8, TM = 32 * NW, T = 64 * NW;
   constexpr int NS = QF ? (CT == VT_F16 ? 2 : 3) : 1, NP = NS;
   constexpr int UK = 32 * CH, UV = D * 4, UNIT = UK + UV;  // chunks
   typedef VRow<QF ? VT_F32 : CT> Q;
-  static_assert(NW == 4, "kv_end");
   struct Main {
     u4v st[R][2][UNIT];
     KvSeen seen[TM];
@@ -1134,8 +1135,6 @@ __device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
     missing[1] = ahead;
     pages(tl.k_lo + 128);
   }
-  // (the waves of a SIMD take turns: one's softmax beside the other's products)
-  if (CT == VT_BF16 && wv < 4) __builtin_amdgcn_s_setprio(1);
   int buf = 0, k0 = tl.k_lo;
   uint32_t lost = 0;
   const auto advance = [&] {
@@ -1266,24 +1265,24 @@ __device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
 
 #define RTQ_KV_ATTEND(SUF, CT, QF, D, FULL, NQ) \
   extern "C" __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void rtq_kv_attend##SUF(KvAttendArgs a) { kv_attend<CT, QF, D, FULL, NQ>(a); }
-#define RTQ_KV_BIG(SUF, CT, QF, D, FULL, NW, R) \
-  extern "C" __global__ __launch_bounds__(64 * NW, 2) void rtq_kv_attend##SUF(KvAttendArgs a) { kv_attend_big<CT, QF, D, FULL, NW, R>(a); }
-#define RTQ_KV_ATTENDS(SUF, CT, QF, NW)              \
-  RTQ_KV_ATTEND(16_64_##SUF, CT, QF, 64, true, 1)    \
-  RTQ_KV_ATTEND(16_128_##SUF, CT, QF, 128, true, 1)  \
+#define RTQ_KV_BIG(SUF, CT, QF, D, FULL, R) \
+  extern "C" __global__ __launch_bounds__(256, 2) void rtq_kv_attend##SUF(KvAttendArgs a) { kv_attend_big<CT, QF, D, FULL, R>(a); }
+#define RTQ_KV_ATTENDS(SUF, CT, QF)                   \
+  RTQ_KV_ATTEND(16_64_##SUF, CT, QF, 64, true, 1)     \
+  RTQ_KV_ATTEND(16_128_##SUF, CT, QF, 128, true, 1)   \
   RTQ_KV_ATTEND(16_128p_##SUF, CT, QF, 128, false, 1) \
   RTQ_KV_ATTEND(16_256p_##SUF, CT, QF, 256, false, 1) \
-  RTQ_KV_ATTEND(32_64_##SUF, CT, QF, 64, true, 2)    \
-  RTQ_KV_ATTEND(32_128_##SUF, CT, QF, 128, true, 2)  \
+  RTQ_KV_ATTEND(32_64_##SUF, CT, QF, 64, true, 2)     \
+  RTQ_KV_ATTEND(32_128_##SUF, CT, QF, 128, true, 2)   \
   RTQ_KV_ATTEND(32_128p_##SUF, CT, QF, 128, false, 2) \
-  RTQ_KV_BIG(_big_64_##SUF, CT, QF, 64, true, 4, 3)    \
-  RTQ_KV_BIG(_big_128_##SUF, CT, QF, 128, true, NW, NW == 4 ? 2 : 3)  \
-  RTQ_KV_BIG(_big_128p_##SUF, CT, QF, 128, false, NW, NW == 4 ? 2 : 3) \
-  RTQ_KV_BIG(_big_256p_##SUF, CT, QF, 256, false, 4, 2)
-RTQ_KV_ATTENDS(f32_f16, VT_F16, true, 4)
-RTQ_KV_ATTENDS(f32_bf16, VT_BF16, true, 4)
-RTQ_KV_ATTENDS(f16, VT_F16, false, 4)
-RTQ_KV_ATTENDS(bf16, VT_BF16, false, 4)
+  RTQ_KV_BIG(_big_64_##SUF, CT, QF, 64, true, 3)      \
+  RTQ_KV_BIG(_big_128_##SUF, CT, QF, 128, true, 2)    \
+  RTQ_KV_BIG(_big_128p_##SUF, CT, QF, 128, false, 2)  \
+  RTQ_KV_BIG(_big_256p_##SUF, CT, QF, 256, false, 2)
+RTQ_KV_ATTENDS(f32_f16, VT_F16, true)
+RTQ_KV_ATTENDS(f32_bf16, VT_BF16, true)
+RTQ_KV_ATTENDS(f16, VT_F16, false)
+RTQ_KV_ATTENDS(bf16, VT_BF16, false)
 
 // the joining kernel: the workgroup of part i of n joins its tile's rows i, i + n, ...
 template <int QT, int CT>

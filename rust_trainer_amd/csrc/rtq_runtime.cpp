@@ -2202,6 +2202,12 @@ rtq_status kv_check_rows(const void* p, int64_t width, int64_t ld, int type, con
   return RTQ_OK;
 }
 
+// a launch holds 2^32 - 1 threads at most
+rtq_status kv_check_grid(int64_t workgroups) {
+  if (workgroups * 256 > 0xffffffffLL) return fail(RTQ_ERR_UNSUPPORTED, "a call of %lld workgroups", (long long)workgroups);
+  return RTQ_OK;
+}
+
 rtq_status kv_check_heads(const rtq_kv_cache* kc, int64_t n, int64_t nh) {
   if (nh < 1 || nh % kc->nkv || nh > 65536 || n * nh > 0x7fffffff)
     return fail(RTQ_ERR_INVALID, "%lld query heads over %lld KV heads", (long long)nh, (long long)kc->nkv);
@@ -2227,6 +2233,7 @@ rtq_status kv_check_append(const rtq_kv_cache* kc, int64_t layer, const rtq_kv_s
   if (n == 0) return RTQ_OK;
   RTQ_TRY(kv_check_rows(k, kc->nkv * kc->d, ldk, type, "k"));
   RTQ_TRY(kv_check_rows(v, kc->nkv * kc->d, ldv, type, "v"));
+  RTQ_TRY(kv_check_grid(n / 4 + RTQ_KV_TARGET + cdiv(n, 32) * kc->nkv));
   if (!q) return RTQ_OK;
   RTQ_TRY(kv_check_heads(kc, n, nh));
   RTQ_TRY(kv_check_rows(q, nh * kc->d, ldq, type, "q"));
@@ -2257,8 +2264,8 @@ rtq_status enqueue_append(rtq_kv_cache* kc, int64_t layer, const KvSeqs& s, int 
 }
 
 // The attention's tiles and partial parts.  Rows of a sequence and KV head average n group / b: tiles of 16 up to
-// that, of 32 (whose registers a head size above 128 has not), else large ones.  `target` items keep every
-// CU's resident workgroups busy; the split tiles' items are at most twice that (each but a tile's last covers C keys).
+// that, of 32 (whose registers a head size above 128 has not), else large ones of 128.  `target` items keep every
+// CU's two resident workgroups busy; the split tiles' items are at most twice that (each but a tile's last covers C keys).
 struct AttendPlan {
   int tm, variant, D;
   bool fused;
@@ -2277,7 +2284,7 @@ AttendPlan attend_plan(const rtq_kv_cache* kc, int64_t n, int64_t b, int64_t ld,
   } else {
     p.tm = 128, p.variant = 7 + size;
   }
-  p.target = std::min(kc->ctx->cu_count * 2, RTQ_KV_TARGET);
+  p.target = kc->ctx ? std::min(kc->ctx->cu_count * 2, RTQ_KV_TARGET) : RTQ_KV_TARGET;
   p.tiles = (cdiv(rows, p.tm) + b) * kc->nkv;
   // a tile's rows times its parts, at most: what one workgroup reads again (up to 256 rows in the time that another kernel takes)
   const int64_t parts = std::min(cdiv(ld * kc->ps, 128), p.target / kc->nkv + 1);
@@ -2293,7 +2300,9 @@ rtq_status kv_check_attend(const rtq_kv_cache* kc, int64_t layer, const rtq_kv_s
   if (!(scale >= 0.0f && scale <= 1e38f)) return fail(RTQ_ERR_INVALID, "attention scale %g", (double)scale);
   if (n == 0) return RTQ_OK;
   RTQ_TRY(kv_check_rows(q, nh * kc->d, ldq, type, "q"));
-  return kv_check_rows(out, nh * kc->d, ldo, type, "out");
+  RTQ_TRY(kv_check_rows(out, nh * kc->d, ldo, type, "out"));
+  const AttendPlan p = attend_plan(kc, n, s->b, s->ld, nh);
+  return kv_check_grid(p.target + p.tiles);
 }
 
 rtq_status enqueue_attend(rtq_kv_cache* kc, int64_t layer, const KvSeqs& s, int type, int64_t nh, float scale, const int32_t* parents,
@@ -2319,7 +2328,7 @@ rtq_status kv_check_keep(const rtq_kv_cache* kc, const rtq_kv_seqs* s, const int
   if (ldk < 1 || ldk > RTQ_TREE_MAX) return fail(RTQ_ERR_INVALID, "%lld kept tokens", (long long)ldk);
   if (!kept) return fail(RTQ_ERR_INVALID, "null kept");
   if (after && after < s->lens + s->b && s->lens < after + s->b) return fail(RTQ_ERR_INVALID, "lens_out overlaps lens");
-  return RTQ_OK;
+  return kv_check_grid(s->b * kc->nkv);
 }
 
 rtq_status enqueue_keep(rtq_kv_cache* kc, const KvSeqs& s, const int32_t* kept, int64_t ldk, int32_t* after, hipStream_t st) {

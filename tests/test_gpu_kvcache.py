@@ -494,6 +494,38 @@ def test_more_tokens_than_the_table_holds(ctx):
     for i in range(2):  # (the last held token as the one new token of its row: the row sees all 64)
         want, bound = attend(q[i:i + 1].astype(np.float64), k, v, 63, 1)
         assert np.all(np.abs(out[i:i + 1].cpu().numpy() - want) <= bound + EPS["f32"] * (np.abs(want) + bound))
+    # a tree whose tokens have no slots: chains that end well see the held tokens, others nothing (small and large tiles)
+    for heads in (1, 70):
+        par = torch.tensor([-1, 5], dtype=torch.int32, device="cuda")
+        q2 = rows_d(np.random.default_rng(1).standard_normal((2, heads * 64)).astype(np.float32))
+        o2 = torch.full((2, heads * 64), 7.0, device="cuda")
+        pg.cache.attend_d(0, s, 2, 0, heads, q2.data_ptr(), heads * 64, o2.data_ptr(), heads * 64, par.data_ptr(), 0.0, stream())
+        got = o2.cpu().numpy()
+        want, bound = attend(q2[:1].cpu().numpy().astype(np.float64), k, v, 63, heads)
+        assert np.all(np.abs(got[:1] - want) <= bound + EPS["f32"] * (np.abs(want) + bound)) and not got[1].any()
+
+
+def test_sequences_that_overlap_stay_in_bounds(ctx):
+    """Starts that fall and rise name the same rows for many sequences, more tiles than the call was planned for: rows are left
+    out or written more than once, and nothing behind them is touched."""
+    b, n = 64, 40
+    lay = Layout([700] * b, [0] * b, 32, wide=2)
+    pg = Pages(ctx, lay, 1, 64, "f16")
+    starts = torch.tensor([0, n] * (b // 2) + [0], dtype=torch.int32, device="cuda")
+    s = seqs_d(b, pg.lens.data_ptr(), pg.table.data_ptr(), lay.table.shape[1], starts.data_ptr())
+    for heads in (1, 8):
+        q = torch.randn(n, heads * 64, device="cuda")
+        buf = torch.full((n + 8, heads * 64), 7.0, device="cuda")
+        pg.cache.attend_d(0, s, n, 0, heads, q.data_ptr(), heads * 64, buf[4:].data_ptr(), heads * 64, 0, 0.0, stream())
+        torch.cuda.synchronize()
+        assert (buf[:4] == 7).all() and (buf[n + 4:] == 7).all() and torch.isfinite(buf).all()
+    # a call of an ordinary sequence after it is as ever
+    s1 = seqs_d(1, pg.lens.data_ptr(), pg.table.data_ptr(), lay.table.shape[1])
+    q, out = torch.randn(1, 64, device="cuda"), torch.zeros(1, 64, device="cuda")
+    pg.cache.attend_d(0, s1, 1, 0, 1, q.data_ptr(), 64, out.data_ptr(), 64, 0, 0.0, stream())
+    k, v = pg.rows(0, 701)
+    want, bound = attend(q.cpu().numpy().astype(np.float64), k, v, 700, 1)
+    assert np.all(np.abs(out.cpu().numpy() - want) <= bound + EPS["f32"] * (np.abs(want) + bound))
 
 
 # ------------------------------------------------------------------ keep

@@ -169,6 +169,21 @@ def test_a_large_tree_is_refused_on_the_host():
     _ffi.lib().rtq_kv_cache_destroy(h)
 
 
+def test_calls_of_more_threads_than_a_launch_holds():
+    st, h = create(kv=1024, d=16)
+    L, b, n = _ffi.lib(), 65536, 65536
+    lens, table = np.zeros(b, np.int32), np.zeros((b, 1), np.int32)
+    s = _ffi.RtqKvSeqs(b, lens.ctypes.data, None, table.ctypes.data, 1)
+    p, ld = lens.ctypes.data, 1024 * 16
+    for n_big, call in ((n, lambda n: L.rtq_kv_attend_d(h, 0, ctypes.byref(s), n, F32, 1024, 0.0, None, p, ld, p, ld, None)),
+                        (2 ** 20, lambda n: L.rtq_kv_append_d(h, 0, ctypes.byref(s), n, F32, ctypes.byref(rope(dim=16)), None, p, ld, p, ld, 0, None, 0, None, 0, None)),
+                        (0, lambda n: L.rtq_kv_keep_d(h, ctypes.byref(s), p, 1, None, None))):
+        assert call(n_big) == UNSUPPORTED and "workgroups" in L.rtq_last_error().decode()
+    s.b = 4096
+    assert L.rtq_kv_keep_d(h, ctypes.byref(s), p, 1, None, None) == INVALID and "context" in L.rtq_last_error().decode()
+    L.rtq_kv_cache_destroy(h)
+
+
 def keep(cache, s, kept, ldk=None, after=True, d=False, alias=False):
     a = np.array(kept, np.int32)
     out = np.zeros(2, np.int32)
