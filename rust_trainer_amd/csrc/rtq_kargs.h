@@ -666,8 +666,9 @@ struct KvAttendArgs {
   const int32_t* parents;  // [n] or null: runs
   int nkv, group, d, ps_shift, n_pages;  // group: query heads a KV head
   float scale2;     // scale log2(e)
-  int target;       // items that the keys are split into (at most this many, and one per tile beside)
+  int target, once; // items that the keys are split into (at most this many, and one per tile beside), that run at once
   int slots;        // partial slots
+  int whole;        // sequences of up to this many slots are not split
   int tm, D;        // rows of a tile, elements of a part's row
   int fused;        // split tiles are joined by their last workgroup, not by a kernel behind it
   float* part;      // [slots][rows of a tile][D]

@@ -20,10 +20,16 @@ __device__ __forceinline__ int kv_held(const int32_t* lens, int i, int ldt, int 
 }
 
 // ------------------------------------------------------------------ append
+// y = x inv_rms (w + off), then pairs (y1, y2) turned by position x freq: (y1 c - y2 s, y2 c + y1 s).  Every element is read
+// and written once: copies bound it (16384 tokens of 16 query and 8 KV heads of 128, f32: 103 us, 4.5 TB/s of a copy's
+// 4.7), and a few tokens their launch (5.6 us).
+//
 // 16 lanes take a head, a lane eight of its elements at a time (a unit: the two sides of four pairs, or eight in a
 // row), a wave four heads.  Few tokens take a workgroup each, its waves sharing the heads; many take a wave
 // each.  The angles are turns: position x freq in 64 bits, of which the whole turns are dropped before sine and cosine
 // are taken in 32 (at position 10^5 a 32-bit angle is off by 4e-3), once per lane and pair for all of its heads.
+// Values are turned over in LDS, 32 tokens of a head at a time: a token's elements lie a page row apart, and
+// stored by themselves they were 2-byte stores (200 us for the call above).
 __device__ __forceinline__ void kv_turn(double pos, double freq, float& c, float& s) {
   double t = pos * freq;
   t -= rint(t);
@@ -244,6 +250,9 @@ RTQ_KV_APPEND(rtq_kv_append_f16, VT_F16, VT_F16)
 RTQ_KV_APPEND(rtq_kv_append_bf16, VT_BF16, VT_BF16)
 
 // ------------------------------------------------------------------ keep
+// A few rows are moved within the cache: what bounds it is that a token's values are 2 bytes of each of d rows, so that a
+// 64-byte piece is read and written for each (32 sequences, 8 tokens of 63 kept, 28 layers of 8 heads of 128: 22 us,
+// 12.5 at a copy's rate for the bytes alone; one sequence: 4.3 us).
 // Workgroup: one KV head of one sequence and layer.  Kept tokens ascend, so the j-th comes from a slot no
 // earlier than its own: a wave that moves its elements in batches of eight tokens, in order, each batch's loads before its
 // stores, never writes a slot that it has yet to read, and no two waves touch the same elements.  Values: eight
@@ -312,15 +321,27 @@ extern "C" __global__ __launch_bounds__(256) void rtq_kv_keep(KvKeepArgs a) {
 }
 
 // ------------------------------------------------------------------ attention
+// o = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q k_j - m), m the running maximum: one pass over the keys and values.
 // Rows of one (sequence, KV head): its new tokens x the head's group of query heads, token by token; a tile
-// takes TM of them.  The keys of a tile are split into ranges of C slots (one C for the call, chosen on the
-// device from the sequences' lengths, so that about `target` items are made in all: the host does not
-// know the lengths); an item is a tile and a range.  Tiles of one range leave o directly, others leave an
-// unnormalised sum, the maximum and the sum of the weights, which rtq_kv_merge joins.
+// takes TM of them, so that a group reads its keys once.  The keys of a tile are split into ranges of C slots (one C for the
+// call, chosen on the device from the sequences' lengths: the host does not know them); an item is a tile and a range.  Tiles
+// of one range leave o directly, others an unnormalised sum, the maximum and the sum of the weights, which are
+// joined by the tile's last workgroup or by a kernel behind.
+//
+// Small tiles (16 rows: single tokens and narrow trees) are bound by the reading of the cache: 64 sequences of up to
+// 8192 tokens, 32 over 8 heads of 128, 1.15 GB: 259 us, 4.4 TB/s; one of 131072: 97 us, 5.5 TB/s (some of it still cached);
+// one of 1000: 14 us, of which the reading takes 1: each item is a chain of dependent loads (lengths, page, keys, values).
+// Large ones (128 rows) are bound by the matrix instructions and the weights between them, which overlap little: 2048
+// tokens behind 6144, 32 over 8 heads of 128: 245 us, 0.98 PFLOP/s of a large product's 1.2, the matrix units busy 53% of
+// the time, at the 1.7 GHz that such work runs at.  (Scores of the next block issued beside a block's weights: the same.)
 //
 // A wave takes 32 slots at a time.  S^T = K q^T and o^T = V^T p^T, so that a lane holds one query row:
 // key row m of tile t is slot 8 (m / 4) + 4 t + m % 4, and the lane that gets the scores of slots 8 g .. 8 g + 7
 // holds them in the order in which it feeds them to the second product: the weights never leave their lane.
+//
+// Weights are rounded to the cache's 16 bits for the second product, in two planes (three of f32 rows over bf16) that keep
+// 16 to 22 bits of them; a large tile of 16-bit rows takes one plane, half a step of that type in a weight of at most
+// 1, as its rows are rounded anyway: a second would be half as many matrix instructions again.  Sums stay in 32 bits.
 struct KvItem {
   int seq, row0, cnt, held, total, tile, hv, split, splits, slot, C;  // slot: of the tile's first part (-1: one part)
 };
@@ -367,25 +388,53 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, int TM, int block
     total = (int)min((int64_t)held + cnt, min((int64_t)a.s.ldt << a.ps_shift, (int64_t)RTQ_KV_SLOTS));
     tiles = (int)(((int64_t)cnt * group + TM - 1) / TM);
   };
-  float w = 0.0f;
+  float w = 0.0f, whole = 0.0f;
   for (int i = i0; i < i1; i++) {
     look(i);
-    w += (float)tiles * (float)total;
+    w += (float)tiles * (float)total, whole += (float)tiles;
   }
-  w = kv_wave_total(w);
-  const int C = max((int)fminf(ceilf(w * (float)a.nkv / (float)a.target / 128.0f), (float)(RTQ_KV_SLOTS / 128)) * 128, 128);
   // a sequence's slots a part, parts
-  const auto cut = [&](int& c, int& ns) {
+  const auto cut = [&](int C, int& c, int& ns) {
     const int64_t least = a.fused ? (int64_t)total * min(max(cnt, 1) * a.group, TM) : total;
     c = max(C, (int)(((least + kKvJoin - 1) / kKvJoin + 127) & ~127));
-    // joining costs a small tile as much as four more turns of its waves (token over 250: 12.8 us in two parts, 9.9 in one)
-    if (TM <= 32 && total <= 512) c = max(c, 512);
+    if (total <= a.whole) c = max(c, a.whole);
     ns = max((total + c - 1) / c, 1);
   };
-  int items = 0, slots = 0, c, ns;
+  // Ranges of about even x 128 slots share the slots out evenly over the items that run at once.  With few tiles
+  // that is it.  With more, what their last ranges leave over makes a second turn of the CUs: then the shortest ranges (of
+  // some) are taken with which all items run at once (32 sequences of 1000 to 7000, 64 rows: 162 -> 133 us).  Tiles that
+  // nearly fill the CUs are not split at all, unless one is far longer than the others (32 of 250 to 1750, 4 rows: 42 -> 34
+  // us; 32 of 75 to 525, 256 rows: 60 -> 36).  Small tiles of long sequences are read evenly by more and shorter ranges,
+  // a second turn or not (32 of 4000 to 28000: 457 us against 550 unsplit).
+  const float even = kv_wave_total(w) * (float)a.nkv / (float)a.once / 128.0f, most = kv_wave_total(whole) * (float)a.nkv;
+  const auto range = [&](float f) { return max((int)fminf(ceilf(even * f), (float)(RTQ_KV_SLOTS / 128)) * 128, 128); };
+  int C = range(1.0f), c, ns;
+  if (TM == 16 && C > 2048) {
+    if (most * 2.0f >= (float)a.once) C = range((float)a.once / (float)a.target);
+  } else if (most * 16.0f > (float)a.once) {
+    constexpr float kTry[] = {1.0f, 1.25f, 1.5f, 2.0f, 3.0f, 4.0f};
+    float n[6] = {}, inv[6];  // items of each (about)
+#pragma unroll
+    for (int f = 0; f < 6; f++) inv[f] = __builtin_amdgcn_rcpf((float)range(kTry[f]));
+    for (int i = i0; i < i1; i++) {
+      if (per > 1) look(i);
+#pragma unroll
+      for (int f = 0; f < 6; f++) n[f] += (float)tiles * (total <= a.whole ? 1.0f : ceilf((float)total * inv[f]));
+    }
+#pragma unroll
+    for (int f = 0; f < 6; f++) n[f] = kv_wave_total(n[f]) * (float)a.nkv;
+    if (most * (TM == 16 ? 2.0f : 1.0f) >= (float)a.once && n[5] <= most) {
+      C = range(kTry[5]);
+    } else {
+#pragma unroll
+      for (int f = 4; f >= 0; f--)
+        if (n[f] <= (float)a.once) C = range(kTry[f]);
+    }
+  }
+  int items = 0, slots = 0;
   for (int i = i0; i < i1; i++) {
     if (per > 1) look(i);
-    cut(c, ns);
+    cut(C, c, ns);
     items += tiles * a.nkv * ns, slots += ns > 1 ? tiles * a.nkv * ns : 0;
   }
   int ei = kv_wave_scan(items) - items, es = kv_wave_scan(slots) - slots;
@@ -395,7 +444,7 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, int TM, int block
   if (block >= ei && block < ei + items) {
     for (int i = i0; i < i1; i++) {
       if (per > 1) look(i);
-      cut(c, ns);
+      cut(C, c, ns);
       const int n = tiles * a.nkv * ns;
       if (block < ei + n) {
         const int at = block - ei;  // tile by tile, so that a range's tiles are a multiple of the XCDs apart
@@ -405,7 +454,7 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, int TM, int block
         const bool found = at >= 0 && it.tile < tiles;  // (sums of sequences that overlap may pass 32 bits)
         // A run's later tiles have more slots: they start first, and where two workgroups a CU take all of them at once, the
         // n-th longest shares its CU with the n-th shortest.
-        if (!a.parents) it.tile = n > a.target || 2 * it.tile < tiles ? tiles - 1 - it.tile : it.tile - (tiles + 1) / 2;
+        if (!a.parents) it.tile = n > a.once || 2 * it.tile < tiles ? tiles - 1 - it.tile : it.tile - (tiles + 1) / 2;
         it.slot = ns > 1 ? es + at - it.split : -1;
         ok = found && (ns == 1 || (it.slot >= 0 && it.slot + ns <= a.slots && block - it.split + ns <= (int)gridDim.x));
         break;
@@ -748,10 +797,10 @@ __device__ __forceinline__ void kv_end(const KvAttendArgs& a, const KvItem& it, 
   kv_rows_again<QT, CT>(a, it, t, 0, 1, nan, sh.again);
 }
 
-// ---- small tiles: 16 or 32 rows, four waves that share the tile's slots, operands straight from the cache
-template <int CT, bool QF, int D, bool FULL, int NQ>
+// ---- small tiles: 16 rows, four waves that share the tile's slots, operands straight from the cache
+template <int CT, bool QF, int D, bool FULL>
 __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
-  constexpr int DC = D / 32, DT = D / 16, TM = 16 * NQ, LDR = D + 4;
+  constexpr int DC = D / 32, DT = D / 16, TM = 16, LDR = D + 4;
   constexpr int NS = QF ? (CT == VT_F16 ? 2 : 3) : 1, NP = QF ? NS : 2;
   typedef VRow<QF ? VT_F32 : CT> Q;
   struct Main {
@@ -774,10 +823,7 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
   const KvTile tl = kv_tile(a, TM, it);
   const int row_lo = tl.row_lo, rows = tl.rows, k_hi = tl.k_hi;
   const bool tree = a.parents != nullptr;
-  // the token (index among the sequence's new ones) of each of this lane's columns
-  int tok[NQ];
-#pragma unroll
-  for (int n = 0; n < NQ; n++) tok[n] = (row_lo + min(16 * n + li, rows - 1)) / group;
+  const int row = row_lo + min(li, rows - 1), tok = row / group;  // of this lane's column (tok: among the sequence's new tokens)
   const int64_t head = (int64_t)d << a.ps_shift, pstride = head * a.nkv;
   const auto page_of = [&](int k0) { return kv_page(a.s, it.seq, k0, a.ps_shift); };
   const auto base_of = [&](int pg) { return ((unsigned)pg < (unsigned)a.n_pages ? pg : 0) * pstride + it.hv * head; };
@@ -808,76 +854,64 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
     load_v(k0, pg);
   }
   constexpr bool SCALED = QF && CT == VT_F16;
-  u4v qf[NS][NQ][DC];
-  float sc[NQ];
+  u4v qf[NS][DC];
+  const int64_t at = (int64_t)(it.row0 + tok) * a.ldq + (int64_t)(it.hv * group + row % group) * d;
+  float sc = a.scale2, x[QF ? DC : 1][8] = {};
 #pragma unroll
-  for (int n = 0; n < NQ; n++) {
-    const int r = row_lo + min(16 * n + li, rows - 1);
-    const int64_t at = (int64_t)(it.row0 + tok[n]) * a.ldq + (int64_t)(it.hv * group + r % group) * d;
-    sc[n] = a.scale2;
-    float x[QF ? DC : 1][8] = {};
+  for (int c = 0; c < DC; c++) {
+    const bool in = (FULL || 32 * c + 8 * g < d) && li < rows;
+    if constexpr (QF) {
+      if (in) {
+        const u4v r1 = Q::load(a.q, at + 32 * c + 8 * g), r2 = Q::load(a.q, at + 32 * c + 8 * g + 4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[c][e] = Q::get(r1, e), x[c][4 + e] = Q::get(r2, e);
+      }
+    } else {
+      qf[0][c] = u4v{0, 0, 0, 0};
+      if (in) qf[0][c] = Q::load(a.q, at + 32 * c + 8 * g);
+    }
+  }
+  if constexpr (QF) {
+    int up = 0;
+    if constexpr (SCALED) {
+      float mx = 0.0f;
+#pragma unroll
+      for (int c = 0; c < DC; c++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[c][e]));
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      up = kv_row_shift(mx);
+      sc = ldexpf(a.scale2, -up);
+    }
 #pragma unroll
     for (int c = 0; c < DC; c++) {
-      const bool in = (FULL || 32 * c + 8 * g < d) && 16 * n + li < rows;
-      if constexpr (QF) {
-        if (in) {
-          const u4v r1 = Q::load(a.q, at + 32 * c + 8 * g), r2 = Q::load(a.q, at + 32 * c + 8 * g + 4);
+      if constexpr (SCALED)
 #pragma unroll
-          for (int e = 0; e < 4; e++) x[c][e] = Q::get(r1, e), x[c][4 + e] = Q::get(r2, e);
-        }
-      } else {
-        qf[0][n][c] = u4v{0, 0, 0, 0};
-        if (in) qf[0][n][c] = Q::load(a.q, at + 32 * c + 8 * g);
-      }
-    }
-    if constexpr (QF) {
-      int up = 0;
-      if constexpr (SCALED) {
-        float mx = 0.0f;
+        for (int e = 0; e < 8; e++) x[c][e] = ldexpf(x[c][e], up);
+      u4v pl[NS];
+      kv_planes<CT, NS>(x[c], pl);
 #pragma unroll
-        for (int c = 0; c < DC; c++)
-#pragma unroll
-          for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[c][e]));
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        up = kv_row_shift(mx);
-        sc[n] = ldexpf(a.scale2, -up);
-      }
-#pragma unroll
-      for (int c = 0; c < DC; c++) {
-        if constexpr (SCALED)
-#pragma unroll
-          for (int e = 0; e < 8; e++) x[c][e] = ldexpf(x[c][e], up);
-        u4v pl[NS];
-        kv_planes<CT, NS>(x[c], pl);
-#pragma unroll
-        for (int i = 0; i < NS; i++) qf[i][n][c] = pl[i];
-      }
+      for (int i = 0; i < NS; i++) qf[i][c] = pl[i];
     }
   }
   if (tree && tl.tail) kv_tree<TM, 256>(a, it, tl, sh.seen, sh.up);
   const int tok0 = row_lo / group;
 
-  f4 acc[NQ][DT];
-  float m[NQ], l[NQ];
+  f4 acc[DT];
+  float m = -INFINITY, l = 0.0f;
 #pragma unroll
-  for (int n = 0; n < NQ; n++) {
-    m[n] = -INFINITY, l[n] = 0.0f;
-#pragma unroll
-    for (int t = 0; t < DT; t++) acc[n][t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  for (int t = 0; t < DT; t++) acc[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
   for (; k0 < k_hi; k0 += 128) {
-    f4 s[NQ][2];
+    f4 s[2];
 #pragma unroll
-    for (int n = 0; n < NQ; n++)
+    for (int t = 0; t < 2; t++) {
+      s[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int t = 0; t < 2; t++) {
-        s[n][t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int c = 0; c < DC; c++)
 #pragma unroll
-        for (int c = 0; c < DC; c++)
-#pragma unroll
-          for (int p = 0; p < NS; p++) s[n][t] = kv_mfma<CT>(kf[t][c], qf[p][n][c], s[n][t]);
-      }
+        for (int p = 0; p < NS; p++) s[t] = kv_mfma<CT>(kf[t][c], qf[p][c], s[t]);
+    }
     const int kn = k0 + 128 < k_hi ? k0 + 128 : k0;  // (the last step loads its own slots again)
     const int pgn = k0 + 128 < k_hi ? pn : pg;
     load_k(kn, pgn);
@@ -885,80 +919,65 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
     const bool there = (unsigned)pg < (unsigned)a.n_pages;
     if (k0 + 32 > it.held || k0 + 32 > k_hi || !there) {
       const int here = there ? min(max(k_hi - k0 - 8 * g, 0), 8) : 0;  // of the lane's eight slots
+      uint32_t bits = tree && tl.tail ? kv_tree_bits(k0 - it.held, sh.seen[tok - tok0]) : kv_run_bits(k0 - it.held, tok);
+      bits = bits >> (8 * g) & ((1u << here) - 1);
+      if (li >= rows) bits = 0;
 #pragma unroll
-      for (int n = 0; n < NQ; n++) {
-        const int r = 16 * n + li;
-        uint32_t bits = tree && tl.tail ? kv_tree_bits(k0 - it.held, sh.seen[tok[n] - tok0]) : kv_run_bits(k0 - it.held, tok[n]);
-        bits = bits >> (8 * g) & ((1u << here) - 1);
-        if (r >= rows) bits = 0;
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (!(bits >> e & 1)) s[n][e >> 2][e & 3] = -INFINITY;
-      }
+      for (int e = 0; e < 8; e++)
+        if (!(bits >> e & 1)) s[e >> 2][e & 3] = -INFINITY;
       // what lies behind the last token may be anything, NaN too: zeros, so that its weight 0 makes 0 of it
 #pragma unroll
       for (int t = 0; t < DT; t++)
         if (FULL || 16 * t < d) vf[t] = kv_clear(vf[t], here);
     }
-    u4v pf[NQ][NP];
+    u4v pf[NP];
+    float mx = s[0][0], p[8];
 #pragma unroll
-    for (int n = 0; n < NQ; n++) {
-      float mx = s[n][0][0], p[8];
+    for (int e = 1; e < 8; e++) mx = fmaxf(mx, s[e >> 2][e & 3]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16));
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const float mn = fmaxf(m, mx * sc), mu = mn == -INFINITY ? 0.0f : mn;
+    const float al = __builtin_amdgcn_exp2f(m - mu);
+    m = mn;
+    float sum = 0.0f;
 #pragma unroll
-      for (int e = 1; e < 8; e++) mx = fmaxf(mx, s[n][e >> 2][e & 3]);
-      mx = fmaxf(mx, __shfl_xor(mx, 16));
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      const float mn = fmaxf(m[n], mx * sc[n]), mu = mn == -INFINITY ? 0.0f : mn;
-      const float al = __builtin_amdgcn_exp2f(m[n] - mu);
-      m[n] = mn;
-      float sum = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        p[e] = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][e & 3], sc[n], kKvUp<CT> - mu));
-        sum += p[e];
-      }
-      l[n] = l[n] * al + sum;
-      if (__any(al != 1.0f)) {
-#pragma unroll
-        for (int t = 0; t < DT; t++) acc[n][t] *= al;
-      }
-      kv_planes<CT, NP>(p, pf[n]);
+    for (int e = 0; e < 8; e++) {
+      p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], sc, kKvUp<CT> - mu));
+      sum += p[e];
     }
+    l = l * al + sum;
+    if (__any(al != 1.0f)) {
+#pragma unroll
+      for (int t = 0; t < DT; t++) acc[t] *= al;
+    }
+    kv_planes<CT, NP>(p, pf);
 #pragma unroll
     for (int t = 0; t < DT; t++)
       if (FULL || 16 * t < d)
 #pragma unroll
-        for (int n = 0; n < NQ; n++)
-#pragma unroll
-          for (int q = 0; q < NP; q++) acc[n][t] = kv_mfma<CT>(vf[t], pf[n][q], acc[n][t]);
+        for (int q = 0; q < NP; q++) acc[t] = kv_mfma<CT>(vf[t], pf[q], acc[t]);
     load_v(kn, pgn);
     pg = pgn;
   }
   // the four waves' parts
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  int nan = 0;
 #pragma unroll
-  for (int n = 0; n < NQ; n++) {
-    l[n] += __shfl_xor(l[n], 16);
-    l[n] += __shfl_xor(l[n], 32);
-    int nan = 0;
+  for (int t = 0; t < DT; t++)
 #pragma unroll
-    for (int t = 0; t < DT; t++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) nan |= (FULL || 16 * t < d) && acc[n][t][r] != acc[n][t][r];
-    nan |= __shfl_xor(nan, 16);
-    nan |= __shfl_xor(nan, 32);
-    if (g == 0) sh.ml[wv][16 * n + li][0] = m[n], sh.ml[wv][16 * n + li][1] = nan ? NAN : l[n];
-  }
+    for (int r = 0; r < 4; r++) nan |= (FULL || 16 * t < d) && acc[t][r] != acc[t][r];
+  nan |= __shfl_xor(nan, 16);
+  nan |= __shfl_xor(nan, 32);
+  if (g == 0) sh.ml[wv][li][0] = m, sh.ml[wv][li][1] = nan ? NAN : l;
   __syncthreads();
+  float top = -INFINITY;
 #pragma unroll
-  for (int n = 0; n < NQ; n++) {
-    float mx = -INFINITY;
+  for (int w = 0; w < 4; w++) top = fmaxf(top, sh.ml[w][li][0]);
+  const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
 #pragma unroll
-    for (int w = 0; w < 4; w++) mx = fmaxf(mx, sh.ml[w][16 * n + li][0]);
-    const float f = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[n] - mx);
-#pragma unroll
-    for (int t = 0; t < DT; t++)
-      if (FULL || 16 * t < d) *reinterpret_cast<f4*>(&sh.o[wv][16 * n + li][16 * t + 4 * g]) = acc[n][t] * f;
-  }
+  for (int t = 0; t < DT; t++)
+    if (FULL || 16 * t < d) *reinterpret_cast<f4*>(&sh.o[wv][li][16 * t + 4 * g]) = acc[t] * f;
   __syncthreads();
   const int vecs = d / 4, slot = it.slot + it.split;
   for (int i = threadIdx.x; i < rows * vecs; i += 256) {
@@ -989,10 +1008,10 @@ __device__ __forceinline__ void kv_attend(const KvAttendArgs& a) {
   kv_end<QF ? VT_F32 : CT, CT, D, TM>(a, it, tl, nan_row, &is_last, all.end);
 }
 
-// ---- large tiles: 32 rows a wave, 64 slots at a time through LDS for all of them
+// ---- large tiles: four waves of 32 rows, 64 slots at a time through LDS for all of them
 //
-// The tile's keys and values reach LDS by buffer loads with the LDS destination, into a ring of R buffers: the next
-// 64 or 128 slots are on their way while these are multiplied.  A unit is 32 slots (of one page): keys [slot][d / 8] and
+// The tile's keys and values reach LDS by buffer loads with the LDS destination, into a ring of R buffers (what
+// two workgroups a CU leave room for: 3 at a head size of 64, else 2): the next slots are on their way while these are multiplied.  A unit is 32 slots (of one page): keys [slot][d / 8] and
 // values [d][4] of 16-byte chunks, a chunk's place swapped by its row so that 16 lanes' reads fall on different
 // banks (64 of 4 bytes); loads past a head's page (rows of a smaller head size, pages that are not there) give zeros.
 // MFMA 32x32x16, again S^T = K q^T and o^T = V^T p^T: key row m of a unit is slot 16 (m / 16) + 8 (m / 4 % 2) +
@@ -1160,6 +1179,7 @@ __device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
       s[u] = f16v{};
 #pragma unroll
       for (int c = 0; c < DK; c++) {
+        if (!FULL && 16 * c >= d) break;
         const u4v kf = kt[(2 * c + h) ^ kx];
 #pragma unroll
         for (int p = 0; p < NS; p++) s[u] = kv_mfma32<CT>(kf, qf[p][c], s[u]);
@@ -1209,6 +1229,7 @@ __device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
       const u4v* vt = sh.st[buf][g >> 1] + UK + q32 * 4;
 #pragma unroll
       for (int t = 0; t < DT; t++) {
+        if (!FULL && 32 * t >= d) break;
         u4v vf = vt[128 * t + ((2 * (g & 1) + h) ^ vx)];
         if constexpr (MASKED) vf = kv_clear(vf, min(max(here - 16 * g - 8 * h, 0), 8));
 #pragma unroll
@@ -1263,21 +1284,18 @@ __device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
   kv_end<QF ? VT_F32 : CT, CT, D, TM>(a, it, tl, all.end.nan_row, &all.end.is_last, all.end.e);
 }
 
-#define RTQ_KV_ATTEND(SUF, CT, QF, D, FULL, NQ) \
-  extern "C" __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void rtq_kv_attend##SUF(KvAttendArgs a) { kv_attend<CT, QF, D, FULL, NQ>(a); }
+#define RTQ_KV_ATTEND(SUF, CT, QF, D, FULL) \
+  extern "C" __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void rtq_kv_attend##SUF(KvAttendArgs a) { kv_attend<CT, QF, D, FULL>(a); }
 #define RTQ_KV_BIG(SUF, CT, QF, D, FULL, R) \
   extern "C" __global__ __launch_bounds__(256, 2) void rtq_kv_attend##SUF(KvAttendArgs a) { kv_attend_big<CT, QF, D, FULL, R>(a); }
-#define RTQ_KV_ATTENDS(SUF, CT, QF)                   \
-  RTQ_KV_ATTEND(16_64_##SUF, CT, QF, 64, true, 1)     \
-  RTQ_KV_ATTEND(16_128_##SUF, CT, QF, 128, true, 1)   \
-  RTQ_KV_ATTEND(16_128p_##SUF, CT, QF, 128, false, 1) \
-  RTQ_KV_ATTEND(16_256p_##SUF, CT, QF, 256, false, 1) \
-  RTQ_KV_ATTEND(32_64_##SUF, CT, QF, 64, true, 2)     \
-  RTQ_KV_ATTEND(32_128_##SUF, CT, QF, 128, true, 2)   \
-  RTQ_KV_ATTEND(32_128p_##SUF, CT, QF, 128, false, 2) \
-  RTQ_KV_BIG(_big_64_##SUF, CT, QF, 64, true, 3)      \
-  RTQ_KV_BIG(_big_128_##SUF, CT, QF, 128, true, 2)    \
-  RTQ_KV_BIG(_big_128p_##SUF, CT, QF, 128, false, 2)  \
+#define RTQ_KV_ATTENDS(SUF, CT, QF)                  \
+  RTQ_KV_ATTEND(16_64_##SUF, CT, QF, 64, true)       \
+  RTQ_KV_ATTEND(16_128_##SUF, CT, QF, 128, true)     \
+  RTQ_KV_ATTEND(16_128p_##SUF, CT, QF, 128, false)   \
+  RTQ_KV_ATTEND(16_256p_##SUF, CT, QF, 256, false)   \
+  RTQ_KV_BIG(_big_64_##SUF, CT, QF, 64, true, 3)     \
+  RTQ_KV_BIG(_big_128_##SUF, CT, QF, 128, true, 2)   \
+  RTQ_KV_BIG(_big_128p_##SUF, CT, QF, 128, false, 2) \
   RTQ_KV_BIG(_big_256p_##SUF, CT, QF, 256, false, 2)
 RTQ_KV_ATTENDS(f32_f16, VT_F16, true)
 RTQ_KV_ATTENDS(f32_bf16, VT_BF16, true)

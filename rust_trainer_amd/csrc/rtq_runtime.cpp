@@ -178,8 +178,8 @@ enum Kid {
   K_VERIFY_PICK = K_VERIFY_MASS + 3,
   K_KV_APPEND = K_VERIFY_PICK + 3,  // + 2 x rows and cache (f32 f16, f32 bf16, f16, bf16) + heads above 128
   K_KV_KEEP = K_KV_APPEND + 8,
-  K_KV_ATTEND,                    // + 11 x rows and cache + tile and head size (attend_plan)
-  K_KV_JOIN = K_KV_ATTEND + 44,  // + rows and cache
+  K_KV_ATTEND,                    // + 8 x rows and cache + tile and head size (attend_plan)
+  K_KV_JOIN = K_KV_ATTEND + 32,  // + rows and cache
   K_ROWS = K_KV_JOIN + 4,  // + format
   K_MODEL = K_ROWS + F_COUNT,  // + RtqModelKernel: the decoder block (rtq_model.cpp)
   K_COUNT = K_MODEL + KM_COUNT
@@ -224,16 +224,12 @@ constexpr const char* kKernelNames[] = {
     "rtq_kv_append_f32_f16", "rtq_kv_append_f32_f16_256", "rtq_kv_append_f32_bf16", "rtq_kv_append_f32_bf16_256",
     "rtq_kv_append_f16", "rtq_kv_append_f16_256", "rtq_kv_append_bf16", "rtq_kv_append_bf16_256", "rtq_kv_keep",
     "rtq_kv_attend16_64_f32_f16", "rtq_kv_attend16_128_f32_f16", "rtq_kv_attend16_128p_f32_f16", "rtq_kv_attend16_256p_f32_f16",
-    "rtq_kv_attend32_64_f32_f16", "rtq_kv_attend32_128_f32_f16", "rtq_kv_attend32_128p_f32_f16",
     "rtq_kv_attend_big_64_f32_f16", "rtq_kv_attend_big_128_f32_f16", "rtq_kv_attend_big_128p_f32_f16", "rtq_kv_attend_big_256p_f32_f16",
     "rtq_kv_attend16_64_f32_bf16", "rtq_kv_attend16_128_f32_bf16", "rtq_kv_attend16_128p_f32_bf16", "rtq_kv_attend16_256p_f32_bf16",
-    "rtq_kv_attend32_64_f32_bf16", "rtq_kv_attend32_128_f32_bf16", "rtq_kv_attend32_128p_f32_bf16",
     "rtq_kv_attend_big_64_f32_bf16", "rtq_kv_attend_big_128_f32_bf16", "rtq_kv_attend_big_128p_f32_bf16", "rtq_kv_attend_big_256p_f32_bf16",
     "rtq_kv_attend16_64_f16", "rtq_kv_attend16_128_f16", "rtq_kv_attend16_128p_f16", "rtq_kv_attend16_256p_f16",
-    "rtq_kv_attend32_64_f16", "rtq_kv_attend32_128_f16", "rtq_kv_attend32_128p_f16",
     "rtq_kv_attend_big_64_f16", "rtq_kv_attend_big_128_f16", "rtq_kv_attend_big_128p_f16", "rtq_kv_attend_big_256p_f16",
     "rtq_kv_attend16_64_bf16", "rtq_kv_attend16_128_bf16", "rtq_kv_attend16_128p_bf16", "rtq_kv_attend16_256p_bf16",
-    "rtq_kv_attend32_64_bf16", "rtq_kv_attend32_128_bf16", "rtq_kv_attend32_128p_bf16",
     "rtq_kv_attend_big_64_bf16", "rtq_kv_attend_big_128_bf16", "rtq_kv_attend_big_128p_bf16", "rtq_kv_attend_big_256p_bf16",
     "rtq_kv_join_f32_f16", "rtq_kv_join_f32_bf16", "rtq_kv_join_f16", "rtq_kv_join_bf16",
     "rtq_rows_q4_0",        "rtq_rows_q8_0",        "rtq_rows_q4_k",        "rtq_rows_q6_k",
@@ -2256,18 +2252,21 @@ rtq_status enqueue_append(rtq_kv_cache* kc, int64_t layer, const KvSeqs& s, int 
     if (i < r.n_factors && r.factors[i] != 0.0f) f /= (double)r.factors[i];
     a.freq[i] = f / 6.283185307179586476925;
   }
-  // a token a wave once that fills every CU's waves twice over
+  // a token a wave once that fills every CU's waves twice over (32 + 8 heads of 128, a workgroup and a wave a token: 1024
+  // tokens 10.0 and 13.6 us, 2048 17.8 and 18.7, 8192 81.6 and 74.5; 8 + 8 of 256: 1024 12.6 and 11.2, 8192 91.0 and 70.5)
   a.wave_tokens = s.n >= 8 * kc->ctx->cu_count;
   a.tw = a.wave_tokens ? (int)cdiv(s.n, 4) : s.n;
   const int64_t vt = cdiv(s.n, 32) * kc->nkv;
   return launch(kc->ctx, K_KV_APPEND + 2 * kv_types(kc, type) + (kc->d > 128 ? 1 : 0), dim3((unsigned)(a.tw + vt)), dim3(256), st, a);
 }
 
-// The attention's tiles and partial parts.  Rows of a sequence and KV head average n group / b: tiles of 16 up to
-// that, of 32 (whose registers a head size above 128 has not), else large ones of 128.  `target` items keep every
-// CU's two resident workgroups busy; the split tiles' items are at most twice that (each but a tile's last covers C keys).
+// The attention's tiles and partial parts.  Small tiles of 16 rows read the cache straight into registers, large ones of
+// 128 through LDS.  Rows of a sequence and KV head average n group / b; measured (bf16, 4 sequences of 1000 slots, head
+// size 128, small and large): 8 rows 16.9 and 21.3 us, 16 rows 21.2 and 16.8 (head size 256, 32 of 4096: 213 and 258), 24
+// rows 32.0 and 17.3; over up to 512 slots (300, head size 64) 24 rows 8.1 and 13.3.  Tiles of 32 rows were never
+// better than both by more than 8%.
 struct AttendPlan {
-  int tm, variant, D;
+  int tm, variant, D, whole;
   bool fused;
   int64_t target, tiles;
   size_t bytes;
@@ -2277,18 +2276,22 @@ AttendPlan attend_plan(const rtq_kv_cache* kc, int64_t n, int64_t b, int64_t ld,
   const int64_t d = kc->d, rows = n * (nh / kc->nkv);
   const int size = d == 64 ? 0 : d == 128 ? 1 : d < 128 ? 2 : 3;
   p.D = d == 64 ? 64 : d <= 128 ? 128 : 256;
-  if (rows <= 16 * b) {
+  if (rows <= 16 * b || (rows <= 32 * b && ld * kc->ps <= 512)) {
     p.tm = 16, p.variant = size;
-  } else if (rows <= 32 * b && d <= 128) {
-    p.tm = 32, p.variant = 4 + size;
   } else {
-    p.tm = 128, p.variant = 7 + size;
+    p.tm = 128, p.variant = 4 + size;
   }
   p.target = kc->ctx ? std::min(kc->ctx->cu_count * 2, RTQ_KV_TARGET) : RTQ_KV_TARGET;
   p.tiles = (cdiv(rows, p.tm) + b) * kc->nkv;
-  // a tile's rows times its parts, at most: what one workgroup reads again (up to 256 rows in the time that another kernel takes)
+  // `target` items: two workgroups for every CU (that run at once, but for head sizes above 128: one); those of split tiles
+  // are at most twice that (each but a tile's last covers C slots).
+  // A tile's rows times its parts, at most, are what its last workgroup would read again: 4 rows x 16 parts 13.2 us, by a
+  // kernel of its own 15.5; 16 x 8 16.7 and 16.8; 16 x 16 19.7 and 16.1.
   const int64_t parts = std::min(cdiv(ld * kc->ps, 128), p.target / kc->nkv + 1);
-  p.fused = std::min<int64_t>(p.tm, rows) * parts <= 256;
+  p.fused = std::min<int64_t>(p.tm, cdiv(rows, b)) * parts <= 128;
+  // Joining costs a small tile as much as four more turns of its waves: one of 300 slots 13.8 us split, 12.1 whole, of
+  // 1000 15.3 and 21.5.
+  p.whole = p.tm == 16 ? 512 : 0;
   p.bytes = (size_t)(2 * p.target * p.tm * (p.D + 2) * 4) + 4 * 256;
   return p;
 }
@@ -2313,13 +2316,13 @@ rtq_status enqueue_attend(rtq_kv_cache* kc, int64_t layer, const KvSeqs& s, int 
   a.q = q, a.o = out, a.ldq = ldq, a.ldo = ldo, a.parents = parents;
   a.nkv = (int)kc->nkv, a.group = (int)(nh / kc->nkv), a.d = (int)kc->d, a.ps_shift = kc->ps_shift, a.n_pages = (int)kc->n_pages;
   a.scale2 = (float)((scale > 0.0f ? (double)scale : 1.0 / std::sqrt((double)kc->d)) * 1.4426950408889634);
-  a.target = (int)p.target, a.slots = (int)(2 * p.target);
+  a.target = (int)p.target, a.once = (int)(p.D > 128 ? p.target / 2 : p.target), a.slots = (int)(2 * p.target);
   a.part = ar.take<float>((size_t)(2 * p.target * p.tm * p.D));
   a.ml = ar.take<float>((size_t)(2 * p.target * p.tm * 2));
-  a.tm = p.tm, a.D = p.D, a.fused = p.fused;
+  a.tm = p.tm, a.D = p.D, a.fused = p.fused, a.whole = p.whole;
   if (ar.off > ar.cap) return fail(RTQ_ERR_INVALID, "internal: workspace too small");
   const dim3 grid((unsigned)(p.target + p.tiles));
-  RTQ_TRY(launch(kc->ctx, K_KV_ATTEND + 11 * kv_types(kc, type) + p.variant, grid, dim3(256), st, a));
+  RTQ_TRY(launch(kc->ctx, K_KV_ATTEND + 8 * kv_types(kc, type) + p.variant, grid, dim3(256), st, a));
   return p.fused ? RTQ_OK : launch(kc->ctx, K_KV_JOIN + kv_types(kc, type), grid, dim3(256), st, a);
 }
 

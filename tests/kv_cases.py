@@ -84,10 +84,10 @@ def visible(m, parents=None):
 
 
 def one_plane(xt, n, b, heads, kv, d):
-    """The half step by which the weights of a call are rounded: large tiles (calls of more than 32 rows a sequence and KV
-    head, of 16 where a head is larger than 128) of 16-bit rows hold each weight in one number of that type; the others'
+    """The half step by which the weights of a call are rounded: large tiles (some of the calls of more than 16 rows a sequence
+    and KV head) of 16-bit rows hold each weight in one number of that type; the others'
     planes are counted with the scores' below."""
-    large = n * (heads // kv) > (32 if d <= 128 else 16) * b
+    large = n * (heads // kv) > 16 * b
     return EPS[xt] if large and xt != "f32" else 0.0
 
 
