@@ -404,12 +404,13 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, int TM, int block
   // that is it.  With more, what their last ranges leave over makes a second turn of the CUs: then the shortest ranges (of
   // some) are taken with which all items run at once (32 sequences of 1000 to 7000, 64 rows: 162 -> 133 us).  Tiles that
   // nearly fill the CUs are not split at all, unless one is far longer than the others (32 of 250 to 1750, 4 rows: 42 -> 34
-  // us; 32 of 75 to 525, 256 rows: 60 -> 36).  Small tiles of long sequences are read evenly by more and shorter ranges,
-  // a second turn or not (32 of 4000 to 28000: 457 us against 550 unsplit).
+  // us; 32 of 75 to 525, 256 rows: 60 -> 36).  Small tiles of long sequences, and large ones that have a CU
+  // each, are better off with ranges as short as the items allow, a second turn or not (32 of 4000 to 28000: 457 us against 550
+  // unsplit; 64 rows and a head size of 256: 1326 against 1650).
   const float even = kv_wave_total(w) * (float)a.nkv / (float)a.once / 128.0f, most = kv_wave_total(whole) * (float)a.nkv;
   const auto range = [&](float f) { return max((int)fminf(ceilf(even * f), (float)(RTQ_KV_SLOTS / 128)) * 128, 128); };
   int C = range(1.0f), c, ns;
-  if (TM == 16 && C > 2048) {
+  if (C > 2048 && (TM == 16 || a.once < a.target)) {
     if (most * 2.0f >= (float)a.once) C = range((float)a.once / (float)a.target);
   } else if (most * 16.0f > (float)a.once) {
     constexpr float kTry[] = {1.0f, 1.25f, 1.5f, 2.0f, 3.0f, 4.0f};
