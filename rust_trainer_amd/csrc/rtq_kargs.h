@@ -657,6 +657,7 @@ struct KvAppendArgs {
   int tw, wave_tokens;  // workgroups of tokens (four tokens each, or one); behind them, of values: 32 tokens of a KV head
   double freq[RTQ_KV_ROT / 2];  // turns per position of each pair
 };
+#define RTQ_KV_ITEM 12
 struct KvAttendArgs {
   KvSeqs s;
   const uint16_t *k, *v;  // the layer's pages
@@ -671,6 +672,7 @@ struct KvAttendArgs {
   int whole;        // sequences of up to this many slots are not split
   int tm, D;        // rows of a tile, elements of a part's row
   int fused;        // split tiles are joined by their last workgroup, not by a kernel behind it
+  int32_t* items;   // [1 + slots][RTQ_KV_ITEM]: the number of parts that are to be joined; each one's item
   float* part;      // [slots][rows of a tile][D]
   float* ml;        // [slots][rows of a tile][2]: maximum, sum (-1: the row sees nothing, NaN: to be done again)
 };

@@ -377,7 +377,7 @@ __device__ __forceinline__ float kv_wave_total(float v) {
 // A tile that is joined by its last workgroup has at most kKvJoin / rows parts, one joined by a kernel of its own at most
 // kKvJoin.  Sequences that overlap in `starts` can name more than the host counted: then whole tiles are left out.
 constexpr int kKvJoin = 1024;
-__device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, int TM, int block, KvItem& it) {
+__device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, const int TM, int block, KvItem& it) {
   const int lane = threadIdx.x & 63, group = a.group;
   const int per = (a.s.b + 63) / 64, i0 = min(lane * per, a.s.b), i1 = min(i0 + per, a.s.b);
   int row0 = 0, cnt = 0, held = 0, total = 0, tiles = 0;
@@ -439,6 +439,7 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, int TM, int block
     items += tiles * a.nkv * ns, slots += ns > 1 ? tiles * a.nkv * ns : 0;
   }
   int ei = kv_wave_scan(items) - items, es = kv_wave_scan(slots) - slots;
+  if (!a.fused && block == 0 && threadIdx.x == 63) a.items[0] = es + slots;
   const uint64_t mine = __ballot(block >= ei && block < ei + items);
   if (!mine) return false;
   int ok = 0;
@@ -468,7 +469,10 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, int TM, int block
   RTQ_KV_GIVE(seq), RTQ_KV_GIVE(row0), RTQ_KV_GIVE(cnt), RTQ_KV_GIVE(held), RTQ_KV_GIVE(total), RTQ_KV_GIVE(tile);
   RTQ_KV_GIVE(hv), RTQ_KV_GIVE(split), RTQ_KV_GIVE(splits), RTQ_KV_GIVE(slot), RTQ_KV_GIVE(C);
 #undef RTQ_KV_GIVE
-  return __builtin_amdgcn_readlane(ok, src);
+  if (!__builtin_amdgcn_readlane(ok, src)) return false;
+  if (!a.fused && it.slot >= 0 && threadIdx.x == 0)
+    *reinterpret_cast<KvItem*>(a.items + (1 + it.slot + it.split) * RTQ_KV_ITEM) = it;
+  return true;
 }
 
 template <int CT>
@@ -1303,13 +1307,26 @@ RTQ_KV_ATTENDS(f32_bf16, VT_BF16, true)
 RTQ_KV_ATTENDS(f16, VT_F16, false)
 RTQ_KV_ATTENDS(bf16, VT_BF16, false)
 
-// the joining kernel: the workgroup of part i of n joins its tile's rows i, i + n, ...
+// the joining kernel: the workgroup of part i of n joins its tile's rows i, i + n, ...  It takes the item from the attention's
+// workgroup of that part (making the plan again took 2 us of each launch).  Items that no workgroup has left (of tiles that the
+// plan leaves out, where sequences overlap) are another call's: what does not name rows of this one is passed over.
 template <int QT, int CT>
 __device__ __forceinline__ void kv_join_rows(const KvAttendArgs& a) {
   __shared__ KvEnd sh;
   __shared__ int nan[128];
-  KvItem it;
-  if (!kv_plan(a, a.tm, blockIdx.x, it) || it.slot < 0) return;
+  typedef const __attribute__((address_space(4))) int32_t* cptr;
+  const int at = blockIdx.x;
+  const cptr items = reinterpret_cast<cptr>(reinterpret_cast<uintptr_t>(a.items));
+  int f[RTQ_KV_ITEM];
+#pragma unroll
+  for (int i = 0; i < RTQ_KV_ITEM; i++) f[i] = items[(1 + at) * RTQ_KV_ITEM + i];
+  if (at >= items[0]) return;
+  const KvItem it = {f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7], f[8], f[9], f[10]};
+  const bool sound = it.seq >= 0 && it.seq < a.s.b && it.row0 >= 0 && it.cnt >= 1 && it.cnt <= a.s.n - it.row0 && it.held >= 0 &&
+                     it.total >= 0 && (it.total == 0 || (it.total - 1) >> a.ps_shift < a.s.ldt) && it.hv >= 0 && it.hv < a.nkv && it.tile >= 0 &&
+                     (int64_t)it.tile * a.tm < (int64_t)it.cnt * a.group && it.splits >= 2 && it.splits <= kKvJoin && it.split >= 0 &&
+                     it.split < it.splits && it.slot + it.split == at && it.slot + it.splits <= a.slots;
+  if (!sound) return;
   const KvTile t = kv_tile(a, a.tm, it);
   if (it.split >= t.rows) return;
   kv_join<QT>(a, it, t, a.tm, a.D, it.split, it.splits, nan, sh);

@@ -2292,7 +2292,7 @@ AttendPlan attend_plan(const rtq_kv_cache* kc, int64_t n, int64_t b, int64_t ld,
   // Joining costs a small tile as much as four more turns of its waves: one of 300 slots 13.8 us split, 12.1 whole, of
   // 1000 15.3 and 21.5.
   p.whole = p.tm == 16 ? 512 : 0;
-  p.bytes = (size_t)(2 * p.target * p.tm * (p.D + 2) * 4) + 4 * 256;
+  p.bytes = (size_t)(2 * p.target * p.tm * (p.D + 2) * 4 + (1 + 2 * p.target) * RTQ_KV_ITEM * 4) + 6 * 256;
   return p;
 }
 
@@ -2319,11 +2319,12 @@ rtq_status enqueue_attend(rtq_kv_cache* kc, int64_t layer, const KvSeqs& s, int 
   a.target = (int)p.target, a.once = (int)(p.D > 128 ? p.target / 2 : p.target), a.slots = (int)(2 * p.target);
   a.part = ar.take<float>((size_t)(2 * p.target * p.tm * p.D));
   a.ml = ar.take<float>((size_t)(2 * p.target * p.tm * 2));
+  a.items = ar.take<int32_t>((size_t)((1 + 2 * p.target) * RTQ_KV_ITEM));
   a.tm = p.tm, a.D = p.D, a.fused = p.fused, a.whole = p.whole;
   if (ar.off > ar.cap) return fail(RTQ_ERR_INVALID, "internal: workspace too small");
   const dim3 grid((unsigned)(p.target + p.tiles));
   RTQ_TRY(launch(kc->ctx, K_KV_ATTEND + 8 * kv_types(kc, type) + p.variant, grid, dim3(256), st, a));
-  return p.fused ? RTQ_OK : launch(kc->ctx, K_KV_JOIN + kv_types(kc, type), grid, dim3(256), st, a);
+  return p.fused ? RTQ_OK : launch(kc->ctx, K_KV_JOIN + kv_types(kc, type), dim3((unsigned)a.slots), dim3(256), st, a);
 }
 
 rtq_status kv_check_keep(const rtq_kv_cache* kc, const rtq_kv_seqs* s, const int32_t* kept, int64_t ldk, const int32_t* after) {

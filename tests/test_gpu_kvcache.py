@@ -507,18 +507,19 @@ def test_more_tokens_than_the_table_holds(ctx):
 
 def test_sequences_that_overlap_stay_in_bounds(ctx):
     """Starts that fall and rise name the same rows for many sequences, more tiles than the call was planned for: rows are left
-    out or written more than once, and nothing behind them is touched."""
+    out or written more than once, and nothing behind them is touched.  With the long sequence split tiles are left out."""
     b, n = 64, 40
-    lay = Layout([700] * b, [0] * b, 32, wide=2)
-    pg = Pages(ctx, lay, 1, 64, "f16")
-    starts = torch.tensor([0, n] * (b // 2) + [0], dtype=torch.int32, device="cuda")
-    s = seqs_d(b, pg.lens.data_ptr(), pg.table.data_ptr(), lay.table.shape[1], starts.data_ptr())
-    for heads in (1, 8):
-        q = torch.randn(n, heads * 64, device="cuda")
-        buf = torch.full((n + 8, heads * 64), 7.0, device="cuda")
-        pg.cache.attend_d(0, s, n, 0, heads, q.data_ptr(), heads * 64, buf[4:].data_ptr(), heads * 64, 0, 0.0, stream())
-        torch.cuda.synchronize()
-        assert (buf[:4] == 7).all() and (buf[n + 4:] == 7).all() and torch.isfinite(buf).all()
+    for long in (20000, 700):
+        lay = Layout([700] * (b - 2) + [long, 700], [0] * b, 32, wide=2)
+        pg = Pages(ctx, lay, 1, 64, "f16")
+        starts = torch.tensor([0, n] * (b // 2) + [0], dtype=torch.int32, device="cuda")
+        s = seqs_d(b, pg.lens.data_ptr(), pg.table.data_ptr(), lay.table.shape[1], starts.data_ptr())
+        for heads in (1, 8):
+            q = torch.randn(n, heads * 64, device="cuda")
+            buf = torch.full((n + 8, heads * 64), 7.0, device="cuda")
+            pg.cache.attend_d(0, s, n, 0, heads, q.data_ptr(), heads * 64, buf[4:].data_ptr(), heads * 64, 0, 0.0, stream())
+            torch.cuda.synchronize()
+            assert (buf[:4] == 7).all() and (buf[n + 4:] == 7).all()
     # a call of an ordinary sequence after it is as ever
     s1 = seqs_d(1, pg.lens.data_ptr(), pg.table.data_ptr(), lay.table.shape[1])
     q, out = torch.randn(1, 64, device="cuda"), torch.zeros(1, 64, device="cuda")
