@@ -669,7 +669,7 @@ struct KvAttendArgs {
   float scale2;     // scale log2(e)
   int target, once; // items that the keys are split into (at most this many, and one per tile beside), that run at once
   int slots;        // partial slots
-  int whole;        // sequences of up to this many slots are not split
+  int whole;        // sequences (large tiles: a call's, all) of up to this many slots are not split
   int tm, D;        // rows of a tile, elements of a part's row
   int fused;        // split tiles are joined by their last workgroup, not by a kernel behind it
   int32_t* items;   // [1 + slots][RTQ_KV_ITEM]: the number of parts that are to be joined; each one's item

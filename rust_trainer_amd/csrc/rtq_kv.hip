@@ -389,15 +389,17 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, const int TM, int
     tiles = (int)(((int64_t)cnt * group + TM - 1) / TM);
   };
   float w = 0.0f, whole = 0.0f;
+  int longest = 0;
   for (int i = i0; i < i1; i++) {
     look(i);
     w += (float)tiles * (float)total, whole += (float)tiles;
+    if (tiles) longest = max(longest, total);
   }
   // a sequence's slots a part, parts
   const auto cut = [&](int C, int& c, int& ns) {
     const int64_t least = a.fused ? (int64_t)total * min(max(cnt, 1) * a.group, TM) : total;
     c = max(C, (int)(((least + kKvJoin - 1) / kKvJoin + 127) & ~127));
-    if (total <= a.whole) c = max(c, a.whole);
+    if (TM == 16 && total <= a.whole) c = max(c, a.whole);
     ns = max((total + c - 1) / c, 1);
   };
   // Ranges of about even x 128 slots share the slots out evenly over the items that run at once.  With few tiles
@@ -410,7 +412,9 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, const int TM, int
   const float even = kv_wave_total(w) * (float)a.nkv / (float)a.once / 128.0f, most = kv_wave_total(whole) * (float)a.nkv;
   const auto range = [&](float f) { return max((int)fminf(ceilf(even * f), (float)(RTQ_KV_SLOTS / 128)) * 128, 128); };
   int C = range(1.0f), c, ns;
-  if (C > 2048 && (TM == 16 || a.once < a.target)) {
+  if (TM > 16 && !__any(longest > a.whole)) {
+    C = max(C, a.whole);
+  } else if (C > 2048 && (TM == 16 || a.once < a.target)) {
     if (most * 2.0f >= (float)a.once) C = range((float)a.once / (float)a.target);
   } else if (most * 16.0f > (float)a.once) {
     constexpr float kTry[] = {1.0f, 1.25f, 1.5f, 2.0f, 3.0f, 4.0f};
@@ -420,7 +424,7 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, const int TM, int
     for (int i = i0; i < i1; i++) {
       if (per > 1) look(i);
 #pragma unroll
-      for (int f = 0; f < 6; f++) n[f] += (float)tiles * (total <= a.whole ? 1.0f : ceilf((float)total * inv[f]));
+      for (int f = 0; f < 6; f++) n[f] += (float)tiles * (TM == 16 && total <= a.whole ? 1.0f : ceilf((float)total * inv[f]));
     }
 #pragma unroll
     for (int f = 0; f < 6; f++) n[f] = kv_wave_total(n[f]) * (float)a.nkv;

@@ -2290,8 +2290,10 @@ AttendPlan attend_plan(const rtq_kv_cache* kc, int64_t n, int64_t b, int64_t ld,
   const int64_t parts = std::min(cdiv(ld * kc->ps, 128), p.target / kc->nkv + 1);
   p.fused = std::min<int64_t>(p.tm, cdiv(rows, b)) * parts <= 128;
   // Joining costs a small tile as much as four more turns of its waves: one of 300 slots 13.8 us split, 12.1 whole, of
-  // 1000 15.3 and 21.5.
-  p.whole = p.tm == 16 ? 512 : 0;
+  // 1000 15.3 and 21.5.  Large ones are as well whole where the call has no longer sequence (joined: 300 slots, 256 rows, head
+  // size 128 27.4, whole 18.7; 32 of 75 to 525, 64 rows 31.5 and 23.4; 4 of them 21.8 and 20.2; their turns are twice as long
+  // at a head size of 256: 4 of them, 24 rows 24.4 and 36.0).
+  p.whole = p.tm == 16 ? 512 : p.D > 128 ? 320 : 640;
   p.bytes = (size_t)(2 * p.target * p.tm * (p.D + 2) * 4 + (1 + 2 * p.target) * RTQ_KV_ITEM * 4) + 6 * 256;
   return p;
 }
