@@ -331,17 +331,15 @@ extern "C" __global__ __launch_bounds__(256) void rtq_kv_keep(KvKeepArgs a) {
 // Small tiles (16 rows: single tokens and narrow trees) are bound by the reading of the cache: 64 sequences of up to
 // 8192 tokens, 32 over 8 heads of 128, 1.15 GB: 259 us, 4.4 TB/s; one of 131072: 97 us, 5.5 TB/s (some of it still cached);
 // one of 1000: 14 us, of which the reading takes 1: each item is a chain of dependent loads (lengths, page, keys, values).
-// Large ones (128 rows) are bound by the matrix instructions and the weights between them, which overlap little: 2048
-// tokens behind 6144, 32 over 8 heads of 128: 245 us, 0.98 PFLOP/s of a large product's 1.2, the matrix units busy 53% of
-// the time, at the 1.7 GHz that such work runs at.  (Scores of the next block issued beside a block's weights: the same.)
+// Large ones (128 rows) are bound by the matrix instructions: 2048 tokens behind 6144, 32 over 8 heads of 128, bf16: 321 us,
+// 0.75 PFLOP/s, and 1.12 with the weights' second plane counted, of a large product's 1.2.
 //
 // A wave takes 32 slots at a time.  S^T = K q^T and o^T = V^T p^T, so that a lane holds one query row:
 // key row m of tile t is slot 8 (m / 4) + 4 t + m % 4, and the lane that gets the scores of slots 8 g .. 8 g + 7
 // holds them in the order in which it feeds them to the second product: the weights never leave their lane.
 //
 // Weights are rounded to the cache's 16 bits for the second product, in two planes (three of f32 rows over bf16) that keep
-// 16 to 22 bits of them; a large tile of 16-bit rows takes one plane, half a step of that type in a weight of at most
-// 1, as its rows are rounded anyway: a second would be half as many matrix instructions again.  Sums stay in 32 bits.
+// 16 to 22 bits of them, in small tiles and in large ones: a row is as exact whatever other rows its call has.  Sums stay in 32 bits.
 struct KvItem {
   int seq, row0, cnt, held, total, tile, hv, split, splits, slot, C;  // slot: of the tile's first part (-1: one part)
 };
@@ -1036,7 +1034,7 @@ __device__ __forceinline__ int kv_swap(int slot) {
 template <int CT, bool QF, int D, bool FULL, int R>
 __device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
   constexpr int NW = 4, DK = D / 16, DT = D / 32, CH = D / 8, TM = 32 * NW, T = 64 * NW;
-  constexpr int NS = QF ? (CT == VT_F16 ? 2 : 3) : 1, NP = NS;
+  constexpr int NS = QF ? (CT == VT_F16 ? 2 : 3) : 1, NP = QF ? NS : 2;
   constexpr int UK = 32 * CH, UV = D * 4, UNIT = UK + UV;  // chunks
   typedef VRow<QF ? VT_F32 : CT> Q;
   struct Main {
