@@ -658,6 +658,18 @@ struct KvAppendArgs {
   double freq[RTQ_KV_ROT / 2];  // turns per position of each pair
 };
 #define RTQ_KV_ITEM 12
+// Slots of an attention tile's range: `least` or more, so that a tile joined by its last workgroup (fused) has about
+// RTQ_KV_JOIN / rows parts, one joined by a kernel about RTQ_KV_JOIN.  Parts are whole: a fused tile's are the quotient rounded up
+// (c >= total rows / RTQ_KV_JOIN, so total / c <= RTQ_KV_JOIN / rows), with its rows fewer than RTQ_KV_JOIN + rows.
+#define RTQ_KV_JOIN 1024
+#define RTQ_KV_ROWS 128  // most rows of a tile
+#define RTQ_KV_JOINED (RTQ_KV_JOIN + RTQ_KV_ROWS)  // what a join's tables hold: rows x parts
+constexpr int kv_range(int total, int rows, int least, bool fused) {
+  const int64_t each = fused ? (int64_t)total * rows : total;
+  const int c = (int)(((each + RTQ_KV_JOIN - 1) / RTQ_KV_JOIN + 127) & ~(int64_t)127);
+  return c > least ? c : least;
+}
+constexpr int kv_parts(int total, int c) { return total > c ? (total - 1) / c + 1 : 1; }
 struct KvAttendArgs {
   KvSeqs s;
   const uint16_t *k, *v;  // the layer's pages

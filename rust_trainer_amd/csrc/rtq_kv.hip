@@ -372,9 +372,7 @@ __device__ __forceinline__ float kv_wave_total(float v) {
 }
 
 // item `block` of the plan (every wave finds it by itself; a lane looks after b / 64 sequences); false: none.
-// A tile that is joined by its last workgroup has at most kKvJoin / rows parts, one joined by a kernel of its own at most
-// kKvJoin.  Sequences that overlap in `starts` can name more than the host counted: then whole tiles are left out.
-constexpr int kKvJoin = 1024;
+// Sequences that overlap in `starts` can name more than the host counted: then whole tiles are left out.
 __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, const int TM, int block, KvItem& it) {
   const int lane = threadIdx.x & 63, group = a.group;
   const int per = (a.s.b + 63) / 64, i0 = min(lane * per, a.s.b), i1 = min(i0 + per, a.s.b);
@@ -395,10 +393,9 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, const int TM, int
   }
   // a sequence's slots a part, parts
   const auto cut = [&](int C, int& c, int& ns) {
-    const int64_t least = a.fused ? (int64_t)total * min(max(cnt, 1) * a.group, TM) : total;
-    c = max(C, (int)(((least + kKvJoin - 1) / kKvJoin + 127) & ~127));
+    c = kv_range(total, (int)min((int64_t)max(cnt, 1) * a.group, (int64_t)TM), C, a.fused);
     if (TM == 16 && total <= a.whole) c = max(c, a.whole);
-    ns = max((total + c - 1) / c, 1);
+    ns = kv_parts(total, c);
   };
   // Ranges of about even x 128 slots share the slots out evenly over the items that run at once.  With few tiles
   // that is it.  With more, what their last ranges leave over makes a second turn of the CUs: then the shortest ranges (of
@@ -672,7 +669,7 @@ __device__ __forceinline__ void kv_row_again(const KvAttendArgs& a, const KvItem
 
 union KvEnd {
   struct {
-    float m[kKvJoin], w[kKvJoin];  // [row][part]: maxima, sums; then weights
+    float m[RTQ_KV_JOINED], w[RTQ_KV_JOINED];  // [row][part]: maxima, sums; then weights
     f4 o[256];
   } j;
   KvAgain again;
@@ -1034,6 +1031,7 @@ __device__ __forceinline__ int kv_swap(int slot) {
 template <int CT, bool QF, int D, bool FULL, int R>
 __device__ __forceinline__ void kv_attend_big(const KvAttendArgs& a) {
   constexpr int NW = 4, DK = D / 16, DT = D / 32, CH = D / 8, TM = 32 * NW, T = 64 * NW;
+  static_assert(TM <= RTQ_KV_ROWS, "a join's tables");
   constexpr int NS = QF ? (CT == VT_F16 ? 2 : 3) : 1, NP = QF ? NS : 2;
   constexpr int UK = 32 * CH, UV = D * 4, UNIT = UK + UV;  // chunks
   typedef VRow<QF ? VT_F32 : CT> Q;
@@ -1326,7 +1324,7 @@ __device__ __forceinline__ void kv_join_rows(const KvAttendArgs& a) {
   const KvItem it = {f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7], f[8], f[9], f[10]};
   const bool sound = it.seq >= 0 && it.seq < a.s.b && it.row0 >= 0 && it.cnt >= 1 && it.cnt <= a.s.n - it.row0 && it.held >= 0 &&
                      it.total >= 0 && (it.total == 0 || (it.total - 1) >> a.ps_shift < a.s.ldt) && it.hv >= 0 && it.hv < a.nkv && it.tile >= 0 &&
-                     (int64_t)it.tile * a.tm < (int64_t)it.cnt * a.group && it.splits >= 2 && it.splits <= kKvJoin && it.split >= 0 &&
+                     (int64_t)it.tile * a.tm < (int64_t)it.cnt * a.group && it.splits >= 2 && it.splits <= RTQ_KV_JOIN && it.split >= 0 &&
                      it.split < it.splits && it.slot + it.split == at && it.slot + it.splits <= a.slots;
   if (!sound) return;
   const KvTile t = kv_tile(a, a.tm, it);

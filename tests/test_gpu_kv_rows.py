@@ -1,4 +1,5 @@
-"""Rows of the cache's attention at the ends of its tables: how exact 16-bit rows are in tiles of either size."""
+"""Rows of the cache's attention where its plan is at its ends: how exact 16-bit rows are in tiles of either size, tiles of so many
+parts that the join's tables are full."""
 import numpy as np
 import pytest
 
@@ -59,3 +60,35 @@ def test_weights_of_16_bit_rows_keep_two_planes(ctx, case, xt, ct):
     q = to_type(0.05 * rng.standard_normal((lay.n, heads * d)), xt)
     parents = np.array([p for m in counts for p in tree(rng, m)[0]], np.int32) if is_tree else None
     check(pg, run(pg, q, xt, heads, parents), q, xt, heads, parents)
+
+
+JOINED = [  # sequences, the one with new tokens: held, new, then heads, kv, d, tree: parts x rows past 1024 in one small tile
+    (12, 10898, 2, 12, 2, 128, False),  # 86 parts of 12 rows
+    (16, 9358, 2, 28, 4, 128, False),   # 74 of 14
+    (16, 10069, 13, 1, 1, 128, False),  # 79 of 13
+    (16, 10069, 13, 1, 1, 64, True),
+    (16, 8705, 15, 4, 4, 64, True),     # 69 of 15
+    (16, 14500, 9, 1, 1, 128, True),    # 114 of 9
+]
+
+
+@pytest.mark.parametrize("xt, ct", [("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("case", range(len(JOINED)))
+def test_tiles_of_many_parts_in_a_batch_of_idle_sequences(ctx, case, xt, ct):
+    """One sequence with some rows, joined by its last workgroup (the call's mean is a row a sequence or less)."""
+    b, held, new, heads, kv, d, is_tree = JOINED[case]
+    lay = Layout([40] * 3 + [held] + [7] * (b - 4), [0] * 3 + [new] + [0] * (b - 4), 64, seed=case)
+    rng = np.random.default_rng(case)
+    pg = Pages(ctx, lay, kv, d, ct, seed=case)
+    q = to_type(2.0 * rng.standard_normal((new, heads * d)), xt)
+    parents = np.array(tree(rng, new)[0], np.int32) if is_tree else None
+    check(pg, run(pg, q, xt, heads, parents), q, xt, heads, parents)
+
+
+def test_fifteen_rows_beside_a_token(ctx):
+    lay = Layout([8705, 100] + [3] * 14, [15, 1] + [0] * 14, 64)
+    rng = np.random.default_rng(1)
+    pg = Pages(ctx, lay, 4, 64, "f16")
+    q = to_type(rng.standard_normal((16, 4 * 64)), "f16")
+    parents = np.array(tree(rng, 15)[0] + [-1], np.int32)
+    check(pg, run(pg, q, "f16", 4, parents), q, "f16", 4, parents)
