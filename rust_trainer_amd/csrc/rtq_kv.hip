@@ -736,7 +736,8 @@ __device__ __forceinline__ void kv_join(const KvAttendArgs& a, const KvItem& it,
     const bool bad = !dead && ls != ls;
     nan[from + r * step] = bad;
     const float inv = dead || ls == 0.0f ? 0.0f : 1.0f / ls;
-    for (int i = part0; i < ns; i += parts) w[i] = bad ? NAN : m[i] * inv;
+    // (a row that sees nothing is 0, also where infinite scores of held keys, which are not its own, make m NaN)
+    for (int i = part0; i < ns; i += parts) w[i] = bad ? NAN : inv == 0.0f ? 0.0f : m[i] * inv;
   }
   __syncthreads();
   for (int r0 = 0; r0 < rows; r0 += G / share) {

@@ -3,7 +3,7 @@ parts that the join's tables are full."""
 import numpy as np
 import pytest
 
-from kv_cases import EPS, TINY, TYPES, Layout, attend, to_type, tree, value
+from kv_cases import EPS, TINY, TYPES, Layout, attend, to_type, tree, value, visible
 from test_gpu_kvcache import NP, Pages, dev, host, rows_d, stream
 
 torch = pytest.importorskip("torch")
@@ -92,3 +92,28 @@ def test_fifteen_rows_beside_a_token(ctx):
     q = to_type(rng.standard_normal((16, 4 * 64)), "f16")
     parents = np.array(tree(rng, 15)[0] + [-1], np.int32)
     check(pg, run(pg, q, "f16", 4, parents), q, "f16", 4, parents)
+
+
+DEAD = [  # held, counts, heads: whole tiles, joined by the last workgroup (small, large tiles) and by a kernel (small, large)
+    (20, [6, 2], 4), (4000, [6, 2], 1), (800, [9, 8], 2), (4000, [6, 2], 4), (4000, [6, 2], 16)]
+
+
+@pytest.mark.parametrize("xt, ct", [("f32", "f16"), ("f32", "bf16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("held, counts, heads", DEAD)
+def test_rows_that_see_nothing_are_zero_beside_infinite_scores(ctx, held, counts, heads, xt, ct):
+    """A held key of +inf is no key of an unused node's row, nor of what hangs from it: those are 0, the others what
+    the formula makes of an infinite score, and the next sequence's are as ever."""
+    lay = Layout([held, 0], counts, 32)
+    rng = np.random.default_rng(4)
+    pg = Pages(ctx, lay, 1, 64, ct)
+    p, s = lay.slots(0)
+    pg.k0[0][p[10], 0, s[10]] = to_type(np.array([np.inf]), ct)[0]
+    pg.k.copy_(dev(pg.k0))
+    parents = np.array([-1, -2, 1, 0, 7, 3, 4, -1, 8][:counts[0]] + [-1, 1, 0, 2, 3, -1, 9, 5][:counts[1]], np.int32)
+    q = to_type(np.abs(rng.standard_normal((lay.n, heads * 64))), xt)
+    got = value(run(pg, q, xt, heads, parents), xt)
+    _, alive = visible(counts[0], parents[:counts[0]])
+    assert not got[:counts[0]][~alive].any() and np.isnan(got[:counts[0]][alive]).all()
+    _, alive = visible(counts[1], parents[counts[0]:])
+    assert not got[counts[0]:][~alive].any()
+    check(pg, to_type(got, xt), q, xt, heads, parents, only=[1])
