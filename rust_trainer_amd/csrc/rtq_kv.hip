@@ -187,7 +187,11 @@ __device__ __forceinline__ void kv_append(const KvAppendArgs& a) {
   typedef VRow<XT> X;
   constexpr int E = X::E;
   const int vecs = a.d / E;
-  for (int i = threadIdx.x; i < nt * vecs; i += 256) {
+  // rows of no sequence, before the first and behind the last, are not read (nor stored)
+  typedef const __attribute__((address_space(4))) int32_t* cptr;
+  const cptr starts = reinterpret_cast<cptr>(reinterpret_cast<uintptr_t>(a.s.starts));
+  const int lo = a.s.starts ? max(starts[0] - t0, 0) : 0, hi = a.s.starts ? min(starts[a.s.b] - t0, nt) : nt;
+  for (int i = lo * vecs + threadIdx.x; i < hi * vecs; i += 256) {
     const int t = i / vecs, c = i % vecs * E;
     const u4v r = X::load(a.vx, (int64_t)(t0 + t) * a.ldv + (int64_t)hv * a.d + c);
 #pragma unroll
@@ -214,7 +218,7 @@ __device__ __forceinline__ void kv_append(const KvAppendArgs& a) {
     }
     if (lane < 32) {
       int64_t at = -1;
-      if (lane < nt && seq >= 0) {
+      if (lane >= lo && lane < hi && seq >= 0) {
         const int64_t slot = (int64_t)max(a.s.lens[seq], 0) + idx;
         const int64_t p = slot >> a.ps_shift;
         const int pid = p < a.s.ldt ? a.s.table[(int64_t)seq * a.s.ldt + p] : -1;

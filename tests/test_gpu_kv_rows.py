@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 from kv_cases import EPS, TINY, TYPES, Layout, attend, to_type, tree, value, visible
+from rust_trainer_amd.kvcache import rope_d, seqs_d
 from test_gpu_kvcache import NP, Pages, dev, host, rows_d, stream
 
 torch = pytest.importorskip("torch")
@@ -117,3 +118,28 @@ def test_rows_that_see_nothing_are_zero_beside_infinite_scores(ctx, held, counts
     _, alive = visible(counts[1], parents[counts[0]:])
     assert not got[counts[0]:][~alive].any()
     check(pg, to_type(got, xt), q, xt, heads, parents, only=[1])
+
+
+@pytest.mark.parametrize("first", [0, 3, 40])
+def test_append_takes_its_sequences_rows_alone(ctx, first):
+    """A call of up to 300 rows, as a captured step makes it, whose sequences have 73 of them: the cache and the queries are those
+    of a call of 73, and the rows before and behind, NaN here, are left."""
+    lay = Layout([5, 31, 0], [40, 0, 33], 32, seed=2)
+    kv, heads, d, n = 3, 6, 80, 300
+    rng = np.random.default_rng(first)
+    a, b = Pages(ctx, lay, kv, d, "f16"), Pages(ctx, lay, kv, d, "f16")
+    rows = [rng.standard_normal((lay.n, h * d)).astype(np.float32) for h in (heads, kv, kv)]
+    wide = [np.full((n, r.shape[1]), np.nan, np.float32) for r in rows]
+    for w, r in zip(wide, rows):
+        w[first:first + lay.n] = r
+    starts = dev(lay.starts + first)
+    seqs = seqs_d(lay.b, a.lens.data_ptr(), a.table.data_ptr(), lay.table.shape[1], starts.data_ptr())
+    outs = []
+    for pg, s, (q, k, v) in ((a, seqs, wide), (b, b.seqs, rows)):
+        qd, kd, vd = dev(q), dev(k), dev(v)
+        outs.append(torch.full((len(q), heads * d), 7.0, device="cuda"))
+        pg.cache.append_d(0, s, len(q), 0, rope_d(32), kd.data_ptr(), kv * d, vd.data_ptr(), kv * d, heads, qd.data_ptr(), heads * d, outs[-1].data_ptr(),
+                          heads * d, stream=stream())
+        torch.cuda.synchronize()
+    assert torch.equal(a.k, b.k) and torch.equal(a.v, b.v) and torch.equal(outs[0][first:first + lay.n], outs[1])
+    assert (outs[0][:first] == 7).all() and (outs[0][first + lay.n:] == 7).all()
