@@ -2935,6 +2935,10 @@ rtq_status kv_check_parents(const rtq_kv_seqs* s, int64_t n, const int32_t* pare
   }
   return RTQ_OK;
 }
+// the call's rows that belong to its sequences: no others are read or written
+void kv_rows(const rtq_kv_seqs* s, int64_t n, int64_t* lo, int64_t* hi) {
+  *lo = s->starts ? s->starts[0] : 0, *hi = s->starts ? s->starts[s->b] : n;
+}
 size_t kv_seq_bytes(const rtq_kv_seqs& s) { return (size_t)(2 * s.b + 1 + s.b * s.ld) * 4 + 3 * 256; }
 rtq_status kv_seq_put(const rtq_kv_seqs& s, int64_t n, Arena& ar, hipStream_t st, KvSeqs* out) {
   int32_t* lens = ar.take<int32_t>((size_t)s.b);
@@ -2954,10 +2958,13 @@ rtq_status rtq_kv_append(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s, 
   RTQ_TRY(kv_check_append(kc, layer, s, n, type, rope, k, ldk, v, ldv, nh, q, ldq, qo, ldo));
   if (n == 0) return RTQ_OK;
   RTQ_TRY(kv_check_lists(kc, s, n));
-  for (int64_t i = 0; pos && i < n; i++)
+  int64_t lo, hi;
+  kv_rows(s, n, &lo, &hi);
+  for (int64_t i = lo; pos && i < hi; i++)
     if (pos[i] < 0) return fail(RTQ_ERR_INVALID, "position %lld is negative", (long long)i);
   rtq_ctx* c = kc->ctx;
   RTQ_TRY(check_ctx(c));
+  if (hi == lo) return RTQ_OK;
   HostCall hc(c);
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = c->stream;
@@ -2974,17 +2981,16 @@ rtq_status rtq_kv_append(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s, 
   float* qn = ar.take<float>((size_t)kc->d);
   float* kn = ar.take<float>((size_t)kc->d);
   if (ar.off > ar.cap) return fail(RTQ_ERR_INVALID, "internal: workspace too small");
-  RTQ_TRY(h2d_rows(kd, k, n, kw, ldk, es, st));
-  RTQ_TRY(h2d_rows(vd, v, n, kw, ldv, es, st));
-  if (q) RTQ_TRY(h2d_rows(qd, q, n, qw, ldq, es, st));
-  if (pd) RTQ_TRY(h2d(pd, pos, (size_t)n * 4, st));
+  RTQ_TRY(h2d_rows(kd + lo * kw * es, (const char*)k + lo * ldk * es, hi - lo, kw, ldk, es, st));
+  RTQ_TRY(h2d_rows(vd + lo * kw * es, (const char*)v + lo * ldv * es, hi - lo, kw, ldv, es, st));
+  if (q) RTQ_TRY(h2d_rows(qd + lo * qw * es, (const char*)q + lo * ldq * es, hi - lo, qw, ldq, es, st));
+  if (pd) RTQ_TRY(h2d(pd + lo, pos + lo, (size_t)(hi - lo) * 4, st));
   if (r.q_norm) RTQ_TRY(h2d(qn, r.q_norm, (size_t)kc->d * 4, st));
   if (r.k_norm) RTQ_TRY(h2d(kn, r.k_norm, (size_t)kc->d * 4, st));
   if (r.q_norm) r.q_norm = qn;
   if (r.k_norm) r.k_norm = kn;
   RTQ_TRY(enqueue_append(kc, layer, sd, type, r, pd, kd, kw, vd, kw, nh, qd, qw, qd, qw, st));
-  const int64_t lo = s->starts ? s->starts[0] : 0, hi = s->starts ? s->starts[s->b] : n;
-  if (q && hi > lo) RTQ_TRY(d2h_rows((char*)qo + lo * ldo * es, qd + lo * qw * es, hi - lo, qw, ldo, es, st));
+  if (q) RTQ_TRY(d2h_rows((char*)qo + lo * ldo * es, qd + lo * qw * es, hi - lo, qw, ldo, es, st));
   HIP_TRY(hipStreamSynchronize(st));
   return RTQ_OK;
 }
@@ -2997,6 +3003,9 @@ rtq_status rtq_kv_attend(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s, 
   RTQ_TRY(kv_check_parents(s, n, parents));
   rtq_ctx* c = kc->ctx;
   RTQ_TRY(check_ctx(c));
+  int64_t lo, hi;
+  kv_rows(s, n, &lo, &hi);
+  if (hi == lo) return RTQ_OK;
   HostCall hc(c);
   HIP_TRY(hipSetDevice(c->device));
   hipStream_t st = c->stream;
@@ -3008,11 +3017,10 @@ rtq_status rtq_kv_attend(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s, 
   RTQ_TRY(kv_seq_put(*s, n, ar, st, &sd));
   char* qd = ar.take<char>((size_t)(n * qw * es));
   int32_t* pd = parents ? ar.take<int32_t>((size_t)n) : nullptr;
-  RTQ_TRY(h2d_rows(qd, q, n, qw, ldq, es, st));
-  if (pd) RTQ_TRY(h2d(pd, parents, (size_t)n * 4, st));
+  RTQ_TRY(h2d_rows(qd + lo * qw * es, (const char*)q + lo * ldq * es, hi - lo, qw, ldq, es, st));
+  if (pd) RTQ_TRY(h2d(pd + lo, parents + lo, (size_t)(hi - lo) * 4, st));
   RTQ_TRY(enqueue_attend(kc, layer, sd, type, nh, scale, pd, qd, qw, qd, qw, p, ar, st));
-  const int64_t lo = s->starts ? s->starts[0] : 0, hi = s->starts ? s->starts[s->b] : n;
-  if (hi > lo) RTQ_TRY(d2h_rows((char*)out + lo * ldo * es, qd + lo * qw * es, hi - lo, qw, ldo, es, st));
+  RTQ_TRY(d2h_rows((char*)out + lo * ldo * es, qd + lo * qw * es, hi - lo, qw, ldo, es, st));
   HIP_TRY(hipStreamSynchronize(st));
   return RTQ_OK;
 }

@@ -207,3 +207,11 @@ def test_keep_refuses(cache):
         assert st == INVALID and "kept" in msg, msg
     st, msg = keep(cache, seqs(table=((0, 9), (2, 3))), ((30, -1), (1, -1)))
     assert st == INVALID and "page" in msg
+
+
+def test_rows_of_no_sequence_are_not_looked_at(cache):
+    """Positions of rows before the first sequence and behind the last may be anything."""
+    for starts, pos in (((0, 2, 4), (0, 1, 2, 3, -1)), ((1, 2, 5), (-7, 1, 2, 3, 4))):
+        assert append(cache, seqs(starts=starts), positions=np.array(pos, np.int32)) == (INVALID, "null context")
+    st, msg = append(cache, seqs(starts=(1, 2, 5)), positions=np.array((0, 1, 2, 3, -1), np.int32))
+    assert st == INVALID and "position" in msg
