@@ -259,8 +259,9 @@ void rtq_kv_cache_destroy(rtq_kv_cache* kc);
 rtq_status rtq_kv_cache_pages(const rtq_kv_cache* kc, int64_t layer, void** k, void** v); /* device addresses */
 /* The sequences of a call.  Sequence i holds lens[i] tokens, slot s of it in page table[i ld + s / page_size]; its new
  * tokens are rows starts[i] .. starts[i + 1] - 1 (ascending; NULL: n / b each) and take the slots after the held
- * ones.  lens is the caller's to advance, after the last layer.  Rows behind starts[b] are neither read nor
- * written.  No two sequences of a call may write one slot (pages that are only read may be shared). */
+ * ones, 2^30 slots at most (host versions: refused; rtq_kv_attend_d sees none behind them).  lens is the caller's to
+ * advance, after the last layer.  Rows before starts[0] and behind starts[b] are neither read nor written.  No two
+ * sequences of a call may write one slot (pages that are only read may be shared). */
 typedef struct rtq_kv_seqs {
   int64_t b;             /* sequences, 1 .. 65536 */
   const int32_t* lens;   /* [b] */

@@ -636,6 +636,7 @@ struct MMaskArgs {
 
 // ---- paged cache of keys and values (rtq_kv.hip)
 #define RTQ_KV_ROT 256  // most rotated elements of a head
+#define RTQ_KV_SLOTS (1 << 30)  // most slots of a sequence that the attention looks at
 #define RTQ_KV_TARGET 4096  // most items that an attention call is split for
 // the sequences of a call: new tokens are rows starts[i] .. starts[i + 1] - 1 (null: n / b each)
 struct KvSeqs {

@@ -13,7 +13,6 @@ __device__ __forceinline__ int kv_start(const KvSeqs& s, int i) {
   if (!s.starts) return (int)((int64_t)s.n / s.b) * i;
   return min(max(s.starts[i], 0), s.n);
 }
-#define RTQ_KV_SLOTS (1 << 30)  // most slots of a sequence that are looked at
 // tokens held by sequence i, as far as its table's slots go
 __device__ __forceinline__ int kv_held(const int32_t* lens, int i, int ldt, int ps_shift) {
   return (int)min((int64_t)max(lens[i], 0), min((int64_t)ldt << ps_shift, (int64_t)RTQ_KV_SLOTS));

@@ -2918,7 +2918,7 @@ rtq_status kv_check_lists(const rtq_kv_cache* kc, const rtq_kv_seqs* s, int64_t 
     if (s->lens[i] < 0) return fail(RTQ_ERR_INVALID, "sequence %lld holds %d tokens", (long long)i, s->lens[i]);
     const int64_t total = s->lens[i] + (s1 - s0), pages = cdiv(total, kc->ps);
     if (s1 == s0) continue;
-    if (pages > s->ld || total > 0x7fffffff)
+    if (pages > s->ld || total > RTQ_KV_SLOTS)
       return fail(RTQ_ERR_INVALID, "sequence %lld: %lld tokens in a table of %lld pages", (long long)i, (long long)total, (long long)s->ld);
     for (int64_t p = 0; p < pages; p++)
       if (s->table[i * s->ld + p] < 0 || s->table[i * s->ld + p] >= kc->n_pages)
@@ -3027,7 +3027,7 @@ rtq_status rtq_kv_attend(rtq_kv_cache* kc, int64_t layer, const rtq_kv_seqs* s, 
 
 rtq_status rtq_kv_keep(rtq_kv_cache* kc, const rtq_kv_seqs* s, const int32_t* kept, int64_t ldk, int32_t* after) {
   RTQ_TRY(kv_check_keep(kc, s, kept, ldk, after));
-  const int64_t slots = s->ld * kc->ps;
+  const int64_t slots = std::min<int64_t>(s->ld * kc->ps, RTQ_KV_SLOTS);
   for (int64_t i = 0; i < s->b; i++) {
     if (s->lens[i] < 0) return fail(RTQ_ERR_INVALID, "sequence %lld holds %d tokens", (long long)i, s->lens[i]);
     int64_t last = -1;

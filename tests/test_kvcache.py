@@ -215,3 +215,20 @@ def test_rows_of_no_sequence_are_not_looked_at(cache):
         assert append(cache, seqs(starts=starts), positions=np.array(pos, np.int32)) == (INVALID, "null context")
     st, msg = append(cache, seqs(starts=(1, 2, 5)), positions=np.array((0, 1, 2, 3, -1), np.int32))
     assert st == INVALID and "position" in msg
+
+
+def test_sequences_longer_than_the_attention_looks_are_refused():
+    """2^30 slots pass, one more does not (one page stands for all of a table's)."""
+    st, h = create(pages=1, page=1024, kv=1, d=16)
+    table = np.zeros((1, 2 ** 20 + 1), np.int32)
+    L = _ffi.lib()
+    for held, word in ((2 ** 30 - 2, "context"), (2 ** 30 - 1, "table")):
+        lens, starts = np.array([held], np.int32), np.array([0, 2], np.int32)
+        s = _ffi.RtqKvSeqs(1, lens.ctypes.data, starts.ctypes.data, table.ctypes.data, table.shape[1])
+        for call, what in ((append, dict(r=rope(dim=16))), (attend, {})):
+            st, msg = call(h, s, n=2, heads=1, **what)
+            assert st == INVALID and word in msg, msg
+        kept, after = np.array([[1]], np.int32), np.zeros(1, np.int32)
+        st = L.rtq_kv_keep(h, ctypes.byref(s), kept.ctypes.data, 1, after.ctypes.data)
+        assert st == INVALID and ("context" if word == "context" else "kept") in L.rtq_last_error().decode()
+    L.rtq_kv_cache_destroy(h)
