@@ -113,9 +113,10 @@ struct rtq_model {
   std::vector<Layer> layers;
   std::vector<void*> owned;  // device allocations of weights, norms, biases and adapters
   std::vector<rtq_weight*> weights;
-  // step buffers, sized for t_cap tokens and n_cap targets
-  int64_t t_cap = 0, n_cap = 0;
+  // step buffers, sized for t_cap tokens and n_cap targets; t_step, n_step: the most of any step that was no extension of a cache
+  int64_t t_cap = 0, n_cap = 0, t_step = 0, n_step = 0;
   void* step_mem = nullptr;
+  size_t step_bytes = 0;
   void* grads = nullptr;  // every adapter's dA and dB (attach_lora), grad_bytes long
   size_t grad_bytes = 0;
   void* hpk_mem = nullptr;  // every group's kept LoRA-down partials
@@ -622,14 +623,14 @@ rtq_status choose_ckpt(rtq_model* m, int64_t t, int64_t n) {
     m->ckpt = false;
     return RTQ_OK;
   }
-  const int64_t T = std::max(t, m->t_cap), N = std::max<int64_t>(std::max(n, m->n_cap), 1);
+  const int64_t T = std::max(t, m->t_step), N = std::max<int64_t>(std::max(n, m->n_step), 1);
   rtq_model probe;
   probe.cfg = m->cfg;
   probe.attn_fused = m->attn_fused;
   const size_t keep = step_layout(&probe, T, N, m->cfg.n_layer, 0);
   size_t free_b = 0, total_b = 0;
   M_HIP(hipMemGetInfo(&free_b, &total_b));
-  const size_t held = m->step_mem ? step_layout(&probe, m->t_cap, std::max<int64_t>(m->n_cap, 1), m->cache_cap, 0) : 0;
+  const size_t held = m->step_mem ? std::min(m->step_bytes, step_layout(&probe, m->t_cap, std::max<int64_t>(m->n_cap, 1), m->cache_cap, 0)) : 0;
   m->ckpt = keep > (free_b + held) / 2;
   return RTQ_OK;
 }
@@ -643,7 +644,7 @@ rtq_status choose_defer(rtq_model* m, int64_t t) {
     for (const Group& g : L.groups) adapted = adapted || g.rank > 0;
   m->defer_lg = false;
   if (m->ckpt || !m->lora_batch || !m->lora_defer || !adapted || c.n_layer < 2) return RTQ_OK;
-  const int64_t T = std::max(t, m->t_cap), qd = c.n_head * c.head_dim, kd = c.n_head_kv * c.head_dim;
+  const int64_t T = std::max(t, m->t_step), qd = c.n_head * c.head_dim, kd = c.n_head_kv * c.head_dim;
   const size_t extra = (size_t)c.n_layer * (size_t)T * (size_t)(2 * c.n_ff + qd + 2 * kd + 2 * c.n_embd) * 4;
   size_t free_b = 0, total_b = 0;
   M_HIP(hipMemGetInfo(&free_b, &total_b));
@@ -657,7 +658,13 @@ rtq_status ensure_step(rtq_model* m, int64_t t, int64_t n) {
   if (t <= m->t_cap && n <= m->n_cap && caches == m->cache_cap && m->layout_fused == (int64_t)m->attn_fused &&
       m->layout_defer == (int64_t)m->defer_lg)
     return RTQ_OK;
-  const int64_t T = std::max(t, m->t_cap), N = std::max<int64_t>(std::max(n, m->n_cap), 1);
+  int64_t T = std::max(t, m->t_cap), N = std::max<int64_t>(std::max(n, m->n_cap), 1);
+  if (!m->kv) {
+    // a prompt that extended a cache may be far longer than any step: a step's buffers (every block's, [t x t] probabilities)
+    // keep room for its length only where that at most doubles them
+    const int64_t T0 = std::max(t, m->t_step), N0 = std::max<int64_t>(std::max(n, m->n_step), 1);
+    if ((T > T0 || N > N0) && step_layout(m, T, N, caches, 0) > 2 * step_layout(m, T0, N0, caches, 0)) T = T0, N = N0;
+  }
   if (m->step_mem) {
     M_HIP(hipStreamSynchronize(stream_of(m)));
     M_HIP(hipFree(m->step_mem));
@@ -666,6 +673,7 @@ rtq_status ensure_step(rtq_model* m, int64_t t, int64_t n) {
   m->t_cap = m->n_cap = m->cache_cap = 0;
   const size_t bytes = step_layout(m, T, N, caches, 0);
   M_HIP(hipMalloc(&m->step_mem, bytes));
+  m->step_bytes = bytes;
   step_layout(m, T, N, caches, reinterpret_cast<uintptr_t>(m->step_mem));
   m->t_cap = T;
   m->n_cap = N;
@@ -2080,6 +2088,7 @@ rtq_status step(rtq_model* m, const int32_t* tokens, int64_t t, const int32_t* p
   m->job = job;
   m->kv = kv;
   if (!kv) {
+    m->t_step = std::max(m->t_step, t), m->n_step = std::max(m->n_step, n);
     m->attn_fused = m->attn_hd_ok && m->attn_mode != 0;
     M_TRY(choose_ckpt(m, t, n));
     M_TRY(choose_defer(m, t));

@@ -187,3 +187,33 @@ def test_refusals(ctx):
             m.extend(c, a["seqs"], a["tokens"], a["k"], a["positions"], a["parents"], a["temperature"])
     m.extend(c, ok, [1, 2], 1)
     m.close()
+
+
+def test_a_long_prompt_leaves_the_steps_their_size(ctx):
+    """A head size without fused attention, whose steps hold [heads x t x t] probabilities: a prompt of 40000 tokens into a cache, and a
+    step of 60 is what it was before, to the bit, in memory of a step of 60."""
+    import torch
+
+    m = load(ctx, head_dim=48, rope_dim=48)
+    toks, pos, tok = sequence(V, 60, 8)
+    targets = [rt.Target(int(a), int(b)) for a, b in zip(pos, tok)]
+
+    def step():
+        m.zero_grad()
+        lp, _ = m.forward_backward(toks, targets, np.ones(8))
+        return [lp] + [x for i in range(m.lora_count()) for x in m.lora(i)[2:]]
+
+    want = step()
+    rng = np.random.default_rng(0)
+    c = m.cache(40, 1024)
+    prompt = rng.integers(0, V, 40000)
+    te = m.extend(c, rt.Seqs([0], [np.arange(40)]), prompt, 1, positions=[39999])
+    assert np.isfinite(te.vals).all()
+    free = torch.cuda.mem_get_info()[0]
+    for _ in range(2):
+        assert all(np.array_equal(a, b) for a, b in zip(step(), want))
+    assert torch.cuda.mem_get_info()[0] > free - (1 << 30)
+    # the next token of the prompt, and a step again
+    assert np.isfinite(m.extend(c, rt.Seqs([40000], [np.arange(40)]), [1], 1).vals).all()
+    assert all(np.array_equal(a, b) for a, b in zip(step(), want))
+    m.close()
