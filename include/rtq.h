@@ -399,7 +399,8 @@ rtq_status rtq_model_verify_draft(rtq_model* m, rtq_model* draft, const int32_t*
  * rtq_kv_append takes them; seqs->lens held before the call and the caller's to advance) enter kc in every block and
  * attend over it, and rtq_top_logits of the rows that `pos` [np] names (0 <= pos < n, each inside a sequence) is
  * returned.  parents [n] or NULL as rtq_kv_attend's: a token's position is its parent's plus one (the held tokens' number for -1).
- * kc: of the model's context, layers, KV heads and head size. */
+ * kc: of the model's context, layers, KV heads and head size.  (No step: rtq_model_checkpointing and _attention_fused
+ * keep telling of the last one.) */
 rtq_status rtq_model_extend(rtq_model* m, rtq_kv_cache* kc, const rtq_kv_seqs* seqs, const int32_t* tokens, int64_t n,
                             const int32_t* parents, const int32_t* pos, int64_t np, int64_t k, float temperature,
                             float* vals, int32_t* ids, float* rest);

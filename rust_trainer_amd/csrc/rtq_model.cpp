@@ -2317,8 +2317,10 @@ rtq_status rtq_model_extend(rtq_model* m, rtq_kv_cache* kc, const rtq_kv_seqs* s
   HeadJob j{HeadJob::TOP};
   j.k = k, j.temp = temperature, j.vals = vals, j.ids = ids, j.rest = rest;
   KvStep kv{kc, seqs, parents, at.data(), {}, nullptr, nullptr};
+  const bool ckpt = m->ckpt, fused = m->attn_fused, defer = m->defer_lg;
   const rtq_status st = step(m, tokens, n, nullptr, nullptr, pos, nullptr, nullptr, np, nullptr, nullptr, &j, &kv);
   m->kv = nullptr;
+  m->ckpt = ckpt, m->attn_fused = fused, m->defer_lg = defer;  // (what the last step chose stays its answer)
   return st;
 }
 

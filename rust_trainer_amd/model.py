@@ -274,5 +274,4 @@ class GpuModel:
         sv = seqs._view()
         _ffi.check(_ffi.lib().rtq_model_extend(self._h, cache.handle, ctypes.byref(sv), toks.ctypes.data, toks.size, _addr(par), pos.ctypes.data, n, k,
                                                temperature, vals.ctypes.data, ids.ctypes.data, rest.ctypes.data), "rtq_model_extend")
-        self._stepped = True
         return Teacher(ids, vals, rest, temperature)

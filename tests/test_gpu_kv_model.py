@@ -217,3 +217,21 @@ def test_a_long_prompt_leaves_the_steps_their_size(ctx):
     assert np.isfinite(m.extend(c, rt.Seqs([40000], [np.arange(40)]), [1], 1).vals).all()
     assert all(np.array_equal(a, b) for a, b in zip(step(), want))
     m.close()
+
+
+@pytest.mark.parametrize("keep, fused, head_dim", [(False, False, 64), (True, True, 64), (False, None, 48)])
+def test_an_extension_is_no_step(ctx, keep, fused, head_dim):
+    """What the last step chose (activations kept, fused attention) is told after an extension as before it, and nothing before any step."""
+    m = load(ctx, head_dim=head_dim, rope_dim=32)
+    m.checkpointing, m.fused_attention = keep, fused
+    c = m.cache(8, 32)
+    m.extend(c, rt.Seqs([0], [np.arange(8)]), np.arange(100), 1)
+    assert m.checkpointing is None and m.fused_attention is None
+    toks, pos, tok = sequence(V, 60, 8)
+    m.forward_backward(toks, [rt.Target(int(a), int(b)) for a, b in zip(pos, tok)], np.ones(8))
+    want = m.checkpointing, m.fused_attention
+    assert want == (keep, bool(fused))
+    for at, n in ((100, 1), (101, 120)):
+        m.extend(c, rt.Seqs([at], [np.arange(8)]), np.arange(n), 1)
+        assert (m.checkpointing, m.fused_attention) == want
+    m.close()
