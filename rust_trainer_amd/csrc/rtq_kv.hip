@@ -402,11 +402,11 @@ __device__ __forceinline__ bool kv_plan(const KvAttendArgs& a, const int TM, int
   };
   // Ranges of about even x 128 slots share the slots out evenly over the items that run at once.  With few tiles
   // that is it.  With more, what their last ranges leave over makes a second turn of the CUs: then the shortest ranges (of
-  // some) are taken with which all items run at once (32 sequences of 1000 to 7000, 64 rows: 162 -> 133 us).  Tiles that
+  // some) are taken with which all items run at once (32 sequences of 1000 to 7000, 64 rows: 174 -> 140 us).  Tiles that
   // nearly fill the CUs are not split at all, unless one is far longer than the others (32 of 250 to 1750, 4 rows: 42 -> 34
-  // us; 32 of 75 to 525, 256 rows: 60 -> 36).  Small tiles of long sequences, and large ones that have a CU
-  // each, are better off with ranges as short as the items allow, a second turn or not (32 of 4000 to 28000: 457 us against 550
-  // unsplit; 64 rows and a head size of 256: 1326 against 1650).
+  // us).  Small tiles of long sequences, and large ones that have a CU each, are better off with ranges as short as the
+  // items allow, a second turn or not (32 of 4000 to 28000: 457 us against 550 unsplit; 64 rows and a head size of 256:
+  // 1676 against 2199 in even ranges).
   const float even = kv_wave_total(w) * (float)a.nkv / (float)a.once / 128.0f, most = kv_wave_total(whole) * (float)a.nkv;
   const auto range = [&](float f) { return max((int)fminf(ceilf(even * f), (float)(RTQ_KV_SLOTS / 128)) * 128, 128); };
   int C = range(1.0f), c, ns;

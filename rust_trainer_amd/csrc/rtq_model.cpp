@@ -659,20 +659,24 @@ rtq_status ensure_step(rtq_model* m, int64_t t, int64_t n) {
       m->layout_defer == (int64_t)m->defer_lg)
     return RTQ_OK;
   int64_t T = std::max(t, m->t_cap), N = std::max<int64_t>(std::max(n, m->n_cap), 1);
-  if (!m->kv) {
-    // a prompt that extended a cache may be far longer than any step: a step's buffers (every block's, [t x t] probabilities)
-    // keep room for its length only where that at most doubles them
-    const int64_t T0 = std::max(t, m->t_step), N0 = std::max<int64_t>(std::max(n, m->n_step), 1);
-    if ((T > T0 || N > N0) && step_layout(m, T, N, caches, 0) > 2 * step_layout(m, T0, N0, caches, 0)) T = T0, N = N0;
-  }
+  // a prompt that extended a cache may be far longer than any step: a step's buffers (every block's, [t x t] probabilities)
+  // keep room for its length only where that at most doubles them, and where the memory is there
+  const int64_t T0 = m->kv ? T : std::max(t, m->t_step), N0 = m->kv ? N : std::max<int64_t>(std::max(n, m->n_step), 1);
+  const bool more = T > T0 || N > N0;
+  if (more && step_layout(m, T, N, caches, 0) > 2 * step_layout(m, T0, N0, caches, 0)) T = T0, N = N0;
   if (m->step_mem) {
     M_HIP(hipStreamSynchronize(stream_of(m)));
     M_HIP(hipFree(m->step_mem));
     m->step_mem = nullptr;
   }
   m->t_cap = m->n_cap = m->cache_cap = 0;
-  const size_t bytes = step_layout(m, T, N, caches, 0);
-  M_HIP(hipMalloc(&m->step_mem, bytes));
+  size_t bytes = step_layout(m, T, N, caches, 0);
+  if (more && hipMalloc(&m->step_mem, bytes) != hipSuccess) {
+    (void)hipGetLastError();
+    m->step_mem = nullptr;
+    T = T0, N = N0, bytes = step_layout(m, T, N, caches, 0);
+  }
+  if (!m->step_mem) M_HIP(hipMalloc(&m->step_mem, bytes));
   m->step_bytes = bytes;
   step_layout(m, T, N, caches, reinterpret_cast<uintptr_t>(m->step_mem));
   m->t_cap = T;

@@ -2261,10 +2261,10 @@ rtq_status enqueue_append(rtq_kv_cache* kc, int64_t layer, const KvSeqs& s, int 
 }
 
 // The attention's tiles and partial parts.  Small tiles of 16 rows read the cache straight into registers, large ones of
-// 128 through LDS.  Rows of a sequence and KV head average n group / b; measured (bf16, 4 sequences of 1000 slots, head
-// size 128, small and large): 8 rows 16.9 and 21.3 us, 16 rows 21.2 and 16.8 (head size 256, 32 of 4096: 213 and 258), 24
-// rows 32.0 and 17.3; over up to 512 slots (300, head size 64) 24 rows 8.1 and 13.3.  Tiles of 32 rows were never
-// better than both by more than 8%.
+// 128 through LDS.  Rows of a sequence and KV head average n group / b; measured (us, small and large; 8 KV heads, lengths
+// between a quarter and 7 / 4 of what is named): bf16, 4 sequences of 1000, head size 128: 8 rows 16.5 and 16.5, 16 rows
+// 18.7 and 16.6, 24 rows 24.4 and 17.7; f16, 32 of 4000, head size 256: 16 rows 263 and 436, 24 rows 416 and 436, 64 rows 567
+// and 460; over up to 512 slots: bf16, one sequence of 300, head size 64: 24 rows 8.3 and 11.6.
 struct AttendPlan {
   int tm, variant, D, whole;
   bool fused;
@@ -2291,8 +2291,8 @@ AttendPlan attend_plan(const rtq_kv_cache* kc, int64_t n, int64_t b, int64_t ld,
   p.fused = std::min<int64_t>(p.tm, cdiv(rows, b)) * parts <= 128;
   // Joining costs a small tile as much as four more turns of its waves: one of 300 slots 13.8 us split, 12.1 whole, of
   // 1000 15.3 and 21.5.  Large ones are as well whole where the call has no longer sequence (joined: 300 slots, 256 rows, head
-  // size 128 27.4, whole 18.7; 32 of 75 to 525, 64 rows 31.5 and 23.4; 4 of them 21.8 and 20.2; their turns are twice as long
-  // at a head size of 256: 4 of them, 24 rows 24.4 and 36.0).
+  // size 128 27.2, whole 19.8; 32 of 75 to 525, 64 rows 33.0 and 25.0; 4 of them 21.5 and 22.2; their turns are twice as long
+  // at a head size of 256: 4 of them, 24 rows 30.8 and 41.2).
   p.whole = p.tm == 16 ? 512 : p.D > 128 ? 320 : 640;
   p.bytes = (size_t)(2 * p.target * p.tm * (p.D + 2) * 4 + (1 + 2 * p.target) * RTQ_KV_ITEM * 4) + 6 * 256;
   return p;

@@ -235,3 +235,26 @@ def test_an_extension_is_no_step(ctx, keep, fused, head_dim):
         m.extend(c, rt.Seqs([at], [np.arange(8)]), np.arange(n), 1)
         assert (m.checkpointing, m.fused_attention) == want
     m.close()
+
+
+@pytest.mark.parametrize("longer", [90, 700])
+def test_steps_after_prompts_of_any_length(ctx, longer):
+    """Steps and prompts in turn, the prompts somewhat or much longer than the steps: each step is what it was, to the bit, and each prompt's last row the
+    whole sequence's."""
+    m = load(ctx, head_dim=64, n_layer=3)
+    toks, pos, tok = sequence(V, 60, 8)
+    targets = [rt.Target(int(a), int(b)) for a, b in zip(pos, tok)]
+    prompt = np.random.default_rng(1).integers(0, V, longer)
+    c = m.cache(22, 32)
+    want = last = None
+    for _ in range(3):
+        m.zero_grad()
+        lp, _ = m.forward_backward(toks, targets, np.ones(8))
+        got = [lp] + [x for i in range(m.lora_count()) for x in m.lora(i)[2:]]
+        want = want or got
+        assert all(np.array_equal(a, b) for a, b in zip(got, want))
+        te = logits(m.extend(c, rt.Seqs([0], [np.arange(22)]), prompt, V, positions=[longer - 1]))
+        last = te if last is None else last
+        assert np.array_equal(te, last)
+    close(last, whole(m, prompt, [longer - 1]), 1e-3)
+    m.close()
