@@ -255,7 +255,7 @@ RTQ_KV_APPEND(rtq_kv_append_bf16, VT_BF16, VT_BF16)
 // ------------------------------------------------------------------ keep
 // A few rows are moved within the cache: what bounds it is that a token's values are 2 bytes of each of d rows, so that a
 // 64-byte piece is read and written for each (32 sequences, 8 tokens of 63 kept, 28 layers of 8 heads of 128: 22 us,
-// 12.5 at a copy's rate for the bytes alone; one sequence: 4.3 us).
+// 12.5 at a copy's rate for the bytes alone; one sequence: 4.4 us).
 // Workgroup: one KV head of one sequence and layer.  Kept tokens ascend, so the j-th comes from a slot no
 // earlier than its own: a wave that moves its elements in batches of eight tokens, in order, each batch's loads before its
 // stores, never writes a slot that it has yet to read, and no two waves touch the same elements.  Values: eight
@@ -334,8 +334,8 @@ extern "C" __global__ __launch_bounds__(256) void rtq_kv_keep(KvKeepArgs a) {
 // Small tiles (16 rows: single tokens and narrow trees) are bound by the reading of the cache: 64 sequences of up to
 // 8192 tokens, 32 over 8 heads of 128, 1.15 GB: 259 us, 4.4 TB/s; one of 131072: 97 us, 5.5 TB/s (some of it still cached);
 // one of 1000: 14 us, of which the reading takes 1: each item is a chain of dependent loads (lengths, page, keys, values).
-// Large ones (128 rows) are bound by the matrix instructions: 2048 tokens behind 6144, 32 over 8 heads of 128, bf16: 321 us,
-// 0.75 PFLOP/s, and 1.12 with the weights' second plane counted, of a large product's 1.2.
+// Large ones (128 rows) are bound by the matrix instructions: 2048 tokens behind 6144, 32 over 8 heads of 128, bf16: 316 us,
+// 0.76 PFLOP/s, and 1.14 with the weights' second plane counted, of a large product's 1.2.
 //
 // A wave takes 32 slots at a time.  S^T = K q^T and o^T = V^T p^T, so that a lane holds one query row:
 // key row m of tile t is slot 8 (m / 4) + 4 t + m % 4, and the lane that gets the scores of slots 8 g .. 8 g + 7
