@@ -663,7 +663,11 @@ rtq_status ensure_step(rtq_model* m, int64_t t, int64_t n) {
   // keep room for its length only where that at most doubles them, and where the memory is there
   const int64_t T0 = m->kv ? T : std::max(t, m->t_step), N0 = m->kv ? N : std::max<int64_t>(std::max(n, m->n_step), 1);
   const bool more = T > T0 || N > N0;
-  if (more && step_layout(m, T, N, caches, 0) > 2 * step_layout(m, T0, N0, caches, 0)) T = T0, N = N0;
+  if (more) {
+    rtq_model probe;
+    probe.cfg = m->cfg, probe.attn_fused = m->attn_fused, probe.defer_lg = m->defer_lg;
+    if (step_layout(&probe, T, N, caches, 0) > 2 * step_layout(&probe, T0, N0, caches, 0)) T = T0, N = N0;
+  }
   if (m->step_mem) {
     M_HIP(hipStreamSynchronize(stream_of(m)));
     M_HIP(hipFree(m->step_mem));
